@@ -319,6 +319,57 @@ int t2t_rms_norm_backward(const void *dy, int64_t dy_stride, const void *x, int6
                           int64_t dx_stride, void *dweight, void *workspace,
                           int64_t workspace_bytes, int32_t N, int32_t C, void *stream);
 
+/*
+ * Attention prologue with per-head norms: the packed projection rows
+ * [Hq + 2 Hkv][D] (query heads, key heads, value heads) of B x T tokens to
+ * q, k, v; each query and key row x becomes R_p(weight x / sqrt(mean(x^2) +
+ * eps)) with the half-split rotation R_p of t2t_qkv_rope at position
+ * p = pos0 + t; values are copied.  fp32 arithmetic, one rounding.
+ *   qkv      dtype 0 = bf16, 1 = float32, strides in elements; 16-byte
+ *            aligned rows (views too).
+ *   q_weight, k_weight  [D], weight_dtype 0 = bf16, 1 = float32.
+ *   cos, sin float32 [table_rows][D / 2], 16-byte aligned.
+ *   D        a multiple of 16, at most 512.
+ *   q, k, v  [B, Hq | Hkv, T, D] views of the same dtype (out).
+ */
+int t2t_qk_norm_rope(const void *qkv, int64_t stride_b, int64_t stride_t, int32_t B, int32_t T,
+                     int32_t Hq, int32_t Hkv, int32_t D, int32_t dtype, const void *q_weight,
+                     const void *k_weight, int32_t weight_dtype, float eps, const float *cos,
+                     const float *sin, int32_t table_rows, int32_t pos0, const t2t_tensor *q,
+                     const t2t_tensor *k, const t2t_tensor *v, void *stream);
+
+/*
+ * The same map for M new tokens a sequence, q rows to q [B, Hq, M, D] and k, v
+ * rows into caches [B, Hkv, cache_rows, D] at their positions: pos0 + m, or
+ * int64 pos[b pos_stride_b + m] (at most 8 rows then).  A device position
+ * outside the tables or the cache stores nothing and gives a query row of
+ * zeros; of rows at the same position the last is stored.
+ */
+int t2t_qk_norm_rope_append(const void *qkv, int64_t stride_b, int64_t stride_t, int32_t B,
+                            int32_t M, int32_t Hq, int32_t Hkv, int32_t D, int32_t dtype,
+                            const void *q_weight, const void *k_weight, int32_t weight_dtype,
+                            float eps, const float *cos, const float *sin, int32_t table_rows,
+                            const int64_t *pos, int64_t pos_stride_b, int32_t pos0,
+                            const t2t_tensor *q, const t2t_tensor *k_cache,
+                            const t2t_tensor *v_cache, int32_t cache_rows, void *stream);
+
+/* Workspace (bytes) of t2t_qk_norm_rope_backward. */
+int64_t t2t_qk_norm_rope_backward_workspace(int32_t B, int32_t T, int32_t Hq, int32_t Hkv,
+                                            int32_t D);
+
+/*
+ * Gradient of t2t_qk_norm_rope: dqkv [B][T][Hq + 2 Hkv][D] (contiguous) and
+ * the norm weights' gradients [D] (weight_dtype), summed in a fixed order
+ * (deterministic, no atomics); all written, not accumulated.
+ */
+int t2t_qk_norm_rope_backward(const t2t_tensor *dq, const t2t_tensor *dk, const t2t_tensor *dv,
+                              const void *qkv, int64_t stride_b, int64_t stride_t, int32_t B,
+                              int32_t T, int32_t Hq, int32_t Hkv, int32_t D, int32_t dtype,
+                              const void *q_weight, const void *k_weight, int32_t weight_dtype,
+                              float eps, const float *cos, const float *sin, int32_t table_rows,
+                              int32_t pos0, void *dqkv, void *dq_weight, void *dk_weight,
+                              void *workspace, int64_t workspace_bytes, void *stream);
+
 /* Epilogues of t2t_rows_linear. */
 #define T2T_ROWS_STORE 0  /* y = W xin */
 #define T2T_ROWS_ADD 1    /* y = res + bf16(W xin) */

@@ -64,6 +64,14 @@ _SIGS = {
     "t2t_qkv_rope": ([_P, _I64, _I64] + [_I32] * 4 + [_P, _P, _I32, _I32] + [_P] * 4,
                      ctypes.c_int),
     "t2t_qkv_rope_backward": ([_P] * 5 + [_I32] * 6 + [_P, _I64, _I64, _P], ctypes.c_int),
+    "t2t_qk_norm_rope": ([_P, _I64, _I64] + [_I32] * 6 + [_P, _P, _I32, ctypes.c_float, _P, _P,
+                         _I32, _I32] + [_P] * 4, ctypes.c_int),
+    "t2t_qk_norm_rope_append": ([_P, _I64, _I64] + [_I32] * 6 + [_P, _P, _I32, ctypes.c_float,
+                                _P, _P, _I32, _P, _I64, _I32] + [_P] * 3 + [_I32, _P],
+                                ctypes.c_int),
+    "t2t_qk_norm_rope_backward_workspace": ([_I32] * 5, ctypes.c_int64),
+    "t2t_qk_norm_rope_backward": ([_P] * 4 + [_I64, _I64] + [_I32] * 6 + [
+        _P, _P, _I32, ctypes.c_float, _P, _P, _I32, _I32] + [_P] * 4 + [_I64, _P], ctypes.c_int),
     "t2t_attn_decode_workspace": ([_I32] * 5, ctypes.c_int64),
     "t2t_rms_norm": ([_P, _I64, _P, _I32, _P, _I64, _P, _I32, _I32, ctypes.c_float, _P],
                      ctypes.c_int),

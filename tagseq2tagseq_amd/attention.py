@@ -326,9 +326,16 @@ class FlexSelfAttention(nn.Module):
     variant, QK-norm, fp8 out-projection) are not available here, so
     ``fp8_out_proj=True`` is accepted for signature compatibility, warned
     about once, and the output projection stays in the module's dtype.
+
+    ``qk_norm=True`` RMS-normalises every query and key head before the
+    rotation, in the same pass (rope.qk_norm_rope), with the weights
+    ``q_norm`` and ``k_norm`` [head_dim].
     """
 
-    def __init__(self, dim: int, num_heads: int, max_seq_len: int, fp8_out_proj: bool = False):
+    NORM_EPS = 1e-6
+
+    def __init__(self, dim: int, num_heads: int, max_seq_len: int, fp8_out_proj: bool = False,
+                 qk_norm: bool = False):
         super().__init__()
         if dim % num_heads != 0:
             raise ValueError("dim must be divisible by num_heads")
@@ -338,15 +345,23 @@ class FlexSelfAttention(nn.Module):
         self.qkv = Linear(dim, 3 * dim, bias=False)
         self.proj = Linear(dim, dim, bias=False)
         self.rotary = Rotary(self.head_dim, max_seq_len)
+        self.qk_norm = qk_norm
+        if qk_norm:
+            self.q_norm = nn.Parameter(torch.ones(self.head_dim))
+            self.k_norm = nn.Parameter(torch.ones(self.head_dim))
         self.fp8_out_proj = fp8_out_proj
         if fp8_out_proj:
             warnings.warn("FlexSelfAttention(fp8_out_proj=True): the fp8 output projection is not "
                           "implemented; the projection runs in the module's dtype", stacklevel=2)
 
     def forward(self, x: torch.Tensor, block_mask: T2TBlockMask) -> torch.Tensor:
-        from .rope import qkv_rope
+        from .rope import qk_norm_rope, qkv_rope
         B, T, C = x.shape
         cos, sin = self.rotary.tables(x.device)
-        q, k, v = qkv_rope(self.qkv(x), cos, sin, self.num_heads)
+        if self.qk_norm:
+            q, k, v = qk_norm_rope(self.qkv(x), self.q_norm, self.k_norm, cos, sin,
+                                   self.num_heads, eps=self.NORM_EPS)
+        else:
+            q, k, v = qkv_rope(self.qkv(x), cos, sin, self.num_heads)
         y = flex_attention(q, k, v, block_mask=block_mask)
         return self.proj(y.transpose(1, 2).reshape(B, T, C))

@@ -105,6 +105,49 @@ hipError_t launch_qkv_rope_bwd(const TensorView& dq, const TensorView& dk, const
                                int pos0, __bf16* dqkv, int64_t sb, int64_t st,
                                hipStream_t stream);
 
+// Prologue with per-head norms: packed rows [B][T][(Hq + 2 Hkv) D] to normed
+// and rotated q, k and plain v views.  append: k / v go to view row = position.
+struct QkNormArgs {
+  const void* packed;
+  int64_t p_sb, p_st;
+  TensorView ops[3];    // q, k, v
+  const void* qw;       // norm weights [D]
+  const void* kw;
+  bool w_f32;
+  float eps;
+  const float* cos;     // [rows][D / 2]
+  const float* sin;
+  const int64_t* pos;   // [B or 1][T] positions (batch stride pos_sb), or NULL for pos0 + t
+  int64_t pos_sb;
+  int pos0, max_pos;    // positions outside [0, max_pos) have no table / cache row
+  int append;
+  int B, T, Hq, Hkv, D;
+  int lp_log2;          // set by the launcher
+};
+
+struct QkNormBwdArgs {
+  TensorView ops[3];    // dq, dk, dv
+  const void* packed;   // the forward's input rows
+  int64_t p_sb, p_st;
+  void* dpacked;        // [B][T][(Hq + 2 Hkv) D], contiguous
+  const void* qw;
+  const void* kw;
+  bool w_f32;
+  float eps;
+  const float* cos;
+  const float* sin;
+  int pos0;
+  float* part;          // [qk_norm_bwd_groups][D]
+  int B, T, Hq, Hkv, D;
+  int lp_log2, groups[3];  // set by the launcher
+};
+
+int64_t qk_norm_items(int64_t B, int64_t T, int Hq, int Hkv, int D);  // threads of the forward
+int qk_norm_bwd_groups(int B, int T, int Hq, int Hkv, int D);
+hipError_t launch_qk_norm_rope(QkNormArgs a, bool f32, hipStream_t stream);
+hipError_t launch_qk_norm_rope_bwd(QkNormBwdArgs a, bool f32, void* dqw, void* dkw,
+                                   hipStream_t stream);
+
 // Decode step: Tq new query rows per batch row against a key/value cache of
 // Tkv filled positions, mask evaluated per key from doc ids and words.
 constexpr int kDecodeMaxRows = 8;  // (Hq / Hkv) * Tq per launch

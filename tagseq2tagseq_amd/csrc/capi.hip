@@ -565,6 +565,161 @@ int t2t_wgrad(const void* a, int64_t lda, const void* b, int64_t ldb, void* out,
 
 namespace {
 
+// Dimensions and operands that the three norm-and-rotate entries share.
+int check_qk_norm(int32_t B, int32_t T, int32_t Hq, int32_t Hkv, int32_t D, int32_t dtype,
+                  const void* qkv, int64_t stride_b, int64_t stride_t, const void* q_weight,
+                  const void* k_weight, int32_t weight_dtype, float eps, const float* cos,
+                  const float* sin, int32_t table_rows, bool need_rows) {
+  if (B < 0 || T < 0 || Hq < 1 || Hkv < 1)
+    return fail(T2T_EINVAL, "B=%d T=%d Hq=%d Hkv=%d", B, T, Hq, Hkv);
+  if (D < 16 || D > 512 || D % 16 != 0)
+    return fail(T2T_EUNSUPPORTED, "head dim D=%d (a multiple of 16, at most 512)", D);
+  if ((dtype != T2T_DTYPE_BF16 && dtype != T2T_DTYPE_F32) ||
+      (weight_dtype != T2T_DTYPE_BF16 && weight_dtype != T2T_DTYPE_F32))
+    return fail(T2T_EUNSUPPORTED, "dtype %d or weight dtype %d not supported here", dtype,
+                weight_dtype);
+  if (!(eps >= 0.f && eps <= FLT_MAX)) return fail(T2T_EINVAL, "eps=%g", (double)eps);
+  if ((int64_t)B * T > 0x7fffffffLL ||
+      t2t::qk_norm_items(B, T, Hq, Hkv, D) > 0x7fffffffLL)
+    return fail(T2T_EUNSUPPORTED, "B=%d T=%d: more head rows than one launch numbers", B, T);
+  const uintptr_t wa = weight_dtype == T2T_DTYPE_F32 ? 4 : 2;
+  if (!q_weight || !k_weight || reinterpret_cast<uintptr_t>(q_weight) % wa ||
+      reinterpret_cast<uintptr_t>(k_weight) % wa)
+    return fail(T2T_EINVAL, "norm weights NULL or misaligned for their dtype");
+  if (table_rows < 0) return fail(T2T_EINVAL, "negative table_rows");
+  if (!need_rows) return T2T_OK;
+  const int64_t align = dtype == T2T_DTYPE_F32 ? 4 : 8;
+  if (!qkv || reinterpret_cast<uintptr_t>(qkv) % 16 || stride_b < 0 || stride_t < 0 ||
+      stride_b % align || stride_t % align)
+    return fail(T2T_EINVAL, "qkv rows must start on 16-byte boundaries");
+  if (!cos || !sin || (reinterpret_cast<uintptr_t>(cos) | reinterpret_cast<uintptr_t>(sin)) % 16)
+    return fail(T2T_EINVAL, "cos / sin NULL or not 16-byte aligned");
+  return T2T_OK;
+}
+
+int check_head_views(const t2t_tensor* const (&views)[3], int32_t dtype) {
+  const int64_t align = dtype == T2T_DTYPE_F32 ? 4 : 8;
+  for (const t2t_tensor* t : views)
+    if (!t || !t->data || reinterpret_cast<uintptr_t>(t->data) % 16 || t->stride_b < 0 ||
+        t->stride_h < 0 || t->stride_t < 0 || t->stride_b % align || t->stride_h % align ||
+        t->stride_t % align)
+      return fail(T2T_EINVAL, "q / k / v view NULL, or its head rows off a 16-byte boundary");
+  return T2T_OK;
+}
+
+}  // namespace
+
+int t2t_qk_norm_rope(const void* qkv, int64_t stride_b, int64_t stride_t, int32_t B, int32_t T,
+                     int32_t Hq, int32_t Hkv, int32_t D, int32_t dtype, const void* q_weight,
+                     const void* k_weight, int32_t weight_dtype, float eps, const float* cos,
+                     const float* sin, int32_t table_rows, int32_t pos0, const t2t_tensor* q,
+                     const t2t_tensor* k, const t2t_tensor* v, void* stream) {
+  const bool any = B > 0 && T > 0;
+  int rc = check_qk_norm(B, T, Hq, Hkv, D, dtype, qkv, stride_b, stride_t, q_weight, k_weight,
+                         weight_dtype, eps, cos, sin, table_rows, any);
+  if (rc) return rc;
+  if (pos0 < 0 || (int64_t)pos0 + T > table_rows)
+    return fail(T2T_EINVAL, "positions %d..%lld exceed the %d table rows", pos0,
+                (long long)pos0 + T - 1, table_rows);
+  if (!any) return T2T_OK;
+  rc = check_head_views({q, k, v}, dtype);
+  if (rc) return rc;
+  t2t::QkNormArgs a{};
+  a.packed = qkv; a.p_sb = stride_b; a.p_st = stride_t;
+  a.ops[0] = as_view(q); a.ops[1] = as_view(k); a.ops[2] = as_view(v);
+  a.qw = q_weight; a.kw = k_weight; a.w_f32 = weight_dtype == T2T_DTYPE_F32; a.eps = eps;
+  a.cos = cos; a.sin = sin; a.pos0 = pos0; a.max_pos = table_rows;
+  a.B = B; a.T = T; a.Hq = Hq; a.Hkv = Hkv; a.D = D;
+  return hip_status(t2t::launch_qk_norm_rope(a, dtype == T2T_DTYPE_F32,
+                                             static_cast<hipStream_t>(stream)),
+                    "t2t_qk_norm_rope launch");
+}
+
+int t2t_qk_norm_rope_append(const void* qkv, int64_t stride_b, int64_t stride_t, int32_t B,
+                            int32_t M, int32_t Hq, int32_t Hkv, int32_t D, int32_t dtype,
+                            const void* q_weight, const void* k_weight, int32_t weight_dtype,
+                            float eps, const float* cos, const float* sin, int32_t table_rows,
+                            const int64_t* pos, int64_t pos_stride_b, int32_t pos0,
+                            const t2t_tensor* q, const t2t_tensor* k_cache,
+                            const t2t_tensor* v_cache, int32_t cache_rows, void* stream) {
+  const bool any = B > 0 && M > 0;
+  int rc = check_qk_norm(B, M, Hq, Hkv, D, dtype, qkv, stride_b, stride_t, q_weight, k_weight,
+                         weight_dtype, eps, cos, sin, table_rows, any);
+  if (rc) return rc;
+  if (cache_rows < 0) return fail(T2T_EINVAL, "negative cache_rows");
+  if (pos) {
+    if (M > t2t::kRowsMaxRows)
+      return fail(T2T_EUNSUPPORTED, "M=%d rows at device positions; at most %d", M,
+                  t2t::kRowsMaxRows);
+    if (reinterpret_cast<uintptr_t>(pos) % 8 || pos_stride_b < 0)
+      return fail(T2T_EINVAL, "pos misaligned or with a negative stride");
+  } else if (pos0 < 0 || (int64_t)pos0 + M > std::min(table_rows, cache_rows)) {
+    return fail(T2T_EINVAL, "positions %d..%lld exceed the %d table rows or %d cache rows", pos0,
+                (long long)pos0 + M - 1, table_rows, cache_rows);
+  }
+  if (!any) return T2T_OK;
+  rc = check_head_views({q, k_cache, v_cache}, dtype);
+  if (rc) return rc;
+  for (const t2t_tensor* t : {k_cache, v_cache})
+    if ((cache_rows > 1 && t->stride_t == 0) || (Hkv > 1 && t->stride_h == 0) ||
+        (B > 1 && t->stride_b == 0))
+      return fail(T2T_EINVAL, "cache rows overlap (stride 0)");
+  t2t::QkNormArgs a{};
+  a.packed = qkv; a.p_sb = stride_b; a.p_st = stride_t;
+  a.ops[0] = as_view(q); a.ops[1] = as_view(k_cache); a.ops[2] = as_view(v_cache);
+  a.qw = q_weight; a.kw = k_weight; a.w_f32 = weight_dtype == T2T_DTYPE_F32; a.eps = eps;
+  a.cos = cos; a.sin = sin; a.pos = pos; a.pos_sb = pos_stride_b; a.pos0 = pos0;
+  a.max_pos = std::min(table_rows, cache_rows); a.append = 1;
+  a.B = B; a.T = M; a.Hq = Hq; a.Hkv = Hkv; a.D = D;
+  return hip_status(t2t::launch_qk_norm_rope(a, dtype == T2T_DTYPE_F32,
+                                             static_cast<hipStream_t>(stream)),
+                    "t2t_qk_norm_rope_append launch");
+}
+
+int64_t t2t_qk_norm_rope_backward_workspace(int32_t B, int32_t T, int32_t Hq, int32_t Hkv,
+                                            int32_t D) {
+  if (B <= 0 || T <= 0 || Hq < 1 || Hkv < 1 || D < 16 || D > 512 || D % 16 != 0) return 0;
+  return (int64_t)t2t::qk_norm_bwd_groups(B, T, Hq, Hkv, D) * D * 4;
+}
+
+int t2t_qk_norm_rope_backward(const t2t_tensor* dq, const t2t_tensor* dk, const t2t_tensor* dv,
+                              const void* qkv, int64_t stride_b, int64_t stride_t, int32_t B,
+                              int32_t T, int32_t Hq, int32_t Hkv, int32_t D, int32_t dtype,
+                              const void* q_weight, const void* k_weight, int32_t weight_dtype,
+                              float eps, const float* cos, const float* sin, int32_t table_rows,
+                              int32_t pos0, void* dqkv, void* dq_weight, void* dk_weight,
+                              void* workspace, int64_t workspace_bytes, void* stream) {
+  const bool any = B > 0 && T > 0;
+  int rc = check_qk_norm(B, T, Hq, Hkv, D, dtype, qkv, stride_b, stride_t, q_weight, k_weight,
+                         weight_dtype, eps, cos, sin, table_rows, any);
+  if (rc) return rc;
+  if (pos0 < 0 || (int64_t)pos0 + T > table_rows)
+    return fail(T2T_EINVAL, "positions %d..%lld exceed the %d table rows", pos0,
+                (long long)pos0 + T - 1, table_rows);
+  if (!dq_weight || !dk_weight) return fail(T2T_EINVAL, "dq_weight or dk_weight is NULL");
+  t2t::QkNormBwdArgs a{};
+  if (any) {
+    rc = check_head_views({dq, dk, dv}, dtype);
+    if (rc) return rc;
+    if (!dqkv || reinterpret_cast<uintptr_t>(dqkv) % 16)
+      return fail(T2T_EINVAL, "dqkv NULL or not 16-byte aligned");
+    const int64_t need = t2t_qk_norm_rope_backward_workspace(B, T, Hq, Hkv, D);
+    if (!workspace || workspace_bytes < need)
+      return fail(T2T_EINVAL, "workspace of %lld bytes, %lld needed", (long long)workspace_bytes,
+                  (long long)need);
+    a.ops[0] = as_view(dq); a.ops[1] = as_view(dk); a.ops[2] = as_view(dv);
+  }
+  a.packed = qkv; a.p_sb = stride_b; a.p_st = stride_t; a.dpacked = dqkv;
+  a.qw = q_weight; a.kw = k_weight; a.w_f32 = weight_dtype == T2T_DTYPE_F32; a.eps = eps;
+  a.cos = cos; a.sin = sin; a.pos0 = pos0; a.part = static_cast<float*>(workspace);
+  a.B = B; a.T = T; a.Hq = Hq; a.Hkv = Hkv; a.D = D;
+  return hip_status(t2t::launch_qk_norm_rope_bwd(a, dtype == T2T_DTYPE_F32, dq_weight, dk_weight,
+                                                 static_cast<hipStream_t>(stream)),
+                    "t2t_qk_norm_rope_backward launch");
+}
+
+namespace {
+
 int check_swiglu(int32_t N, int32_t H, const void* const* ptrs, int np, const int64_t* strides,
                  int ns, const int64_t* min_strides) {
   if (N < 0 || H <= 0 || H % 8 != 0)

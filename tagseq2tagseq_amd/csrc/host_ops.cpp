@@ -18,6 +18,8 @@
 #include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 
+#include <cmath>
+#include <cstdint>
 #include <tuple>
 #include <vector>
 
@@ -203,6 +205,192 @@ Tensor qkv_rope_backward(const Tensor& dq_in, const Tensor& dk_in, const Tensor&
                               dqkv.stride(1), stream_of(dq)),
         "t2t_qkv_rope_backward");
   return dqkv;
+}
+
+// ---- QKV split + norms of queries and keys + rotary embedding
+
+// bfloat16 or float32 rows as the kernels read them: unit stride along the
+// last dimension, the other strides (of dimensions that are stepped) and the
+// start on 16-byte boundaries; anything else is copied.
+Tensor vector_rows(const Tensor& t) {
+  const int64_t align = 16 / t.element_size();
+  bool ok = t.stride(-1) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+  for (int64_t d = 0; d + 1 < t.dim(); ++d)
+    ok = ok && (t.size(d) == 1 || (t.stride(d) >= 0 && t.stride(d) % align == 0));
+  return ok ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+
+t2t_tensor heads_of(const Tensor& t) {
+  const auto stride = [&](int d) { return t.size(d) == 1 ? 0 : t.stride(d); };
+  return t2t_tensor{t.data_ptr(), stride(0), stride(1), stride(2)};
+}
+
+// What the three calls below take, checked: the packed rows (copied where the
+// kernels cannot read them), weights and tables.
+struct QkNorm {
+  Tensor qkv, qw, kw, cos, sin;
+  int64_t B, T, H, Hkv, D, sb, st;
+  int code, wcode;
+  QkNorm(const Tensor& qkv_in, const Tensor& qw_in, const Tensor& kw_in, const Tensor& cos_in,
+         const Tensor& sin_in, int64_t heads, int64_t kv_heads, double eps) {
+    TORCH_CHECK_VALUE(qkv_in.dim() == 3, "qkv must be [B, T, (H + 2 Hkv) D], got shape ",
+                      qkv_in.sizes());
+    TORCH_CHECK_VALUE(heads > 0 && kv_heads > 0, "num_heads=", heads, " and num_kv_heads=",
+                      kv_heads, " must be positive");
+    H = heads;
+    Hkv = kv_heads;
+    // (as a quotient: twice a huge count would not fit)
+    TORCH_CHECK_VALUE(H <= qkv_in.size(2) && Hkv <= qkv_in.size(2) &&
+                          qkv_in.size(2) % (H + 2 * Hkv) == 0,
+                      "last dim ", qkv_in.size(2), " is not (num_heads + 2 num_kv_heads) * "
+                      "head_dim (num_heads=", H, ", num_kv_heads=", Hkv, ")");
+    TORCH_CHECK_NOT_IMPLEMENTED(
+        qkv_in.scalar_type() == at::kBFloat16 || qkv_in.scalar_type() == at::kFloat, "qkv dtype ",
+        qkv_in.scalar_type(), " is not supported (bfloat16 or float32)");
+    D = qkv_in.size(2) / (H + 2 * Hkv);
+    TORCH_CHECK_VALUE(qw_in.dim() == 1 && qw_in.size(0) == D && kw_in.sizes() == qw_in.sizes(),
+                      "q_weight ", qw_in.sizes(), " and k_weight ", kw_in.sizes(),
+                      " must be [head_dim] = [", D, "]");
+    TORCH_CHECK_VALUE(qw_in.scalar_type() == kw_in.scalar_type(),
+                      "q_weight and k_weight differ in dtype");
+    TORCH_CHECK_VALUE(cos_in.dim() == 2 && cos_in.size(1) * 2 == D &&
+                          sin_in.sizes() == cos_in.sizes() &&
+                          cos_in.scalar_type() == at::kFloat &&
+                          sin_in.scalar_type() == at::kFloat,
+                      "cos ", cos_in.sizes(), " and sin ", sin_in.sizes(),
+                      " must be float32 [rows, head_dim / 2]");
+    TORCH_CHECK_VALUE(eps >= 0 && std::isfinite(eps), "eps=", eps);
+    need_gpu(qkv_in, qw_in, kw_in, cos_in, sin_in);
+    for (const Tensor* t : {&qw_in, &kw_in, &cos_in, &sin_in})
+      TORCH_CHECK_VALUE(t->device() == qkv_in.device(), "operands on different devices");
+    const c10::DeviceGuard guard(qkv_in.device());
+    code = qkv_in.scalar_type() == at::kFloat ? T2T_DTYPE_F32 : T2T_DTYPE_BF16;
+    wcode = weight_code(qw_in);
+    qkv = vector_rows(qkv_in);
+    qw = qw_in.contiguous();
+    kw = kw_in.contiguous();
+    cos = vector_rows(cos_in.contiguous());
+    sin = vector_rows(sin_in.contiguous());
+    B = qkv.size(0);
+    T = qkv.size(1);
+    sb = B == 1 ? 0 : qkv.stride(0);
+    st = T == 1 ? 0 : qkv.stride(1);
+    TORCH_CHECK_VALUE(B <= INT32_MAX && T <= INT32_MAX && H <= INT32_MAX && D <= INT32_MAX,
+                      "qkv ", qkv.sizes(), " is too large");
+  }
+  int64_t rows() const { return std::min<int64_t>(cos.size(0), INT32_MAX); }
+  int64_t first(int64_t pos0) const {
+    TORCH_CHECK_VALUE(pos0 >= 0 && pos0 <= rows() && pos0 + T <= rows(), "positions ", pos0,
+                      " .. ", pos0 + T - 1, " exceed the ", rows(), " table rows");
+    return pos0;
+  }
+};
+
+std::tuple<Tensor, Tensor, Tensor> qk_norm_rope(const Tensor& qkv_in, const Tensor& q_weight,
+                                                const Tensor& k_weight, const Tensor& cos_in,
+                                                const Tensor& sin_in, int64_t heads,
+                                                int64_t kv_heads, int64_t pos0, double eps) {
+  const QkNorm a(qkv_in, q_weight, k_weight, cos_in, sin_in, heads, kv_heads, eps);
+  const c10::DeviceGuard guard(a.qkv.device());
+  a.first(pos0);
+  Tensor q = at::empty({a.B, a.H, a.T, a.D}, a.qkv.options()),
+         k = at::empty({a.B, a.Hkv, a.T, a.D}, a.qkv.options()), v = at::empty_like(k);
+  const t2t_tensor qs = heads_of(q), ks = heads_of(k), vs = heads_of(v);
+  check(t2t_qk_norm_rope(a.qkv.data_ptr(), a.sb, a.st, a.B, a.T, a.H, a.Hkv, a.D, a.code,
+                         a.qw.data_ptr(), a.kw.data_ptr(), a.wcode, static_cast<float>(eps),
+                         a.cos.data_ptr<float>(), a.sin.data_ptr<float>(), a.rows(), pos0, &qs,
+                         &ks, &vs, stream_of(a.qkv)),
+        "t2t_qk_norm_rope");
+  return {q, k, v};
+}
+
+std::tuple<Tensor, Tensor, Tensor> qk_norm_rope_backward(
+    const Tensor& dq_in, const Tensor& dk_in, const Tensor& dv_in, const Tensor& qkv_in,
+    const Tensor& q_weight, const Tensor& k_weight, const Tensor& cos_in, const Tensor& sin_in,
+    int64_t heads, int64_t kv_heads, int64_t pos0, double eps) {
+  const QkNorm a(qkv_in, q_weight, k_weight, cos_in, sin_in, heads, kv_heads, eps);
+  const c10::DeviceGuard guard(a.qkv.device());
+  a.first(pos0);
+  need_gpu(dq_in, dk_in, dv_in);
+  const std::vector<int64_t> qshape{a.B, a.H, a.T, a.D}, kshape{a.B, a.Hkv, a.T, a.D};
+  TORCH_CHECK_VALUE(dq_in.sizes() == at::IntArrayRef(qshape) &&
+                        dk_in.sizes() == at::IntArrayRef(kshape) &&
+                        dv_in.sizes() == at::IntArrayRef(kshape),
+                    "gradients ", dq_in.sizes(), ", ", dk_in.sizes(), ", ", dv_in.sizes(),
+                    " do not fit qkv ", qkv_in.sizes());
+  for (const Tensor* t : {&dq_in, &dk_in, &dv_in})
+    TORCH_CHECK_VALUE(t->scalar_type() == a.qkv.scalar_type() && t->device() == a.qkv.device(),
+                      "gradients differ from qkv in dtype or device");
+  const Tensor dq = vector_rows(dq_in), dk = vector_rows(dk_in), dv = vector_rows(dv_in);
+  Tensor dqkv = at::empty(a.qkv.sizes(), a.qkv.options());
+  Tensor dqw = at::empty_like(a.qw), dkw = at::empty_like(a.kw);
+  const int64_t bytes = t2t_qk_norm_rope_backward_workspace(a.B, a.T, a.H, a.Hkv, a.D);
+  Tensor ws = at::empty({std::max<int64_t>(1, bytes / 4)}, a.cos.options());
+  const t2t_tensor qs = heads_of(dq), ks = heads_of(dk), vs = heads_of(dv);
+  check(t2t_qk_norm_rope_backward(&qs, &ks, &vs, a.qkv.data_ptr(), a.sb, a.st, a.B, a.T, a.H,
+                                  a.Hkv, a.D, a.code, a.qw.data_ptr(), a.kw.data_ptr(), a.wcode,
+                                  static_cast<float>(eps), a.cos.data_ptr<float>(),
+                                  a.sin.data_ptr<float>(), a.rows(), pos0, dqkv.data_ptr(),
+                                  dqw.data_ptr(), dkw.data_ptr(), ws.data_ptr(), ws.numel() * 4,
+                                  stream_of(a.qkv)),
+        "t2t_qk_norm_rope_backward");
+  return {dqkv, dqw, dkw};
+}
+
+// pos: int64 [M] or [B, M] on the device, or undefined for pos0 + m.
+Tensor qk_norm_rope_append(const Tensor& qkv_in, const Tensor& q_weight, const Tensor& k_weight,
+                           const Tensor& cos_in, const Tensor& sin_in, int64_t heads,
+                           const c10::optional<Tensor>& pos_in, int64_t pos0,
+                           const Tensor& k_cache, const Tensor& v_cache, double eps) {
+  TORCH_CHECK_VALUE(k_cache.dim() == 4 && k_cache.sizes() == v_cache.sizes(), "caches ",
+                    k_cache.sizes(), " and ", v_cache.sizes(),
+                    " must both be [B, Hkv, capacity, D]");
+  const QkNorm a(qkv_in, q_weight, k_weight, cos_in, sin_in, heads, k_cache.size(1), eps);
+  const c10::DeviceGuard guard(a.qkv.device());
+  TORCH_CHECK_VALUE(k_cache.size(0) == a.B && k_cache.size(3) == a.D, "caches ", k_cache.sizes(),
+                    " do not fit qkv ", qkv_in.sizes(), " of ", heads, " query heads");
+  for (const Tensor* t : {&k_cache, &v_cache}) {
+    need_gpu(*t);
+    TORCH_CHECK_VALUE(t->scalar_type() == a.qkv.scalar_type() && t->device() == a.qkv.device(),
+                      "the caches differ from qkv in dtype or device");
+    // written in place, so not copied
+    TORCH_CHECK_VALUE(t->stride(3) == 1 || t->numel() == 0,
+                      "the cache rows must have unit stride");
+  }
+  const int64_t cap = std::min<int64_t>(k_cache.size(2), INT32_MAX);
+  Tensor pos;
+  int64_t pos_sb = 0;
+  if (pos_in.has_value()) {
+    TORCH_CHECK_VALUE(pos_in->is_cuda() && pos_in->device() == a.qkv.device() &&
+                          pos_in->scalar_type() == at::kLong,
+                      "pos must be an int64 tensor on qkv's device");
+    const bool each = pos_in->dim() == 2;
+    TORCH_CHECK_VALUE((pos_in->dim() == 1 && pos_in->size(0) == a.T) ||
+                          (each && pos_in->size(0) == a.B && pos_in->size(1) == a.T),
+                      "pos ", pos_in->sizes(), " must be [", a.T, "] or [", a.B, ", ", a.T, "]");
+    pos = pos_in->contiguous();
+    pos_sb = each ? a.T : 0;
+  } else {
+    TORCH_CHECK_VALUE(pos0 >= 0 && pos0 <= std::min(cap, a.rows()) &&
+                          pos0 + a.T <= std::min(cap, a.rows()),
+                      "positions ", pos0, " .. ", pos0 + a.T - 1, " exceed the ", a.rows(),
+                      " table rows or the ", cap, " cache rows");
+  }
+  Tensor q = at::empty({a.B, a.H, a.T, a.D}, a.qkv.options());
+  const auto cache = [](const Tensor& t) {
+    t2t_tensor s = heads_of(t);
+    s.stride_t = t.stride(2);
+    return s;
+  };
+  const t2t_tensor qs = heads_of(q), ks = cache(k_cache), vs = cache(v_cache);
+  check(t2t_qk_norm_rope_append(a.qkv.data_ptr(), a.sb, a.st, a.B, a.T, a.H, a.Hkv, a.D, a.code,
+                                a.qw.data_ptr(), a.kw.data_ptr(), a.wcode,
+                                static_cast<float>(eps), a.cos.data_ptr<float>(),
+                                a.sin.data_ptr<float>(), a.rows(),
+                                pos.defined() ? pos.data_ptr<int64_t>() : nullptr, pos_sb,
+                                pos.defined() ? 0 : pos0, &qs, &ks, &vs, cap, stream_of(a.qkv)),
+        "t2t_qk_norm_rope_append");
+  return q;
 }
 
 // ---- SwiGLU
@@ -410,6 +598,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("rms_norm_backward", &rms_norm_backward, no_gil);
   m.def("qkv_rope", &qkv_rope, no_gil);
   m.def("qkv_rope_backward", &qkv_rope_backward, no_gil);
+  m.def("qk_norm_rope", &qk_norm_rope, no_gil);
+  m.def("qk_norm_rope_backward", &qk_norm_rope_backward, no_gil);
+  m.def("qk_norm_rope_append", &qk_norm_rope_append, no_gil);
   m.def("swiglu", &swiglu, no_gil);
   m.def("swiglu_backward",
         [](const Tensor& g2, const Tensor& dh, const std::vector<int64_t>& shape) {

@@ -39,7 +39,7 @@ from .attention import flex_attention
 from .block_mask import T2TBlockMask, build_block_mask
 from .decode import MAX_ROWS, attn_decode
 from .modules import RMSNorm, TS2TSBackbone
-from .rope import qkv_rope
+from .rope import qk_norm_rope_append, qkv_rope
 from .rows import applies as rows_apply, rows_linear, rows_qkv_rope
 
 
@@ -132,10 +132,10 @@ class TS2TSModel:
                     max_seq_len: int, dropout: float, drop_path_rate: float,
                     block_mask_creator: Callable, fp8: bool = False, weight_tying: bool = True,
                     ignore_index: int = -100, tokenizer=None, link_detector=None,
-                    layout_policy=None) -> "TS2TSModel":
+                    layout_policy=None, qk_norm: bool = False) -> "TS2TSModel":
         backbone = TS2TSBackbone(num_layers=num_layers, model_dim=model_dim, num_heads=num_heads,
                                  max_seq_len=max_seq_len, dropout=dropout,
-                                 drop_path_rate=drop_path_rate, fp8=fp8)
+                                 drop_path_rate=drop_path_rate, fp8=fp8, qk_norm=qk_norm)
         embedding = nn.Embedding(vocab_size, model_dim)
         norm = RMSNorm(model_dim)
         if weight_tying:
@@ -302,7 +302,10 @@ class TS2TSModel:
             attn = layer.attn
             C = x.shape[-1]
             nxt = self._next_skip(i, skips) if fused else None
-            if fused:
+            if attn.qk_norm:
+                q = self._normed_rows(layer, x, fused, buf.pos, cos_t, sin_t, cache.k[i],
+                                      cache.v[i])
+            elif fused:
                 q = rows_qkv_rope(x, attn.qkv.weight, attn.num_heads, cos_t, sin_t, buf.pos,
                                   cache.k[i], cache.v[i], norm=layer.ln_1)
             else:
@@ -318,6 +321,16 @@ class TS2TSModel:
         if fused:
             return rows_linear(x, self.lm_head_weight, norm=self.norm)
         return F.linear(self.norm(x), self.lm_head_weight)
+
+    @staticmethod
+    def _normed_rows(layer, x, fused: bool, pos, cos, sin, k_cache, v_cache):
+        """Query rows of a layer with query / key norms; its keys and values go
+        to the cache rows at their positions (an int or a device tensor)."""
+        attn = layer.attn
+        h = (rows_linear(x, attn.qkv.weight, norm=layer.ln_1) if fused else
+             attn.qkv(layer.ln_1(x)))
+        return qk_norm_rope_append(h, attn.q_norm, attn.k_norm, cos, sin, attn.num_heads, pos,
+                                   k_cache, v_cache, eps=attn.NORM_EPS)
 
     def _rows_fusable(self, x) -> bool:
         """Whether the layers of a few-row step can run on the fused row
@@ -395,7 +408,10 @@ class TS2TSModel:
         B, n, C = x.shape
         T = p0 + n
         cos, sin = attn.rotary.tables(x.device)
-        if fused:
+        if attn.qk_norm:
+            q = self._normed_rows(layer, x, fused, p0, cos, sin, cache.k[i], cache.v[i])
+            k, v = cache.k[i, :, :, p0:T], cache.v[i, :, :, p0:T]
+        elif fused:
             q = rows_qkv_rope(x, attn.qkv.weight, attn.num_heads, cos, sin, p0, cache.k[i],
                               cache.v[i], norm=layer.ln_1)
         else:

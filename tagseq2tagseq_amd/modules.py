@@ -89,15 +89,16 @@ class DropPath(nn.Module):
 
 
 class Layer(nn.Module):
-    """model/modules/layer.py:11-35."""
+    """model/modules/layer.py:11-35; ``qk_norm``: norms of the attention's query
+    and key heads (FlexSelfAttention)."""
 
     def __init__(self, n_embd: int, n_head: int, dropout: float, max_seq_len: int, fp8: bool,
-                 drop_path_rate: float):
+                 drop_path_rate: float, qk_norm: bool = False):
         super().__init__()
         self.drop_path = DropPath(drop_path_rate)
         self.ln_1 = RMSNorm(n_embd)
         self.attn = FlexSelfAttention(dim=n_embd, num_heads=n_head, max_seq_len=max_seq_len,
-                                      fp8_out_proj=fp8)
+                                      fp8_out_proj=fp8, qk_norm=qk_norm)
         self.ln_2 = RMSNorm(n_embd)
         self.mlp = GLU(in_dim=n_embd, out_dim=n_embd, hidden_dim=int(8 / 3 * n_embd),
                        activation="silu", dropout=dropout, fp8=fp8)
@@ -115,13 +116,13 @@ class TS2TSBackbone(nn.Module):
 
     def __init__(self, num_layers: int, model_dim: int, num_heads: int, max_seq_len: int,
                  dropout: float, drop_path_rate: float, fp8: bool = False,
-                 activation_checkpointing: bool = False, **kwargs):
+                 activation_checkpointing: bool = False, qk_norm: bool = False, **kwargs):
         super().__init__()
         self.model_dim = model_dim
         self.max_seq_len = max_seq_len
         self.layers = nn.ModuleList([
             Layer(n_embd=model_dim, n_head=num_heads, max_seq_len=max_seq_len, dropout=dropout,
-                  drop_path_rate=drop_path_rate, fp8=fp8) for _ in range(num_layers)])
+                  drop_path_rate=drop_path_rate, fp8=fp8, qk_norm=qk_norm) for _ in range(num_layers)])
         self.skip_weights = nn.Parameter(torch.ones(num_layers // 2))
         self.activation_checkpointing = activation_checkpointing
 
@@ -203,11 +204,13 @@ class TS2TSTrainingModule(nn.Module):
                     max_seq_len: int, dropout: float, drop_path_rate: float,
                     block_mask_creator: Callable, fp8: bool = False, weight_tying: bool = True,
                     ignore_index: int = -100, dtype: torch.dtype = torch.bfloat16,
-                    activation_checkpointing: bool = False) -> "TS2TSTrainingModule":
+                    activation_checkpointing: bool = False,
+                    qk_norm: bool = False) -> "TS2TSTrainingModule":
         backbone = TS2TSBackbone(num_layers=num_layers, model_dim=model_dim, num_heads=num_heads,
                                  max_seq_len=max_seq_len, dropout=dropout,
                                  drop_path_rate=drop_path_rate, fp8=fp8,
-                                 activation_checkpointing=activation_checkpointing)
+                                 activation_checkpointing=activation_checkpointing,
+                                 qk_norm=qk_norm)
         embedding = nn.Embedding(vocab_size, model_dim)
         norm = RMSNorm(model_dim)
         loss_fn = LinearCELoss(D=model_dim, V=vocab_size, dtype=dtype, ignore_index=ignore_index,

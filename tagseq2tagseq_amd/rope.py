@@ -12,12 +12,24 @@ is the textbook form and its parity with tunalab is unpinned).
     cos, sin = rope_tables(head_dim, rows, device)      # float32 [rows, D/2]
 
 Kernels: libt2t_attn.so ``t2t_qkv_rope`` / ``t2t_qkv_rope_backward``.
+
+With RMS norms of every query and key head before the rotation (one weight of
+head_dim for the queries, one for the keys; the norm that keeps attention
+logits bounded), and with fewer key / value heads than query heads:
+
+    q, k, v = qk_norm_rope(qkv, q_weight, k_weight, cos, sin, num_heads)
+    q = qk_norm_rope_append(qkv, q_weight, k_weight, cos, sin, num_heads, pos,
+                            k_cache, v_cache)       # new tokens, k / v cached
+
+Kernels: ``t2t_qk_norm_rope``, ``t2t_qk_norm_rope_backward`` and
+``t2t_qk_norm_rope_append`` (bf16 and float32).
 """
 from __future__ import annotations
 
-from typing import Dict, Tuple
+from typing import Dict, Optional, Tuple, Union
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 
@@ -140,3 +152,114 @@ def qkv_rope(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, num_heads:
     if _lib.unwatched(qkv, cos, sin):
         return _qkv_rope_impl(qkv, cos, sin, int(num_heads), int(pos0))
     return QKVRopeFn.apply(qkv, cos, sin, int(num_heads), int(pos0))
+
+
+# ---- with norms of queries and keys
+
+def _qk_norm_dims(qkv: torch.Tensor, num_heads: int, num_kv_heads: int):
+    B, T, W = qkv.shape
+    return B, T, W // (num_heads + 2 * num_kv_heads)
+
+
+@torch.library.custom_op("t2t::qk_norm_rope", mutates_args=())
+def qk_norm_rope_op(qkv: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor,
+                    cos: torch.Tensor, sin: torch.Tensor, num_heads: int, num_kv_heads: int,
+                    pos0: int, eps: float) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """q [B, H, T, D] and k, v [B, Hkv, T, D] from qkv [B, T, (H + 2 Hkv) D];
+    q and k normed per head and rotated."""
+    return _lib.host().qk_norm_rope(qkv, q_weight, k_weight, cos, sin, num_heads, num_kv_heads,
+                                    pos0, eps)
+
+
+@qk_norm_rope_op.register_fake
+def _qk_norm_rope_fake(qkv, q_weight, k_weight, cos, sin, num_heads, num_kv_heads, pos0, eps):
+    B, T, D = _qk_norm_dims(qkv, num_heads, num_kv_heads)
+    return tuple(qkv.new_empty((B, h, T, D)) for h in (num_heads, num_kv_heads, num_kv_heads))
+
+
+@torch.library.custom_op("t2t::qk_norm_rope_backward", mutates_args=())
+def qk_norm_rope_backward_op(
+        dq: torch.Tensor, dk: torch.Tensor, dv: torch.Tensor, qkv: torch.Tensor,
+        q_weight: torch.Tensor, k_weight: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
+        num_heads: int, num_kv_heads: int, pos0: int,
+        eps: float) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(dqkv, dq_weight, dk_weight)."""
+    return _lib.host().qk_norm_rope_backward(dq, dk, dv, qkv, q_weight, k_weight, cos, sin,
+                                             num_heads, num_kv_heads, pos0, eps)
+
+
+@qk_norm_rope_backward_op.register_fake
+def _qk_norm_rope_backward_fake(dq, dk, dv, qkv, q_weight, k_weight, cos, sin, num_heads,
+                                num_kv_heads, pos0, eps):
+    return (qkv.new_empty(qkv.shape), q_weight.new_empty(q_weight.shape),
+            k_weight.new_empty(k_weight.shape))
+
+
+def _qk_norm_rope_setup(ctx, inputs, output):
+    ctx.save_for_backward(*inputs[:5])
+    ctx.args = inputs[5:]
+
+
+def _qk_norm_rope_bwd(ctx, dq, dk, dv):
+    dqkv, dqw, dkw = qk_norm_rope_backward_op(dq, dk, dv, *ctx.saved_tensors, *ctx.args)
+    return dqkv, dqw, dkw, None, None, None, None, None, None
+
+
+qk_norm_rope_op.register_autograd(_qk_norm_rope_bwd, setup_context=_qk_norm_rope_setup)
+
+
+class QKNormRopeFn(torch.autograd.Function):
+    """The same kernels as t2t::qk_norm_rope for eager execution (as QKVRopeFn
+    is for t2t::qkv_rope)."""
+
+    @staticmethod
+    def forward(ctx, qkv, q_weight, k_weight, cos, sin, *args):
+        ctx.save_for_backward(qkv, q_weight, k_weight, cos, sin)
+        ctx.args = args
+        return _lib.host().qk_norm_rope(qkv, q_weight, k_weight, cos, sin, *args)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dq, dk, dv):
+        got = _lib.host().qk_norm_rope_backward(dq, dk, dv, *ctx.saved_tensors, *ctx.args)
+        return (*got, None, None, None, None, None, None)
+
+
+def qk_norm_rope(qkv: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor,
+                 cos: torch.Tensor, sin: torch.Tensor, num_heads: int,
+                 num_kv_heads: Optional[int] = None, pos0: int = 0, eps: float = 1e-6):
+    """Split qkv [B, T, (H + 2 Hkv) D] (query heads, key heads, value heads;
+    Hkv = H unless ``num_kv_heads`` is given) into q [B, H, T, D] and k, v
+    [B, Hkv, T, D] (contiguous): every query and key row RMS-normalised with
+    q_weight / k_weight [D] and then rotated at positions pos0 .. pos0 + T - 1
+    (table rows), value rows copied.  bf16 or float32 rows, head_dim a
+    multiple of 16 up to 512, bf16 or float32 weights; fp32 arithmetic with one
+    rounding.  Gradients for qkv and the weights."""
+    args = (int(num_heads), int(num_heads if num_kv_heads is None else num_kv_heads), int(pos0),
+            float(eps))
+    if torch.compiler.is_compiling():
+        return qk_norm_rope_op(qkv, q_weight, k_weight, cos, sin, *args)
+    if _lib.unwatched(qkv, q_weight, k_weight, cos, sin):
+        return _lib.host().qk_norm_rope(qkv, q_weight, k_weight, cos, sin, *args)
+    return QKNormRopeFn.apply(qkv, q_weight, k_weight, cos, sin, *args)
+
+
+def qk_norm_rope_append(qkv: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor,
+                        cos: torch.Tensor, sin: torch.Tensor, num_heads: int,
+                        pos: Union[int, torch.Tensor], k_cache: torch.Tensor,
+                        v_cache: torch.Tensor, eps: float = 1e-6) -> torch.Tensor:
+    """``qk_norm_rope`` of M new tokens' rows qkv [B, M, (H + 2 Hkv) D] with
+    the keys and values written into k_cache / v_cache [B, Hkv, capacity, D]
+    at their positions; returns q [B, H, M, D].  Every other cache row is left
+    as it is.
+
+    pos: the first token's position (rows at pos .. pos + M - 1), or a device
+    int64 tensor [M] or [B, M] of positions, read by the kernel (M at most 8).
+    A device position outside the tables or the cache stores nothing and gives
+    a query row of zeros; of rows at the same position the last is stored.
+    No gradient: for rows that autograd records, use ``qk_norm_rope``."""
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (qkv, q_weight, k_weight)):
+        raise RuntimeError("qk_norm_rope_append has no gradient: call it under torch.no_grad()")
+    at, pos0 = (pos, 0) if isinstance(pos, torch.Tensor) else (None, int(pos))
+    return _lib.host().qk_norm_rope_append(qkv, q_weight, k_weight, cos, sin, int(num_heads), at,
+                                           pos0, k_cache, v_cache, float(eps))
