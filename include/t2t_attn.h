@@ -370,6 +370,74 @@ int t2t_qk_norm_rope_backward(const t2t_tensor *dq, const t2t_tensor *dk, const 
                               int32_t pos0, void *dqkv, void *dq_weight, void *dk_weight,
                               void *workspace, int64_t workspace_bytes, void *stream);
 
+/*
+ * Scaled embedding lookup: out[i] = scale weight[tokens[i]] for N ids (int64),
+ * computed in fp32 and rounded once; an id outside [0, V) gives a row of NaN.
+ *   weight   [V][C], dtype 0 = bf16, 1 = float32, row stride weight_stride >= C
+ *            (elements); V at most 2^24.
+ *   out      [N][C] contiguous, same dtype.
+ * Rows are moved in 16-byte pieces where C, the stride and the addresses allow
+ * it, element by element otherwise.
+ */
+int t2t_embedding(const int64_t *tokens, int64_t N, const void *weight, int64_t weight_stride,
+                  int64_t V, int32_t C, int32_t dtype, float scale, void *out, void *stream);
+
+/* Workspace (bytes) of t2t_embedding_backward. */
+int64_t t2t_embedding_backward_workspace(int64_t N, int64_t V, int32_t C);
+
+/*
+ * Gradient of t2t_embedding: dweight[v] = scale * sum of dy[i] over the i with
+ * tokens[i] == v, in fp32 in the order of the positions (deterministic, no
+ * atomics on values), rounded once.  Every row of dweight [V][C] (contiguous)
+ * is written; the row `padding` (-1: none) and those of ids that do not occur
+ * are zero; ids outside [0, V) are left out.
+ *   dy       [N][C] rows of the dtype with row stride dy_stride.
+ */
+int t2t_embedding_backward(const int64_t *tokens, int64_t N, const void *dy, int64_t dy_stride,
+                           int64_t V, int32_t C, int32_t dtype, float scale, int64_t padding,
+                           void *dweight, void *workspace, int64_t workspace_bytes,
+                           void *stream);
+
+/*
+ * Distillation loss of logit rows z [rows][V] from a teacher's top logits, and
+ * its gradient, in one pass.  For row r, with teacher logits t_k at columns
+ * i_k = idx[r][k] (slots of i_k < 0 are empty), T = temperature, a = alpha:
+ *   p = softmax over the slots of t / T,  q = softmax(z / T)
+ *   row_loss = a T^2 sum_k p_k (ln p_k - ln q(i_k))
+ *            + (1 - a) (logsumexp(z) - z[target])
+ *   grad_j   = s (a T ([slots] q_j - sum over k with i_k = j of p_k)
+ *            + (1 - a) (softmax(z)_j - [j = target]))
+ * with s = scale * *scale_dev * g[r g_stride] (the last two where given).
+ * T is 0.01 to 100.  Slots of one column add up.  A row whose slots are all empty or -inf has no
+ * first part; a row whose target is ignore_index has loss and gradient 0 and
+ * is not read; a target outside [0, V) or a column i_k >= V makes the row's
+ * loss NaN and its gradient 0.
+ *   logits   dtype 0 = bf16, 1 = float32; rows at any address of the type,
+ *            stride ld >= V (elements; grad likewise).
+ *   idx      int32 or int64 (idx_bytes 4 or 8); teacher dtype 0 / 1; K <= 1024.
+ *   target   int64 [rows], or NULL with alpha 1.
+ *   row_loss float [rows] or NULL; grad (dtype) or NULL, may be the logits.
+ *   unless_one  nonzero: nothing is done where *g is 1 (g_stride 0), for a
+ *            gradient written earlier with g taken as 1.
+ */
+int t2t_distill_rows(const void *logits, int64_t ld, int64_t rows, int32_t V, int32_t dtype,
+                     const void *idx, int32_t idx_bytes, int64_t idx_ld, const void *teacher,
+                     int32_t teacher_dtype, int64_t teacher_ld, int32_t K, const int64_t *target,
+                     int64_t ignore_index, float temperature, float alpha, float scale,
+                     const float *scale_dev, const float *g, int64_t g_stride,
+                     int32_t unless_one, float *row_loss, void *grad, int64_t grad_ld,
+                     void *stream);
+
+/* out[0] = 1 / max(n, 1), out[1] = 1 / n (NaN for n = 0), n the rows whose
+ * target is not ignore_index. */
+int t2t_distill_count(const int64_t *target, int64_t rows, int64_t ignore_index, float *out,
+                      void *stream);
+
+/* *loss = scale (*scale_dev where given) times the sum of the row losses, added
+ * in 64 bits in a fixed order. */
+int t2t_distill_mean(const float *row_loss, int64_t rows, const float *scale_dev, float scale,
+                     float *loss, void *stream);
+
 /* Epilogues of t2t_rows_linear. */
 #define T2T_ROWS_STORE 0  /* y = W xin */
 #define T2T_ROWS_ADD 1    /* y = res + bf16(W xin) */

@@ -72,6 +72,16 @@ _SIGS = {
     "t2t_qk_norm_rope_backward_workspace": ([_I32] * 5, ctypes.c_int64),
     "t2t_qk_norm_rope_backward": ([_P] * 4 + [_I64, _I64] + [_I32] * 6 + [
         _P, _P, _I32, ctypes.c_float, _P, _P, _I32, _I32] + [_P] * 4 + [_I64, _P], ctypes.c_int),
+    "t2t_embedding": ([_P, _I64, _P, _I64, _I64, _I32, _I32, ctypes.c_float, _P, _P],
+                      ctypes.c_int),
+    "t2t_embedding_backward_workspace": ([_I64, _I64, _I32], ctypes.c_int64),
+    "t2t_embedding_backward": ([_P, _I64, _P, _I64, _I64, _I32, _I32, ctypes.c_float, _I64, _P,
+                               _P, _I64, _P], ctypes.c_int),
+    "t2t_distill_rows": ([_P, _I64, _I64, _I32, _I32, _P, _I32, _I64, _P, _I32, _I64, _I32, _P,
+                          _I64] + [ctypes.c_float] * 3 + [_P, _P, _I64, _I32, _P, _P, _I64, _P],
+                         ctypes.c_int),
+    "t2t_distill_count": ([_P, _I64, _I64, _P, _P], ctypes.c_int),
+    "t2t_distill_mean": ([_P, _I64, _P, ctypes.c_float, _P, _P], ctypes.c_int),
     "t2t_attn_decode_workspace": ([_I32] * 5, ctypes.c_int64),
     "t2t_rms_norm": ([_P, _I64, _P, _I32, _P, _I64, _P, _I32, _I32, ctypes.c_float, _P],
                      ctypes.c_int),

@@ -148,6 +148,78 @@ hipError_t launch_qk_norm_rope(QkNormArgs a, bool f32, hipStream_t stream);
 hipError_t launch_qk_norm_rope_bwd(QkNormBwdArgs a, bool f32, void* dqw, void* dkw,
                                    hipStream_t stream);
 
+// Scaled embedding lookup: out[i] = scale W[tokens[i]] (rows of C, contiguous
+// out); ids outside [0, V) give NaN rows.  vector: rows in 16-byte pieces.
+struct EmbedArgs {
+  const int64_t* tokens;
+  int64_t N;
+  const void* weight;
+  int64_t w_stride;
+  int64_t V;
+  int C;
+  float scale;
+  void* out;
+};
+hipError_t launch_embed(const EmbedArgs& a, bool f32, bool vector, hipStream_t stream);
+
+// Its weight gradient [V][C] (contiguous, every row written).
+struct EmbedGradArgs {
+  const int64_t* tokens;
+  int N;
+  int64_t V;
+  int64_t padding;      // id whose row's gradient is zero, or -1
+  const void* dy;
+  int64_t dy_stride;
+  int C;
+  float scale;
+  void* dweight;
+  // set by the launcher, in the workspace:
+  int* count;           // positions in the list
+  int2* list;           // (position, token), grouped by token
+  float* part;          // [pieces][2][C]: a token that came from / goes on behind the piece
+  int group_log2, rows_per_group, piece;
+};
+struct EmbedPlan {
+  int group_log2, rows_per_group, piece;
+  int64_t list_at, part_at, bytes;
+};
+EmbedPlan embed_plan(int64_t N, int64_t V, int C);
+hipError_t launch_embed_grad(EmbedGradArgs a, void* workspace, bool f32, bool vector,
+                             hipStream_t stream);
+
+// Distillation loss of logit rows from a teacher's top logits, and its gradient.
+constexpr int kDistillMaxSlots = 1024;
+struct DistillArgs {
+  const void* logits;
+  int64_t ld, rows;
+  int V;
+  const void* idx;        // [rows][idx_ld] columns, int64 or int32; < 0: an empty slot
+  bool idx64;
+  int64_t idx_ld;
+  const void* teacher;    // [rows][teacher_ld] logits, bf16 or fp32
+  bool teacher_f32;
+  int64_t teacher_ld;
+  int K;
+  const int64_t* target;  // or NULL: every row counts, alpha 1
+  int64_t ignore_index;
+  float temp, inv_temp, alpha;
+  float scale;            // of the gradient, times *scale_dev and g[row * g_stride]
+  const float* scale_dev;
+  const float* g;
+  int64_t g_stride;
+  int unless_one;         // do nothing where *g is 1
+  float* row_loss;        // or NULL
+  void* grad;             // or NULL; may be the logits
+  int64_t grad_ld;
+};
+hipError_t launch_distill_rows(const DistillArgs& a, bool f32, hipStream_t stream);
+// out[0] = 1 / max(n, 1), out[1] = 1 / n (NaN for 0) of n counted rows.
+hipError_t launch_distill_count(const int64_t* target, int64_t rows, int64_t ignore_index,
+                                float* out, hipStream_t stream);
+// *loss = scale (*scale_dev where given) times the sum of the row losses.
+hipError_t launch_distill_mean(const float* row_loss, int64_t rows, const float* scale_dev,
+                               float scale, float* loss, hipStream_t stream);
+
 // Decode step: Tq new query rows per batch row against a key/value cache of
 // Tkv filled positions, mask evaluated per key from doc ids and words.
 constexpr int kDecodeMaxRows = 8;  // (Hq / Hkv) * Tq per launch

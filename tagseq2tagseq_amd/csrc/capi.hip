@@ -720,6 +720,145 @@ int t2t_qk_norm_rope_backward(const t2t_tensor* dq, const t2t_tensor* dk, const 
 
 namespace {
 
+constexpr int64_t kEmbedMaxV = 1 << 24;
+
+int check_embed(const void* tokens, int64_t N, int64_t V, int32_t C, int32_t dtype) {
+  if (N < 0 || V < 1 || C < 1)
+    return fail(T2T_EINVAL, "N=%lld V=%lld C=%d", (long long)N, (long long)V, C);
+  if (dtype != T2T_DTYPE_BF16 && dtype != T2T_DTYPE_F32)
+    return fail(T2T_EUNSUPPORTED, "dtype %d not supported here", dtype);
+  if (V > kEmbedMaxV || N >= (1LL << 31) - 4096 || N * C > 1LL << 38)
+    return fail(T2T_EUNSUPPORTED, "N=%lld V=%lld C=%d: more than one launch numbers",
+                (long long)N, (long long)V, C);
+  if (N > 0 && (!tokens || reinterpret_cast<uintptr_t>(tokens) % 8))
+    return fail(T2T_EINVAL, "tokens NULL or misaligned");
+  return T2T_OK;
+}
+
+// Whether rows of C elements at these addresses and strides can be read in
+// 16-byte pieces; -1 where an address is off its own type.
+int embed_vector(int32_t C, int32_t dtype, const void* a, const void* b, int64_t stride) {
+  const int64_t size = dtype == T2T_DTYPE_F32 ? 4 : 2, piece = 16 / size;
+  const uintptr_t at = reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b);
+  if (at % size) return -1;
+  return C % piece == 0 && stride % piece == 0 && at % 16 == 0;
+}
+
+}  // namespace
+
+int t2t_embedding(const int64_t* tokens, int64_t N, const void* weight, int64_t weight_stride,
+                  int64_t V, int32_t C, int32_t dtype, float scale, void* out, void* stream) {
+  const int rc = check_embed(tokens, N, V, C, dtype);
+  if (rc) return rc;
+  if (N == 0) return T2T_OK;
+  const int vec = embed_vector(C, dtype, weight, out, weight_stride);
+  if (!weight || !out || vec < 0 || weight_stride < C)
+    return fail(T2T_EINVAL, "weight or out NULL, misaligned, or a row stride below C");
+  return hip_status(t2t::launch_embed({tokens, N, weight, weight_stride, V, C, scale, out},
+                                      dtype == T2T_DTYPE_F32, vec,
+                                      static_cast<hipStream_t>(stream)),
+                    "t2t_embedding launch");
+}
+
+int64_t t2t_embedding_backward_workspace(int64_t N, int64_t V, int32_t C) {
+  if (N < 0 || V < 1 || V > kEmbedMaxV || C < 1 || N >= (1LL << 31) - 4096) return 0;
+  return t2t::embed_plan(N, V, C).bytes;
+}
+
+int t2t_embedding_backward(const int64_t* tokens, int64_t N, const void* dy, int64_t dy_stride,
+                           int64_t V, int32_t C, int32_t dtype, float scale, int64_t padding,
+                           void* dweight, void* workspace, int64_t workspace_bytes,
+                           void* stream) {
+  const int rc = check_embed(tokens, N, V, C, dtype);
+  if (rc) return rc;
+  if (padding < -1 || padding >= V)
+    return fail(T2T_EINVAL, "padding id %lld outside [-1, V)", (long long)padding);
+  const int vec = embed_vector(C, dtype, dy, dweight, dy_stride);
+  if (!dweight || vec < 0 || (N > 0 && (!dy || dy_stride < 0)))
+    return fail(T2T_EINVAL, "dy or dweight NULL, misaligned, or a negative row stride");
+  const int64_t need = t2t_embedding_backward_workspace(N, V, C);
+  if (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16)
+    return fail(T2T_EINVAL, "workspace of %lld bytes (16-byte aligned), %lld needed",
+                (long long)workspace_bytes, (long long)need);
+  t2t::EmbedGradArgs a{};
+  a.tokens = tokens; a.N = (int)N; a.V = V; a.padding = padding; a.dy = dy;
+  a.dy_stride = dy_stride; a.C = C; a.scale = scale; a.dweight = dweight;
+  return hip_status(t2t::launch_embed_grad(a, workspace, dtype == T2T_DTYPE_F32, vec,
+                                           static_cast<hipStream_t>(stream)),
+                    "t2t_embedding_backward launch");
+}
+
+int t2t_distill_rows(const void* logits, int64_t ld, int64_t rows, int32_t V, int32_t dtype,
+                     const void* idx, int32_t idx_bytes, int64_t idx_ld, const void* teacher,
+                     int32_t teacher_dtype, int64_t teacher_ld, int32_t K, const int64_t* target,
+                     int64_t ignore_index, float temperature, float alpha, float scale,
+                     const float* scale_dev, const float* g, int64_t g_stride, int32_t unless_one,
+                     float* row_loss, void* grad, int64_t grad_ld, void* stream) {
+  if (rows < 0 || V < 1 || K < 0)
+    return fail(T2T_EINVAL, "rows=%lld V=%d K=%d", (long long)rows, V, K);
+  if (K > t2t::kDistillMaxSlots)
+    return fail(T2T_EUNSUPPORTED, "K=%d slots a row; at most %d", K, t2t::kDistillMaxSlots);
+  if ((dtype != T2T_DTYPE_BF16 && dtype != T2T_DTYPE_F32) ||
+      (K > 0 && teacher_dtype != T2T_DTYPE_BF16 && teacher_dtype != T2T_DTYPE_F32))
+    return fail(T2T_EUNSUPPORTED, "dtype %d or teacher dtype %d not supported here", dtype,
+                teacher_dtype);
+  if (K > 0 && idx_bytes != 4 && idx_bytes != 8)
+    return fail(T2T_EUNSUPPORTED, "indices of %d bytes (4 or 8)", idx_bytes);
+  // (the loss is a difference of logarithms, rounded at 1e-6, times its square)
+  if (!(temperature >= 0.01f && temperature <= 100.f))
+    return fail(T2T_EINVAL, "temperature=%g outside [0.01, 100]", (double)temperature);
+  if (!(alpha >= 0.f && alpha <= 1.f))
+    return fail(T2T_EINVAL, "alpha=%g outside [0, 1]", (double)alpha);
+  if (alpha < 1.f && !target) return fail(T2T_EINVAL, "alpha below 1 needs targets");
+  if (ld < V || (grad && grad_ld < V)) return fail(T2T_EINVAL, "row stride below V");
+  if (unless_one && (!g || g_stride != 0))
+    return fail(T2T_EINVAL, "unless_one needs one incoming gradient");
+  if (rows == 0) return T2T_OK;
+  if (rows > 0x7fffffffLL)
+    return fail(T2T_EUNSUPPORTED, "rows=%lld: more than one launch numbers", (long long)rows);
+  const uintptr_t size = dtype == T2T_DTYPE_F32 ? 4 : 2;
+  if (!logits || (!row_loss && !grad) || reinterpret_cast<uintptr_t>(logits) % size ||
+      reinterpret_cast<uintptr_t>(grad) % size)
+    return fail(T2T_EINVAL, "logits NULL, nothing to write, or an address off its type");
+  if (grad == logits && grad_ld != ld)
+    return fail(T2T_EINVAL, "a gradient over the logits has their row stride");
+  if (K > 0 && (!idx || !teacher || idx_ld < 0 || teacher_ld < 0 ||
+                reinterpret_cast<uintptr_t>(idx) % idx_bytes ||
+                reinterpret_cast<uintptr_t>(teacher) % (teacher_dtype == T2T_DTYPE_F32 ? 4 : 2)))
+    return fail(T2T_EINVAL, "idx or teacher NULL, misaligned or with a negative stride");
+  t2t::DistillArgs a{};
+  a.logits = logits; a.ld = ld; a.rows = rows; a.V = V;
+  a.idx = idx; a.idx64 = idx_bytes == 8; a.idx_ld = idx_ld;
+  a.teacher = teacher; a.teacher_f32 = teacher_dtype == T2T_DTYPE_F32; a.teacher_ld = teacher_ld;
+  a.K = K; a.target = target; a.ignore_index = ignore_index;
+  a.temp = temperature; a.inv_temp = 1.f / temperature; a.alpha = alpha;
+  a.scale = scale; a.scale_dev = scale_dev; a.g = g; a.g_stride = g_stride;
+  a.unless_one = unless_one; a.row_loss = row_loss; a.grad = grad; a.grad_ld = grad_ld;
+  return hip_status(t2t::launch_distill_rows(a, dtype == T2T_DTYPE_F32,
+                                             static_cast<hipStream_t>(stream)),
+                    "t2t_distill_rows launch");
+}
+
+int t2t_distill_count(const int64_t* target, int64_t rows, int64_t ignore_index, float* out,
+                      void* stream) {
+  if (rows < 0 || rows > 0x7fffffffLL) return fail(T2T_EINVAL, "rows=%lld", (long long)rows);
+  if (!out || (rows > 0 && !target)) return fail(T2T_EINVAL, "target or out is NULL");
+  return hip_status(t2t::launch_distill_count(target, rows, ignore_index, out,
+                                              static_cast<hipStream_t>(stream)),
+                    "t2t_distill_count launch");
+}
+
+int t2t_distill_mean(const float* row_loss, int64_t rows, const float* scale_dev, float scale,
+                     float* loss, void* stream) {
+  if (rows < 0) return fail(T2T_EINVAL, "rows=%lld", (long long)rows);
+  if (!loss || (rows > 0 && !row_loss)) return fail(T2T_EINVAL, "row_loss or loss is NULL");
+  return hip_status(t2t::launch_distill_mean(row_loss, rows, scale_dev, scale, loss,
+                                             static_cast<hipStream_t>(stream)),
+                    "t2t_distill_mean launch");
+}
+
+namespace {
+
 int check_swiglu(int32_t N, int32_t H, const void* const* ptrs, int np, const int64_t* strides,
                  int ns, const int64_t* min_strides) {
   if (N < 0 || H <= 0 || H % 8 != 0)

@@ -393,6 +393,270 @@ Tensor qk_norm_rope_append(const Tensor& qkv_in, const Tensor& q_weight, const T
   return q;
 }
 
+// ---- scaled embedding
+
+int embed_code(const Tensor& w) {
+  TORCH_CHECK_NOT_IMPLEMENTED(w.scalar_type() == at::kBFloat16 || w.scalar_type() == at::kFloat,
+                              "weight dtype ", w.scalar_type(),
+                              " is not supported (bfloat16 or float32)");
+  return w.scalar_type() == at::kFloat ? T2T_DTYPE_F32 : T2T_DTYPE_BF16;
+}
+
+Tensor embed_ids(const Tensor& tokens) {
+  TORCH_CHECK_VALUE(tokens.scalar_type() == at::kLong || tokens.scalar_type() == at::kInt,
+                    "tokens must be int64 or int32, not ", tokens.scalar_type());
+  return tokens.to(at::kLong).contiguous();
+}
+
+Tensor embedding(const Tensor& tokens, const Tensor& weight, double scale) {
+  TORCH_CHECK_VALUE(weight.dim() == 2, "weight must be [V, C], got shape ", weight.sizes());
+  const int code = embed_code(weight);
+  need_gpu(tokens, weight);
+  TORCH_CHECK_VALUE(tokens.device() == weight.device(), "tokens and weight on different devices");
+  const c10::DeviceGuard guard(weight.device());
+  const Tensor ids = embed_ids(tokens);
+  const int64_t V = weight.size(0), C = weight.size(1);
+  const bool rows = (weight.stride(1) == 1 || C == 1) && weight.stride(0) >= C;
+  const Tensor w = rows ? weight : weight.contiguous();
+  std::vector<int64_t> shape = tokens.sizes().vec();
+  shape.push_back(C);
+  Tensor out = at::empty(shape, weight.options());
+  if (out.numel())
+    check(t2t_embedding(ids.data_ptr<int64_t>(), ids.numel(), w.data_ptr(),
+                        V == 1 ? C : w.stride(0), V, static_cast<int32_t>(C), code,
+                        static_cast<float>(scale), out.data_ptr(), stream_of(weight)),
+          "t2t_embedding");
+  return out;
+}
+
+// dy [..., C] of the tokens; the gradient [V, C] of dy's dtype.
+Tensor embedding_backward(const Tensor& tokens, const Tensor& dy_in, int64_t V, double scale,
+                          int64_t padding) {
+  const int code = embed_code(dy_in);
+  need_gpu(tokens, dy_in);
+  TORCH_CHECK_VALUE(tokens.device() == dy_in.device(), "tokens and gradient on different devices");
+  const c10::DeviceGuard guard(dy_in.device());
+  const Tensor ids = embed_ids(tokens);
+  const int64_t C = dy_in.size(-1), N = ids.numel();
+  TORCH_CHECK_VALUE(dy_in.numel() == N * C, "gradient ", dy_in.sizes(), " does not fit tokens ",
+                    tokens.sizes());
+  Tensor dw = at::empty({V, C}, dy_in.options());
+  if (dw.numel() == 0) return dw;
+  Tensor dy = dy_in.dim() == 2 ? dy_in : dy_in.reshape({N, C});
+  if (dy.stride(1) != 1) dy = dy.contiguous();
+  Tensor ws = at::empty({t2t_embedding_backward_workspace(N, V, C)},
+                        dy.options().dtype(at::kByte));
+  check(t2t_embedding_backward(ids.data_ptr<int64_t>(), N, dy.data_ptr(),
+                               N == 1 ? C : dy.stride(0), V, static_cast<int32_t>(C), code,
+                               static_cast<float>(scale), padding, dw.data_ptr(), ws.data_ptr(),
+                               ws.numel(), stream_of(dy)),
+        "t2t_embedding_backward");
+  return dw;
+}
+
+// ---- distillation loss
+
+int float_code(const Tensor& t, const char* what) {
+  TORCH_CHECK_NOT_IMPLEMENTED(t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kFloat,
+                              what, " dtype ", t.scalar_type(),
+                              " is not supported (bfloat16 or float32)");
+  return t.scalar_type() == at::kFloat ? T2T_DTYPE_F32 : T2T_DTYPE_BF16;
+}
+
+// The last dimension's rows with unit stride and a row stride of at least
+// their length.
+Tensor plain_rows(const Tensor& t) {
+  Tensor r = t.dim() == 2 ? t : t.reshape({-1, t.size(-1)});
+  const bool ok = (r.stride(1) == 1 || r.size(1) == 1) &&
+                  (r.size(0) == 1 || r.stride(0) >= r.size(1));
+  return ok ? r : r.clone(at::MemoryFormat::Contiguous);
+}
+
+// What the distillation calls take, checked; reduction: 0 none, 1 sum, 2 mean.
+struct Distill {
+  Tensor z, idx, teacher, target;
+  std::vector<int64_t> shape;  // of the logits
+  int64_t rows = 0, V = 0, K = 0, ignore = 0;
+  int code = 0, teacher_code = 0;
+  double temp = 1, alpha = 1;
+  Distill(const Tensor& logits, const Tensor& idx_in, const Tensor& teacher_in,
+          const c10::optional<Tensor>& target_in, double temperature, double alpha_in,
+          int64_t ignore_index)
+      : ignore(ignore_index), temp(temperature), alpha(alpha_in) {
+    TORCH_CHECK_VALUE(logits.dim() >= 1 && logits.size(-1) >= 1 && logits.size(-1) <= INT32_MAX,
+                      "logits must be [..., V], got shape ", logits.sizes());
+    TORCH_CHECK_VALUE(idx_in.sizes() == teacher_in.sizes() && idx_in.dim() == logits.dim() &&
+                          idx_in.sizes().slice(0, idx_in.dim() - 1) ==
+                              logits.sizes().slice(0, logits.dim() - 1),
+                      "teacher_idx ", idx_in.sizes(), " and teacher_logits ", teacher_in.sizes(),
+                      " must be [..., K] of logits ", logits.sizes());
+    TORCH_CHECK_VALUE(idx_in.scalar_type() == at::kLong || idx_in.scalar_type() == at::kInt,
+                      "teacher_idx must be int64 or int32, not ", idx_in.scalar_type());
+    TORCH_CHECK_VALUE(temp >= 0.01 && temp <= 100, "temperature=", temp,
+                      " must be in [0.01, 100]");
+    TORCH_CHECK_VALUE(alpha >= 0 && alpha <= 1, "alpha=", alpha, " must be in [0, 1]");
+    TORCH_CHECK_VALUE(alpha == 1 || target_in.has_value(), "alpha below 1 needs targets");
+    code = float_code(logits, "logits");
+    teacher_code = float_code(teacher_in, "teacher_logits");
+    need_gpu(logits, idx_in, teacher_in);
+    TORCH_CHECK_VALUE(idx_in.device() == logits.device() && teacher_in.device() == logits.device(),
+                      "logits and teacher on different devices");
+    shape = logits.sizes().vec();
+    V = logits.size(-1);
+    rows = logits.numel() / V;
+    K = idx_in.size(-1);
+    const c10::DeviceGuard guard(logits.device());
+    if (target_in.has_value()) {
+      TORCH_CHECK_VALUE(target_in->sizes() == logits.sizes().slice(0, logits.dim() - 1) &&
+                            (target_in->scalar_type() == at::kLong ||
+                             target_in->scalar_type() == at::kInt),
+                        "targets ", target_in->sizes(), " must be int64 or int32 ids of logits ",
+                        logits.sizes());
+      need_gpu(*target_in);
+      TORCH_CHECK_VALUE(target_in->device() == logits.device(),
+                        "logits and targets on different devices");
+      target = target_in->to(at::kLong).contiguous().view({-1});
+    }
+    if (rows == 0) return;
+    z = plain_rows(logits);
+    if (K > 0) {
+      idx = plain_rows(idx_in);
+      teacher = plain_rows(teacher_in);
+    }
+  }
+  // One launch over the rows; any of the outputs may be undefined.  grad: rows
+  // of stride grad_ld, the logits themselves among them.
+  void launch(const Tensor& row_loss, const Tensor& grad, int64_t grad_ld, double scale,
+              const Tensor& scale_dev, const Tensor& g, bool unless_one) const {
+    if (rows == 0) return;
+    const auto ptr = [](const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; };
+    check(t2t_distill_rows(
+              z.data_ptr(), step(z), rows, static_cast<int32_t>(V), code, ptr(idx),
+              idx.defined() && idx.scalar_type() == at::kInt ? 4 : 8, step(idx), ptr(teacher),
+              teacher_code, step(teacher), static_cast<int32_t>(K),
+              static_cast<const int64_t*>(ptr(target)), ignore, static_cast<float>(temp),
+              static_cast<float>(alpha), static_cast<float>(scale),
+              static_cast<const float*>(ptr(scale_dev)), static_cast<const float*>(ptr(g)),
+              g.defined() && g.numel() > 1 ? 1 : 0, unless_one,
+              static_cast<float*>(ptr(row_loss)), ptr(grad), grad_ld, stream_of(z)),
+          "t2t_distill_rows");
+  }
+  static int64_t step(const Tensor& t) {
+    return !t.defined() ? 0 : t.size(0) == 1 ? t.size(1) : t.stride(0);
+  }
+};
+
+// (loss, gradient for an incoming gradient of 1, [1 / max(n, 1), 1 / n]); the
+// second only when asked for, and never for the rows' own losses.
+std::tuple<Tensor, Tensor, Tensor> distill_loss(
+    const Tensor& logits, const Tensor& idx, const Tensor& teacher,
+    const c10::optional<Tensor>& target, double temperature, double alpha, int64_t ignore_index,
+    int64_t reduction, bool with_grad) {
+  const Distill a(logits, idx, teacher, target, temperature, alpha, ignore_index);
+  const c10::DeviceGuard guard(logits.device());
+  const auto f32 = logits.options().dtype(at::kFloat);
+  Tensor row_loss = at::empty(logits.sizes().slice(0, logits.dim() - 1), f32);
+  if (reduction == 0) {
+    a.launch(row_loss, Tensor(), a.V, 1.0, Tensor(), Tensor(), false);
+    return {row_loss, Tensor(), Tensor()};
+  }
+  Tensor inv;
+  double scale = 1.0;
+  if (reduction == 2) {
+    if (a.target.defined()) {
+      inv = at::empty({2}, f32);
+      check(t2t_distill_count(a.target.data_ptr<int64_t>(), a.rows, ignore_index,
+                              inv.data_ptr<float>(), stream_of(logits)),
+            "t2t_distill_count");
+    } else {
+      scale = a.rows ? 1.0 / static_cast<double>(a.rows) : NAN;
+    }
+  }
+  Tensor grad = with_grad ? at::empty(a.shape, logits.options()) : Tensor();
+  a.launch(row_loss, grad, a.V, scale, inv, Tensor(), false);
+  Tensor loss = at::empty({}, f32);
+  check(t2t_distill_mean(row_loss.data_ptr<float>(), a.rows,
+                         inv.defined() ? inv.data_ptr<float>() + 1 : nullptr,
+                         static_cast<float>(scale), loss.data_ptr<float>(), stream_of(logits)),
+        "t2t_distill_mean");
+  return {loss, grad, inv};
+}
+
+// The logits' gradient for the incoming gradient g (one value, or one a row for
+// reduction 0).  kept: the gradient of distill_loss, which stands where g is 1
+// and is written again where it is not.
+Tensor distill_loss_backward(const Tensor& g_in, const Tensor& logits, const Tensor& idx,
+                             const Tensor& teacher, const c10::optional<Tensor>& target,
+                             double temperature, double alpha, int64_t ignore_index,
+                             int64_t reduction, const c10::optional<Tensor>& inv_in,
+                             const c10::optional<Tensor>& kept) {
+  const Distill a(logits, idx, teacher, target, temperature, alpha, ignore_index);
+  need_gpu(g_in);
+  const c10::DeviceGuard guard(logits.device());
+  TORCH_CHECK_VALUE(g_in.scalar_type() == at::kFloat && g_in.device() == logits.device() &&
+                        g_in.numel() == (reduction == 0 ? a.rows : 1),
+                    "gradient ", g_in.sizes(), " ", g_in.scalar_type(), " does not fit the loss");
+  const Tensor g = g_in.contiguous();
+  Tensor inv = inv_in.has_value() ? *inv_in : Tensor();
+  double scale = 1.0;
+  if (reduction == 2 && !inv.defined()) {
+    if (a.target.defined()) {
+      inv = at::empty({2}, g.options());
+      check(t2t_distill_count(a.target.data_ptr<int64_t>(), a.rows, ignore_index,
+                              inv.data_ptr<float>(), stream_of(logits)),
+            "t2t_distill_count");
+    } else if (a.rows) {
+      scale = 1.0 / static_cast<double>(a.rows);
+    }
+  }
+  Tensor grad = kept.has_value() ? *kept : at::empty(a.shape, logits.options());
+  a.launch(Tensor(), grad, a.V, scale, inv, g, kept.has_value());
+  return grad;
+}
+
+// Over chunk rows of a head's logits: the gradient in place of the logits.
+void distill_rows_(const Tensor& logits, const Tensor& idx, const Tensor& teacher,
+                   const c10::optional<Tensor>& target, double temperature, double alpha,
+                   int64_t ignore_index, const c10::optional<Tensor>& inv, double scale,
+                   const Tensor& row_loss, bool with_grad) {
+  const Distill a(logits, idx, teacher, target, temperature, alpha, ignore_index);
+  const c10::DeviceGuard guard(logits.device());
+  TORCH_CHECK(logits.dim() == 2 && (a.rows == 0 || a.z.data_ptr() == logits.data_ptr()) &&
+                  row_loss.is_cuda() && row_loss.scalar_type() == at::kFloat &&
+                  row_loss.is_contiguous() && row_loss.numel() == a.rows,
+              "logits of unit stride [rows, V] and float32 row losses [rows]");
+  if (a.rows)
+    a.launch(row_loss, with_grad ? a.z : Tensor(), Distill::step(a.z), scale,
+             inv.has_value() ? *inv : Tensor(), Tensor(), false);
+}
+
+// [1 / max(n, 1), 1 / n] of the targets, n the counted ones.
+Tensor distill_count(const Tensor& target, int64_t ignore_index) {
+  need_gpu(target);
+  TORCH_CHECK_VALUE(target.scalar_type() == at::kLong && target.is_contiguous(),
+                    "targets must be contiguous int64");
+  const c10::DeviceGuard guard(target.device());
+  Tensor inv = at::empty({2}, target.options().dtype(at::kFloat));
+  check(t2t_distill_count(target.data_ptr<int64_t>(), target.numel(), ignore_index,
+                          inv.data_ptr<float>(), stream_of(target)),
+        "t2t_distill_count");
+  return inv;
+}
+
+// scale (inv[1] where given) times the sum of row losses.
+Tensor distill_mean(const Tensor& row_loss, const c10::optional<Tensor>& inv, double scale) {
+  need_gpu(row_loss);
+  TORCH_CHECK_VALUE(row_loss.scalar_type() == at::kFloat && row_loss.is_contiguous(),
+                    "row losses must be contiguous float32");
+  const c10::DeviceGuard guard(row_loss.device());
+  Tensor loss = at::empty({}, row_loss.options());
+  check(t2t_distill_mean(row_loss.data_ptr<float>(), row_loss.numel(),
+                         inv.has_value() ? inv->data_ptr<float>() + 1 : nullptr,
+                         static_cast<float>(scale), loss.data_ptr<float>(), stream_of(row_loss)),
+        "t2t_distill_mean");
+  return loss;
+}
+
 // ---- SwiGLU
 
 std::tuple<Tensor, Tensor> swiglu(const Tensor& gu) {
@@ -601,6 +865,13 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("qk_norm_rope", &qk_norm_rope, no_gil);
   m.def("qk_norm_rope_backward", &qk_norm_rope_backward, no_gil);
   m.def("qk_norm_rope_append", &qk_norm_rope_append, no_gil);
+  m.def("embedding", &embedding, no_gil);
+  m.def("embedding_backward", &embedding_backward, no_gil);
+  m.def("distill_loss", &distill_loss, no_gil);
+  m.def("distill_loss_backward", &distill_loss_backward, no_gil);
+  m.def("distill_rows_", &distill_rows_, no_gil);
+  m.def("distill_count", &distill_count, no_gil);
+  m.def("distill_mean", &distill_mean, no_gil);
   m.def("swiglu", &swiglu, no_gil);
   m.def("swiglu_backward",
         [](const Tensor& g2, const Tensor& dh, const std::vector<int64_t>& shape) {

@@ -46,6 +46,20 @@ def _mm_f32(a: torch.Tensor, b: torch.Tensor) -> torch.Tensor:
         return torch.mm(a, b).float()
 
 
+def head_weight(weight: torch.Tensor, dev) -> torch.Tensor:
+    """The head's weight as the products take it: bf16, contiguous, its rows
+    padded with zeros to a multiple of 8 (the weight itself where it is that)."""
+    V, D = weight.shape
+    ld = (V + 7) // 8 * 8
+    if (ld == V and weight.device == dev and weight.dtype == torch.bfloat16
+            and weight.is_contiguous()):
+        return weight.detach()
+    w = torch.empty((ld, D), dtype=torch.bfloat16, device=dev)
+    w[:V].copy_(weight)
+    w[V:].zero_()
+    return w
+
+
 def _head_pass(x, weight, targets, ignore_index: int, chunk: Optional[int], grads: bool):
     """Per chunk of rows: logits, t2t_ce_rows (row losses, and the logit
     gradient in place over the logits), then -- when ``grads`` -- dx and the
@@ -53,20 +67,14 @@ def _head_pass(x, weight, targets, ignore_index: int, chunk: Optional[int], grad
     dw are None without ``grads``."""
     N, D = x.shape
     V = weight.shape[0]
-    ld = (V + 7) // 8 * 8
     dev = x.device
     t = targets.reshape(-1).to(device=dev, dtype=torch.int64).contiguous()
     if t.numel() != N:
         raise ValueError(f"{t.numel()} targets for {N} rows")
     if weight.shape[1] != D:
         raise ValueError(f"weight {tuple(weight.shape)} does not match rows of width {D}")
-    if (ld == V and weight.device == dev and weight.dtype == torch.bfloat16
-            and weight.is_contiguous()):
-        w = weight.detach()
-    else:
-        w = torch.empty((ld, D), dtype=torch.bfloat16, device=dev)
-        w[:V].copy_(weight)
-        w[V:].zero_()
+    w = head_weight(weight, dev)
+    ld = w.shape[0]
     n = (t != ignore_index).sum()
     # gradient scale 1 / n; with every row ignored no row has a gradient, so
     # the scale only has to be finite

@@ -38,6 +38,7 @@ from . import _lib
 from .attention import flex_attention
 from .block_mask import T2TBlockMask, build_block_mask
 from .decode import MAX_ROWS, attn_decode
+from .embedding import embedding
 from .modules import RMSNorm, TS2TSBackbone
 from .rope import qk_norm_rope_append, qkv_rope
 from .rows import applies as rows_apply, rows_linear, rows_qkv_rope
@@ -108,7 +109,7 @@ class TS2TSModel:
     def __init__(self, backbone: TS2TSBackbone, embedding_weight: torch.Tensor,
                  lm_head_weight: torch.Tensor, norm: nn.Module, block_mask_creator: Callable,
                  vocab_size: int, ignore_index: int = -100, tokenizer=None, link_detector=None,
-                 layout_policy=None):
+                 layout_policy=None, embedding_scale: Optional[float] = None):
         self.backbone = backbone
         self.embedding_weight = embedding_weight
         self.lm_head_weight = lm_head_weight
@@ -119,6 +120,7 @@ class TS2TSModel:
         self.tokenizer = tokenizer
         self.link_detector = link_detector
         self.layout_policy = layout_policy
+        self.embedding_scale = embedding_scale  # factor on the embedding's rows, or None
         self.kv_cache: Optional[KVCache] = None
         self.prefill_rows = 64
         self.use_graphs = True
@@ -132,19 +134,21 @@ class TS2TSModel:
                     max_seq_len: int, dropout: float, drop_path_rate: float,
                     block_mask_creator: Callable, fp8: bool = False, weight_tying: bool = True,
                     ignore_index: int = -100, tokenizer=None, link_detector=None,
-                    layout_policy=None, qk_norm: bool = False) -> "TS2TSModel":
+                    layout_policy=None, qk_norm: bool = False,
+                    embedding_scale: Optional[float] = None) -> "TS2TSModel":
         backbone = TS2TSBackbone(num_layers=num_layers, model_dim=model_dim, num_heads=num_heads,
                                  max_seq_len=max_seq_len, dropout=dropout,
                                  drop_path_rate=drop_path_rate, fp8=fp8, qk_norm=qk_norm)
-        embedding = nn.Embedding(vocab_size, model_dim)
+        table = nn.Embedding(vocab_size, model_dim)
         norm = RMSNorm(model_dim)
         if weight_tying:
-            lm_head_weight = embedding.weight
+            lm_head_weight = table.weight
         else:
             lm_head_weight = nn.Parameter(torch.empty(vocab_size, model_dim))
             nn.init.normal_(lm_head_weight, mean=0.0, std=0.02)
-        return cls(backbone, embedding.weight, lm_head_weight, norm, block_mask_creator,
-                   vocab_size, ignore_index, tokenizer, link_detector, layout_policy)
+        return cls(backbone, table.weight, lm_head_weight, norm, block_mask_creator,
+                   vocab_size, ignore_index, tokenizer, link_detector, layout_policy,
+                   embedding_scale)
 
     def eval(self):
         self.backbone.eval()
@@ -186,18 +190,24 @@ class TS2TSModel:
                                  for name, prm in m._parameters.items() if prm is not None]
         params = [m._parameters.get(name) for m, name in self._param_slots]
         params += (self.embedding_weight, self.lm_head_weight)
-        return self.backbone.training, tuple(None if p is None else (p.data_ptr(), p._version)
-                                             for p in params)
+        return (self.backbone.training, self.embedding_scale,
+                tuple(None if p is None else (p.data_ptr(), p._version)
+                      for p in params))
 
     @torch.no_grad()
     def forward_inference(self, tokens: torch.Tensor, doc_spans: Optional[List[Any]] = None,
                           **kwargs) -> torch.Tensor:
         """model/model.py:214-237: logits [1, T, V] over the whole sequence."""
         block_mask = self.block_mask_creator(tokens=tokens, doc_spans=doc_spans or [], **kwargs)
-        x = F.embedding(tokens, self.embedding_weight)
+        x = self._embed(tokens)
         x = self.backbone(x, block_mask=block_mask)
         x = self.norm(x)
         return F.linear(x, self.lm_head_weight)
+
+    def _embed(self, tokens: torch.Tensor) -> torch.Tensor:
+        if self.embedding_scale is None:
+            return F.embedding(tokens, self.embedding_weight)
+        return embedding(tokens, self.embedding_weight, self.embedding_scale)
 
     # -- cached path -------------------------------------------------------
 
@@ -260,7 +270,7 @@ class TS2TSModel:
             logits = self._graph_step(cache, tokens, bm, p0)
             cache.length = T
             return logits
-        x = F.embedding(tokens[:, p0:], self.embedding_weight)
+        x = self._embed(tokens[:, p0:])
         x = self._backbone_rows(x, bm, cache, p0, full)
         cache.length = T
         x = x[:, -1:]
@@ -286,7 +296,7 @@ class TS2TSModel:
         qdoc = cache.doc.index_select(1, buf.pos)
         qbits = cache.q_bits.index_select(2, buf.pos) if cache.words else None
         qpos = buf.pos.to(torch.int32).view(1, 1)
-        x = F.embedding(tok, self.embedding_weight)
+        x = self._embed(tok)
         cos_t, sin_t = self._layers()[0].attn.rotary.tables(x.device)
         fused = self._rows_fusable(x)
         if not fused:

@@ -30,6 +30,7 @@ import torch.utils.checkpoint
 
 from . import norm
 from .attention import FlexSelfAttention
+from .embedding import ScaledEmbedding
 from .glu import swiglu_applies, swiglu_rows
 from .head_loss import HeadCEFn, fused_head_applies, head_loss_needs_grad, head_loss_value
 from .linear import Linear
@@ -204,21 +205,39 @@ class TS2TSTrainingModule(nn.Module):
                     max_seq_len: int, dropout: float, drop_path_rate: float,
                     block_mask_creator: Callable, fp8: bool = False, weight_tying: bool = True,
                     ignore_index: int = -100, dtype: torch.dtype = torch.bfloat16,
-                    activation_checkpointing: bool = False,
-                    qk_norm: bool = False) -> "TS2TSTrainingModule":
+                    activation_checkpointing: bool = False, qk_norm: bool = False,
+                    embedding_scale: Optional[float] = None,
+                    distill_alpha: Optional[float] = None,
+                    distill_temperature: float = 1.0) -> "TS2TSTrainingModule":
+        """``qk_norm``: norms of the attention's query and key heads;
+        ``embedding_scale``: a factor on the embedding's rows (ScaledEmbedding);
+        ``distill_alpha``, ``distill_temperature``: the loss distils where a
+        batch has a teacher's top logits (distill.LinearDistillLoss)."""
         backbone = TS2TSBackbone(num_layers=num_layers, model_dim=model_dim, num_heads=num_heads,
                                  max_seq_len=max_seq_len, dropout=dropout,
                                  drop_path_rate=drop_path_rate, fp8=fp8,
                                  activation_checkpointing=activation_checkpointing,
                                  qk_norm=qk_norm)
-        embedding = nn.Embedding(vocab_size, model_dim)
+        embedding = (nn.Embedding(vocab_size, model_dim) if embedding_scale is None else
+                     ScaledEmbedding(vocab_size, model_dim, embedding_scale))
         norm = RMSNorm(model_dim)
-        loss_fn = LinearCELoss(D=model_dim, V=vocab_size, dtype=dtype, ignore_index=ignore_index,
-                               weight=embedding.weight if weight_tying else None)
+        head = dict(D=model_dim, V=vocab_size, dtype=dtype, ignore_index=ignore_index,
+                    weight=embedding.weight if weight_tying else None)
+        if distill_alpha is None:
+            loss_fn = LinearCELoss(**head)
+        else:
+            from .distill import LinearDistillLoss
+            loss_fn = LinearDistillLoss(temperature=distill_temperature, alpha=distill_alpha,
+                                        **head)
         return cls(backbone, embedding, norm, loss_fn, block_mask_creator, vocab_size,
                    ignore_index)
 
     def forward(self, batch: Dict[str, Any]) -> torch.Tensor:
+        """Mean loss of ``batch["tokens"]`` [B, T + 1]; with ``teacher_idx`` and
+        ``teacher_logits`` [B, T, K] in the batch, the teacher's top logits at
+        positions 0 .. T - 1, that of distilling from them."""
+        batch = dict(batch)
+        teacher = [batch.pop(n) for n in ("teacher_idx", "teacher_logits") if n in batch]
         tokens = batch["tokens"]
         input_ids = tokens[:, :-1].contiguous()
         target_ids = tokens[:, 1:].contiguous()
@@ -226,4 +245,4 @@ class TS2TSTrainingModule(nn.Module):
         x = self.embedding(input_ids)
         x = self.backbone(x, block_mask=block_mask)
         x = self.norm(x)
-        return self.loss_fn(x, target_ids)
+        return self.loss_fn(x, target_ids, *teacher)
