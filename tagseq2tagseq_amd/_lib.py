@@ -150,6 +150,12 @@ def unwatched(*tensors) -> bool:
     return forward_ad._current_level < 0 and host().unwatched(*tensors)
 
 
+def only_recorded(*tensors) -> bool:
+    """True when nothing but autograd's graph watches a call on these tensors,
+    so that it may be recorded by the host module's own functions."""
+    return forward_ad._current_level < 0 and host().plain(*tensors)
+
+
 def replaces_torch(*tensors) -> bool:
     """True when a kernel may stand in for a torch function of these tensors
     unseen: as unwatched (a recorded graph, which its caller is, aside), and

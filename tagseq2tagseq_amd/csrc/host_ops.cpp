@@ -14,6 +14,8 @@
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
@@ -801,6 +803,117 @@ std::vector<Tensor> token_inputs(const Tensor& lists, int64_t grants, int64_t co
   return t;
 }
 
+// ---- the same calls recorded by autograd, from C++
+//
+// A call that only autograd watches (plain() below) is recorded here: a Python
+// autograd.Function costs its own host time forward, and backward a switch to
+// the engine's thread that waits for the interpreter.
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+// Results of a backward that itself has no gradient: an error where one is asked for.
+variable_list once(variable_list grads, const char* what) {
+  if (!c10::GradMode::is_enabled()) return grads;
+  return torch::autograd::DelayedError(std::string(what) + " is differentiable once",
+                                       static_cast<int64_t>(grads.size()))(std::move(grads));
+}
+
+struct QkNormAd : torch::autograd::Function<QkNormAd> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& qkv, const Tensor& qw,
+                               const Tensor& kw, const Tensor& cos, const Tensor& sin,
+                               int64_t heads, int64_t kv_heads, int64_t pos0, double eps) {
+    ctx->save_for_backward({qkv, qw, kw, cos, sin});
+    ctx->saved_data["n"] = std::vector<int64_t>{heads, kv_heads, pos0};
+    ctx->saved_data["eps"] = eps;
+    auto [q, k, v] = qk_norm_rope(qkv, qw, kw, cos, sin, heads, kv_heads, pos0, eps);
+    return {q, k, v};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    const variable_list t = ctx->get_saved_variables();
+    const std::vector<int64_t> n = ctx->saved_data["n"].toIntVector();
+    auto [dqkv, dqw, dkw] = qk_norm_rope_backward(g[0], g[1], g[2], t[0], t[1], t[2], t[3], t[4],
+                                                  n[0], n[1], n[2],
+                                                  ctx->saved_data["eps"].toDouble());
+    variable_list d = once({dqkv, dqw, dkw}, "qk_norm_rope");
+    d.resize(9);
+    return d;
+  }
+};
+
+std::tuple<Tensor, Tensor, Tensor> qk_norm_rope_ad(const Tensor& qkv, const Tensor& qw,
+                                                   const Tensor& kw, const Tensor& cos,
+                                                   const Tensor& sin, int64_t heads,
+                                                   int64_t kv_heads, int64_t pos0, double eps) {
+  variable_list o = QkNormAd::apply(qkv, qw, kw, cos, sin, heads, kv_heads, pos0, eps);
+  return {o[0], o[1], o[2]};
+}
+
+struct EmbeddingAd : torch::autograd::Function<EmbeddingAd> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& tokens, const Tensor& weight,
+                        double scale, int64_t padding) {
+    ctx->save_for_backward({tokens});
+    ctx->saved_data["n"] = std::vector<int64_t>{weight.size(0), padding};
+    ctx->saved_data["scale"] = scale;
+    return embedding(tokens, weight, scale);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    const std::vector<int64_t> n = ctx->saved_data["n"].toIntVector();
+    variable_list d = once({embedding_backward(ctx->get_saved_variables()[0], g[0], n[0],
+                                               ctx->saved_data["scale"].toDouble(), n[1])},
+                           "embedding");
+    return {Tensor(), d[0], Tensor(), Tensor()};
+  }
+};
+
+Tensor embedding_ad(const Tensor& tokens, const Tensor& weight, double scale, int64_t padding) {
+  return EmbeddingAd::apply(tokens, weight, scale, padding);
+}
+
+// A sum or mean is differentiated with an incoming gradient of 1 as a rule, so
+// the forward's pass over the logits writes its gradient.
+struct DistillAd : torch::autograd::Function<DistillAd> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& logits, const Tensor& idx,
+                        const Tensor& teacher, const c10::optional<Tensor>& target,
+                        double temperature, double alpha, int64_t ignore_index,
+                        int64_t reduction) {
+    auto [loss, grad, inv] =
+        distill_loss(logits, idx, teacher, target, temperature, alpha, ignore_index, reduction,
+                     reduction != 0 && logits.requires_grad());
+    ctx->save_for_backward({logits, idx, teacher, target.has_value() ? *target : Tensor(), inv});
+    ctx->saved_data["x"] = std::vector<double>{temperature, alpha};
+    ctx->saved_data["n"] = std::vector<int64_t>{ignore_index, reduction};
+    if (grad.defined()) ctx->saved_data["kept"] = grad;
+    return loss;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    const auto given = [](const Tensor& t) {
+      return t.defined() ? c10::optional<Tensor>(t) : c10::nullopt;
+    };
+    const variable_list t = ctx->get_saved_variables();
+    const std::vector<double> x = ctx->saved_data["x"].toDoubleVector();
+    const std::vector<int64_t> n = ctx->saved_data["n"].toIntVector();
+    c10::optional<Tensor> kept;  // handed over: a second backward computes its own
+    const auto at = ctx->saved_data.find("kept");
+    if (at != ctx->saved_data.end()) {
+      kept = at->second.toTensor();
+      ctx->saved_data.erase(at);
+    }
+    variable_list d = once({distill_loss_backward(g[0], t[0], t[1], t[2], given(t[3]), x[0], x[1],
+                                                  n[0], n[1], given(t[4]), kept)},
+                           "distill_loss");
+    d.resize(8);
+    return d;
+  }
+};
+
+Tensor distill_loss_ad(const Tensor& logits, const Tensor& idx, const Tensor& teacher,
+                       const c10::optional<Tensor>& target, double temperature, double alpha,
+                       int64_t ignore_index, int64_t reduction) {
+  return DistillAd::apply(logits, idx, teacher, target, temperature, alpha, ignore_index,
+                          reduction);
+}
+
 // ---- what may be watching a call
 
 // Nothing but the caller sees the call, and the tensors are what their
@@ -865,6 +978,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("qk_norm_rope", &qk_norm_rope, no_gil);
   m.def("qk_norm_rope_backward", &qk_norm_rope_backward, no_gil);
   m.def("qk_norm_rope_append", &qk_norm_rope_append, no_gil);
+  m.def("qk_norm_rope_ad", &qk_norm_rope_ad, no_gil);
+  m.def("embedding_ad", &embedding_ad, no_gil);
+  m.def("distill_loss_ad", &distill_loss_ad, no_gil);
   m.def("embedding", &embedding, no_gil);
   m.def("embedding_backward", &embedding_backward, no_gil);
   m.def("distill_loss", &distill_loss, no_gil);

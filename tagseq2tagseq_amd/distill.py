@@ -92,7 +92,8 @@ distill_loss_op.register_autograd(_backward, setup_context=_setup)
 
 
 class DistillFn(torch.autograd.Function):
-    """The same kernels for eager execution.  A sum or mean is differentiated
+    """The same kernels for eager calls that something besides autograd watches
+    (the others are recorded by the host module, in the same way).  A sum or mean is differentiated
     with an incoming gradient of 1 as a rule, so its gradient is written by the
     forward's pass over the logits; the backward hands it over, having the rows
     computed again (on the device, without waiting) where the incoming gradient is
@@ -143,6 +144,8 @@ def distill_loss(logits: torch.Tensor, teacher_idx: torch.Tensor, teacher_logits
     if _lib.unwatched(*watched):
         return _lib.host().distill_loss(logits, teacher_idx, teacher_logits, targets, *args,
                                         False)[0]
+    if _lib.only_recorded(*watched):
+        return _lib.host().distill_loss_ad(logits, teacher_idx, teacher_logits, targets, *args)
     return DistillFn.apply(logits, teacher_idx, teacher_logits, targets, *args)
 
 

@@ -66,7 +66,8 @@ embedding_op.register_autograd(_backward, setup_context=_setup)
 
 
 class EmbeddingFn(torch.autograd.Function):
-    """The same kernels as t2t::embedding for eager execution."""
+    """The same kernels as t2t::embedding for eager calls that something besides
+    autograd watches (the others are recorded by the host module)."""
 
     @staticmethod
     def forward(ctx, tokens, weight, scale, padding):
@@ -103,6 +104,8 @@ def embedding(tokens: torch.Tensor, weight: torch.Tensor, scale: float = 1.0,
         return embedding_op(tokens, weight, scale, padding)
     if _lib.unwatched(tokens, weight):
         return _lib.host().embedding(tokens, weight, scale)
+    if _lib.only_recorded(tokens, weight):
+        return _lib.host().embedding_ad(tokens, weight, scale, padding)
     return EmbeddingFn.apply(tokens, weight, scale, padding)
 
 

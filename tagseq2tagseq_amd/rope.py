@@ -209,8 +209,8 @@ qk_norm_rope_op.register_autograd(_qk_norm_rope_bwd, setup_context=_qk_norm_rope
 
 
 class QKNormRopeFn(torch.autograd.Function):
-    """The same kernels as t2t::qk_norm_rope for eager execution (as QKVRopeFn
-    is for t2t::qkv_rope)."""
+    """The same kernels as t2t::qk_norm_rope for eager calls that something
+    besides autograd watches (the others are recorded by the host module)."""
 
     @staticmethod
     def forward(ctx, qkv, q_weight, k_weight, cos, sin, *args):
@@ -241,6 +241,8 @@ def qk_norm_rope(qkv: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tens
         return qk_norm_rope_op(qkv, q_weight, k_weight, cos, sin, *args)
     if _lib.unwatched(qkv, q_weight, k_weight, cos, sin):
         return _lib.host().qk_norm_rope(qkv, q_weight, k_weight, cos, sin, *args)
+    if _lib.only_recorded(qkv, q_weight, k_weight, cos, sin):
+        return _lib.host().qk_norm_rope_ad(qkv, q_weight, k_weight, cos, sin, *args)
     return QKNormRopeFn.apply(qkv, q_weight, k_weight, cos, sin, *args)
 
 
