@@ -22,14 +22,16 @@
 //   sum_k w_k ((t_k - max t) - (z(i_k) - max z)) / (T sum w) - ln sum w + ln sum_j
 // with w_k = e^((t_k - max t) / T), whose terms are small where the result is.
 // The gradient is first written without the teacher's and the target's terms;
-// behind a barrier, one thread for each of those columns writes its value
-// again, the slots of equal columns added in their order.  The gradient may
+// behind a barrier, a thread for each of those columns writes its value again,
+// the weights of equal columns added, in their order.  The gradient may
 // overwrite the logits: everything is read before the barriers ahead of the
 // first write.
 //
 // Addresses: rows start anywhere on their type (V = 50257 columns of bf16 have
-// every second row off a 4-byte boundary); 16-byte pieces are read and written
-// at that alignment, which global memory instructions allow.
+// every second row off a 4-byte boundary); whole pieces start at the row's first
+// 16-byte boundary (so the order of a row's additions goes by its address
+// modulo 16).  A gradient whose rows lie otherwise is written in pieces
+// off that boundary, which global memory instructions allow.
 #include "attn_kernels.h"
 
 namespace t2t {
@@ -40,6 +42,8 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr int kMaxSlots = kDistillMaxSlots;
 
+typedef float float2v __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2v __attribute__((ext_vector_type(2)));
 typedef short short2v __attribute__((ext_vector_type(2)));
 typedef unsigned short ushort2v __attribute__((ext_vector_type(2)));
 
@@ -59,11 +63,9 @@ struct Elem<__bf16> {
   }
   __device__ static void pack(const float (&x)[8], Piece& p) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const __bf16 lo = (__bf16)x[2 * e], hi = (__bf16)x[2 * e + 1];
-      p.w[e] = (uint32_t)__builtin_bit_cast(uint16_t, lo) |
-               ((uint32_t)__builtin_bit_cast(uint16_t, hi) << 16);
-    }
+    for (int e = 0; e < 4; ++e)
+      p.w[e] = __builtin_bit_cast(
+          uint32_t, __builtin_convertvector((float2v{x[2 * e], x[2 * e + 1]}), bf16x2v));
   }
   // Maximum over pieces on the packed bits.  Values of sign 0 are ordered as
   // signed 16-bit numbers and above all others; only a row without any looks
@@ -117,8 +119,9 @@ struct Elem<float> {
   __device__ static float negative(Least m) { return m; }
 };
 
-// A row of V columns: V / VEC whole pieces, and the columns behind them, which
-// the first V % VEC threads hold one each (Tail).
+// A row of V columns: the columns up to its first 16-byte boundary, whole pieces
+// from there (body), and the columns behind them.  The first threads hold one
+// of the columns outside the pieces each (`last`).
 template <typename T>
 __device__ __forceinline__ typename Elem<T>::Piece load_piece(const T* row, uint32_t i) {
   // (an unsigned 32-bit offset from the uniform row: one register an address)
@@ -132,12 +135,6 @@ __device__ __forceinline__ void store_piece(T* row, uint32_t i,
   typename Elem<T>::Piece p;
   Elem<T>::pack(x, p);
   *reinterpret_cast<typename Elem<T>::Piece*>(reinterpret_cast<char*>(row) + 16 * i) = p;
-}
-
-template <typename T>
-__device__ __forceinline__ int tail_column(int V) {
-  const int col = V / Elem<T>::kVec * Elem<T>::kVec + threadIdx.x;
-  return col < V ? col : -1;
 }
 
 // Combines n values over the work-group, all threads getting the results; red:
@@ -167,13 +164,6 @@ __device__ __forceinline__ void combine(float (&x)[n], float (*red)[n]) {
   for (int j = 0; j < n; ++j) x[j] = red[lane % (NT / 64)][j];
   combine_lanes<n, Max>(x, NT / 64);
 }
-
-// A row's slots in LDS, the target behind them as a slot without mass.
-struct Slots {
-  int column[kMaxSlots + 1];  // -1: empty
-  float t[kMaxSlots + 1];     // the teacher's logit, then its probability
-  float z[kMaxSlots + 1];     // the student's logit there
-};
 
 // The exponentials of a row.  P: 1, one softmax; 0, two of unrelated
 // temperatures; n >= 2, e^(z - max) is the n-th power of e^((z - max) / T).
@@ -213,118 +203,85 @@ struct Exps {
   }
 };
 
+// seen: a bit for every column of a slot (modulo its size: two columns of one
+// bit only cost time).  A column that is met twice sends the row to the search
+// through `column`; looking for equal columns in every row took 15 % of its time.
+constexpr int kSeenWords = 2048;
 struct Shared {
-  Slots slots;
-  float max[2][16][2], sum[16][4];  // of the waves
-  int flags[2];                     // a column >= V; a slot with a say
+  int column[kMaxSlots];  // of the slots; -1: empty
+  float w[kMaxSlots];     // their weights
+  uint32_t seen[kSeenWords];
+  int twice, target_in;   // a bit of `seen` met twice; a slot at the target's column
+  float max[2][16][4], sum[16][4];  // of the waves
 };
 
-// A row of the loss with everything but its own logits known.
+// A row, and what a thread holds of it before the work begins.
 template <typename T>
 struct RowAt {
   const T* z;
   T* out;
+  const T* body;   // the first piece
+  T* out_body;
   uint32_t pieces;
-  int last;    // the thread's column behind the pieces, or -1
-  float tail;  // its logit
+  int last;        // the thread's column outside the pieces, or -1
+  float tail;      // its logit
+  int64_t target;
+  int64_t column;  // of the thread's slot; -1: none
+  float t;         // the teacher's logit there
 };
 
-template <typename T, int NT, int P, bool Far, typename Row>
-__device__ __forceinline__ void finish_row(const DistillArgs& a, int64_t row, const RowAt<T>& at,
-                                           Row& held, Shared& sh, float m, float m_teacher,
-                                           bool taught, bool hard, float c, float ct) {
-  Slots& s = sh.slots;
-  const Exps<P, Far> ex(m, c, kLog2e);
-
-  // Sums: e^((z - m) / T), e^(z - m), the teacher's weights, and KD's terms.
-  float sum[4] = {};
-  held.sums(at, ex, sum[0], sum[1]);
-  if (at.last >= 0) ex.sum(at.tail, sum[0], sum[1]);
-  if (taught)
-#pragma unroll 1
-    for (int k = threadIdx.x; k < a.K; k += NT) {
-      const float w = s.column[k] < 0 ? 0.f : fast_exp2((s.t[k] - m_teacher) * ct);
-      if (w != 0.f) {  // (NaN too)
-        sum[2] += w;
-        sum[3] += w * ((s.t[k] - m_teacher) - (s.z[k] - m));
-      }
-      s.t[k] = w;  // by the thread that reads it here only; by all behind the barrier
-    }
-  combine<NT, 4, false>(sum, sh.sum);
-
-  if (threadIdx.x == 0 && a.row_loss) {
-    float loss = 0.f;
-    if (taught)
-      loss = a.alpha * a.temp * a.temp *
-             (sum[3] / sum[2] * a.inv_temp + (ex.log2_first(sum[0]) - __log2f(sum[2])) * kLn2);
-    if (hard) {
-      const float lse = P == 1 ? ex.log2_first(sum[0]) : ex.log2_other(sum[1]);
-      loss += (1.f - a.alpha) * (lse * kLn2 - (s.z[a.K] - m));
-    }
-    a.row_loss[row] = loss;
+template <typename T>
+__device__ __forceinline__ RowAt<T> row_at(const DistillArgs& a, int64_t row) {
+  RowAt<T> at;
+  at.z = static_cast<const T*>(a.logits) + row * a.ld;
+  at.out = a.grad ? static_cast<T*>(a.grad) + row * a.grad_ld : nullptr;
+  const int ahead = min((int)(-reinterpret_cast<uintptr_t>(at.z) & 15) / (int)sizeof(T), a.V);
+  at.body = at.z + ahead;
+  at.out_body = at.out + ahead;
+  at.pieces = (uint32_t)(a.V - ahead) / Elem<T>::kVec;
+  const int behind = ahead + at.pieces * Elem<T>::kVec;
+  const int i = threadIdx.x, col = i < ahead ? i : behind + i - ahead;
+  at.last = col < a.V && (i < ahead || i - ahead < Elem<T>::kVec) ? col : -1;
+  at.target = a.target ? a.target[row] : 0;
+  at.column = -1;
+  at.t = -INFINITY;
+  const int k = threadIdx.x;
+  if (k < a.K) {
+    at.column = a.idx64 ? static_cast<const int64_t*>(a.idx)[row * a.idx_ld + k]
+                        : static_cast<const int32_t*>(a.idx)[row * a.idx_ld + k];
+    const int64_t slot = row * a.teacher_ld + k;
+    at.t = a.teacher_f32 ? static_cast<const float*>(a.teacher)[slot]
+                         : (float)static_cast<const __bf16*>(a.teacher)[slot];
   }
-  if (!at.out) {
-    __syncthreads();
-    return;
-  }
-
-  float scale = a.scale;
-  if (a.scale_dev) scale *= *a.scale_dev;
-  if (a.g) scale *= a.g[row * a.g_stride];
-  const float from_soft = taught ? a.alpha * a.temp * scale : 0.f;
-  const float from_hard = hard ? (1.f - a.alpha) * scale : 0.f;
-  // Factors of the two exponentials (of the one, with both parts at T = 1).
-  const float f0 = (P == 1 ? from_soft + from_hard : from_soft) / sum[0];
-  const float f1 = P == 1 ? 0.f : from_hard / sum[1];
-  held.grads(at, ex, f0, f1);
-  if (at.last >= 0) at.out[at.last] = (T)ex.grad(at.tail, f0, f1);
-  __syncthreads();
-
-  // The slots' and the target's columns.
-  const float per_weight = taught ? from_soft / sum[2] : 0.f;
-  for (int k = threadIdx.x; k <= a.K; k += NT) {
-    const int col = s.column[k];
-    if (col < 0 || (k < a.K && !taught && !(hard && col == s.column[a.K]))) continue;
-    float w = 0.f;
-    bool first = true;
-    for (int j = 0; j <= a.K; ++j)
-      if (s.column[j] == col) {
-        if (j < k) first = false;
-        if (j < a.K && taught) w += s.t[j];
-      }
-    if (!first) continue;
-    float x = ex.grad(s.z[k], f0, f1) - w * per_weight;
-    if (hard && col == s.column[a.K]) x -= from_hard;
-    at.out[col] = (T)x;
-  }
-  __syncthreads();
+  at.tail = at.last >= 0 ? (float)at.z[at.last] : -INFINITY;  // (no share of a sum)
+  return at;
 }
 
 // A row wider than the registers hold: read for the maximum, for the sums and
 // for the gradient.  In place, a thread's writes follow its own last reading.
 template <typename T, int NT>
 struct ReadRow {
-  static constexpr int kWaves = NT == 1024 ? 8 : 4;
+  static constexpr int kWaves = NT == 1024 ? 8 : 4;  // a SIMD, for the register budget
   static constexpr bool kLoop = true;
   static constexpr int VEC = Elem<T>::kVec;
+  static constexpr bool kTwoMax = false;
   __device__ void load(const RowAt<T>&) {}
   __device__ float max(const RowAt<T>& at) {
     float m = -INFINITY;
     for (uint32_t i = threadIdx.x; i < at.pieces; i += NT) {
       float x[VEC];
-      Elem<T>::unpack(load_piece(at.z, i), x);
+      Elem<T>::unpack(load_piece(at.body, i), x);
 #pragma unroll
       for (int e = 0; e < VEC; ++e) m = fmaxf(m, x[e]);
     }
     return m;
   }
-  static constexpr bool kTwoMax = false;
   __device__ float least_negative() { return -INFINITY; }
   template <typename E>
   __device__ void sums(const RowAt<T>& at, const E& ex, float& s0, float& s1) {
     for (uint32_t i = threadIdx.x; i < at.pieces; i += NT) {
       float x[VEC];
-      Elem<T>::unpack(load_piece(at.z, i), x);
+      Elem<T>::unpack(load_piece(at.body, i), x);
 #pragma unroll
       for (int e = 0; e < VEC; ++e) ex.sum(x[e], s0, s1);
     }
@@ -333,10 +290,10 @@ struct ReadRow {
   __device__ void grads(const RowAt<T>& at, const E& ex, float f0, float f1) {
     for (uint32_t i = threadIdx.x; i < at.pieces; i += NT) {
       float x[VEC];
-      Elem<T>::unpack(load_piece(at.z, i), x);
+      Elem<T>::unpack(load_piece(at.body, i), x);
 #pragma unroll
       for (int e = 0; e < VEC; ++e) x[e] = ex.grad(x[e], f0, f1);
-      store_piece(at.out, i, x);
+      store_piece(at.out_body, i, x);
     }
   }
 };
@@ -345,7 +302,7 @@ struct ReadRow {
 // the other (sched_barrier): unpacked all at once, they would spill.
 template <typename T, int NT, int NP>
 struct HeldRow {
-  static constexpr int kWaves = NP <= 7 ? 8 : 4;  // a SIMD, for the register budget
+  static constexpr int kWaves = NP <= 8 ? 8 : 4;
   static constexpr bool kLoop = false;
   static constexpr int VEC = Elem<T>::kVec;
   static constexpr bool kTwoMax = Elem<T>::kTwoMax;
@@ -363,7 +320,7 @@ struct HeldRow {
       constexpr uint32_t none = Elem<T>::kNone;
       q[p] = make_uint4(none, none, none, none);
       if (i < at.pieces) {
-        const typename Elem<T>::Piece x = load_piece(at.z, i);
+        const typename Elem<T>::Piece x = load_piece(at.body, i);
         q[p] = make_uint4(x.w[0], x.w[1], x.w[2], x.w[3]);
       }
     }
@@ -414,105 +371,138 @@ struct HeldRow {
       Elem<T>::unpack(piece(p), x);
 #pragma unroll
       for (int e = 0; e < VEC; ++e) x[e] = ex.grad(x[e], f0, f1);
-      if (i < at.pieces) store_piece(at.out, i, x);
+      if (i < at.pieces) store_piece(at.out_body, i, x);
       __builtin_amdgcn_sched_barrier(0);
     }
   }
 };
 
+// The row's sums, its loss and its gradient; m and m_teacher are the maxima.
+template <typename T, int NT, int P, bool Far, typename Row>
+__device__ __forceinline__ void finish_row(const DistillArgs& a, int64_t row, const RowAt<T>& at,
+                                           Row& held, Shared& sh, float z_slot, float z_target,
+                                           float m, float m_teacher, bool taught, bool hard,
+                                           float c, float ct, float scale) {
+  const Exps<P, Far> ex(m, c, kLog2e);
+  const int k0 = threadIdx.x;
+
+  // Sums: e^((z - m) / T), e^(z - m), the teacher's weights, and KD's terms.
+  float sum[4] = {};
+  if (k0 < a.K) {
+    const bool in = at.column >= 0;
+    const float w = taught && in ? fast_exp2((at.t - m_teacher) * ct) : 0.f;
+    if (w != 0.f) {  // (NaN too)
+      sum[2] = w;
+      sum[3] = w * ((at.t - m_teacher) - (z_slot - m));
+    }
+    sh.column[k0] = in ? (int)at.column : -1;
+    sh.w[k0] = w;
+    if (in) {
+      const uint32_t bit = (uint32_t)at.column % (32 * kSeenWords);
+      if (atomicOr(&sh.seen[bit / 32], 1u << bit % 32) >> bit % 32 & 1) sh.twice = 1;
+      if (hard && at.column == at.target) sh.target_in = 1;
+    }
+  }
+  held.sums(at, ex, sum[0], sum[1]);
+  if (at.last >= 0) ex.sum(at.tail, sum[0], sum[1]);
+  combine<NT, 4, false>(sum, sh.sum);
+
+  if (k0 == 0 && a.row_loss) {
+    float loss = 0.f;
+    if (taught)
+      loss = a.alpha * a.temp * a.temp *
+             (sum[3] / sum[2] * a.inv_temp + (ex.log2_first(sum[0]) - __log2f(sum[2])) * kLn2);
+    if (hard) {
+      const float lse = P == 1 ? ex.log2_first(sum[0]) : ex.log2_other(sum[1]);
+      loss += (1.f - a.alpha) * (lse * kLn2 - (z_target - m));
+    }
+    a.row_loss[row] = loss;
+  }
+  if (!at.out) return;
+
+  const float from_soft = taught ? a.alpha * a.temp * scale : 0.f;
+  const float from_hard = hard ? (1.f - a.alpha) * scale : 0.f;
+  // Factors of the two exponentials (of the one, with both parts at T = 1).
+  const float f0 = (P == 1 ? from_soft + from_hard : from_soft) / sum[0];
+  const float f1 = P == 1 ? 0.f : from_hard / sum[1];
+  held.grads(at, ex, f0, f1);
+  if (at.last >= 0) at.out[at.last] = (T)ex.grad(at.tail, f0, f1);
+  __syncthreads();
+
+  // The slots' columns, each by its first slot, and the target's.
+  const float per_weight = taught ? from_soft / sum[2] : 0.f;
+  const int64_t target = hard ? at.target : -1;
+  if (k0 < a.K && at.column >= 0 && (taught || at.column == target)) {
+    float w = sh.w[k0];
+    bool first = true;
+    if (sh.twice)
+      for (int j = 0; j < a.K; ++j)
+        if (j != k0 && sh.column[j] == (int)at.column) {
+          first = first && j > k0;
+          w += sh.w[j];
+        }
+    if (first) {
+      float x = ex.grad(z_slot, f0, f1) - w * per_weight;
+      if (at.column == target) x -= from_hard;
+      at.out[at.column] = (T)x;
+    }
+  }
+  if (k0 == 0 && hard && !sh.target_in) at.out[target] = (T)(ex.grad(z_target, f0, f1) - from_hard);
+}
+
 // One row of the loss.  Row: how the logits are read (all at once, or again in
 // each phase).
 template <typename T, int NT, int P, typename Row>
-__device__ __forceinline__ void distill_row(const DistillArgs& a, int64_t row, Shared& sh) {
+__device__ __forceinline__ void distill_row(const DistillArgs& a, int64_t row, const RowAt<T>& at,
+                                            Row& held, Shared& sh, float scale) {
   constexpr int VEC = Elem<T>::kVec;
-  Slots& s = sh.slots;
   const int V = a.V;
-  RowAt<T> at;
-  at.z = static_cast<const T*>(a.logits) + row * a.ld;
-  at.out = a.grad ? static_cast<T*>(a.grad) + row * a.grad_ld : nullptr;
-  at.pieces = (uint32_t)V / VEC;
-  at.last = tail_column<T>(V);
-  at.tail = -INFINITY;
+  const bool hard = a.alpha < 1.f, soft = a.alpha > 0.f;
   const auto no_gradient = [&](float loss) {
     if (threadIdx.x == 0 && a.row_loss) a.row_loss[row] = loss;
     if (at.out) {
       const float zero[VEC] = {};
-      for (uint32_t i = threadIdx.x; i < at.pieces; i += NT) store_piece(at.out, i, zero);
+      for (uint32_t i = threadIdx.x; i < at.pieces; i += NT) store_piece(at.out_body, i, zero);
       if (at.last >= 0) at.out[at.last] = (T)0.f;
     }
-    __syncthreads();
   };
-  const int64_t target = a.target ? a.target[row] : 0;
-  const bool hard = a.alpha < 1.f, soft = a.alpha > 0.f;
-  if (a.target && (target == a.ignore_index || target < 0 || target >= V)) {
-    no_gradient(target == a.ignore_index ? 0.f : __builtin_nanf(""));
+  if (a.target && (at.target == a.ignore_index || at.target < 0 || at.target >= V)) {
+    no_gradient(at.target == a.ignore_index ? 0.f : __builtin_nanf(""));
     return;
   }
+  if (a.K > 0 && at.out)
+    for (int i = threadIdx.x; i < kSeenWords; i += NT) sh.seen[i] = 0;
+  if (threadIdx.x == 0) sh.twice = sh.target_in = 0;
+  const bool in = at.column >= 0 && at.column < V;
+  const float z_slot = in ? (float)at.z[at.column] : 0.f;
+  const float z_target = hard && threadIdx.x == 0 ? (float)at.z[at.target] : 0.f;
 
-  const auto column = [&](int k) {
-    return a.idx64 ? static_cast<const int64_t*>(a.idx)[row * a.idx_ld + k]
-                   : static_cast<const int32_t*>(a.idx)[row * a.idx_ld + k];
-  };
-  const auto teacher = [&](int k) {
-    const int64_t i = row * a.teacher_ld + k;
-    return a.teacher_f32 ? static_cast<const float*>(a.teacher)[i]
-                         : (float)static_cast<const __bf16*>(a.teacher)[i];
-  };
-  // The thread's first slot ahead of the row: the student's logit there, loaded
-  // behind it, waits for its column alone.
-  int64_t c0 = -1;
-  float t0 = 0.f;
-  if ((int)threadIdx.x < a.K) {
-    c0 = column(threadIdx.x);
-    t0 = teacher(threadIdx.x);
-  }
-  Row held;
-  held.load(at);
-  if (at.last >= 0) at.tail = (float)at.z[at.last];
-  if (threadIdx.x < 2) sh.flags[threadIdx.x] = 0;
-  __syncthreads();
-#pragma unroll 1  // (the row's registers are live)
-  for (int k = threadIdx.x; k < a.K; k += NT) {
-    const bool ahead = k == (int)threadIdx.x;
-    const int64_t c = ahead ? c0 : column(k);
-    const bool in = c >= 0 && c < V;
-    if (c >= V) atomicOr(&sh.flags[0], 1);
-    s.column[k] = in ? (int)c : -1;
-    const float t = !in ? -INFINITY : ahead ? t0 : teacher(k);
-    // (a maximum passes NaN over; slots of -inf alone say nothing)
-    if (t != -INFINITY) atomicOr(&sh.flags[1], 1);
-    s.t[k] = t;
-    s.z[k] = in ? (float)at.z[c] : 0.f;
-  }
-  if (threadIdx.x == 0) {
-    s.column[a.K] = hard ? (int)target : -1;
-    s.t[a.K] = 0.f;
-    s.z[a.K] = hard ? (float)at.z[target] : 0.f;
-  }
-
-  // Maxima of the student's and the teacher's logits.
-  float m[2] = {fmaxf(held.max(at), at.tail), -INFINITY};
-#pragma unroll 1
-  for (int k = threadIdx.x; k < a.K; k += NT) m[1] = fmaxf(m[1], s.t[k]);
-  combine<NT, 2, true>(m, sh.max[0]);  // its barrier also ends the slots
-  const bool bad = soft && sh.flags[0], taught = soft && sh.flags[1];
+  // Maxima: the student's and the teacher's logits, a column outside the
+  // vocabulary, a slot with a say (slots of -inf alone have none; a maximum
+  // passes NaN over).
+  float m[4] = {fmaxf(held.max(at), at.tail), in ? at.t : -INFINITY, at.column >= V ? 1.f : 0.f,
+                in && at.t != -INFINITY ? 1.f : 0.f};
+  combine<NT, 4, true>(m, sh.max[0]);
+  const bool bad = soft && m[2] != 0.f, taught = soft && m[3] != 0.f;
   if (bad || !(taught || hard)) {
     no_gradient(bad ? __builtin_nanf("") : 0.f);
     return;
   }
   if (Row::kTwoMax && m[0] < 0.f) {  // no value of sign 0 among the pieces
-    float n[2] = {fmaxf(held.least_negative(), at.tail), -INFINITY};
-    combine<NT, 2, true>(n, sh.max[1]);
+    float n[4] = {fmaxf(held.least_negative(), at.tail)};
+    combine<NT, 4, true>(n, sh.max[1]);
     m[0] = n[0];
   }
   const float ct = kLog2e * a.inv_temp;
   const float c = soft ? ct : kLog2e;  // of the only softmax, where there is one
   // |max| c below the largest float, for c up to 144
   if (fabsf(m[0]) < 1e36f) {
-    finish_row<T, NT, P, false>(a, row, at, held, sh, m[0], m[1], taught, hard, c, ct);
+    finish_row<T, NT, P, false>(a, row, at, held, sh, z_slot, z_target, m[0], m[1], taught, hard,
+                                c, ct, scale);
   } else {
     ReadRow<T, NT> again;
-    finish_row<T, NT, P, true>(a, row, at, again, sh, m[0], m[1], taught, hard, c, ct);
+    finish_row<T, NT, P, true>(a, row, at, again, sh, z_slot, z_target, m[0], m[1], taught, hard,
+                               c, ct, scale);
   }
 }
 
@@ -522,10 +512,21 @@ template <typename T, int NT, int P, typename Row>
 __global__ __launch_bounds__(NT, Row::kWaves) void distill_kernel(DistillArgs a) {
   __shared__ Shared sh;
   if (a.unless_one && *a.g == 1.f) return;
+  const auto one = [&](int64_t row) {
+    const RowAt<T> at = row_at<T>(a, row);
+    Row held;
+    held.load(at);
+    const float scale = (a.scale_dev ? a.scale * *a.scale_dev : a.scale) *
+                        (a.g ? a.g[row * a.g_stride] : 1.f);
+    distill_row<T, NT, P>(a, row, at, held, sh, scale);
+  };
   if constexpr (Row::kLoop) {
-    for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) distill_row<T, NT, P, Row>(a, r, sh);
+    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+      one(row);
+      __syncthreads();  // LDS is the next row's
+    }
   } else {  // (what a loop keeps from one row to the next costs the registers of a piece)
-    distill_row<T, NT, P, Row>(a, blockIdx.x, sh);
+    one(blockIdx.x);
   }
 }
 
@@ -588,24 +589,24 @@ hipError_t launch_row(const DistillArgs& a, unsigned grid, hipStream_t stream) {
 template <typename T>
 hipError_t launch_distill_t(const DistillArgs& a, hipStream_t stream) {
   const int64_t pieces = a.V / Elem<T>::kVec;
-  // A gradient that stands as a rule: few work-groups, which end at once or
-  // read their rows (with the held row's threads, so in its order of additions).
-  const int64_t most = 1024;
-  const unsigned all = (unsigned)a.rows, few = (unsigned)(a.rows < most ? a.rows : most);
+  const unsigned all = (unsigned)a.rows, few = all < 1024 ? all : 1024;
 #define READ(NT) return launch_row<T, NT, ReadRow<T, NT>>(a, few, stream)
 #define ROW(NT, NP) return launch_row<T, NT, HeldRow<T, NT, NP>>(a, all, stream)
-  if (pieces <= 1024) {
+  // At least a thread a slot.
+  // (a gradient that stands as a rule is read, not held, with the threads that
+  // hold it: in the same order of additions)
+  if (pieces <= 1024 && a.K <= 256) {
     if (a.unless_one) READ(256);
     if (pieces <= 256) ROW(256, 1);
     if (pieces <= 512) ROW(256, 2);
     ROW(256, 4);
   }
-  if (pieces <= 2048) {
+  if (pieces <= 2048 && a.K <= 512) {
     if (a.unless_one) READ(512);
     ROW(512, 4);
   }
-  if (a.unless_one || pieces > 16 * 1024)
-    return launch_row<T, 1024, ReadRow<T, 1024>>(a, a.unless_one ? few : all, stream);
+  if (a.unless_one || pieces > 16 * 1024) READ(1024);
+  if (pieces <= 2 * 1024) ROW(1024, 2);
   if (pieces <= 4 * 1024) ROW(1024, 4);
   if (pieces <= 5 * 1024) ROW(1024, 5);
   if (pieces <= 6 * 1024) ROW(1024, 6);

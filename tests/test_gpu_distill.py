@@ -363,12 +363,19 @@ def test_strides_alignments_and_leading_dimensions(dt):
         return loss.detach(), torch.autograd.grad(loss, leaf)[0].reshape(N, V)
 
     want = run(z, idx, t, target)
+    # Where a row starts between two 16-byte boundaries, the columns that a thread
+    # adds up are others: another order of the same additions.  Each order's
+    # result is within the tolerance of the sums (rel(S) holds for any chain of
+    # that length), so that is what both have to keep.
+    rows, tol, grad, size = _reference(z, idx, t, target, 2.0, 0.5)
+    n = int((target != IGNORE).sum())
     wide = torch.full((N, V + 20), float("nan"), dtype=dt, device=DEV)
     for off in (0, 1, 8):
         view = wide[:, off:off + V]
         view.copy_(z)
-        for a, b in zip(run(view, idx, t, target), want):
-            assert torch.equal(a, b)
+        loss, dz = run(view, idx, t, target)
+        _within(loss, rows.sum() / n, (tol.sum() + 4 * U * rows.abs().sum()) / n, "mean")
+        _within(dz, grad / n, _grad_tol(dt, grad / n, size / n), "gradient")
     pad = torch.cat((idx, idx), 1)[:, :K], torch.cat((t, t), 1)[:, :K]
     for a, b in zip(run(z, *pad, target.int()), want):
         assert torch.equal(a, b)
