@@ -388,8 +388,8 @@ int64_t t2t_embedding_backward_workspace(int64_t N, int64_t V, int32_t C);
 /*
  * Gradient of t2t_embedding: dweight[v] = scale * sum of dy[i] over the i with
  * tokens[i] == v, in fp32 in the order of the positions (deterministic, no
- * atomics on values), rounded once.  Every row of dweight [V][C] (contiguous)
- * is written; the row `padding` (-1: none) and those of ids that do not occur
+ * atomics on values), rounded once.  Every row of dweight [V][C] (contiguous,
+ * 16-byte aligned) is written; the row `padding` (-1: none) and those of ids that do not occur
  * are zero; ids outside [0, V) are left out.
  *   dy       [N][C] rows of the dtype with row stride dy_stride.
  */

@@ -177,7 +177,8 @@ struct EmbedGradArgs {
   int* count;           // positions in the list
   int2* list;           // (position, token), grouped by token
   float* part;          // [pieces][2][C]: a token that came from / goes on behind the piece
-  int group_log2, rows_per_group, piece;
+  int group_log2, rows_per_group, piece, fill_groups;
+  int64_t zero_bytes;
 };
 struct EmbedPlan {
   int group_log2, rows_per_group, piece;

@@ -776,6 +776,8 @@ int t2t_embedding_backward(const int64_t* tokens, int64_t N, const void* dy, int
   const int vec = embed_vector(C, dtype, dy, dweight, dy_stride);
   if (!dweight || vec < 0 || (N > 0 && (!dy || dy_stride < 0)))
     return fail(T2T_EINVAL, "dy or dweight NULL, misaligned, or a negative row stride");
+  if (reinterpret_cast<uintptr_t>(dweight) % 16)
+    return fail(T2T_EINVAL, "dweight must be 16-byte aligned");
   const int64_t need = t2t_embedding_backward_workspace(N, V, C);
   if (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16)
     return fail(T2T_EINVAL, "workspace of %lld bytes (16-byte aligned), %lld needed",

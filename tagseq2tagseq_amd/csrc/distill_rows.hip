@@ -302,7 +302,7 @@ struct ReadRow {
 // the other (sched_barrier): unpacked all at once, they would spill.
 template <typename T, int NT, int NP>
 struct HeldRow {
-  static constexpr int kWaves = NP <= 8 ? 8 : 4;
+  static constexpr int kWaves = NP <= 8 ? 8 : NT < 1024 ? 6 : 4;
   static constexpr bool kLoop = false;
   static constexpr int VEC = Elem<T>::kVec;
   static constexpr bool kTwoMax = Elem<T>::kTwoMax;
@@ -601,16 +601,20 @@ hipError_t launch_distill_t(const DistillArgs& a, hipStream_t stream) {
     if (pieces <= 512) ROW(256, 2);
     ROW(256, 4);
   }
-  if (pieces <= 2048 && a.K <= 512) {
+  // Rows in as few threads as still hold them: each thread has about 30 registers
+  // beside its pieces, and what is left of them is further rows on the CU, whose
+  // loads run while another row is computed (8192 rows of 50257: three rows of
+  // 512 threads 363 us, two of 1024 372 us).
+  if (pieces <= 13 * 512 && a.K <= 512) {
     if (a.unless_one) READ(512);
-    ROW(512, 4);
+    if (pieces <= 4 * 512) ROW(512, 4);
+    if (pieces <= 8 * 512) ROW(512, 8);
+    if (pieces <= 10 * 512) ROW(512, 10);
+    ROW(512, 13);
   }
   if (a.unless_one || pieces > 16 * 1024) READ(1024);
   if (pieces <= 2 * 1024) ROW(1024, 2);
   if (pieces <= 4 * 1024) ROW(1024, 4);
-  if (pieces <= 5 * 1024) ROW(1024, 5);
-  if (pieces <= 6 * 1024) ROW(1024, 6);
-  if (pieces <= 7 * 1024) ROW(1024, 7);
   if (pieces <= 8 * 1024) ROW(1024, 8);
   if (pieces <= 12 * 1024) ROW(1024, 12);
   ROW(1024, 16);

@@ -47,7 +47,7 @@ def _backward(**kw):
 @no_gpu
 @pytest.mark.parametrize("kw,rc,text", [
     (dict(pad=-2), -1, "padding"), (dict(pad=10), -1, "padding"), (dict(dw=None), -1, "dweight"),
-    (dict(dy=None), -1, "dy"), (dict(ds=-1), -1, "stride"), (dict(ws=None), -1, "workspace"),
+    (dict(dy=None), -1, "dy"), (dict(dw=ctypes.c_void_p(0x1008)), -1, "16-byte"), (dict(ds=-1), -1, "stride"), (dict(ws=None), -1, "workspace"),
     (dict(bytes=16), -1, "workspace"), (dict(ws=ctypes.c_void_p(0x1008)), -1, "workspace"),
     (dict(V=1 << 25), -2, "one launch"),
 ])
