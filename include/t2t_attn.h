@@ -374,7 +374,7 @@ int t2t_qk_norm_rope_backward(const t2t_tensor *dq, const t2t_tensor *dk, const 
  * Scaled embedding lookup: out[i] = scale weight[tokens[i]] for N ids (int64),
  * computed in fp32 and rounded once; an id outside [0, V) gives a row of NaN.
  *   weight   [V][C], dtype 0 = bf16, 1 = float32, row stride weight_stride >= C
- *            (elements); V at most 2^24.
+ *            (elements); V at most 2^20.
  *   out      [N][C] contiguous, same dtype.
  * Rows are moved in 16-byte pieces where C, the stride and the addresses allow
  * it, element by element otherwise.

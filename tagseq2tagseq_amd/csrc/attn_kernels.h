@@ -174,15 +174,16 @@ struct EmbedGradArgs {
   float scale;
   void* dweight;
   // set by the launcher, in the workspace:
-  int* count;           // positions in the list
-  int2* list;           // (position, token), grouped by token
+  int2* list;           // [N] (position, token), grouped by token; (0, -1): no gradient
+  int2* split;          // [N] (position, id), blocks of positions sorted by group
+  int* bounds;          // [blocks][groups + 1]: where a group starts in a block's part
   float* part;          // [pieces][2][C]: a token that came from / goes on behind the piece
-  int group_log2, rows_per_group, piece, fill_groups;
-  int64_t zero_bytes;
+  int group_log2, rows_per_group, row_bits, piece, blocks;
+  int64_t zero_bytes, zero_split;  // of dweight; those that the first launch fills
 };
 struct EmbedPlan {
-  int group_log2, rows_per_group, piece;
-  int64_t list_at, part_at, bytes;
+  int group_log2, rows_per_group, piece, blocks;
+  int64_t split_at, bounds_at, part_at, bytes;
 };
 EmbedPlan embed_plan(int64_t N, int64_t V, int C);
 hipError_t launch_embed_grad(EmbedGradArgs a, void* workspace, bool f32, bool vector,

@@ -720,7 +720,7 @@ int t2t_qk_norm_rope_backward(const t2t_tensor* dq, const t2t_tensor* dk, const 
 
 namespace {
 
-constexpr int64_t kEmbedMaxV = 1 << 24;
+constexpr int64_t kEmbedMaxV = 1 << 20;
 
 int check_embed(const void* tokens, int64_t N, int64_t V, int32_t C, int32_t dtype) {
   if (N < 0 || V < 1 || C < 1)

@@ -9,15 +9,17 @@
 // the rows of dy read once in that order.  HBM bound: dy is read once and the
 // V rows of dW are written once, most of them zeros.
 //
-//   1. embed_group_kernel: work-group r of G takes the tokens with
-//      id mod G = r (G a power of two, so neighbouring ids, whose frequencies
-//      are alike, spread over the work-groups).  Every work-group reads all ids
-//      (from L2): it counts those with a smaller remainder, which is where its
-//      list starts, and the occurrences of its own ids; on a second reading
-//      each wave places its positions, in order, behind those of the waves
-//      before it.  No work-group waits for another.  Further work-groups of the
-//      same launch fill dW with zeros meanwhile (a wave's loads wait for its
-//      own earlier stores, so not the same ones).
+//   1. Group r of G has the ids with id mod G = r (G a power of two, so
+//      neighbouring ids, whose frequencies are alike, spread over the groups).
+//      embed_split_kernel sorts blocks of 2048 positions by group, in LDS;
+//      embed_group_kernel, a work-group a group, sorts the group's parts of all
+//      blocks by id: each wave counts its share of them, and places them in order
+//      behind those of the waves before it.  Short lists are grouped
+//      without the split, every work-group reading all ids (with long ones, which
+//      all work-groups read in step from the same L2 channels, that took
+//      70 us for 131072 ids).  Further work-groups of both launches fill dW
+//      with zeros meanwhile (a wave's loads wait for its own earlier stores,
+//      so not the same ones).
 //   2. embed_sum_kernel: the list in pieces of S positions; a wave sums 64 VEC
 //      columns over a piece, all its loads in flight at once, and stores a
 //      token's row where all its positions lie within the piece, and a partial
@@ -34,9 +36,12 @@ namespace {
 constexpr int kEmbThreads = 256;
 constexpr int kEmbItems = 4;
 constexpr int kSumBatch = 16;
-constexpr int kGroupThreads = 1024;
+constexpr int kEmbedDirect = 4096;     // positions grouped without the split
+constexpr int kGroupThreads = 512;
 constexpr int kGroupWaves = kGroupThreads / 64;
 constexpr int kGroupSteps = 8;         // of 64 positions, loaded at once
+constexpr int kSplitItems = 4;         // positions a thread
+constexpr int kSplitBlock = kGroupThreads * kSplitItems;
 constexpr int kSumThreads = 256;
 constexpr int kJoinWaves = 16;
 constexpr int kLongRun = 32;           // pieces: from here the work-group joins a token
@@ -80,55 +85,55 @@ __global__ __launch_bounds__(kEmbThreads) void embed_kernel(EmbedArgs a) {
   }
 }
 
-// cursor[wave][row]: first the occurrences of the group's row in the wave's
-// part of the tokens, then where the wave's next one goes.
-__global__ __launch_bounds__(kGroupThreads) void embed_group_kernel(EmbedGradArgs a) {
-  extern __shared__ int lds[];
-  if (blockIdx.x >= 1u << a.group_log2) {  // the zeros of dW, bytes of whole 16-byte pieces
-    const int64_t n = a.zero_bytes / 16, step = (int64_t)a.fill_groups * kGroupThreads;
-    const int64_t i0 = (int64_t)(blockIdx.x - (1u << a.group_log2)) * kGroupThreads + threadIdx.x;
-    uint4* dst = static_cast<uint4*>(a.dweight);
-    for (int64_t i = i0; i < n; i += step) dst[i] = make_uint4(0, 0, 0, 0);
-    const int rest = (int)(a.zero_bytes % 16) / 2;  // and the 16-bit words behind them
-    if (i0 < rest) reinterpret_cast<uint16_t*>(dst + n)[i0] = 0;
-    return;
+// An id as 32 bits; one outside 32 bits as the largest number, which is no row.
+__device__ __forceinline__ uint32_t id_of(int64_t t) {
+  return (uint64_t)t >> 32 ? 0xffffffffu : (uint32_t)t;
+}
+
+// Bytes [from, to) of dW, multiples of 16 but for the end of dW.
+__device__ __forceinline__ void fill_zeros(void* dw, int64_t from, int64_t to, int block,
+                                           int blocks) {
+  const int64_t n = to / 16, step = (int64_t)blocks * kGroupThreads;
+  const int64_t first = (int64_t)block * kGroupThreads + threadIdx.x;
+  uint4* dst = static_cast<uint4*>(dw);
+  for (int64_t i = from / 16 + first; i < n; i += step) dst[i] = make_uint4(0, 0, 0, 0);
+  const int rest = (int)(to % 16) / 2;  // the 16-bit words behind the whole pieces
+  if (first < rest) reinterpret_cast<uint16_t*>(dst + n)[first] = 0;
+}
+
+// The lanes of `active` whose v, of `bits` bits, is this lane's.
+__device__ __forceinline__ uint64_t same_lanes(uint32_t v, int bits, uint64_t active) {
+  uint64_t same = active;
+  for (int b = 0; b < bits; ++b) {
+    const bool one = v >> b & 1;
+    const uint64_t ones = __ballot(one);
+    same &= one ? ones : ~ones;
   }
-  const int R = a.rows_per_group;
-  int* cursor = lds;                  // [kGroupWaves][R]
-  int* red = lds + kGroupWaves * R;   // [kGroupWaves]
+  return same;
+}
+
+// Where the active lanes' values go: behind the earlier ones of the same v,
+// counted in cursor[v], in the order of the lanes.
+__device__ __forceinline__ int place(int* cursor, uint32_t v, int bits, bool active) {
+  const int lane = threadIdx.x & 63;
+  const uint64_t same = same_lanes(v, bits, __ballot(active));
+  const int leader = __ffsll((unsigned long long)same) - 1;
+  int at = 0;
+  if (active && lane == leader) at = atomicAdd(&cursor[v], __popcll(same));
+  at = __shfl(at, active ? leader : lane, 64);
+  return at + __popcll(same & ((1ull << lane) - 1));
+}
+
+// counts[wave][n] to where the first value of each kind goes: behind those of
+// smaller kinds and of earlier waves, from `base` on.  Returns the end.
+__device__ __forceinline__ int starts_of(int* counts, int n, int base, int* red) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const uint32_t G = 1u << a.group_log2, r = blockIdx.x;
-  for (int i = threadIdx.x; i < kGroupWaves * R; i += kGroupThreads) cursor[i] = 0;
-  __syncthreads();
-
-  const int N = a.N;
-  const int part = ((N + kGroupWaves - 1) / kGroupWaves + 63) & ~63;
-  const int i0 = wave * part, i1 = min(N, i0 + part);
-  int before = 0;
-#pragma unroll 8
-  for (int i = i0 + lane; i < i1; i += 64) {
-    const int64_t t = a.tokens[i];
-    const bool valid = (uint64_t)t < (uint64_t)a.V && t != a.padding;
-    const uint32_t rest = (uint32_t)t & (G - 1);
-    before += valid && rest < r;
-    if (valid && rest == r) atomicAdd(&cursor[wave * R + (int)(t >> a.group_log2)], 1);
-  }
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) before += __shfl_xor(before, off, 64);
-  if (lane == 0) red[wave] = before;
-  __syncthreads();  // the counts too
-  int base = 0;
-#pragma unroll
-  for (int w = 0; w < kGroupWaves; ++w) base += red[w];
-  __syncthreads();
-
-  // Exclusive sums over rows, then over the waves within a row.
-  for (int r0 = 0; r0 < R; r0 += kGroupThreads) {
-    const int row = r0 + threadIdx.x;
+  for (int k0 = 0; k0 < n; k0 += kGroupThreads) {
+    const int k = k0 + threadIdx.x;
     int count = 0;
-    if (row < R)
+    if (k < n)
 #pragma unroll
-      for (int w = 0; w < kGroupWaves; ++w) count += cursor[w * R + row];
+      for (int w = 0; w < kGroupWaves; ++w) count += counts[w * n + k];
     int x = count;  // inclusive over the wave
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) {
@@ -137,54 +142,161 @@ __global__ __launch_bounds__(kGroupThreads) void embed_group_kernel(EmbedGradArg
     }
     if (lane == 63) red[wave] = x;
     __syncthreads();
-    int at = base + x - count, all = 0;
+    int at = base + x - count;
 #pragma unroll
     for (int w = 0; w < kGroupWaves; ++w) {
       if (w < wave) at += red[w];
-      all += red[w];
+      base += red[w];
     }
-    if (row < R)
+    if (k < n)
 #pragma unroll
       for (int w = 0; w < kGroupWaves; ++w) {
-        const int c = cursor[w * R + row];
-        cursor[w * R + row] = at;
+        const int c = counts[w * n + k];
+        counts[w * n + k] = at;
         at += c;
       }
-    base += all;
     __syncthreads();
   }
-  if (r == G - 1 && threadIdx.x == 0) *a.count = base;
+  return base;
+}
 
-  // Second reading: 64 positions at a time, one token id after the other.
-  for (int s0 = i0; s0 < i1; s0 += 64 * kGroupSteps) {
-    int64_t ts[kGroupSteps];
+// A block of 2048 positions sorted by group: (position, id) to split[block],
+// where each group's part starts to bounds[block][G + 1].
+__global__ __launch_bounds__(kGroupThreads) void embed_split_kernel(EmbedGradArgs a) {
+  extern __shared__ int lds[];
+  if ((int)blockIdx.x >= a.blocks) {
+    fill_zeros(a.dweight, 0, a.zero_split, blockIdx.x - a.blocks, gridDim.x - a.blocks);
+    return;
+  }
+  const int G = 1 << a.group_log2, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int* cursor = lds;                  // [kGroupWaves][G]
+  int* red = lds + kGroupWaves * G;   // [kGroupWaves]
+  const int64_t b0 = (int64_t)blockIdx.x * kSplitBlock;
+  const int i0 = wave * 64 * kSplitItems + lane;
+  uint32_t id[kSplitItems];
+#pragma unroll
+  for (int k = 0; k < kSplitItems; ++k) {
+    const int64_t i = b0 + i0 + 64 * k;
+    id[k] = i < a.N ? id_of(a.tokens[i]) : 0;
+  }
+  for (int i = threadIdx.x; i < kGroupWaves * G; i += kGroupThreads) cursor[i] = 0;
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < kSplitItems; ++k)
+    if (b0 + i0 + 64 * k < a.N) atomicAdd(&cursor[wave * G + (id[k] & (G - 1))], 1);
+  __syncthreads();
+  const int all = starts_of(cursor, G, 0, red);
+  int* bounds = a.bounds + (int64_t)blockIdx.x * (G + 1);
+  for (int g = threadIdx.x; g < G; g += kGroupThreads) bounds[g] = cursor[g];  // wave 0's start
+  if (threadIdx.x == 0) bounds[G] = all;
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < kSplitItems; ++k) {
+    const bool in = b0 + i0 + 64 * k < a.N;
+    const int at = place(cursor + wave * G, id[k] & (G - 1), a.group_log2, in);
+    if (in) a.split[b0 + at] = make_int2((int)(b0 + i0 + 64 * k), (int)id[k]);
+  }
+}
+
+// Calls f(position, id, active) for the wave's share of the group's positions,
+// in order, all lanes at once; other groups' lanes are inactive.
+template <bool Split, typename F>
+__device__ __forceinline__ void group_share(const EmbedGradArgs& a, uint32_t r, const F& f) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const uint32_t G = 1u << a.group_log2;
+  if (!Split) {
+    const int part = ((a.N + kGroupWaves - 1) / kGroupWaves + 63) & ~63;
+    const int i0 = wave * part, i1 = min(a.N, i0 + part);
+    for (int s = i0; s < i1; s += 64 * kGroupSteps) {
+      uint32_t id[kGroupSteps];
+#pragma unroll
+      for (int k = 0; k < kGroupSteps; ++k) {
+        const int i = s + 64 * k + lane;
+        id[k] = i < i1 ? id_of(a.tokens[i]) : r ^ 1;
+      }
+#pragma unroll
+      for (int k = 0; k < kGroupSteps; ++k) {
+        const bool own = (id[k] & (G - 1)) == r;
+        if (__ballot(own)) f(s + 64 * k + lane, id[k], own);
+      }
+    }
+    return;
+  }
+  const int part = (a.blocks + kGroupWaves - 1) / kGroupWaves;
+  const int b0 = wave * part, b1 = min(a.blocks, b0 + part);
+  for (int b = b0; b < b1; b += kGroupSteps) {
+    int at[kGroupSteps], end[kGroupSteps];
+    int2 e[kGroupSteps];
 #pragma unroll
     for (int k = 0; k < kGroupSteps; ++k) {
-      const int i = s0 + 64 * k + lane;
-      ts[k] = i < i1 ? a.tokens[i] : -1;
+      const int* bounds = a.bounds + (int64_t)min(b + k, b1 - 1) * (G + 1) + r;
+      at[k] = bounds[0];
+      end[k] = b + k < b1 ? bounds[1] : at[k];
     }
 #pragma unroll
     for (int k = 0; k < kGroupSteps; ++k) {
-      const int64_t t = ts[k];
-      const bool own =
-          (uint64_t)t < (uint64_t)a.V && t != a.padding && ((uint32_t)t & (G - 1)) == r;
-      const int row = own ? (int)(t >> a.group_log2) : -1;
-      uint64_t left = __ballot(own);
-      while (left) {
-        const int leader = __ffsll((unsigned long long)left) - 1;
-        const int lrow = __builtin_amdgcn_readlane(row, leader);
-        const uint64_t same = __ballot(row == lrow);
-        int at = 0;
-        if (lane == leader) at = atomicAdd(&cursor[wave * R + lrow], __popcll(same));
-        at = __builtin_amdgcn_readlane(at, leader);
-        if (row == lrow) {
-          at += __popcll(same & ((1ull << lane) - 1));
-          a.list[at] = make_int2(s0 + 64 * k + lane, (int)t);
-        }
-        left &= ~same;
+      e[k] = make_int2(0, 0);
+      if (at[k] + lane < end[k]) e[k] = a.split[(int64_t)(b + k) * kSplitBlock + at[k] + lane];
+    }
+#pragma unroll
+    for (int k = 0; k < kGroupSteps; ++k) {
+      if (at[k] < end[k]) f(e[k].x, (uint32_t)e[k].y, at[k] + lane < end[k]);
+      for (int i = at[k] + 64; i < end[k]; i += 64) {
+        int2 more = make_int2(0, 0);
+        if (i + lane < end[k]) more = a.split[(int64_t)(b + k) * kSplitBlock + i + lane];
+        f(more.x, (uint32_t)more.y, i + lane < end[k]);
       }
     }
   }
+}
+
+// The list of a group's positions by id.  Row R, behind the others, takes ids
+// without a gradient; they are in the list as token -1, so that it has every
+// position and needs no count.
+template <bool Split>
+__global__ __launch_bounds__(kGroupThreads) void embed_group_kernel(EmbedGradArgs a) {
+  extern __shared__ int lds[];
+  const uint32_t G = 1u << a.group_log2;
+  if (blockIdx.x >= G) {
+    fill_zeros(a.dweight, a.zero_split, a.zero_bytes, blockIdx.x - G, gridDim.x - G);
+    return;
+  }
+  const uint32_t r = blockIdx.x, V = (uint32_t)a.V, pad = (uint32_t)a.padding;
+  const int R = a.rows_per_group + 1, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int* cursor = lds;                  // [kGroupWaves][R]
+  int* red = lds + kGroupWaves * R;   // [kGroupWaves]
+  for (int i = threadIdx.x; i < kGroupWaves * R; i += kGroupThreads) cursor[i] = 0;
+  // Positions of smaller groups.
+  int before = 0;
+  if (Split) {
+    for (int b = threadIdx.x; b < a.blocks; b += kGroupThreads)
+      before += a.bounds[(int64_t)b * (G + 1) + r];
+  } else {
+#pragma unroll 8
+    for (int i = threadIdx.x; i < a.N; i += kGroupThreads)
+      before += (id_of(a.tokens[i]) & (G - 1)) < r;
+  }
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) before += __shfl_xor(before, off, 64);
+  if (lane == 0) red[wave] = before;
+  __syncthreads();
+  int base = 0;
+#pragma unroll
+  for (int w = 0; w < kGroupWaves; ++w) base += red[w];
+
+  const auto row_of = [&](uint32_t t) {
+    return t < V && t != pad ? (int)(t >> a.group_log2) : R - 1;
+  };
+  group_share<Split>(a, r, [&](int, uint32_t id, bool own) {
+    if (own) atomicAdd(&cursor[wave * R + row_of(id)], 1);
+  });
+  __syncthreads();
+  starts_of(cursor, R, base, red);
+  group_share<Split>(a, r, [&](int i, uint32_t id, bool own) {
+    const int row = own ? row_of(id) : 0;
+    const int at = place(cursor + wave * R, row, a.row_bits, own);
+    if (own) a.list[at] = row == R - 1 ? make_int2(0, -1) : make_int2(i, (int)id);
+  });
 }
 
 // A wave sums 64 VEC columns of a piece of S positions, lane l the columns
@@ -192,7 +304,7 @@ __global__ __launch_bounds__(kGroupThreads) void embed_group_kernel(EmbedGradArg
 // The positions are the same for all lanes.
 template <typename T, int VEC, int S>
 __global__ __launch_bounds__(kSumThreads) void embed_sum_kernel(EmbedGradArgs a) {
-  const int M = *a.count, lane = threadIdx.x & 63;
+  const int M = a.N, lane = threadIdx.x & 63;
   const int blocks = (a.C + 64 * VEC - 1) / (64 * VEC);
   const int item = __builtin_amdgcn_readfirstlane(
       (int)(blockIdx.x * (kSumThreads / 64) + (threadIdx.x >> 6)));
@@ -204,7 +316,7 @@ __global__ __launch_bounds__(kSumThreads) void embed_sum_kernel(EmbedGradArgs a)
   const int2* __restrict__ list = a.list + e0;
   const bool in = c < a.C;
   const T* __restrict__ dy = static_cast<const T*>(a.dy) + (in ? c : 0);
-  const int before = e0 ? list[-1].y : -1, after = e0 + n < M ? list[n].y : -1;
+  const int before = e0 ? list[-1].y : -2, after = e0 + n < M ? list[n].y : -2;
   float acc[VEC] = {};
   bool from_before = list[0].y == before;
 #pragma unroll
@@ -230,7 +342,7 @@ __global__ __launch_bounds__(kSumThreads) void embed_sum_kernel(EmbedGradArgs a)
       const int follows = ends ? after : e + 1 < kSumBatch ? token[(e + 1) % kSumBatch] : next;
       if (!ends && follows == token[e]) continue;
       const bool to_after = ends && follows == token[e];
-      if (in) {
+      if (in && token[e] >= 0) {
         if (from_before || to_after) {
           float* p = a.part + (2 * (int64_t)piece + !from_before) * a.C + c;
 #pragma unroll
@@ -276,7 +388,7 @@ template <typename T, int VEC>
 __global__ __launch_bounds__(64 * kJoinWaves) void embed_join_kernel(EmbedGradArgs a) {
   __shared__ float red[kJoinWaves][64 * VEC];
   __shared__ int long_piece, ends;
-  const int M = *a.count, S = a.piece;
+  const int M = a.N, S = a.piece;
   const int pieces = (int)(((int64_t)M + S - 1) / S);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int piece = blockIdx.x * kJoinWaves + wave;
@@ -289,7 +401,7 @@ __global__ __launch_bounds__(64 * kJoinWaves) void embed_join_kernel(EmbedGradAr
   __syncthreads();
   if (e1 < M) {
     const int token = a.list[e1].y;
-    const bool starts = a.list[e1 - 1].y == token &&
+    const bool starts = token >= 0 && a.list[e1 - 1].y == token &&
                         !(a.list[e0].y == token && e0 && a.list[e0 - 1].y == token);
     if (starts) {
       // Lane l: does piece + 1 + l start with the token?
@@ -374,9 +486,23 @@ hipError_t launch_join(const EmbedGradArgs& a, int64_t pieces, hipStream_t strea
 
 template <typename T>
 hipError_t launch_grad_t(const EmbedGradArgs& a, bool vector, hipStream_t stream) {
-  const int lds = (kGroupWaves * a.rows_per_group + kGroupWaves) * 4;
-  hipLaunchKernelGGL(embed_group_kernel, dim3((1u << a.group_log2) + a.fill_groups),
-                     dim3(kGroupThreads), lds, stream, a);
+  const int G = 1 << a.group_log2;
+  const int lds = (kGroupWaves * (a.rows_per_group + 1) + kGroupWaves) * 4;
+  const auto fills = [](int64_t bytes) {  // work-groups; four 16-byte pieces a thread at least
+    const int64_t n = (bytes / 16 + 4 * kGroupThreads - 1) / (4 * kGroupThreads);
+    return (int)(n < 1 ? 1 : n < 768 ? n : 768);
+  };
+  if (a.blocks) {
+    hipLaunchKernelGGL(embed_split_kernel, dim3(a.blocks + fills(a.zero_split)),
+                       dim3(kGroupThreads), (kGroupWaves * G + kGroupWaves) * 4, stream, a);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL(embed_group_kernel<true>, dim3(G + fills(a.zero_bytes - a.zero_split)),
+                       dim3(kGroupThreads), lds, stream, a);
+  } else {
+    hipLaunchKernelGGL(embed_group_kernel<false>, dim3(G + fills(a.zero_bytes)),
+                       dim3(kGroupThreads), lds, stream, a);
+  }
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || a.N == 0) return e;
   const int64_t pieces = ((int64_t)a.N + a.piece - 1) / a.piece;
@@ -396,19 +522,23 @@ hipError_t launch_grad_t(const EmbedGradArgs& a, bool vector, hipStream_t stream
 
 }  // namespace
 
-// Grouping work-groups: 256 (each reads every id), more where a group's rows
-// would not fit the LDS counters (16 ints a row: 40 KiB).  Positions a piece: few
-// for short lists, whose waves would not fill the card.
+// Groups: 256, more where a group's rows would not fit the LDS counters (8 ints
+// a row: 32 KiB).  Positions a piece: few for short lists, whose waves would not
+// fill the card.
 EmbedPlan embed_plan(int64_t N, int64_t V, int C) {
   EmbedPlan p{};
   p.group_log2 = 8;
-  while ((V >> p.group_log2) >= 640) ++p.group_log2;
-  p.rows_per_group = (int)((V + (1ll << p.group_log2) - 1) >> p.group_log2);
+  while ((V >> p.group_log2) > 1024) ++p.group_log2;
+  const int64_t G = 1ll << p.group_log2;
+  p.rows_per_group = (int)((V + G - 1) >> p.group_log2);
   p.piece = N <= 32768 ? 16 : 32;
+  p.blocks = N <= kEmbedDirect ? 0 : (int)((N + kSplitBlock - 1) / kSplitBlock);
+  const auto whole = [](int64_t n) { return (n + 255) / 256 * 256; };
   const int64_t pieces = (N + p.piece - 1) / p.piece;
-  p.list_at = 256;  // behind the count
-  p.part_at = (p.list_at + N * (int64_t)sizeof(int2) + 255) / 256 * 256;
-  p.bytes = p.part_at + 2 * pieces * C * 4;
+  p.split_at = whole(N * (int64_t)sizeof(int2));
+  p.bounds_at = p.split_at + (p.blocks ? whole(N * (int64_t)sizeof(int2)) : 0);
+  p.part_at = p.bounds_at + whole(p.blocks * (G + 1) * 4);
+  p.bytes = p.part_at + 2 * pieces * C * 4 + 256;  // (never none)
   return p;
 }
 
@@ -422,15 +552,18 @@ hipError_t launch_embed_grad(EmbedGradArgs a, void* workspace, bool f32, bool ve
                              hipStream_t stream) {
   const EmbedPlan p = embed_plan(a.N, a.V, a.C);
   char* ws = static_cast<char*>(workspace);
-  a.count = reinterpret_cast<int*>(ws);
-  a.list = reinterpret_cast<int2*>(ws + p.list_at);
+  a.list = reinterpret_cast<int2*>(ws);
+  a.split = reinterpret_cast<int2*>(ws + p.split_at);
+  a.bounds = reinterpret_cast<int*>(ws + p.bounds_at);
   a.part = reinterpret_cast<float*>(ws + p.part_at);
   a.group_log2 = p.group_log2;
   a.rows_per_group = p.rows_per_group;
+  a.row_bits = 0;
+  while (p.rows_per_group >> a.row_bits) ++a.row_bits;  // the row behind the last too
   a.piece = p.piece;
+  a.blocks = p.blocks;
   a.zero_bytes = a.V * a.C * (f32 ? 4 : 2);
-  const int64_t fills = (a.zero_bytes / 16 + 4 * kGroupThreads - 1) / (4 * kGroupThreads);
-  a.fill_groups = (int)(fills < 1 ? 1 : fills < 512 ? fills : 512);
+  a.zero_split = p.blocks ? a.zero_bytes / 32 * 16 : 0;  // about half in each launch
   return f32 ? launch_grad_t<float>(a, vector, stream) : launch_grad_t<__bf16>(a, vector, stream);
 }
 

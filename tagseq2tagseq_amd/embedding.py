@@ -85,7 +85,7 @@ class EmbeddingFn(torch.autograd.Function):
 def embedding(tokens: torch.Tensor, weight: torch.Tensor, scale: float = 1.0,
               padding_idx: Optional[int] = None) -> torch.Tensor:
     """``scale * weight[tokens]``: rows [..., C] (weight's dtype, bf16 or
-    float32) of tokens [...] (int64 or int32) from weight [V, C], V up to 2^24.
+    float32) of tokens [...] (int64 or int32) from weight [V, C], V up to 2^20.
 
     The weight's gradient is dense; the row ``padding_idx`` (counted from the
     end when negative) gets none.  An id outside [0, V) gives a row of NaN and

@@ -27,7 +27,7 @@ def _forward(**kw):
 @no_gpu
 @pytest.mark.parametrize("kw,rc,text", [
     (dict(N=-1), -1, "N=-1"), (dict(V=0), -1, "V=0"), (dict(C=0), -1, "C=0"),
-    (dict(dtype=2), -2, "dtype"), (dict(V=(1 << 24) + 1), -2, "one launch"),
+    (dict(dtype=2), -2, "dtype"), (dict(V=(1 << 20) + 1), -2, "one launch"),
     (dict(N=1 << 31), -2, "one launch"), (dict(N=1 << 30, C=1 << 10), -2, "one launch"),
     (dict(tokens=None), -1, "tokens"), (dict(tokens=ctypes.c_void_p(0x1004)), -1, "tokens"),
     (dict(w=None), -1, "weight"), (dict(out=ctypes.c_void_p(0x1001)), -1, "misaligned"),
@@ -49,7 +49,7 @@ def _backward(**kw):
     (dict(pad=-2), -1, "padding"), (dict(pad=10), -1, "padding"), (dict(dw=None), -1, "dweight"),
     (dict(dy=None), -1, "dy"), (dict(dw=ctypes.c_void_p(0x1008)), -1, "16-byte"), (dict(ds=-1), -1, "stride"), (dict(ws=None), -1, "workspace"),
     (dict(bytes=16), -1, "workspace"), (dict(ws=ctypes.c_void_p(0x1008)), -1, "workspace"),
-    (dict(V=1 << 25), -2, "one launch"),
+    (dict(V=1 << 21), -2, "one launch"),
 ])
 def test_backward_entry_refuses(kw, rc, text):
     assert _backward(**kw) == rc and text in _err()
@@ -57,7 +57,7 @@ def test_backward_entry_refuses(kw, rc, text):
 
 def test_workspace_sizes():
     ws = _lib.lib().t2t_embedding_backward_workspace
-    assert ws(-1, 5, 5) == ws(5, 0, 5) == ws(5, 5, 0) == ws(5, 1 << 25, 5) == 0
+    assert ws(-1, 5, 5) == ws(5, 0, 5) == ws(5, 5, 0) == ws(5, 1 << 21, 5) == 0
     assert 0 < ws(0, 5, 5) < ws(1000, 5, 5) < ws(1 << 20, 50257, 768) < 1 << 30
 
 
