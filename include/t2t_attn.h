@@ -327,7 +327,8 @@ int t2t_rms_norm_backward(const void *dy, int64_t dy_stride, const void *x, int6
  * p = pos0 + t; values are copied.  fp32 arithmetic, one rounding.
  *   qkv      dtype 0 = bf16, 1 = float32, strides in elements; 16-byte
  *            aligned rows (views too).
- *   q_weight, k_weight  [D], weight_dtype 0 = bf16, 1 = float32.
+ *   q_weight, k_weight  [D], weight_dtype 0 = bf16, 1 = float32, 16-byte
+ *            aligned.
  *   cos, sin float32 [table_rows][D / 2], 16-byte aligned.
  *   D        a multiple of 16, at most 512.
  *   q, k, v  [B, Hq | Hkv, T, D] views of the same dtype (out).

@@ -122,7 +122,7 @@ struct QkNormArgs {
   int pos0, max_pos;    // positions outside [0, max_pos) have no table / cache row
   int append;
   int B, T, Hq, Hkv, D;
-  int lp_log2;          // set by the launcher
+  int lp_log2, tokens_log2;  // set by the launcher
 };
 
 struct QkNormBwdArgs {
@@ -137,13 +137,12 @@ struct QkNormBwdArgs {
   const float* cos;
   const float* sin;
   int pos0;
-  float* part;          // [qk_norm_bwd_groups][D]
+  float* part;          // [2][qk_norm_bwd_groups][D]
   int B, T, Hq, Hkv, D;
-  int lp_log2, groups[3];  // set by the launcher
+  int lp_log2, tokens_log2;  // set by the launcher
 };
 
-int64_t qk_norm_items(int64_t B, int64_t T, int Hq, int Hkv, int D);  // threads of the forward
-int qk_norm_bwd_groups(int B, int T, int Hq, int Hkv, int D);
+int qk_norm_bwd_groups(int B, int T, int Hq, int D);
 hipError_t launch_qk_norm_rope(QkNormArgs a, bool f32, hipStream_t stream);
 hipError_t launch_qk_norm_rope_bwd(QkNormBwdArgs a, bool f32, void* dqw, void* dkw,
                                    hipStream_t stream);

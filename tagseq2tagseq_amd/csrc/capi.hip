@@ -579,13 +579,13 @@ int check_qk_norm(int32_t B, int32_t T, int32_t Hq, int32_t Hkv, int32_t D, int3
     return fail(T2T_EUNSUPPORTED, "dtype %d or weight dtype %d not supported here", dtype,
                 weight_dtype);
   if (!(eps >= 0.f && eps <= FLT_MAX)) return fail(T2T_EINVAL, "eps=%g", (double)eps);
-  if ((int64_t)B * T > 0x7fffffffLL ||
-      t2t::qk_norm_items(B, T, Hq, Hkv, D) > 0x7fffffffLL)
-    return fail(T2T_EUNSUPPORTED, "B=%d T=%d: more head rows than one launch numbers", B, T);
-  const uintptr_t wa = weight_dtype == T2T_DTYPE_F32 ? 4 : 2;
-  if (!q_weight || !k_weight || reinterpret_cast<uintptr_t>(q_weight) % wa ||
-      reinterpret_cast<uintptr_t>(k_weight) % wa)
-    return fail(T2T_EINVAL, "norm weights NULL or misaligned for their dtype");
+  // (with the tokens past the end that a last wave's lanes number)
+  if ((int64_t)B * T > 0x7fffffffLL - 64 || (int64_t)Hq + 2 * (int64_t)Hkv > 1 << 20)
+    return fail(T2T_EUNSUPPORTED, "B=%d T=%d Hq=%d Hkv=%d: more tokens or heads than one launch "
+                "numbers", B, T, Hq, Hkv);
+  if (!q_weight || !k_weight || reinterpret_cast<uintptr_t>(q_weight) % 16 ||
+      reinterpret_cast<uintptr_t>(k_weight) % 16)
+    return fail(T2T_EINVAL, "norm weights NULL or not 16-byte aligned");
   if (table_rows < 0) return fail(T2T_EINVAL, "negative table_rows");
   if (!need_rows) return T2T_OK;
   const int64_t align = dtype == T2T_DTYPE_F32 ? 4 : 8;
@@ -678,8 +678,8 @@ int t2t_qk_norm_rope_append(const void* qkv, int64_t stride_b, int64_t stride_t,
 
 int64_t t2t_qk_norm_rope_backward_workspace(int32_t B, int32_t T, int32_t Hq, int32_t Hkv,
                                             int32_t D) {
-  if (B <= 0 || T <= 0 || Hq < 1 || Hkv < 1 || D < 16 || D > 512 || D % 16 != 0) return 0;
-  return (int64_t)t2t::qk_norm_bwd_groups(B, T, Hq, Hkv, D) * D * 4;
+  if (B <= 0 || T <= 0 || Hq < 1 || Hq > 1 << 20 || Hkv < 1 || D < 16 || D > 512 || D % 16 != 0) return 0;
+  return 2 * (int64_t)t2t::qk_norm_bwd_groups(B, T, Hq, D) * D * 4;
 }
 
 int t2t_qk_norm_rope_backward(const t2t_tensor* dq, const t2t_tensor* dk, const t2t_tensor* dv,

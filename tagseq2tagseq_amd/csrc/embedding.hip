@@ -35,11 +35,10 @@ namespace {
 
 constexpr int kEmbThreads = 256;
 constexpr int kEmbItems = 4;
-constexpr int kSumBatch = 16;
 constexpr int kEmbedDirect = 4096;     // positions grouped without the split
 constexpr int kGroupThreads = 512;
 constexpr int kGroupWaves = kGroupThreads / 64;
-constexpr int kGroupSteps = 8;         // of 64 positions, loaded at once
+constexpr int kGroupSteps = 4;         // of 64 positions, loaded at once
 constexpr int kSplitItems = 4;         // positions a thread
 constexpr int kSplitBlock = kGroupThreads * kSplitItems;
 constexpr int kSumThreads = 256;
@@ -300,10 +299,11 @@ __global__ __launch_bounds__(kGroupThreads) void embed_group_kernel(EmbedGradArg
 }
 
 // A wave sums 64 VEC columns of a piece of S positions, lane l the columns
-// VEC l .. of the wave's block, kSumBatch positions' loads in flight at once.
+// VEC l .. of the wave's block, the loads of half a piece in flight at once.
 // The positions are the same for all lanes.
 template <typename T, int VEC, int S>
 __global__ __launch_bounds__(kSumThreads) void embed_sum_kernel(EmbedGradArgs a) {
+  constexpr int kSumBatch = S / 2;
   const int M = a.N, lane = threadIdx.x & 63;
   const int blocks = (a.C + 64 * VEC - 1) / (64 * VEC);
   const int item = __builtin_amdgcn_readfirstlane(
@@ -319,9 +319,8 @@ __global__ __launch_bounds__(kSumThreads) void embed_sum_kernel(EmbedGradArgs a)
   const int before = e0 ? list[-1].y : -2, after = e0 + n < M ? list[n].y : -2;
   float acc[VEC] = {};
   bool from_before = list[0].y == before;
-#pragma unroll
-  for (int b = 0; b < S; b += kSumBatch) {
-    if (b >= n) break;
+#pragma unroll 1  // (unrolled, most of a short list's time went into fetching code)
+  for (int b = 0; b < n; b += kSumBatch) {
     // (positions behind the piece's end: its last one again, unused)
     int token[kSumBatch];
     Pack<T, VEC> d[kSumBatch];
@@ -506,16 +505,10 @@ hipError_t launch_grad_t(const EmbedGradArgs& a, bool vector, hipStream_t stream
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || a.N == 0) return e;
   const int64_t pieces = ((int64_t)a.N + a.piece - 1) / a.piece;
-  // Columns a lane: 16 bytes, or half where that leaves fewer lanes idle (768
-  // columns of bf16: three waves of 256 instead of one and a half of 512).
-  constexpr int kWide = 16 / sizeof(T), kHalf = kWide / 2;
-  const auto covered = [&](int vec) { return (a.C + 64 * vec - 1) / (64 * vec) * vec; };
-  if (!vector)
-    e = launch_sum_piece<T, 1>(a, pieces, stream);
-  else if (covered(kHalf) < covered(kWide))
-    e = launch_sum_piece<T, kHalf>(a, pieces, stream);
-  else
-    e = launch_sum_piece<T, kWide>(a, pieces, stream);
+  // 16 bytes a lane, also where 768 columns leave half of every second wave idle
+  // (131072 positions: 59 us; lanes of 8 bytes, all of them busy, 75 us)
+  e = vector ? launch_sum_piece<T, 16 / (int)sizeof(T)>(a, pieces, stream)
+             : launch_sum_piece<T, 1>(a, pieces, stream);
   if (e != hipSuccess || pieces < 2) return e;
   return vector ? launch_join<T, 4>(a, pieces, stream) : launch_join<T, 1>(a, pieces, stream);
 }

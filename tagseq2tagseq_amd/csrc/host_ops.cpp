@@ -269,8 +269,8 @@ struct QkNorm {
     code = qkv_in.scalar_type() == at::kFloat ? T2T_DTYPE_F32 : T2T_DTYPE_BF16;
     wcode = weight_code(qw_in);
     qkv = vector_rows(qkv_in);
-    qw = qw_in.contiguous();
-    kw = kw_in.contiguous();
+    qw = vector_rows(qw_in.contiguous());
+    kw = vector_rows(kw_in.contiguous());
     cos = vector_rows(cos_in.contiguous());
     sin = vector_rows(sin_in.contiguous());
     B = qkv.size(0);

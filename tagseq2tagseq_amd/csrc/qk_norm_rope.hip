@@ -17,7 +17,11 @@
 // reads the three gradients and the query and key part of the row, and writes
 // the row's gradient.  A group of LP lanes (D / 16 rounded up to a power of
 // two) holds a head row, lane j the values 8j .. 8j + 7 of both halves, so the
-// rotation pairs sit in one lane and the mean is log2 LP shuffles.
+// rotation pairs sit in one lane and the mean is log2 LP shuffles.  A wave takes
+// whole tokens -- one, or as many as its groups hold the query heads of --
+// and their query, key and value heads one after the other, so that the lanes
+// load a token's angles once for all heads (one head row a group, whatever its
+// token, read them with every row: 16384 tokens of 36 heads of 64, 48 us).
 #include "attn_kernels.h"
 
 namespace t2t {
@@ -26,18 +30,32 @@ namespace {
 
 constexpr int kQkThreads = 256;
 constexpr int kQkWaves = kQkThreads / 64;
+constexpr int kBwdThreads = 256;
+constexpr int kBwdWaves = kBwdThreads / 64;
+constexpr int kBwdGroups = 768;  // work-groups of the backward: three on each CU
 
-__device__ __forceinline__ void load8(const __bf16* p, float (&x)[8]) {
-  const bf16x8 v = *reinterpret_cast<const bf16x8*>(p);
+// Eight values as they are stored.
+struct Raw16 { bf16x8 v; };
+struct Raw32 { float4 a, b; };
+__device__ __forceinline__ Raw16 raw8(const __bf16* p) {
+  return {*reinterpret_cast<const bf16x8*>(p)};
+}
+__device__ __forceinline__ Raw32 raw8(const float* p) {
+  return {reinterpret_cast<const float4*>(p)[0], reinterpret_cast<const float4*>(p)[1]};
+}
+__device__ __forceinline__ void values(const Raw16& r, float (&x)[8]) {
 #pragma unroll
-  for (int e = 0; e < 8; ++e) x[e] = (float)v[e];
+  for (int e = 0; e < 8; ++e) x[e] = (float)r.v[e];
 }
+__device__ __forceinline__ void values(const Raw32& r, float (&x)[8]) {
+  x[0] = r.a.x; x[1] = r.a.y; x[2] = r.a.z; x[3] = r.a.w;
+  x[4] = r.b.x; x[5] = r.b.y; x[6] = r.b.z; x[7] = r.b.w;
+}
+template <typename T>
+using RawOf = decltype(raw8(static_cast<const T*>(nullptr)));
 
-__device__ __forceinline__ void load8(const float* p, float (&x)[8]) {
-  const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-  x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
-  x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-}
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, float (&x)[8]) { values(raw8(p), x); }
 
 __device__ __forceinline__ void store8(__bf16* p, const float (&x)[8]) {
   bf16x8 v;
@@ -51,11 +69,11 @@ __device__ __forceinline__ void store8(float* p, const float (&x)[8]) {
   reinterpret_cast<float4*>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
 }
 
-// Norm weights have any alignment that their type has.
 __device__ __forceinline__ void load_weight8(const void* w, bool f32, int i, float (&out)[8]) {
-#pragma unroll
-  for (int e = 0; e < 8; ++e)
-    out[e] = f32 ? static_cast<const float*>(w)[i + e] : (float)static_cast<const __bf16*>(w)[i + e];
+  if (f32)
+    load8(static_cast<const float*>(w) + i, out);
+  else
+    load8(static_cast<const __bf16*>(w) + i, out);
 }
 
 __device__ __forceinline__ float group_sum(float x, int LP) {
@@ -63,198 +81,246 @@ __device__ __forceinline__ float group_sum(float x, int LP) {
   return x;
 }
 
-// One group of LP lanes per (token, head); heads are the Hq query, Hkv key
-// and Hkv value heads of the packed row, in that order.
+// A lane's place in a wave that works on `tokens` tokens: the token among
+// them, the first head of its group, how many heads further the next one is.
+struct Place {
+  int token, head, step, j8, half;
+  bool in;  // the lane has columns
+  __device__ Place(int lp_log2, int tokens_log2, int D) {
+    const int lane = threadIdx.x & 63, group = lane >> lp_log2;
+    const int per = 6 - lp_log2 - tokens_log2;  // log2 of the groups a token
+    token = group >> per;
+    head = group & ((1 << per) - 1);
+    step = 1 << per;
+    half = D >> 1;
+    j8 = 8 * (lane & ((1 << lp_log2) - 1));
+    in = j8 < half;
+  }
+};
+
 template <typename T>
 __global__ __launch_bounds__(kQkThreads) void qk_norm_rope_kernel(QkNormArgs a) {
-  const uint32_t item = blockIdx.x * kQkThreads + threadIdx.x;
-  const uint32_t heads = a.Hq + 2 * a.Hkv;
-  const uint32_t row = item >> a.lp_log2;
-  const uint32_t n = row / heads;
-  if (n >= (uint32_t)(a.B * a.T)) return;  // whole groups: the shuffles below stay within one
-  const int head = row - n * heads;
-  const int b = n / (uint32_t)a.T, t = n - b * a.T;
-  const int LP = 1 << a.lp_log2, half = a.D >> 1;
-  const int j8 = 8 * (item & (LP - 1));
-  const bool in = j8 < half;
+  const Place at(a.lp_log2, a.tokens_log2, a.D);
+  const int LP = 1 << a.lp_log2, half = at.half, j8 = at.j8;
+  const int64_t tokens = (int64_t)a.B * a.T, stride = (int64_t)gridDim.x * kQkWaves << a.tokens_log2;
+  int64_t n0 = ((int64_t)blockIdx.x * kQkWaves + (threadIdx.x >> 6)) << a.tokens_log2;
+  for (; n0 < tokens; n0 += stride) {
+    const uint32_t n = (uint32_t)n0 + at.token;  // (at most 2^31 tokens)
+    const bool ok = at.in && n < tokens;
+    const int b = n / (uint32_t)a.T, t = n - b * a.T;
+    const T* src = static_cast<const T*>(a.packed) + b * a.p_sb + (int64_t)t * a.p_st + j8;
 
-  // The position, its cache row where there is a cache, and whether a row of
-  // the same position follows (the later one is kept).
-  int64_t p = a.pos0 + t;
-  bool stored = true;
-  if (a.pos) {
-    const int64_t* pos = a.pos + b * a.pos_sb;
-    p = pos[t];
-    for (int u = t + 1; u < a.T; ++u) stored = stored && pos[u] != p;
-  }
-  const bool known = p >= 0 && p < a.max_pos;
-
-  const int which = head < a.Hq ? 0 : (head < a.Hq + a.Hkv ? 1 : 2);
-  const int h = which == 0 ? head : (which == 1 ? head - a.Hq : head - a.Hq - a.Hkv);
-  const T* src = static_cast<const T*>(a.packed) + b * a.p_sb + (int64_t)t * a.p_st +
-                 (int64_t)head * a.D + j8;
-  float x1[8] = {}, x2[8] = {};
-  if (in) {
-    load8(src, x1);
-    load8(src + half, x2);
-  }
-  if (which < 2) {
-    float w1[8] = {}, w2[8] = {}, c[8] = {}, s[8] = {};
-    if (in) {
-      const void* w = which ? a.kw : a.qw;
-      load_weight8(w, a.w_f32, j8, w1);
-      load_weight8(w, a.w_f32, half + j8, w2);
-      if (known) {
-        load8(a.cos + p * half + j8, c);
-        load8(a.sin + p * half + j8, s);
+    // The first head row of each kind: all loads in flight at once.
+    const int heads[3] = {a.Hq, a.Hkv, a.Hkv};
+    RawOf<T> r1[3] = {}, r2[3] = {};
+    float c[8] = {}, s[8] = {};
+    int first = 0;
+#pragma unroll
+    for (int w = 0; w < 3; ++w) {
+      if (ok && at.head < heads[w]) {
+        const T* row = src + (int64_t)(first + at.head) * a.D;
+        r1[w] = raw8(row);
+        r2[w] = raw8(row + half);
       }
+      first += heads[w];
     }
-    float ss = 0.f;
+    // The position, and whether a row of the same position follows (the later
+    // one is kept).
+    int64_t p = a.pos0 + t;
+    bool stored = true;
+    if (a.pos && ok) {
+      const int64_t* pos = a.pos + b * a.pos_sb;
+      p = pos[t];
+      for (int u = t + 1; u < a.T; ++u) stored = stored && pos[u] != p;
+    }
+    const bool known = p >= 0 && p < a.max_pos;
+    if (ok && known) {
+      load8(a.cos + p * half + j8, c);
+      load8(a.sin + p * half + j8, s);
+    }
+    first = 0;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) ss = fmaf(x1[e], x1[e], fmaf(x2[e], x2[e], ss));
-    const float r = rsqrtf(group_sum(ss, LP) / (float)a.D + a.eps);
+    for (int w = 0; w < 3; ++w) {
+      float w1[8] = {}, w2[8] = {};
+      if (w < 2 && at.in) {
+        load_weight8(w ? a.kw : a.qw, a.w_f32, j8, w1);
+        load_weight8(w ? a.kw : a.qw, a.w_f32, half + j8, w2);
+      }
+      for (int h0 = 0; h0 < heads[w]; h0 += at.step) {
+        const int h = h0 + at.head;
+        const bool row_ok = ok && h < heads[w];
+        if (h0) {
+          r1[w] = r2[w] = RawOf<T>{};
+          if (row_ok) {
+            const T* row = src + (int64_t)(first + h) * a.D;
+            r1[w] = raw8(row);
+            r2[w] = raw8(row + half);
+          }
+        }
+        float x1[8], x2[8];
+        values(r1[w], x1);
+        values(r2[w], x2);
+        if (w < 2) {
+          float ss = 0.f;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float y1 = x1[e] * r * w1[e], y2 = x2[e] * r * w2[e];
-      x1[e] = fmaf(y1, c[e], y2 * s[e]);
-      x2[e] = fmaf(y2, c[e], -(y1 * s[e]));
+          for (int e = 0; e < 8; ++e) ss = fmaf(x1[e], x1[e], fmaf(x2[e], x2[e], ss));
+          const float r = rsqrtf(group_sum(ss, LP) / (float)a.D + a.eps);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float y1 = x1[e] * r * w1[e], y2 = x2[e] * r * w2[e];
+            x1[e] = fmaf(y1, c[e], y2 * s[e]);
+            x2[e] = fmaf(y2, c[e], -(y1 * s[e]));
+          }
+        }
+        if (!row_ok) continue;
+        int64_t to = t;
+        if (a.append) {
+          if (!known) {  // no table row: a query of zeros, nothing into the cache
+            if (w) continue;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x1[e] = x2[e] = 0.f;
+          } else if (w) {
+            if (!stored) continue;
+            to = p;
+          }
+        }
+        const TensorView& o = a.ops[w];
+        T* dst = static_cast<T*>(o.data) + b * o.sb + h * o.sh + to * o.st + j8;
+        store8(dst, x1);
+        store8(dst + half, x2);
+      }
+      first += heads[w];
     }
   }
-  if (!in) return;
-  const TensorView& o = a.ops[which];
-  int64_t at = t;
-  if (a.append) {
-    if (!known) {  // no table row: a query of zeros, nothing into the cache
-      if (which) return;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) x1[e] = x2[e] = 0.f;
-    } else if (which) {
-      if (!stored) return;
-      at = p;
-    }
-  }
-  T* dst = static_cast<T*>(o.data) + b * o.sb + h * o.sh + at * o.st + j8;
-  store8(dst, x1);
-  store8(dst + half, x2);
 }
 
-// Each work-group takes rounds of kQkThreads / LP rows of one kind (query, key
-// or value heads, by block index), so that a lane holds the same columns
-// throughout and its share of dw stays in registers; per work-group the shares
-// are summed by shuffles and through LDS into part[group][D].
+// A lane holds the same columns throughout, so its shares of the two dw stay in
+// registers; per work-group they are summed by shuffles and through LDS into
+// part[2][group][D].
 template <typename T>
-__global__ __launch_bounds__(kQkThreads) void qk_norm_rope_bwd_kernel(QkNormBwdArgs a) {
-  __shared__ float red[kQkWaves][2 * 256];
-  int which = 0;
-  uint32_t group = blockIdx.x;
-  while (group >= (uint32_t)a.groups[which]) group -= a.groups[which++];
-  const uint32_t H = which ? a.Hkv : a.Hq;
-  const int head0 = which == 0 ? 0 : (which == 1 ? a.Hq : a.Hq + a.Hkv);
-  const int LP = 1 << a.lp_log2, half = a.D >> 1;
-  const int j8 = 8 * (threadIdx.x & (LP - 1));
-  const bool in = j8 < half;
-  const uint32_t rows = (uint32_t)a.B * a.T * H, per = kQkThreads >> a.lp_log2;
-  const TensorView& g = a.ops[which];
-
-  float w1[8] = {}, w2[8] = {}, acc1[8] = {}, acc2[8] = {};
-  if (in && which < 2) {
-    load_weight8(which ? a.kw : a.qw, a.w_f32, j8, w1);
-    load_weight8(which ? a.kw : a.qw, a.w_f32, half + j8, w2);
-  }
-  for (uint32_t r0 = group * per; r0 < rows; r0 += a.groups[which] * per) {
-    const uint32_t row = r0 + (threadIdx.x >> a.lp_log2);
-    const bool ok = in && row < rows;
-    const uint32_t n = row / H, h = row - n * H;
+__global__ __launch_bounds__(kBwdThreads, 3) void qk_norm_rope_bwd_kernel(QkNormBwdArgs a) {
+  __shared__ float red[kBwdWaves][2 * 256];
+  const Place at(a.lp_log2, a.tokens_log2, a.D);
+  const int LP = 1 << a.lp_log2, half = at.half, j8 = at.j8, wave = threadIdx.x >> 6;
+  const int all_heads = a.Hq + 2 * a.Hkv;
+  const int64_t tokens = (int64_t)a.B * a.T;
+  const int64_t stride = (int64_t)gridDim.x * kBwdWaves << a.tokens_log2;
+  float acc1[2][8] = {}, acc2[2][8] = {};
+  for (int64_t n0 = ((int64_t)blockIdx.x * kBwdWaves + wave) << a.tokens_log2; n0 < tokens;
+       n0 += stride) {
+    const uint32_t n = (uint32_t)n0 + at.token;
+    const bool ok = at.in && n < tokens;
     const int b = n / (uint32_t)a.T, t = n - b * a.T;
-    float d1[8] = {}, d2[8] = {}, x1[8] = {}, x2[8] = {}, c[8] = {}, s[8] = {};
-    const int64_t at = b * a.p_sb + (int64_t)t * a.p_st + (int64_t)(head0 + h) * a.D + j8;
-    const int64_t to =
-        ((int64_t)n * (a.Hq + 2 * a.Hkv) + head0 + h) * a.D + j8;
+    const T* src = static_cast<const T*>(a.packed) + b * a.p_sb + (int64_t)t * a.p_st + j8;
+    T* out = static_cast<T*>(a.dpacked) + (int64_t)n * all_heads * a.D + j8;
+    float c[8] = {}, s[8] = {};
     if (ok) {
-      const T* src = static_cast<const T*>(g.data) + b * g.sb + h * g.sh + (int64_t)t * g.st + j8;
-      load8(src, d1);
-      load8(src + half, d2);
+      load8(a.cos + (int64_t)(a.pos0 + t) * half + j8, c);
+      load8(a.sin + (int64_t)(a.pos0 + t) * half + j8, s);
     }
-    if (which < 2) {
-      if (ok) {
-        const T* x = static_cast<const T*>(a.packed) + at;
-        load8(x, x1);
-        load8(x + half, x2);
-        load8(a.cos + (int64_t)(a.pos0 + t) * half + j8, c);
-        load8(a.sin + (int64_t)(a.pos0 + t) * half + j8, s);
-      }
-      float ss = 0.f, dot = 0.f;
+    int first = 0;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float y1 = fmaf(d1[e], c[e], -(d2[e] * s[e]));
-        const float y2 = fmaf(d2[e], c[e], d1[e] * s[e]);
-        d1[e] = y1;
-        d2[e] = y2;
-        ss = fmaf(x1[e], x1[e], fmaf(x2[e], x2[e], ss));
-        dot = fmaf(y1 * w1[e], x1[e], fmaf(y2 * w2[e], x2[e], dot));
+    for (int w = 0; w < 3; ++w) {
+      const int H = w ? a.Hkv : a.Hq;
+      const TensorView& g = a.ops[w];
+      float w1[8] = {}, w2[8] = {};
+      if (w < 2 && at.in) {
+        load_weight8(w ? a.kw : a.qw, a.w_f32, j8, w1);
+        load_weight8(w ? a.kw : a.qw, a.w_f32, half + j8, w2);
       }
-      ss = group_sum(ss, LP);
-      dot = group_sum(dot, LP);
-      const float r = rsqrtf(ss / (float)a.D + a.eps);
-      const float m = dot * r / (float)a.D;  // mean(g n)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float n1 = x1[e] * r, n2 = x2[e] * r;
-        if (ok) {
-          acc1[e] = fmaf(d1[e], n1, acc1[e]);
-          acc2[e] = fmaf(d2[e], n2, acc2[e]);
+      for (int h0 = 0; h0 < H; h0 += at.step) {
+        const int h = h0 + at.head;
+        const bool row_ok = ok && h < H;
+        const int64_t col = (int64_t)(first + h) * a.D;
+        float d1[8] = {}, d2[8] = {};
+        if (row_ok) {
+          const T* d =
+              static_cast<const T*>(g.data) + b * g.sb + h * g.sh + (int64_t)t * g.st + j8;
+          load8(d, d1);
+          load8(d + half, d2);
         }
-        d1[e] = r * (d1[e] * w1[e] - n1 * m);
-        d2[e] = r * (d2[e] * w2[e] - n2 * m);
+        if (w < 2) {
+          float x1[8] = {}, x2[8] = {};
+          if (row_ok) {
+            load8(src + col, x1);
+            load8(src + col + half, x2);
+          }
+          float ss = 0.f, dot = 0.f;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float y1 = fmaf(d1[e], c[e], -(d2[e] * s[e]));
+            const float y2 = fmaf(d2[e], c[e], d1[e] * s[e]);
+            d1[e] = y1;
+            d2[e] = y2;
+            ss = fmaf(x1[e], x1[e], fmaf(x2[e], x2[e], ss));
+            dot = fmaf(y1 * w1[e], x1[e], fmaf(y2 * w2[e], x2[e], dot));
+          }
+          ss = group_sum(ss, LP);
+          dot = group_sum(dot, LP);
+          const float r = rsqrtf(ss / (float)a.D + a.eps);
+          const float m = dot * r / (float)a.D;  // mean(g n)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float n1 = x1[e] * r, n2 = x2[e] * r;
+            if (row_ok) {  // (0 times the r of no row is not a number at eps = 0)
+              acc1[w & 1][e] = fmaf(d1[e], n1, acc1[w & 1][e]);
+              acc2[w & 1][e] = fmaf(d2[e], n2, acc2[w & 1][e]);
+            }
+            d1[e] = r * (d1[e] * w1[e] - n1 * m);
+            d2[e] = r * (d2[e] * w2[e] - n2 * m);
+          }
+        }
+        if (row_ok) {
+          store8(out + col, d1);
+          store8(out + col + half, d2);
+        }
+      }
+      first += H;
+    }
+  }
+  // The lanes with the same columns: 64 / LP in a wave, then the waves.
+#pragma unroll
+  for (int w = 0; w < 2; ++w) {
+    for (int off = LP; off < 64; off <<= 1) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        acc1[w][e] += __shfl_xor(acc1[w][e], off, 64);
+        acc2[w][e] += __shfl_xor(acc2[w][e], off, 64);
       }
     }
-    if (ok) {
-      T* dst = static_cast<T*>(a.dpacked) + to;
-      store8(dst, d1);
-      store8(dst + half, d2);
-    }
-  }
-  if (which == 2) return;
-  // The lanes with the same columns: 64 / LP in a wave, then the waves.
-  for (int off = LP; off < 64; off <<= 1) {
+    if ((threadIdx.x & 63) < LP && at.in) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      acc1[e] += __shfl_xor(acc1[e], off, 64);
-      acc2[e] += __shfl_xor(acc2[e], off, 64);
+      for (int e = 0; e < 8; ++e) {
+        red[wave][j8 + e] = acc1[w][e];
+        red[wave][half + j8 + e] = acc2[w][e];
+      }
     }
-  }
-  const int wave = threadIdx.x >> 6;
-  if ((threadIdx.x & 63) < LP && in) {
+    __syncthreads();
+    float* part = a.part + ((int64_t)w * gridDim.x + blockIdx.x) * a.D;
+    for (int i = threadIdx.x; i < a.D; i += kBwdThreads) {
+      float sum = 0.f;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      red[wave][j8 + e] = acc1[e];
-      red[wave][half + j8 + e] = acc2[e];
+      for (int v = 0; v < kBwdWaves; ++v) sum += red[v][i];
+      part[i] = sum;
     }
-  }
-  __syncthreads();
-  float* part = a.part + ((int64_t)(which ? a.groups[0] : 0) + group) * a.D;
-  for (int i = threadIdx.x; i < a.D; i += kQkThreads) {
-    float sum = 0.f;
-#pragma unroll
-    for (int v = 0; v < kQkWaves; ++v) sum += red[v][i];
-    part[i] = sum;
+    __syncthreads();
   }
 }
 
 // dw[i] = sum over the work-groups of their shares, in a fixed order: 16 waves
 // per 64 columns, wave s summing groups s, s + 16, ..., then the waves.
 constexpr int kDwWaves = 16;
-__global__ __launch_bounds__(64 * kDwWaves) void qk_norm_dw_kernel(const float* part, int nq,
-                                                                   int nk, int D, void* dqw,
-                                                                   void* dkw, bool w_f32) {
+__global__ __launch_bounds__(64 * kDwWaves) void qk_norm_dw_kernel(const float* part, int groups,
+                                                                   int D, void* dqw, void* dkw,
+                                                                   bool w_f32) {
   __shared__ float red[kDwWaves][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int col = blockIdx.x * 64 + lane;
-  const int first = blockIdx.y ? nq : 0, count = blockIdx.y ? nk : nq;
+  const int first = blockIdx.y ? groups : 0;
   float sum = 0.f;
   if (col < D) {
 #pragma unroll 8
-    for (int g = wave; g < count; g += kDwWaves) sum += part[(int64_t)(first + g) * D + col];
+    for (int g = wave; g < groups; g += kDwWaves) sum += part[(int64_t)(first + g) * D + col];
   }
   red[wave][lane] = sum;
   __syncthreads();
@@ -275,29 +341,31 @@ int lanes_log2(int D) {
   return l;
 }
 
-// Work-groups for `rows` head rows: four rounds each, at most 1024.
-int groups_of(int64_t rows, int lp_log2) {
-  const int64_t per = kQkThreads >> lp_log2;
-  const int64_t n = (rows + 4 * per - 1) / (4 * per);
-  return (int)(n < 1024 ? n : 1024);
+// log2 of the tokens a wave takes: as many as its groups hold the query heads of.
+int tokens_log2(int lp_log2, int Hq) {
+  int l = 0;
+  while ((Hq << lp_log2 << (l + 1)) <= 64) ++l;
+  return l;
+}
+
+// Waves for all tokens, in work-groups of `waves`, at most `most` of these.
+int groups_of(int64_t tokens, int tokens_log2, int waves, int most) {
+  const int64_t per = (int64_t)waves << tokens_log2, n = (tokens + per - 1) / per;
+  return (int)(n < most ? n : most);
 }
 
 }  // namespace
 
-int64_t qk_norm_items(int64_t B, int64_t T, int Hq, int Hkv, int D) {
-  return (B * T * (Hq + 2 * (int64_t)Hkv)) << lanes_log2(D);
-}
-
-int qk_norm_bwd_groups(int B, int T, int Hq, int Hkv, int D) {
-  const int l = lanes_log2(D);
-  return groups_of((int64_t)B * T * Hq, l) + groups_of((int64_t)B * T * Hkv, l);
+int qk_norm_bwd_groups(int B, int T, int Hq, int D) {
+  return groups_of((int64_t)B * T, tokens_log2(lanes_log2(D), Hq), kBwdWaves, kBwdGroups);
 }
 
 hipError_t launch_qk_norm_rope(QkNormArgs a, bool f32, hipStream_t stream) {
   a.lp_log2 = lanes_log2(a.D);
-  const int64_t items = qk_norm_items(a.B, a.T, a.Hq, a.Hkv, a.D);
-  if (items == 0) return hipSuccess;
-  const dim3 grid((unsigned)((items + kQkThreads - 1) / kQkThreads));
+  a.tokens_log2 = tokens_log2(a.lp_log2, a.Hq);
+  const int64_t tokens = (int64_t)a.B * a.T;
+  if (tokens == 0) return hipSuccess;
+  const dim3 grid((unsigned)groups_of(tokens, a.tokens_log2, kQkWaves, 1 << 20));
   if (f32)
     hipLaunchKernelGGL(qk_norm_rope_kernel<float>, grid, dim3(kQkThreads), 0, stream, a);
   else
@@ -308,22 +376,20 @@ hipError_t launch_qk_norm_rope(QkNormArgs a, bool f32, hipStream_t stream) {
 hipError_t launch_qk_norm_rope_bwd(QkNormBwdArgs a, bool f32, void* dqw, void* dkw,
                                    hipStream_t stream) {
   a.lp_log2 = lanes_log2(a.D);
-  const int64_t n = (int64_t)a.B * a.T;
-  a.groups[0] = groups_of(n * a.Hq, a.lp_log2);
-  a.groups[1] = groups_of(n * a.Hkv, a.lp_log2);
-  a.groups[2] = a.groups[1];
-  const int total = a.groups[0] + 2 * a.groups[1];
-  if (total) {
+  a.tokens_log2 = tokens_log2(a.lp_log2, a.Hq);
+  const int groups = qk_norm_bwd_groups(a.B, a.T, a.Hq, a.D);
+  if (groups) {
     if (f32)
-      hipLaunchKernelGGL(qk_norm_rope_bwd_kernel<float>, dim3(total), dim3(kQkThreads), 0, stream, a);
-    else
-      hipLaunchKernelGGL(qk_norm_rope_bwd_kernel<__bf16>, dim3(total), dim3(kQkThreads), 0, stream,
+      hipLaunchKernelGGL(qk_norm_rope_bwd_kernel<float>, dim3(groups), dim3(kBwdThreads), 0, stream,
                          a);
+    else
+      hipLaunchKernelGGL(qk_norm_rope_bwd_kernel<__bf16>, dim3(groups), dim3(kBwdThreads), 0,
+                         stream, a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
   hipLaunchKernelGGL(qk_norm_dw_kernel, dim3((unsigned)((a.D + 63) / 64), 2), dim3(64 * kDwWaves),
-                     0, stream, a.part, a.groups[0], a.groups[1], a.D, dqw, dkw, a.w_f32);
+                     0, stream, a.part, groups, a.D, dqw, dkw, a.w_f32);
   return hipGetLastError();
 }
 

@@ -40,9 +40,10 @@ def _forward(**kw):
     (dict(dtype=2), -2, "dtype"), (dict(wdt=7), -2, "dtype"),
     (dict(eps=-1e-6), -1, "eps"), (dict(eps=float("nan")), -1, "eps"),
     (dict(eps=float("inf")), -1, "eps"),
-    (dict(B=1 << 20, T=1 << 20), -2, "more head rows"),
-    (dict(T=1 << 30, rows=2 ** 31 - 1), -2, "more head rows"),
-    (dict(qw=None), -1, "norm weights"), (dict(kw=ctypes.c_void_p(0x1001)), -1, "norm weights"),
+    (dict(B=1 << 20, T=1 << 20), -2, "more tokens"),
+    (dict(B=2, T=1 << 30, rows=2 ** 31 - 1), -2, "more tokens"),
+    (dict(Hq=1 << 20, st=1 << 30), -2, "more tokens or heads"),
+    (dict(qw=None), -1, "norm weights"), (dict(kw=ctypes.c_void_p(0x1008)), -1, "norm weights"),
     (dict(qkv=None), -1, "16-byte"), (dict(qkv=ctypes.c_void_p(0x1008)), -1, "16-byte"),
     (dict(st=257), -1, "16-byte"), (dict(sb=-8), -1, "16-byte"),
     (dict(cos=None), -1, "cos"), (dict(sin=ctypes.c_void_p(0x1004)), -1, "cos"),
@@ -103,7 +104,7 @@ def test_workspace_sizes():
     ws = _lib.lib().t2t_qk_norm_rope_backward_workspace
     assert ws(0, 5, 2, 2, 64) == ws(1, 5, 2, 2, 20) == ws(1, 5, 0, 2, 64) == 0
     assert ws(1, 1, 1, 1, 64) == 2 * 64 * 4
-    assert ws(8, 1 << 20, 16, 16, 128) == 2 * 1024 * 128 * 4  # bounded
+    assert ws(8, 1 << 20, 16, 16, 128) == 2 * 768 * 128 * 4  # bounded
 
 
 def _cpu(H=2, Hkv=2, D=64, dt=torch.bfloat16, T=3):
