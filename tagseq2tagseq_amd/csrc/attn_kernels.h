@@ -137,12 +137,12 @@ struct QkNormBwdArgs {
   const float* cos;
   const float* sin;
   int pos0;
-  float* part;          // [2][qk_norm_bwd_groups][D]
+  float* part;          // [qk_norm_bwd_groups][D]
   int B, T, Hq, Hkv, D;
-  int lp_log2, tokens_log2;  // set by the launcher
+  int lp_log2, groups[3];  // set by the launcher
 };
 
-int qk_norm_bwd_groups(int B, int T, int Hq, int D);
+int qk_norm_bwd_groups(int B, int T, int Hq, int Hkv, int D);
 hipError_t launch_qk_norm_rope(QkNormArgs a, bool f32, hipStream_t stream);
 hipError_t launch_qk_norm_rope_bwd(QkNormBwdArgs a, bool f32, void* dqw, void* dkw,
                                    hipStream_t stream);

@@ -678,8 +678,8 @@ int t2t_qk_norm_rope_append(const void* qkv, int64_t stride_b, int64_t stride_t,
 
 int64_t t2t_qk_norm_rope_backward_workspace(int32_t B, int32_t T, int32_t Hq, int32_t Hkv,
                                             int32_t D) {
-  if (B <= 0 || T <= 0 || Hq < 1 || Hq > 1 << 20 || Hkv < 1 || D < 16 || D > 512 || D % 16 != 0) return 0;
-  return 2 * (int64_t)t2t::qk_norm_bwd_groups(B, T, Hq, D) * D * 4;
+  if (B <= 0 || T <= 0 || Hq < 1 || Hkv < 1 || D < 16 || D > 512 || D % 16 != 0) return 0;
+  return (int64_t)t2t::qk_norm_bwd_groups(B, T, Hq, Hkv, D) * D * 4;
 }
 
 int t2t_qk_norm_rope_backward(const t2t_tensor* dq, const t2t_tensor* dk, const t2t_tensor* dv,

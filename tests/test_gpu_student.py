@@ -1,0 +1,221 @@
+"""The operators that distilling and serving a student model adds, run
+together as a user runs them: a training step of TS2TSTrainingModule (scaled
+embedding, layers with query / key norms, distillation loss) and cached
+generation of TS2TSModel with the same weights.
+
+Both are compared with the same model written in plain torch operations in 64
+bits.  The loss and gradients of a bf16 model carry the roundings of every
+layer's activations: each tensor that is stored rounds by half a step, 2^-8 of
+itself at most and 2^-9.8 in the mean square; with about 12 stored activations
+a layer and 3 layers, adding up as independent errors, a relative error of
+sqrt(36) 2^-9.8 < 0.7 % reaches the logits, and the backward, with as many
+roundings again on top of it, 1 %.  The bounds below are 3 times that for whole
+tensors (2-norms), 3 %.  The float32 model has 2^-16 of those errors; its
+bound, 1e-4, is the float32 attention's own.
+"""
+import math
+
+import pytest
+import torch
+
+from tagseq2tagseq_amd import synth
+from tagseq2tagseq_amd.mask_creators import create_doc_causal_block_mask
+from tagseq2tagseq_amd.model import TS2TSModel
+from tagseq2tagseq_amd.modules import TS2TSTrainingModule
+
+pytestmark = pytest.mark.gpu
+
+DEV = torch.device("cuda:0")
+V, C, H, LAYERS, T, K = 515, 256, 4, 3, 192, 6
+SCALE, TAU, ALPHA = math.sqrt(C), 2.0, 0.5
+IGNORE = -100
+SPANS = [synth.DocSpan(doc_id=7, start=0, end=70), synth.DocSpan(doc_id=3, start=70, end=T)]
+
+
+def _student(dtype, seed=0):
+    torch.manual_seed(seed)
+    m = TS2TSTrainingModule.from_config(
+        vocab_size=V, num_layers=LAYERS, model_dim=C, num_heads=H, max_seq_len=256, dropout=0.0,
+        drop_path_rate=0.0, block_mask_creator=create_doc_causal_block_mask, qk_norm=True,
+        embedding_scale=SCALE, distill_alpha=ALPHA, distill_temperature=TAU)
+    with torch.no_grad():
+        m.embedding.weight.mul_(C ** -0.5)
+        for layer in m.backbone.layers:
+            for w in (layer.attn.q_norm, layer.attn.k_norm):
+                w.add_(0.2 * torch.randn_like(w))
+    return m.to(DEV, dtype)
+
+
+def _batch(seed=0):
+    g = torch.Generator().manual_seed(seed)
+    tokens = torch.randint(0, V, (1, T + 1), generator=g)
+    idx = torch.stack([torch.randperm(V, generator=g)[:K] for _ in range(T)])[None]
+    idx[0, ::5, 3:] = -1
+    top = 4 * torch.randn(1, T, K, generator=g)
+    return dict(tokens=tokens.to(DEV), doc_spans=SPANS, teacher_idx=idx.to(DEV),
+                teacher_logits=top.to(DEV))
+
+
+# ---- the model in 64 bits
+
+def _rms(x, w):
+    return x / torch.sqrt((x * x).mean(-1, keepdim=True) + 1e-6) * w
+
+
+def _logits(p, ids):
+    """Logits [T, V] from parameters p (float64, by name) of one sequence."""
+    n = ids.shape[0]
+    doc = torch.empty(n, dtype=torch.int64, device=DEV)
+    for s in SPANS:
+        doc[s.start:min(s.end, n)] = s.doc_id
+    mask = (doc[:, None] == doc[None]).tril()
+    D = C // H
+    inv = 10000.0 ** (-torch.arange(D // 2, dtype=torch.float64, device=DEV) / (D // 2))
+    ang = torch.arange(n, dtype=torch.float64, device=DEV)[:, None] * inv
+    cos, sin = ang.cos(), ang.sin()
+
+    def turn(x):
+        a, b = x[..., :D // 2], x[..., D // 2:]
+        return torch.cat((a * cos + b * sin, b * cos - a * sin), -1)
+
+    x = p["embedding.weight"][ids] * SCALE
+    skips, n_skip = [], LAYERS // 2
+    for i in range(LAYERS):
+        q = f"backbone.layers.{i}."
+        if i >= n_skip and skips:
+            x = x + p["backbone.skip_weights"][i - n_skip] * skips.pop()
+        h = _rms(x, p[q + "ln_1.weight"]) @ p[q + "attn.qkv.weight"].t()
+        a, b, v = h.view(n, 3, H, D).permute(1, 2, 0, 3)
+        a, b = turn(_rms(a, p[q + "attn.q_norm"])), turn(_rms(b, p[q + "attn.k_norm"]))
+        s = (a @ b.transpose(-1, -2) / math.sqrt(D)).masked_fill(~mask, -math.inf)
+        y = (torch.softmax(s, -1) @ v).transpose(0, 1).reshape(n, C)
+        x = x + y @ p[q + "attn.proj.weight"].t()
+        g, u = (_rms(x, p[q + "ln_2.weight"]) @ p[q + "mlp.gate_up.weight"].t()).chunk(2, -1)
+        x = x + (torch.nn.functional.silu(g) * u) @ p[q + "mlp.down.weight"].t()
+        if i < n_skip:
+            skips.append(x)
+    return _rms(x, p["norm.weight"]) @ p["embedding.weight"].t()
+
+
+def _loss(p, batch):
+    ids, target = batch["tokens"][0, :-1], batch["tokens"][0, 1:]
+    z = _logits(p, ids)
+    idx, t = batch["teacher_idx"][0], batch["teacher_logits"][0].double()
+    valid = idx >= 0
+    pk = torch.softmax((t / TAU).masked_fill(~valid, -math.inf), -1)
+    log_q = torch.log_softmax(z / TAU, -1).gather(1, idx.clamp(min=0))
+    kd = (pk * torch.where(valid, pk.clamp(min=1e-300).log() - log_q, 0.0)).sum(-1)
+    ce = -torch.log_softmax(z, -1).gather(1, target[:, None])[:, 0]
+    rows = ALPHA * TAU ** 2 * kd + (1 - ALPHA) * ce
+    return rows[target != IGNORE].mean()
+
+
+def _params64(m):
+    named = {n: t for n, t in m.state_dict().items()}
+    return {n: named[n].double().requires_grad_(True) for n, _ in m.named_parameters()}
+
+
+@pytest.mark.parametrize("dtype,bound", [(torch.bfloat16, 3e-2), (torch.float32, 1e-4)])
+def test_training_step(dtype, bound):
+    m, batch = _student(dtype), _batch()
+    loss = m(batch)
+    loss.backward()
+    p = _params64(m)
+    ref = _loss(p, batch)
+    grads = dict(zip(p, torch.autograd.grad(ref, list(p.values()))))
+    assert abs(float(loss.detach()) - float(ref)) <= bound * float(ref)
+    for name, prm in m.named_parameters():
+        want = grads[name]
+        off = float((prm.grad.double() - want).norm() / want.norm())
+        assert prm.grad.dtype == dtype and off <= bound, f"{name}: {off:.3g}"
+
+
+def test_steps_are_the_same_again():
+    """Two runs of three optimizer steps end with the same bits: no operator's
+    sums depend on the order that work-groups run in."""
+    ends = []
+    for _ in range(2):
+        m = _student(torch.bfloat16)
+        opt = torch.optim.SGD(m.parameters(), lr=1e-2)
+        for step in range(3):
+            opt.zero_grad()
+            loss = m(_batch(step))
+            loss.backward()
+            opt.step()
+        ends.append([loss.detach()] + [p.detach().clone() for p in m.parameters()])
+    for a, b in zip(*ends):
+        assert torch.equal(a, b)
+
+
+def test_step_without_a_teacher_is_the_cross_entropy():
+    m, batch = _student(torch.bfloat16), _batch()
+    for n in ("teacher_idx", "teacher_logits"):
+        del batch[n]
+    loss = float(m(batch).detach())
+    with torch.no_grad():
+        z = _logits(_params64(m), batch["tokens"][0, :-1])
+    ref = float(torch.nn.functional.cross_entropy(z, batch["tokens"][0, 1:]))
+    assert abs(loss - ref) <= 3e-2 * ref
+
+
+@pytest.mark.parametrize("graphs,fused", [(True, True), (True, False), (False, True)])
+def test_generation(graphs, fused):
+    """Cached generation of the student against the whole sequence in 64 bits:
+    the prefill, single tokens (captured or eager, on the fused row kernels or
+    not), several rows at once, and after an earlier token changed."""
+    m = _student(torch.bfloat16)
+    serve = TS2TSModel(m.backbone, m.embedding.weight, m.embedding.weight, m.norm,
+                       create_doc_causal_block_mask, V, embedding_scale=SCALE).eval()
+    serve.use_graphs, serve.fuse_rows = graphs, fused
+    p = {n: t.detach() for n, t in _params64(m).items()}
+    ids = _batch(3)["tokens"][:, :T]
+
+    def check(tokens, what):
+        spans = [s for s in SPANS if s.start < tokens.shape[1]]
+        spans[-1] = synth.DocSpan(doc_id=spans[-1].doc_id, start=spans[-1].start,
+                                  end=tokens.shape[1])
+        got = serve.forward_inference_last(tokens, spans)[0, 0].double()
+        want = _logits(p, tokens[0])[-1]
+        off = float((got - want).norm() / want.norm())
+        assert off <= 3e-2, f"{what}: {off:.3g}"
+        whole = serve.forward_inference(tokens, spans)[0, -1].double()
+        assert float((whole - want).norm() / want.norm()) <= 3e-2, what
+
+    check(ids[:, :100], "prefill")
+    for n in range(101, 106):
+        check(ids[:, :n], f"token {n}")
+    check(ids[:, :110], "five rows")
+    changed = ids.clone()
+    changed[0, 90] = (changed[0, 90] + 1) % V
+    check(changed[:, :111], "an earlier token changed")
+    check(changed[:, :112], "and one more")
+    # another factor on the embedding: nothing cached or captured is used again
+    serve.embedding_scale = None
+    p["embedding.weight"] = p["embedding.weight"] / SCALE
+    tied = p["embedding.weight"]
+    spans = [SPANS[0], synth.DocSpan(doc_id=3, start=70, end=113)]
+    got = serve.forward_inference_last(changed[:, :113], spans)[0, 0].double()
+    p["embedding.weight"] = tied
+    want = _logits(p, changed[0, :113])[-1] * SCALE  # the head keeps its own size
+    assert float((got - want).norm() / want.norm()) <= 3e-2
+
+
+def test_float32_student_serves():
+    m = _student(torch.float32)
+    serve = TS2TSModel(m.backbone, m.embedding.weight, m.embedding.weight, m.norm,
+                       create_doc_causal_block_mask, V, embedding_scale=SCALE).eval()
+    ids = _batch(4)["tokens"][:, :T]
+    got = serve.forward_inference_last(ids, SPANS)[0, 0].double()
+    want = _logits({n: t.detach() for n, t in _params64(m).items()}, ids[0])[-1]
+    assert float((got - want).norm() / want.norm()) <= 1e-4
+
+
+def test_from_config_of_both():
+    kw = dict(vocab_size=64, num_layers=2, model_dim=128, num_heads=2, max_seq_len=32, dropout=0.0,
+              drop_path_rate=0.0, block_mask_creator=create_doc_causal_block_mask, qk_norm=True,
+              embedding_scale=3.0)
+    train, serve = TS2TSTrainingModule.from_config(**kw), TS2TSModel.from_config(**kw)
+    assert serve.embedding_scale == train.embedding.scale == 3.0
+    a, b = (dict(x.backbone.named_parameters()) for x in (train, serve))
+    assert {n: t.shape for n, t in a.items()} == {n: t.shape for n, t in b.items()}
+    assert "layers.0.attn.q_norm" in a

@@ -104,7 +104,7 @@ def test_workspace_sizes():
     ws = _lib.lib().t2t_qk_norm_rope_backward_workspace
     assert ws(0, 5, 2, 2, 64) == ws(1, 5, 2, 2, 20) == ws(1, 5, 0, 2, 64) == 0
     assert ws(1, 1, 1, 1, 64) == 2 * 64 * 4
-    assert ws(8, 1 << 20, 16, 16, 128) == 2 * 768 * 128 * 4  # bounded
+    assert 0 < ws(8, 1 << 20, 16, 16, 128) <= 1024 * 128 * 4  # bounded
 
 
 def _cpu(H=2, Hkv=2, D=64, dt=torch.bfloat16, T=3):
