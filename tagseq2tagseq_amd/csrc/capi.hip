@@ -660,6 +660,7 @@ int t2t_qk_norm_rope_append(const void* qkv, int64_t stride_b, int64_t stride_t,
   if (!any) return T2T_OK;
   rc = check_head_views({q, k_cache, v_cache}, dtype);
   if (rc) return rc;
+  if (k_cache->data == v_cache->data) return fail(T2T_EINVAL, "k_cache and v_cache are one");
   for (const t2t_tensor* t : {k_cache, v_cache})
     if ((cache_rows > 1 && t->stride_t == 0) || (Hkv > 1 && t->stride_h == 0) ||
         (B > 1 && t->stride_b == 0))
@@ -727,7 +728,7 @@ int check_embed(const void* tokens, int64_t N, int64_t V, int32_t C, int32_t dty
     return fail(T2T_EINVAL, "N=%lld V=%lld C=%d", (long long)N, (long long)V, C);
   if (dtype != T2T_DTYPE_BF16 && dtype != T2T_DTYPE_F32)
     return fail(T2T_EUNSUPPORTED, "dtype %d not supported here", dtype);
-  if (V > kEmbedMaxV || N >= (1LL << 31) - 4096 || N * C > 1LL << 38)
+  if (V > kEmbedMaxV || C > 1 << 20 || N >= (1LL << 31) - 4096 || N * C > 1LL << 38)
     return fail(T2T_EUNSUPPORTED, "N=%lld V=%lld C=%d: more than one launch numbers",
                 (long long)N, (long long)V, C);
   if (N > 0 && (!tokens || reinterpret_cast<uintptr_t>(tokens) % 8))
@@ -761,7 +762,8 @@ int t2t_embedding(const int64_t* tokens, int64_t N, const void* weight, int64_t 
 }
 
 int64_t t2t_embedding_backward_workspace(int64_t N, int64_t V, int32_t C) {
-  if (N < 0 || V < 1 || V > kEmbedMaxV || C < 1 || N >= (1LL << 31) - 4096) return 0;
+  if (N < 0 || V < 1 || V > kEmbedMaxV || C < 1 || C > 1 << 20 || N >= (1LL << 31) - 4096)
+    return 0;
   return t2t::embed_plan(N, V, C).bytes;
 }
 
@@ -798,6 +800,8 @@ int t2t_distill_rows(const void* logits, int64_t ld, int64_t rows, int32_t V, in
                      float* row_loss, void* grad, int64_t grad_ld, void* stream) {
   if (rows < 0 || V < 1 || K < 0)
     return fail(T2T_EINVAL, "rows=%lld V=%d K=%d", (long long)rows, V, K);
+  if (V > 1 << 28)  // (a row's byte offsets have 32 bits)
+    return fail(T2T_EUNSUPPORTED, "V=%d columns; at most 2^28", V);
   if (K > t2t::kDistillMaxSlots)
     return fail(T2T_EUNSUPPORTED, "K=%d slots a row; at most %d", K, t2t::kDistillMaxSlots);
   if ((dtype != T2T_DTYPE_BF16 && dtype != T2T_DTYPE_F32) ||

@@ -243,6 +243,8 @@ class LinearDistillLoss(LinearCELoss):
     bf16 rows run ``head_distill``; float32 rows on the GPU are evaluated in
     chunks with recomputation.  Without a teacher it is the cross-entropy."""
 
+    distils = True
+
     def __init__(self, D: int, V: int, temperature: float = 1.0, alpha: float = 0.5, **kwargs):
         super().__init__(D, V, **kwargs)
         self.temperature = float(temperature)

@@ -16,7 +16,6 @@ Kernels: libt2t_attn.so ``t2t_embedding`` / ``t2t_embedding_backward``.
 """
 from __future__ import annotations
 
-import math
 from typing import Optional
 
 import torch
@@ -91,8 +90,8 @@ def embedding(tokens: torch.Tensor, weight: torch.Tensor, scale: float = 1.0,
     end when negative) gets none.  An id outside [0, V) gives a row of NaN and
     no gradient: the ids stay on the device and are not waited for."""
     scale = float(scale)
-    if not math.isfinite(scale):
-        raise ValueError(f"scale={scale!r} must be finite")
+    if not abs(scale) <= torch.finfo(torch.float32).max:
+        raise ValueError(f"scale={scale!r} must be finite in float32")
     if weight.dim() != 2:
         raise ValueError(f"weight must be [V, C], got shape {tuple(weight.shape)}")
     padding, V = -1, weight.shape[0]

@@ -200,6 +200,11 @@ class TS2TSTrainingModule(nn.Module):
         self.vocab_size = vocab_size
         self.ignore_index = ignore_index
 
+    @property
+    def distils(self) -> bool:
+        """Whether the loss takes a teacher's top logits."""
+        return getattr(self.loss_fn, "distils", False)
+
     @classmethod
     def from_config(cls, vocab_size: int, num_layers: int, model_dim: int, num_heads: int,
                     max_seq_len: int, dropout: float, drop_path_rate: float,
@@ -238,6 +243,11 @@ class TS2TSTrainingModule(nn.Module):
         positions 0 .. T - 1, that of distilling from them."""
         batch = dict(batch)
         teacher = [batch.pop(n) for n in ("teacher_idx", "teacher_logits") if n in batch]
+        if teacher and not self.distils:
+            raise ValueError("the batch has a teacher, and the loss does not distil (build the "
+                             "module with distill_alpha)")
+        if len(teacher) == 1:
+            raise ValueError("teacher_idx and teacher_logits go together")
         tokens = batch["tokens"]
         input_ids = tokens[:, :-1].contiguous()
         target_ids = tokens[:, 1:].contiguous()

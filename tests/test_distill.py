@@ -29,7 +29,7 @@ def _rows(**kw):
 @no_gpu
 @pytest.mark.parametrize("kw,rc,text", [
     (dict(rows=-1), -1, "rows=-1"), (dict(V=0), -1, "V=0"), (dict(K=-1), -1, "K=-1"),
-    (dict(K=1025), -2, "at most 1024"), (dict(dt=2), -2, "dtype"), (dict(tdt=3), -2, "dtype"),
+    (dict(K=1025), -2, "at most 1024"), (dict(V=(1 << 28) + 1, ld=1 << 29, gld=1 << 29), -2, "2^28"), (dict(dt=2), -2, "dtype"), (dict(tdt=3), -2, "dtype"),
     (dict(ib=2), -2, "indices"), (dict(temp=0.0), -1, "temperature"),
     (dict(temp=-1.0), -1, "temperature"), (dict(temp=float("nan")), -1, "temperature"),
     (dict(temp=100.5), -1, "temperature"), (dict(alpha=-0.1), -1, "alpha"),
@@ -123,3 +123,8 @@ def test_training_module_takes_a_teacher():
     assert "teacher_idx" in batch and torch.equal(got["y"], tokens[:, 1:])
     m(dict(tokens=tokens, doc_spans=["a"]))
     assert got["i"] is None and got["t"] is None
+    for missing in ("teacher_idx", "teacher_logits"):
+        with pytest.raises(ValueError, match="together"):
+            m({k: v for k, v in batch.items() if k != missing})
+    with pytest.raises(ValueError, match="distill_alpha"):
+        plain(batch)

@@ -28,7 +28,7 @@ def _forward(**kw):
 @pytest.mark.parametrize("kw,rc,text", [
     (dict(N=-1), -1, "N=-1"), (dict(V=0), -1, "V=0"), (dict(C=0), -1, "C=0"),
     (dict(dtype=2), -2, "dtype"), (dict(V=(1 << 20) + 1), -2, "one launch"),
-    (dict(N=1 << 31), -2, "one launch"), (dict(N=1 << 30, C=1 << 10), -2, "one launch"),
+    (dict(N=1 << 31), -2, "one launch"), (dict(C=(1 << 20) + 1, ws=1 << 21), -2, "one launch"), (dict(N=1 << 30, C=1 << 10), -2, "one launch"),
     (dict(tokens=None), -1, "tokens"), (dict(tokens=ctypes.c_void_p(0x1004)), -1, "tokens"),
     (dict(w=None), -1, "weight"), (dict(out=ctypes.c_void_p(0x1001)), -1, "misaligned"),
     (dict(ws=63), -1, "stride"),
@@ -66,7 +66,7 @@ def test_python_layer_refuses():
     t = torch.zeros(3, dtype=torch.int64)
     with pytest.raises(RuntimeError, match="GPU"):
         embedding(t, w)
-    for scale in (float("nan"), float("inf")):
+    for scale in (float("nan"), float("inf"), -1e39):
         with pytest.raises(ValueError, match="finite"):
             embedding(t, w, scale)
     for pad in (10, -11):

@@ -18,6 +18,8 @@ import math
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwad
+import torch.utils.checkpoint
 
 from tagseq2tagseq_amd.distill import LinearDistillLoss, distill_loss, head_distill
 from tagseq2tagseq_amd.head_loss import head_cross_entropy
@@ -474,6 +476,35 @@ def test_custom_op():
         assert torch.equal(loss, want)
         assert torch.equal(dz, torch.autograd.grad(want, other, torch.ones_like(want))[0])
     torch.library.opcheck(torch.ops.t2t.distill_loss, (z, idx, t, target, 2.0, 0.5, IGNORE, 2))
+
+
+def test_what_else_may_watch_a_call():
+    """Traces hold the call, forward-mode levels and batched calls are refused;
+    a function mode and recorded hooks see an ordinary call."""
+    z, idx, t, target = _case(9, 100, 4, F32)
+
+    def call(x):
+        return distill_loss(x, idx, t, target, alpha=0.5)
+
+    other = torch.randn_like(z)
+    with torch.no_grad():
+        traced = torch.jit.trace(call, z, check_trace=False)
+        assert torch.equal(traced(other), call(other))
+    with torch.no_grad(), fwad.dual_level():
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            call(fwad.make_dual(z, torch.ones_like(z)))
+    with torch.no_grad(), pytest.raises(RuntimeError):
+        torch.func.vmap(call)(torch.stack([z, z]))
+    loss = call(z.requires_grad_(True))
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(loss, z, torch.ones(2, device=DEV), is_grads_batched=True)
+    loss = call(z)
+    (want,) = torch.autograd.grad(loss, z)
+    with torch.autograd.graph.save_on_cpu():
+        loss = call(z)
+    assert torch.equal(torch.autograd.grad(loss, z)[0], want)
+    again = torch.utils.checkpoint.checkpoint(call, z, use_reentrant=False)
+    assert torch.equal(torch.autograd.grad(again, z)[0], want)
 
 
 def test_second_order_is_refused():

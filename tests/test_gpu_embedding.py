@@ -8,6 +8,7 @@ scales (2 U), then rounds once.
 """
 import pytest
 import torch
+import torch.autograd.forward_ad as fwad
 
 from tagseq2tagseq_amd.embedding import ScaledEmbedding, embedding
 
@@ -265,6 +266,27 @@ def test_module_and_custom_op():
     op = torch.ops.t2t.embedding(tokens, w, 5.5, 3)
     assert torch.equal(op, out) and torch.equal(torch.autograd.grad(op, w, dy)[0], dw)
     torch.library.opcheck(torch.ops.t2t.embedding, (tokens, w.detach(), 5.5, 3))
+
+
+def test_what_else_may_watch_a_call():
+    """Traces hold the call, forward-mode levels and batched calls are refused."""
+    tokens, w, dy = _case(30, 20, 16, BF)
+
+    def call(x):
+        return embedding(tokens, x, 2.0)
+
+    other = torch.randn_like(w)
+    with torch.no_grad():
+        traced = torch.jit.trace(call, w, check_trace=False)
+        assert torch.equal(traced(other), call(other))
+    with torch.no_grad(), fwad.dual_level():
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            call(fwad.make_dual(w, torch.ones_like(w)))
+    with torch.no_grad(), pytest.raises(RuntimeError):
+        torch.func.vmap(call)(torch.stack([w, w]))
+    out = call(w.requires_grad_(True))
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(out, w, torch.stack([dy, dy]), is_grads_batched=True)
 
 
 def test_second_order_is_refused():

@@ -16,6 +16,7 @@ eps / 2 of the value.  Before that stands fp32 arithmetic, U = 2^-24 a step:
 """
 import pytest
 import torch
+import torch.autograd.forward_ad as fwad
 
 from tagseq2tagseq_amd.rope import qk_norm_rope, qk_norm_rope_append, rope_tables
 
@@ -412,6 +413,47 @@ def test_custom_op():
                           (qkv.detach(), qw.detach(), kw.detach(), cos, sin, 4, 2, 1, EPS))
 
 
+def test_what_else_may_watch_a_call():
+    """Traces hold the call, forward-mode levels and batched calls are refused."""
+    qkv, qw, kw, cos, sin = _inputs(1, 12, 4, 2, 64, BF, BF, 0)
+
+    def call(x):
+        return qk_norm_rope(x, qw, kw, cos, sin, 4, 2)[0]
+
+    other = torch.randn_like(qkv)
+    with torch.no_grad():
+        traced = torch.jit.trace(call, qkv, check_trace=False)
+        assert torch.equal(traced(other), call(other))
+    with torch.no_grad(), fwad.dual_level():
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            call(fwad.make_dual(qkv, torch.ones_like(qkv)))
+    with torch.no_grad(), pytest.raises(RuntimeError):
+        torch.func.vmap(call)(torch.stack([qkv, qkv]))
+    q = call(qkv.requires_grad_(True))
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(q, qkv, torch.stack([q, q]).detach(), is_grads_batched=True)
+
+
+def test_leaves_keep_their_gradients_and_hooks():
+    """Accumulated gradients, a hook on an output, saved tensors kept elsewhere."""
+    qkv, qw, kw, cos, sin = _inputs(1, 30, 4, 4, 64, BF, BF, 0)
+    leaves = [t.requires_grad_(True) for t in (qkv, qw, kw)]
+    out = qk_norm_rope(*leaves, cos, sin, 4)
+    grads = _grads(out)
+    want = torch.autograd.grad(out, leaves, grads)
+    seen = []
+    with torch.autograd.graph.save_on_cpu():
+        out = qk_norm_rope(*leaves, cos, sin, 4)
+    out[0].register_hook(lambda g: seen.append(g))
+    torch.autograd.backward(out, grads)
+    assert len(seen) == 1 and torch.equal(seen[0], grads[0])
+    for leaf, w in zip(leaves, want):
+        assert torch.equal(leaf.grad, w)
+    torch.autograd.backward(qk_norm_rope(*leaves, cos, sin, 4), grads)
+    for leaf, w in zip(leaves, want):
+        assert torch.equal(leaf.grad, w + w)
+
+
 # ---- refusals that need GPU tensors
 
 def test_refusals():
@@ -439,6 +481,8 @@ def test_refusals():
         qk_norm_rope_append(qkv, qw, kw, cos, sin, 2, 0, kc.float(), vc.float())
     with pytest.raises(RuntimeError, match="overlap"):
         qk_norm_rope_append(qkv, qw, kw, cos, sin, 2, 0, kc[:, :, :1].expand(1, 1, 8, 64), vc)
+    with pytest.raises(RuntimeError, match="are one"):
+        qk_norm_rope_append(qkv, qw, kw, cos, sin, 2, 0, kc, kc)
     with pytest.raises(RuntimeError, match="boundary"):
         odd = torch.zeros(8 * 64 + 1, dtype=BF, device=DEV)[1:].view(1, 1, 8, 64)
         qk_norm_rope_append(qkv, qw, kw, cos, sin, 2, 0, odd, vc)

@@ -64,7 +64,7 @@ def test_nothing_to_do_is_no_error():
 def _append(**kw):
     a = dict(qkv=P, sb=0, st=256, B=1, M=4, Hq=2, Hkv=1, D=64, dtype=0, qw=P, kw=P, wdt=0,
              eps=1e-6, cos=P, sin=P, rows=16, pos=None, pos_sb=0, pos0=0, q=_view(), k=_view(),
-             v=_view(), cache=16)
+             v=_view(data=0x2000), cache=16)
     a.update(kw)
     return _lib.lib().t2t_qk_norm_rope_append(*a.values(), None)
 
@@ -74,7 +74,8 @@ def _append(**kw):
     (dict(pos=P, M=9), -2, "at most 8"), (dict(pos=ctypes.c_void_p(0x1004)), -1, "misaligned"),
     (dict(pos=P, pos_sb=-4), -1, "stride"), (dict(pos0=-1), -1, "positions"),
     (dict(pos0=13), -1, "exceed"), (dict(cache=3), -1, "exceed"), (dict(cache=-1), -1, "cache"),
-    (dict(k=_view(stride_t=0)), -1, "overlap"), (dict(B=2, v=_view()), -1, "overlap"),
+    (dict(k=_view(stride_t=0)), -1, "overlap"), (dict(B=2), -1, "overlap"),
+    (dict(v=_view()), -1, "are one"),
     (dict(Hkv=2, k=_view(stride_h=0)), -1, "overlap"), (dict(D=20), -2, "head dim"),
 ])
 def test_append_entry_refuses(kw, rc, text):
