@@ -14,19 +14,25 @@
 //      embed_split_kernel sorts blocks of 2048 positions by group, in LDS;
 //      embed_group_kernel, a work-group a group, sorts the group's parts of all
 //      blocks by id: each wave counts its share of them, and places them in order
-//      behind those of the waves before it.  Short lists are grouped
-//      without the split, every work-group reading all ids (with long ones, which
-//      all work-groups read in step from the same L2 channels, that took
-//      70 us for 131072 ids).  Further work-groups of both launches fill dW
-//      with zeros meanwhile (a wave's loads wait for its own earlier stores,
-//      so not the same ones).
+//      behind those of the waves before it.  (Without the split, every
+//      work-group reading all ids, in step and from the same L2 channels, 131072
+//      ids took 70 us, 20 this way.)  Further work-groups of both launches
+//      fill dW with zeros meanwhile (a wave's loads wait for its own
+//      earlier stores, so not the same ones).
 //   2. embed_sum_kernel: the list in pieces of S positions; a wave sums 64 VEC
 //      columns over a piece, all its loads in flight at once, and stores a
 //      token's row where all its positions lie within the piece, and a partial
 //      sum where they do not.
 //   3. embed_join_kernel: tokens that cross pieces, from their partial sums.
 //
+// Up to 2048 positions, whose four launches would be latency, embed_small_kernel
+// does all but the zeros: a work-group reads all ids, sorts its group's positions
+// in LDS and sums them.  (Writing the rows of its absent ids too, 77 MB of rows
+// 256 ids apart, took 35 us; the fill ahead of it takes 13.)
+//
 // Every order is that of the positions: results do not change from run to run.
+#include <algorithm>
+
 #include "attn_kernels.h"
 
 namespace t2t {
@@ -35,7 +41,8 @@ namespace {
 
 constexpr int kEmbThreads = 256;
 constexpr int kEmbItems = 4;
-constexpr int kEmbedDirect = 4096;     // positions grouped without the split
+constexpr int kEmbedSmall = 2048;      // positions that embed_small_kernel sums
+constexpr int kLongRow = 64;           // positions: from here a row is all waves' there
 constexpr int kGroupThreads = 512;
 constexpr int kGroupWaves = kGroupThreads / 64;
 constexpr int kGroupSteps = 4;         // of 64 positions, loaded at once
@@ -197,30 +204,12 @@ __global__ __launch_bounds__(kGroupThreads) void embed_split_kernel(EmbedGradArg
   }
 }
 
-// Calls f(position, id, active) for the wave's share of the group's positions,
-// in order, all lanes at once; other groups' lanes are inactive.
-template <bool Split, typename F>
+// Calls f(position, id, active) for the wave's share of the group's positions
+// in the sorted blocks, in order, all lanes at once.
+template <typename F>
 __device__ __forceinline__ void group_share(const EmbedGradArgs& a, uint32_t r, const F& f) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const uint32_t G = 1u << a.group_log2;
-  if (!Split) {
-    const int part = ((a.N + kGroupWaves - 1) / kGroupWaves + 63) & ~63;
-    const int i0 = wave * part, i1 = min(a.N, i0 + part);
-    for (int s = i0; s < i1; s += 64 * kGroupSteps) {
-      uint32_t id[kGroupSteps];
-#pragma unroll
-      for (int k = 0; k < kGroupSteps; ++k) {
-        const int i = s + 64 * k + lane;
-        id[k] = i < i1 ? id_of(a.tokens[i]) : r ^ 1;
-      }
-#pragma unroll
-      for (int k = 0; k < kGroupSteps; ++k) {
-        const bool own = (id[k] & (G - 1)) == r;
-        if (__ballot(own)) f(s + 64 * k + lane, id[k], own);
-      }
-    }
-    return;
-  }
   const int part = (a.blocks + kGroupWaves - 1) / kGroupWaves;
   const int b0 = wave * part, b1 = min(a.blocks, b0 + part);
   for (int b = b0; b < b1; b += kGroupSteps) {
@@ -249,10 +238,14 @@ __device__ __forceinline__ void group_share(const EmbedGradArgs& a, uint32_t r, 
   }
 }
 
+// The row of an id in its group; `none` for one without a gradient.
+__device__ __forceinline__ int row_in_group(const EmbedGradArgs& a, uint32_t id, int none) {
+  return id < (uint32_t)a.V && id != (uint32_t)a.padding ? (int)(id >> a.group_log2) : none;
+}
+
 // The list of a group's positions by id.  Row R, behind the others, takes ids
 // without a gradient; they are in the list as token -1, so that it has every
 // position and needs no count.
-template <bool Split>
 __global__ __launch_bounds__(kGroupThreads) void embed_group_kernel(EmbedGradArgs a) {
   extern __shared__ int lds[];
   const uint32_t G = 1u << a.group_log2;
@@ -260,21 +253,15 @@ __global__ __launch_bounds__(kGroupThreads) void embed_group_kernel(EmbedGradArg
     fill_zeros(a.dweight, a.zero_split, a.zero_bytes, blockIdx.x - G, gridDim.x - G);
     return;
   }
-  const uint32_t r = blockIdx.x, V = (uint32_t)a.V, pad = (uint32_t)a.padding;
+  const uint32_t r = blockIdx.x;
   const int R = a.rows_per_group + 1, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   int* cursor = lds;                  // [kGroupWaves][R]
   int* red = lds + kGroupWaves * R;   // [kGroupWaves]
   for (int i = threadIdx.x; i < kGroupWaves * R; i += kGroupThreads) cursor[i] = 0;
   // Positions of smaller groups.
   int before = 0;
-  if (Split) {
-    for (int b = threadIdx.x; b < a.blocks; b += kGroupThreads)
-      before += a.bounds[(int64_t)b * (G + 1) + r];
-  } else {
-#pragma unroll 8
-    for (int i = threadIdx.x; i < a.N; i += kGroupThreads)
-      before += (id_of(a.tokens[i]) & (G - 1)) < r;
-  }
+  for (int b = threadIdx.x; b < a.blocks; b += kGroupThreads)
+    before += a.bounds[(int64_t)b * (G + 1) + r];
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) before += __shfl_xor(before, off, 64);
   if (lane == 0) red[wave] = before;
@@ -283,18 +270,127 @@ __global__ __launch_bounds__(kGroupThreads) void embed_group_kernel(EmbedGradArg
 #pragma unroll
   for (int w = 0; w < kGroupWaves; ++w) base += red[w];
 
-  const auto row_of = [&](uint32_t t) {
-    return t < V && t != pad ? (int)(t >> a.group_log2) : R - 1;
-  };
-  group_share<Split>(a, r, [&](int, uint32_t id, bool own) {
-    if (own) atomicAdd(&cursor[wave * R + row_of(id)], 1);
+  group_share(a, r, [&](int, uint32_t id, bool own) {
+    if (own) atomicAdd(&cursor[wave * R + row_in_group(a, id, R - 1)], 1);
   });
   __syncthreads();
   starts_of(cursor, R, base, red);
-  group_share<Split>(a, r, [&](int i, uint32_t id, bool own) {
-    const int row = own ? row_of(id) : 0;
+  group_share(a, r, [&](int i, uint32_t id, bool own) {
+    const int row = own ? row_in_group(a, id, R - 1) : 0;
     const int at = place(cursor + wave * R, row, a.row_bits, own);
     if (own) a.list[at] = row == R - 1 ? make_int2(0, -1) : make_int2(i, (int)id);
+  });
+}
+
+__global__ __launch_bounds__(kGroupThreads) void embed_zero_kernel(EmbedGradArgs a) {
+  fill_zeros(a.dweight, 0, a.zero_bytes, blockIdx.x, gridDim.x);
+}
+
+// The rows of a short list (at most kEmbedSmall positions) in one launch, a
+// work-group a group of ids.  A row of up to kLongRow positions is summed by a
+// wave, a longer one by all of them: each a contiguous share, then the shares.
+template <typename T, int VEC>
+__global__ __launch_bounds__(kGroupThreads) void embed_small_kernel(EmbedGradArgs a) {
+  extern __shared__ int lds[];
+  const uint32_t G = 1u << a.group_log2, r = blockIdx.x;
+  const int R = a.rows_per_group + 1, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  // The counters, and when they are done with, the shares [kGroupWaves][64 VEC].
+  int* cursor = lds;
+  float* shares = reinterpret_cast<float*>(lds);
+  int* start = lds + kGroupWaves * max(R, 64 * VEC);  // [R + 1]: a row's first in the list
+  int* list = start + R + 1;                          // [N]: positions
+  int* red = list + a.N;                              // [kGroupWaves]
+  for (int i = threadIdx.x; i < kGroupWaves * R; i += kGroupThreads) cursor[i] = 0;
+  // A wave has kEmbedSmall / 8 positions at most, in order.
+  constexpr int kSteps = kEmbedSmall / kGroupThreads;
+  const int part = ((a.N + kGroupWaves - 1) / kGroupWaves + 63) & ~63;
+  const int i0 = wave * part + lane, i1 = min(a.N, (wave + 1) * part);
+  int row[kSteps];  // -1: another group's
+#pragma unroll
+  for (int k = 0; k < kSteps; ++k) {
+    const int i = i0 + 64 * k;
+    const uint32_t id = i < i1 ? id_of(a.tokens[i]) : r ^ 1;
+    row[k] = (id & (G - 1)) == r ? row_in_group(a, id, R - 1) : -1;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < kSteps; ++k)
+    if (row[k] >= 0) atomicAdd(&cursor[wave * R + row[k]], 1);
+  __syncthreads();
+  const int all = starts_of(cursor, R, 0, red);
+  for (int i = threadIdx.x; i < R; i += kGroupThreads) start[i] = cursor[i];  // wave 0's
+  if (threadIdx.x == 0) start[R] = all;
+  __syncthreads();
+  for (int k = 0; k < kSteps; ++k) {
+    int mine = -1;
+#pragma unroll
+    for (int j = 0; j < kSteps; ++j) mine = j == k ? row[j] : mine;
+    if (!__ballot(mine >= 0)) continue;
+    const int at = place(cursor + wave * R, mine < 0 ? 0 : mine, a.row_bits, mine >= 0);
+    if (mine >= 0) list[at] = i0 + 64 * k;
+  }
+  __syncthreads();
+
+  // The sum of positions [s, e) of the list in the lane's columns, in order.
+  const auto sum = [&](int s, int e, int c, float (&acc)[VEC]) {
+    const T* dy = static_cast<const T*>(a.dy) + c;
+    for (; s < e; s += 8) {
+      Pack<T, VEC> d[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k)  // (behind the end: the last one again, unused)
+        d[k] = *reinterpret_cast<const Pack<T, VEC>*>(dy +
+                                                      (int64_t)list[min(s + k, e - 1)] * a.dy_stride);
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (s + k < e)
+#pragma unroll
+          for (int v = 0; v < VEC; ++v) acc[v] += (float)d[k].v[v];
+    }
+  };
+  const auto store = [&](int row, int c, const float (&acc)[VEC]) {
+    Pack<T, VEC> o;
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) o.v[v] = (T)(acc[v] * a.scale);
+    *reinterpret_cast<Pack<T, VEC>*>(static_cast<T*>(a.dweight) +
+                                     (((int64_t)row << a.group_log2) + r) * a.C + c) = o;
+  };
+  // Rows by their number of positions: f(row) for each, in turn by wave where
+  // the waves share them out.
+  const auto rows = [&](int least, int most, bool shared, const auto& f) {
+    int turn = 0;
+    for (int r0 = 0; r0 < R - 1; r0 += 64) {
+      const int mine = r0 + lane;
+      const bool there = mine < R - 1 && ((int64_t)mine << a.group_log2) + r < a.V;
+      const int count = there ? start[mine + 1] - start[mine] : -1;
+      for (uint64_t left = __ballot(count >= least && count <= most); left; left &= left - 1) {
+        if (!shared || turn++ % kGroupWaves == wave) f(r0 + __ffsll((unsigned long long)left) - 1);
+      }
+    }
+  };
+  rows(1, kLongRow, true, [&](int row) {
+    for (int c = lane * VEC; c < a.C; c += 64 * VEC) {
+      float acc[VEC] = {};
+      sum(start[row], start[row + 1], c, acc);
+      store(row, c, acc);
+    }
+  });
+  rows(kLongRow + 1, kEmbedSmall, false, [&](int row) {
+    const int s = start[row], e = start[row + 1], share = (e - s + kGroupWaves - 1) / kGroupWaves;
+    for (int c0 = 0; c0 < a.C; c0 += 64 * VEC) {
+      const int c = c0 + lane * VEC;
+      float acc[VEC] = {};
+      if (c < a.C) sum(min(e, s + wave * share), min(e, s + (wave + 1) * share), c, acc);
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) shares[(wave * 64 + lane) * VEC + v] = acc[v];
+      __syncthreads();
+      if (wave == 0 && c < a.C) {
+        for (int w = 1; w < kGroupWaves; ++w)
+#pragma unroll
+          for (int v = 0; v < VEC; ++v) acc[v] += shares[(w * 64 + lane) * VEC + v];
+        store(row, c, acc);
+      }
+      __syncthreads();
+    }
   });
 }
 
@@ -485,31 +581,40 @@ hipError_t launch_join(const EmbedGradArgs& a, int64_t pieces, hipStream_t strea
 
 template <typename T>
 hipError_t launch_grad_t(const EmbedGradArgs& a, bool vector, hipStream_t stream) {
-  const int G = 1 << a.group_log2;
-  const int lds = (kGroupWaves * (a.rows_per_group + 1) + kGroupWaves) * 4;
+  constexpr int kVec = 16 / (int)sizeof(T);
+  const int G = 1 << a.group_log2, R = a.rows_per_group + 1;
   const auto fills = [](int64_t bytes) {  // work-groups; four 16-byte pieces a thread at least
     const int64_t n = (bytes / 16 + 4 * kGroupThreads - 1) / (4 * kGroupThreads);
     return (int)(n < 1 ? 1 : n < 768 ? n : 768);
   };
-  if (a.blocks) {
-    hipLaunchKernelGGL(embed_split_kernel, dim3(a.blocks + fills(a.zero_split)),
-                       dim3(kGroupThreads), (kGroupWaves * G + kGroupWaves) * 4, stream, a);
+  if (a.N <= kEmbedSmall) {
+    hipLaunchKernelGGL(embed_zero_kernel, dim3(fills(a.zero_bytes)), dim3(kGroupThreads), 0,
+                       stream, a);
     const hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
-    hipLaunchKernelGGL(embed_group_kernel<true>, dim3(G + fills(a.zero_bytes - a.zero_split)),
-                       dim3(kGroupThreads), lds, stream, a);
-  } else {
-    hipLaunchKernelGGL(embed_group_kernel<false>, dim3(G + fills(a.zero_bytes)),
-                       dim3(kGroupThreads), lds, stream, a);
+    if (e != hipSuccess || a.N == 0) return e;
+    const int vec = vector ? kVec : 1;
+    const int lds = (kGroupWaves * std::max(R, 64 * vec) + R + 1 + a.N + kGroupWaves) * 4;
+    if (vector)
+      hipLaunchKernelGGL((embed_small_kernel<T, kVec>), dim3(G), dim3(kGroupThreads), lds, stream,
+                         a);
+    else
+      hipLaunchKernelGGL((embed_small_kernel<T, 1>), dim3(G), dim3(kGroupThreads), lds, stream, a);
+    return hipGetLastError();
   }
+  hipLaunchKernelGGL(embed_split_kernel, dim3(a.blocks + fills(a.zero_split)),
+                     dim3(kGroupThreads), (kGroupWaves * G + kGroupWaves) * 4, stream, a);
   hipError_t e = hipGetLastError();
-  if (e != hipSuccess || a.N == 0) return e;
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL(embed_group_kernel, dim3(G + fills(a.zero_bytes - a.zero_split)),
+                     dim3(kGroupThreads), (kGroupWaves * R + kGroupWaves) * 4, stream, a);
+  e = hipGetLastError();
+  if (e != hipSuccess) return e;
   const int64_t pieces = ((int64_t)a.N + a.piece - 1) / a.piece;
   // 16 bytes a lane, also where 768 columns leave half of every second wave idle
   // (131072 positions: 59 us; lanes of 8 bytes, all of them busy, 75 us)
-  e = vector ? launch_sum_piece<T, 16 / (int)sizeof(T)>(a, pieces, stream)
+  e = vector ? launch_sum_piece<T, kVec>(a, pieces, stream)
              : launch_sum_piece<T, 1>(a, pieces, stream);
-  if (e != hipSuccess || pieces < 2) return e;
+  if (e != hipSuccess) return e;
   return vector ? launch_join<T, 4>(a, pieces, stream) : launch_join<T, 1>(a, pieces, stream);
 }
 
@@ -525,13 +630,15 @@ EmbedPlan embed_plan(int64_t N, int64_t V, int C) {
   const int64_t G = 1ll << p.group_log2;
   p.rows_per_group = (int)((V + G - 1) >> p.group_log2);
   p.piece = N <= 32768 ? 16 : 32;
-  p.blocks = N <= kEmbedDirect ? 0 : (int)((N + kSplitBlock - 1) / kSplitBlock);
+  p.bytes = 256;  // (never none)
+  if (N <= kEmbedSmall) return p;
+  p.blocks = (int)((N + kSplitBlock - 1) / kSplitBlock);
   const auto whole = [](int64_t n) { return (n + 255) / 256 * 256; };
   const int64_t pieces = (N + p.piece - 1) / p.piece;
   p.split_at = whole(N * (int64_t)sizeof(int2));
-  p.bounds_at = p.split_at + (p.blocks ? whole(N * (int64_t)sizeof(int2)) : 0);
+  p.bounds_at = p.split_at + whole(N * (int64_t)sizeof(int2));
   p.part_at = p.bounds_at + whole(p.blocks * (G + 1) * 4);
-  p.bytes = p.part_at + 2 * pieces * C * 4 + 256;  // (never none)
+  p.bytes = p.part_at + 2 * pieces * C * 4;
   return p;
 }
 
@@ -556,7 +663,7 @@ hipError_t launch_embed_grad(EmbedGradArgs a, void* workspace, bool f32, bool ve
   a.piece = p.piece;
   a.blocks = p.blocks;
   a.zero_bytes = a.V * a.C * (f32 ? 4 : 2);
-  a.zero_split = p.blocks ? a.zero_bytes / 32 * 16 : 0;  // about half in each launch
+  a.zero_split = a.zero_bytes / 32 * 16;  // about half in each launch
   return f32 ? launch_grad_t<float>(a, vector, stream) : launch_grad_t<__bf16>(a, vector, stream);
 }
 

@@ -58,7 +58,7 @@ def test_backward_entry_refuses(kw, rc, text):
 def test_workspace_sizes():
     ws = _lib.lib().t2t_embedding_backward_workspace
     assert ws(-1, 5, 5) == ws(5, 0, 5) == ws(5, 5, 0) == ws(5, 1 << 21, 5) == 0
-    assert 0 < ws(0, 5, 5) < ws(1000, 5, 5) < ws(1 << 20, 50257, 768) < 1 << 30
+    assert 0 < ws(0, 5, 5) == ws(2048, 5, 5) < ws(2049, 5, 5) < ws(1 << 20, 50257, 768) < 1 << 30
 
 
 def test_python_layer_refuses():

@@ -74,7 +74,8 @@ def test_rows_and_gradient(N, V, C, dt, scale):
     assert torch.equal(out.detach(), embedding(tokens, w.detach(), scale))
 
 
-@pytest.mark.parametrize("N", [15, 16, 17, 31, 32, 33, 64, 1000, 70000])
+@pytest.mark.parametrize("N", [1, 15, 16, 17, 63, 64, 65, 66, 1000, 2047, 2048, 2049, 2064, 2065,
+                               4097, 32768, 32769, 32800, 70000])
 def test_one_token_throughout(N):
     """A token that crosses every piece of the list; its neighbours get zeros."""
     C = 40
@@ -85,11 +86,15 @@ def test_one_token_throughout(N):
     _check_grad(dw, tokens, dy, 9, 1.0)
 
 
+@pytest.mark.parametrize("more", [0, 2048, 32768])
 @pytest.mark.parametrize("lengths", [(16, 16, 16), (15, 1, 16), (1, 31, 1), (40, 3, 50, 5),
-                                     (17, 64, 15, 1, 1, 1), (5, 200, 5)])
-def test_runs_that_end_at_and_cross_pieces(lengths):
+                                     (17, 64, 15, 1, 1, 1), (5, 200, 5), (64, 65, 66),
+                                     (32, 32, 33, 31, 600, 1)])
+def test_runs_that_end_at_and_cross_pieces(lengths, more):
     """Runs of equal tokens (ids of one work-group, in ascending order) of
-    given lengths, in shuffled positions."""
+    given lengths behind one of `more`, in shuffled positions: short lists, and
+    longer ones with pieces of 16 and of 32."""
+    lengths = (more,) * (more > 0) + lengths
     ids = torch.cat([torch.full((n,), 512 * i + 3) for i, n in enumerate(lengths)])
     g = torch.Generator().manual_seed(len(ids))
     tokens = ids[torch.randperm(len(ids), generator=g)].to(DEV)
@@ -101,21 +106,23 @@ def test_runs_that_end_at_and_cross_pieces(lengths):
     _check_grad(dw, tokens, dy, V, 1.0)
 
 
-def test_order_of_the_positions():
+@pytest.mark.parametrize("more", [0, 3000])
+def test_order_of_the_positions(more):
     """Additions in the order of the positions: 2^24 + 1 - 2^24 is 0 in fp32, and
     2^24 - 2^24 + 1 is 1."""
     big = 2.0 ** 24
-    tokens = torch.tensor([5, 9, 5, 9, 5, 9], device=DEV)
-    vals = torch.tensor([big, big, 1.0, -big, -big, 1.0], device=DEV)
+    tokens = torch.tensor([5, 9, 5, 9, 5, 9] + [3] * more, device=DEV)
+    vals = torch.tensor([big, big, 1.0, -big, -big, 1.0] + [0.0] * more, device=DEV)
     w = torch.zeros(10, 4, device=DEV, requires_grad=True)
-    (dw,) = torch.autograd.grad(embedding(tokens, w), w, vals[:, None].expand(6, 4))
+    (dw,) = torch.autograd.grad(embedding(tokens, w), w, vals[:, None].expand(6 + more, 4))
     assert dw[5].tolist() == [0.0] * 4 and dw[9].tolist() == [1.0] * 4
 
 
+@pytest.mark.parametrize("N", [400, 5000])
 @pytest.mark.parametrize("pad", [0, 7, -1])
-def test_padding_row(pad):
+def test_padding_row(pad, N):
     V, C = 50, 32
-    tokens, w, dy = _case(400, V, C, BF)
+    tokens, w, dy = _case(N, V, C, BF)
     tokens[::3] = pad % V
     w.requires_grad_(True)
     out = embedding(tokens, w, 2.0, padding_idx=pad)
@@ -125,15 +132,16 @@ def test_padding_row(pad):
     assert not dw[pad].any()
 
 
-def test_ids_outside_the_table():
+@pytest.mark.parametrize("N", [64, 3000, 40000])
+def test_ids_outside_the_table(N):
     V, C = 20, 16
-    tokens, w, dy = _case(64, V, C, BF)
+    tokens, w, dy = _case(N, V, C, BF)
     bad = {3: -1, 10: V, 40: 1 << 40, 41: -(1 << 62), 63: (1 << 32) + 2}
     for i, t in bad.items():
         tokens[i] = t
     w.requires_grad_(True)
     out = embedding(tokens, w, 1.0)
-    rows = torch.zeros(64, dtype=torch.bool, device=DEV)
+    rows = torch.zeros(N, dtype=torch.bool, device=DEV)
     rows[list(bad)] = True
     assert out[rows].isnan().all() and not out[~rows].isnan().any()
     _check_rows(out.detach()[~rows], tokens[~rows], w.detach(), 1.0)
