@@ -390,14 +390,16 @@ int64_t t2t_embedding_backward_workspace(int64_t N, int64_t V, int32_t C);
  * Gradient of t2t_embedding: dweight[v] = scale * sum of dy[i] over the i with
  * tokens[i] == v, in fp32 in the order of the positions (deterministic, no
  * atomics on values), rounded once.  Every row of dweight [V][C] (contiguous,
- * 16-byte aligned) is written; the row `padding` (-1: none) and those of ids that do not occur
- * are zero; ids outside [0, V) are left out.
+ * 16-byte aligned) is written; the row `padding` (-1: none) and those of ids
+ * that do not occur are zero; ids outside [0, V) are left out.
  *   dy       [N][C] rows of the dtype with row stride dy_stride.
  */
 int t2t_embedding_backward(const int64_t *tokens, int64_t N, const void *dy, int64_t dy_stride,
                            int64_t V, int32_t C, int32_t dtype, float scale, int64_t padding,
                            void *dweight, void *workspace, int64_t workspace_bytes,
                            void *stream);
+
+#define T2T_DISTILL_MAX_SLOTS 1024
 
 /*
  * Distillation loss of logit rows z [rows][V] from a teacher's top logits, and
@@ -409,10 +411,10 @@ int t2t_embedding_backward(const int64_t *tokens, int64_t N, const void *dy, int
  *   grad_j   = s (a T ([slots] q_j - sum over k with i_k = j of p_k)
  *            + (1 - a) (softmax(z)_j - [j = target]))
  * with s = scale * *scale_dev * g[r g_stride] (the last two where given).
- * T is 0.01 to 100.  Slots of one column add up.  A row whose slots are all empty or -inf has no
- * first part; a row whose target is ignore_index has loss and gradient 0 and
- * is not read; a target outside [0, V) or a column i_k >= V makes the row's
- * loss NaN and its gradient 0.
+ * T is 0.01 to 100.  Slots of one column add up.  A row whose slots are all
+ * empty or -inf has no first part; a row whose target is ignore_index has loss
+ * and gradient 0 and is not read; a target outside [0, V) or a column i_k >= V
+ * makes the row's loss NaN and its gradient 0.  With a = 0 the slots are not read.
  *   logits   dtype 0 = bf16, 1 = float32; rows at any address of the type,
  *            stride ld >= V (elements; grad likewise).
  *   idx      int32 or int64 (idx_bytes 4 or 8); teacher dtype 0 / 1; K <= 1024.

@@ -792,6 +792,8 @@ int t2t_embedding_backward(const int64_t* tokens, int64_t N, const void* dy, int
                     "t2t_embedding_backward launch");
 }
 
+static_assert(t2t::kDistillMaxSlots == T2T_DISTILL_MAX_SLOTS);
+
 int t2t_distill_rows(const void* logits, int64_t ld, int64_t rows, int32_t V, int32_t dtype,
                      const void* idx, int32_t idx_bytes, int64_t idx_ld, const void* teacher,
                      int32_t teacher_dtype, int64_t teacher_ld, int32_t K, const int64_t* target,
@@ -836,7 +838,8 @@ int t2t_distill_rows(const void* logits, int64_t ld, int64_t rows, int32_t V, in
   a.logits = logits; a.ld = ld; a.rows = rows; a.V = V;
   a.idx = idx; a.idx64 = idx_bytes == 8; a.idx_ld = idx_ld;
   a.teacher = teacher; a.teacher_f32 = teacher_dtype == T2T_DTYPE_F32; a.teacher_ld = teacher_ld;
-  a.K = K; a.target = target; a.ignore_index = ignore_index;
+  a.K = alpha > 0.f ? K : 0;  // (without a say, not read)
+  a.target = target; a.ignore_index = ignore_index;
   a.temp = temperature; a.inv_temp = 1.f / temperature; a.alpha = alpha;
   a.scale = scale; a.scale_dev = scale_dev; a.g = g; a.g_stride = g_stride;
   a.unless_one = unless_one; a.row_loss = row_loss; a.grad = grad; a.grad_ld = grad_ld;

@@ -624,9 +624,28 @@ hipError_t launch_distill_t(const DistillArgs& a, hipStream_t stream) {
 
 }  // namespace
 
-hipError_t launch_distill_rows(const DistillArgs& a, bool f32, hipStream_t stream) {
-  if (a.rows == 0) return hipSuccess;
-  return f32 ? launch_distill_t<float>(a, stream) : launch_distill_t<__bf16>(a, stream);
+// A launch has fewer than 2^32 threads: of more rows than that there are several.
+hipError_t launch_distill_rows(const DistillArgs& all, bool f32, hipStream_t stream) {
+  constexpr int64_t kRows = 1 << 21;
+  const int64_t size = f32 ? 4 : 2;
+  for (int64_t r0 = 0; r0 < all.rows; r0 += kRows) {
+    DistillArgs a = all;
+    const auto from = [r0](auto* p, int64_t bytes) {
+      return p ? reinterpret_cast<decltype(p)>(reinterpret_cast<uintptr_t>(p) + r0 * bytes) : p;
+    };
+    a.rows = all.rows - r0 < kRows ? all.rows - r0 : kRows;
+    a.logits = from(a.logits, a.ld * size);
+    a.grad = from(a.grad, a.grad_ld * size);
+    a.idx = from(a.idx, a.idx_ld * (a.idx64 ? 8 : 4));
+    a.teacher = from(a.teacher, a.teacher_ld * (a.teacher_f32 ? 4 : 2));
+    a.target = from(a.target, 8);
+    a.g = from(a.g, a.g_stride * 4);
+    a.row_loss = from(a.row_loss, 4);
+    const hipError_t e =
+        f32 ? launch_distill_t<float>(a, stream) : launch_distill_t<__bf16>(a, stream);
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
 }
 
 hipError_t launch_distill_count(const int64_t* target, int64_t rows, int64_t ignore_index,

@@ -548,11 +548,20 @@ __global__ __launch_bounds__(64 * kJoinWaves) void embed_join_kernel(EmbedGradAr
 
 template <typename T, int VEC>
 hipError_t launch_embed_t(const EmbedArgs& a, hipStream_t stream) {
-  const int64_t items = a.N * (a.C / VEC);
+  // (a launch has fewer than 2^32 threads: of more pieces there are several)
+  const int64_t nv = a.C / VEC, most = (1ll << 31) / nv;
   constexpr int per = kEmbThreads * kEmbItems;
-  const dim3 grid((unsigned)((items + per - 1) / per));
-  hipLaunchKernelGGL((embed_kernel<T, VEC>), grid, dim3(kEmbThreads), 0, stream, a);
-  return hipGetLastError();
+  for (int64_t n0 = 0; n0 < a.N; n0 += most) {
+    EmbedArgs part = a;
+    part.tokens += n0;
+    part.out = static_cast<T*>(a.out) + n0 * a.C;
+    part.N = std::min(a.N - n0, most);
+    hipLaunchKernelGGL((embed_kernel<T, VEC>), dim3((unsigned)((part.N * nv + per - 1) / per)),
+                       dim3(kEmbThreads), 0, stream, part);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
 }
 
 template <typename T, int VEC, int S>

@@ -410,6 +410,11 @@ Tensor embed_ids(const Tensor& tokens) {
   return tokens.to(at::kLong).contiguous();
 }
 
+// (before a count of columns is handed on as 32 bits)
+void need_columns(int64_t C) {
+  TORCH_CHECK_NOT_IMPLEMENTED(C <= INT32_MAX, "rows of ", C, " columns are not supported");
+}
+
 Tensor embedding(const Tensor& tokens, const Tensor& weight, double scale) {
   TORCH_CHECK_VALUE(weight.dim() == 2, "weight must be [V, C], got shape ", weight.sizes());
   const int code = embed_code(weight);
@@ -418,6 +423,7 @@ Tensor embedding(const Tensor& tokens, const Tensor& weight, double scale) {
   const c10::DeviceGuard guard(weight.device());
   const Tensor ids = embed_ids(tokens);
   const int64_t V = weight.size(0), C = weight.size(1);
+  need_columns(C);
   const bool rows = (weight.stride(1) == 1 || C == 1) && weight.stride(0) >= C;
   const Tensor w = rows ? weight : weight.contiguous();
   std::vector<int64_t> shape = tokens.sizes().vec();
@@ -440,6 +446,7 @@ Tensor embedding_backward(const Tensor& tokens, const Tensor& dy_in, int64_t V, 
   const c10::DeviceGuard guard(dy_in.device());
   const Tensor ids = embed_ids(tokens);
   const int64_t C = dy_in.size(-1), N = ids.numel();
+  need_columns(C);
   TORCH_CHECK_VALUE(dy_in.numel() == N * C, "gradient ", dy_in.sizes(), " does not fit tokens ",
                     tokens.sizes());
   Tensor dw = at::empty({V, C}, dy_in.options());
@@ -492,6 +499,8 @@ struct Distill {
                               logits.sizes().slice(0, logits.dim() - 1),
                       "teacher_idx ", idx_in.sizes(), " and teacher_logits ", teacher_in.sizes(),
                       " must be [..., K] of logits ", logits.sizes());
+    TORCH_CHECK_NOT_IMPLEMENTED(idx_in.size(-1) <= T2T_DISTILL_MAX_SLOTS, "K=", idx_in.size(-1),
+                                " slots a row; at most ", T2T_DISTILL_MAX_SLOTS);
     TORCH_CHECK_VALUE(idx_in.scalar_type() == at::kLong || idx_in.scalar_type() == at::kInt,
                       "teacher_idx must be int64 or int32, not ", idx_in.scalar_type());
     TORCH_CHECK_VALUE(temp >= 0.01 && temp <= 100, "temperature=", temp,

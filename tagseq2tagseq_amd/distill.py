@@ -16,7 +16,7 @@ averaged over the rows whose target is not ignore_index (all rows without
 targets).  Slots with a negative id are empty: a row may have fewer than K, or
 none, and then only its second part.  Slots of the same id add up.  An id
 outside the vocabulary makes the loss NaN, as a target outside it does: ids
-stay on the device and are not waited for.
+stay on the device and are not waited for.  With alpha 0 the teacher is not read.
 
     loss = distill_loss(logits, teacher_idx, teacher_logits, targets,
                         temperature=2.0, alpha=0.5)
@@ -42,7 +42,6 @@ from .head_loss import AUTO_CHUNK_BYTES, _mm_f32, fused_head_applies, head_weigh
 from .modules import LinearCELoss
 
 _REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
-MAX_SLOTS = 1024  # K
 
 
 @torch.library.custom_op("t2t::distill_loss", mutates_args=())
@@ -258,9 +257,9 @@ class LinearDistillLoss(LinearCELoss):
         if teacher_idx is None:
             return super().forward(x, targets)
         x = x.reshape(-1, x.shape[-1])
-        t = targets.reshape(-1)
-        K = teacher_idx.shape[-1]
-        idx, top = teacher_idx.reshape(-1, K), teacher_logits.reshape(-1, K)
+        N, K = x.shape[0], teacher_idx.shape[-1]
+        t = targets.reshape(N)
+        idx, top = teacher_idx.reshape(N, K), teacher_logits.reshape(N, K)
         if fused_head_applies(x, self.weight) and not torch.compiler.is_compiling():
             return head_distill(x, self.weight, idx, top, t, temperature=self.temperature,
                                 alpha=self.alpha, ignore_index=self.ignore_index,

@@ -123,7 +123,8 @@ class TS2TSBackbone(nn.Module):
         self.max_seq_len = max_seq_len
         self.layers = nn.ModuleList([
             Layer(n_embd=model_dim, n_head=num_heads, max_seq_len=max_seq_len, dropout=dropout,
-                  drop_path_rate=drop_path_rate, fp8=fp8, qk_norm=qk_norm) for _ in range(num_layers)])
+                  drop_path_rate=drop_path_rate, fp8=fp8, qk_norm=qk_norm)
+            for _ in range(num_layers)])
         self.skip_weights = nn.Parameter(torch.ones(num_layers // 2))
         self.activation_checkpointing = activation_checkpointing
 

@@ -29,6 +29,7 @@ from __future__ import annotations
 from typing import Dict, Optional, Tuple, Union
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -235,6 +236,8 @@ def qk_norm_rope(qkv: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tens
     (table rows), value rows copied.  bf16 or float32 rows, head_dim a
     multiple of 16 up to 512, bf16 or float32 weights; fp32 arithmetic with one
     rounding.  Gradients for qkv and the weights."""
+    if (cos.requires_grad or sin.requires_grad) and torch.is_grad_enabled():
+        raise RuntimeError("the rotary tables get no gradient: detach cos and sin")
     args = (int(num_heads), int(num_heads if num_kv_heads is None else num_kv_heads), int(pos0),
             float(eps))
     if torch.compiler.is_compiling():
@@ -244,6 +247,22 @@ def qk_norm_rope(qkv: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tens
     if _lib.only_recorded(qkv, q_weight, k_weight, cos, sin):
         return _lib.host().qk_norm_rope_ad(qkv, q_weight, k_weight, cos, sin, *args)
     return QKNormRopeFn.apply(qkv, q_weight, k_weight, cos, sin, *args)
+
+
+@torch.library.custom_op("t2t::qk_norm_rope_append", mutates_args=("k_cache", "v_cache"))
+def qk_norm_rope_append_op(qkv: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor,
+                           cos: torch.Tensor, sin: torch.Tensor, num_heads: int,
+                           pos: Optional[torch.Tensor], pos0: int, k_cache: torch.Tensor,
+                           v_cache: torch.Tensor, eps: float) -> torch.Tensor:
+    """The append for traces: q, with rows of the caches overwritten."""
+    return _lib.host().qk_norm_rope_append(qkv, q_weight, k_weight, cos, sin, num_heads, pos, pos0,
+                                           k_cache, v_cache, eps)
+
+
+@qk_norm_rope_append_op.register_fake
+def _qk_norm_rope_append_fake(qkv, q_weight, k_weight, cos, sin, num_heads, pos, pos0, k_cache,
+                              v_cache, eps):
+    return qkv.new_empty((qkv.shape[0], num_heads, qkv.shape[1], q_weight.shape[0]))
 
 
 def qk_norm_rope_append(qkv: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor,
@@ -260,8 +279,14 @@ def qk_norm_rope_append(qkv: torch.Tensor, q_weight: torch.Tensor, k_weight: tor
     A device position outside the tables or the cache stores nothing and gives
     a query row of zeros; of rows at the same position the last is stored.
     No gradient: for rows that autograd records, use ``qk_norm_rope``."""
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (qkv, q_weight, k_weight)):
+    rows = (qkv, q_weight, k_weight, cos, sin)
+    if (torch.is_grad_enabled() and any(t.requires_grad for t in rows)
+            or forward_ad._current_level >= 0
+            and any(forward_ad.unpack_dual(t).tangent is not None for t in rows)):
         raise RuntimeError("qk_norm_rope_append has no gradient: call it under torch.no_grad()")
     at, pos0 = (pos, 0) if isinstance(pos, torch.Tensor) else (None, int(pos))
-    return _lib.host().qk_norm_rope_append(qkv, q_weight, k_weight, cos, sin, int(num_heads), at,
-                                           pos0, k_cache, v_cache, float(eps))
+    args = (*rows, int(num_heads), at, pos0, k_cache, v_cache, float(eps))
+    watched = (*rows, k_cache, v_cache) if at is None else (*rows, k_cache, v_cache, at)
+    if torch.compiler.is_compiling() or not _lib.only_recorded(*watched):
+        return qk_norm_rope_append_op(*args)
+    return _lib.host().qk_norm_rope_append(*args)

@@ -78,6 +78,9 @@ def test_python_layer_refuses():
     for bad in (idx[:2], idx[:, :1], idx.view(1, 3, 2)):
         with pytest.raises(ValueError, match="teacher_idx"):
             distill_loss(z, bad, t, target)
+    for k in (1025, 1 << 32):  # (also where 32 bits hold none of it)
+        with pytest.raises(NotImplementedError, match="at most 1024"):
+            distill_loss(z, idx[:, :1].expand(3, k), t[:, :1].expand(3, k), target)
     with pytest.raises(ValueError, match="teacher_idx must"):
         distill_loss(z, idx.float(), t, target)
     with pytest.raises(NotImplementedError, match="dtype"):
@@ -86,6 +89,12 @@ def test_python_layer_refuses():
         distill_loss(z, idx, t.clone().requires_grad_(True), target)
     with pytest.raises(RuntimeError, match="bf16 rows"):
         head_distill(z, z, idx, t)
+    # (rows that the chunks would not reach)
+    m = LinearDistillLoss(4, 10)
+    x = torch.zeros(2, 4)
+    for bad in ((target, idx[:2], t[:2]), (target[:2], idx, t[:2]), (target[:2], idx[:2], t)):
+        with pytest.raises(RuntimeError, match="shape"):
+            m(x, *bad)
 
 
 def test_shapes_of_the_traced_op():

@@ -287,6 +287,34 @@ def test_columns_and_targets_outside_the_vocabulary():
     (dz,) = torch.autograd.grad(rows, leaf, torch.ones_like(rows))
     assert not dz[1:5].any() and dz[[0, 5]].any()
     assert distill_loss(z, idx, t, target, alpha=0.5).isnan()
+    # alpha 0: the teacher has no say, whatever its columns
+    target[:] = 3
+    idx[:, 0] = (1 << 32) + 3
+    idx[:, 1] = 3
+    want = distill_loss(leaf, idx[:, :0], t[:, :0], target, alpha=0.0)
+    got = distill_loss(leaf, idx, t, target, alpha=0.0)
+    assert torch.equal(got, want) and got.isfinite()
+    assert torch.equal(*(torch.autograd.grad(x, leaf)[0] for x in (got, want)))
+
+
+def test_more_rows_than_a_launch_takes():
+    """The rows at and behind the end of a launch, against the same rows alone."""
+    N, V, K = (1 << 21) + 70, 40, 2
+    g = torch.Generator(device=DEV).manual_seed(5)
+    z = torch.randn(N, V, generator=g, device=DEV).to(BF).requires_grad_(True)
+    idx = torch.randint(-1, V, (N, K), generator=g, device=DEV)
+    t = torch.randn(N, K, generator=g, device=DEV)
+    target = torch.randint(0, V, (N,), generator=g, device=DEV)
+    up = torch.randn(N, generator=g, device=DEV)
+    kw = dict(temperature=2.0, alpha=0.5, reduction="none")
+    rows = distill_loss(z, idx, t, target, **kw)
+    (dz,) = torch.autograd.grad(rows, z, up)
+    for part in (slice(0, 64), slice((1 << 21) - 64, N)):
+        alone = z.detach()[part].clone().requires_grad_(True)
+        want = distill_loss(alone, idx[part], t[part], target[part], **kw)
+        (d,) = torch.autograd.grad(want, alone, up[part])
+        # (rows of 80 bytes: whole pieces from the same column on in both)
+        assert torch.equal(rows[part], want) and torch.equal(dz[part], d)
 
 
 def test_no_counted_rows_and_no_rows():
@@ -591,6 +619,10 @@ def test_module():
     assert torch.equal(m(x, target).detach(), head_cross_entropy(x, w, target, IGNORE))
     with pytest.raises(ValueError, match="together"):
         m(x, target, idx)
+    # no slots at all: the second part alone
+    assert torch.equal(m(x, target, idx[:, :0], t[:, :0]).detach(),
+                       head_distill(x, w, idx[:, :0], t[:, :0], target, temperature=2.0,
+                                    alpha=0.5))
     # float32 rows: chunks of logits in float32, gradients by recomputation
     f = LinearDistillLoss(64, 400, temperature=2.0, alpha=0.5,
                           weight=torch.nn.Parameter(w.float()), chunk=8)

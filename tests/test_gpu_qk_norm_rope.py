@@ -385,6 +385,29 @@ def test_captured_append():
             assert not q.any()
 
 
+def test_traced_append():
+    """A trace, and a call that a dispatch mode watches, hold the append."""
+    B, M, H, Hkv, D, cap = 2, 3, 4, 2, 64, 16
+    qkv, qw, kw, _, _ = _inputs(B, M, H, Hkv, D, BF, BF, 0)
+    cos, sin = rope_tables(D, cap, DEV)
+    caches = [torch.zeros(B, Hkv, cap, D, dtype=BF, device=DEV) for _ in range(2)]
+    pos = torch.tensor([4, 5, 6], device=DEV)
+
+    def call(x, at, kc, vc):
+        return qk_norm_rope_append(x, qw, kw, cos, sin, H, at, kc, vc)
+
+    with torch.no_grad():
+        traced = torch.jit.trace(call, (qkv, pos, *caches), check_trace=False)
+        for seed in (1, 2):
+            x = _inputs(B, M, H, Hkv, D, BF, BF, 0, seed=seed)[0]
+            want, got = ([c.clone() for c in caches] for _ in range(2))
+            assert torch.equal(traced(x, pos + seed, *got), call(x, pos + seed, *want))
+            for a, b in zip(got, want):
+                assert torch.equal(a, b) and b[:, :, 4 + seed:7 + seed].any()
+    torch.library.opcheck(torch.ops.t2t.qk_norm_rope_append,
+                          (qkv, qw, kw, cos, sin, H, pos, 0, *caches, EPS))
+
+
 def test_another_stream():
     qkv, qw, kw, cos, sin = _inputs(1, 512, 4, 4, 64, BF, BF, 0)
     want = qk_norm_rope(qkv, qw, kw, cos, sin, 4)

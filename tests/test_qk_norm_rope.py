@@ -5,6 +5,7 @@ import ctypes
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwad
 from torch._subclasses.fake_tensor import FakeTensorMode
 
 from tagseq2tagseq_amd import _lib
@@ -135,6 +136,21 @@ def test_python_layer_refuses():
         qk_norm_rope(*a[:3], a[3].double(), a[4].double(), 2)
     with pytest.raises(ValueError, match="eps"):
         qk_norm_rope(*a, 2, eps=-1.0)
+    for i in (3, 4):
+        b = list(a)
+        b[i] = b[i].clone().requires_grad_(True)
+        with pytest.raises(RuntimeError, match="tables get no gradient"):
+            qk_norm_rope(*b, 2)
+        with torch.no_grad(), pytest.raises(RuntimeError, match="GPU"):
+            qk_norm_rope(*b, 2)
+    caches = [torch.zeros(1, 2, 8, 64, dtype=torch.bfloat16) for _ in range(2)]
+    for i in range(5):
+        b = list(a)
+        b[i] = b[i].clone().requires_grad_(True)
+        with pytest.raises(RuntimeError, match="append has no gradient"):
+            qk_norm_rope_append(*b, 2, 0, *caches)
+    with fwad.dual_level(), pytest.raises(RuntimeError, match="append has no gradient"):
+        qk_norm_rope_append(fwad.make_dual(a[0], a[0].clone()), *a[1:], 2, 0, *caches)
     with pytest.raises(ValueError, match="caches"):
         qk_norm_rope_append(*a, 2, 0, torch.zeros(1, 2, 8, 64), torch.zeros(1, 2, 9, 64))
 
@@ -144,6 +160,9 @@ def test_shapes_of_the_traced_op():
         a = _cpu(H=4, Hkv=2, D=32, T=7)
         q, k, v = torch.ops.t2t.qk_norm_rope(*a, 4, 2, 0, 1e-6)
         assert q.shape == (1, 4, 7, 32) and k.shape == v.shape == (1, 2, 7, 32)
+        cache = torch.zeros(1, 2, 8, 32, dtype=torch.bfloat16)
+        q = torch.ops.t2t.qk_norm_rope_append(*a, 4, None, 1, cache, cache.clone(), 1e-6)
+        assert q.shape == (1, 4, 7, 32)
 
 
 def test_module_parameters():
