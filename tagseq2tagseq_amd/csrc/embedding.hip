@@ -19,11 +19,15 @@
 //      ids took 70 us, 20 this way.)  Further work-groups of both launches
 //      fill dW with zeros meanwhile (a wave's loads wait for its own
 //      earlier stores, so not the same ones).
-//   2. embed_sum_kernel: the list in pieces of S positions; a wave sums 64 VEC
-//      columns over a piece, all its loads in flight at once, and stores a
-//      token's row where all its positions lie within the piece, and a partial
-//      sum where they do not.
+//   2. embed_sum_kernel: the list in pieces of S positions; each is summed by
+//      token, and a token's row is stored where all its positions lie within the
+//      piece, a partial sum where they do not.
 //   3. embed_join_kernel: tokens that cross pieces, from their partial sums.
+//
+// 16384 positions of 768 columns in bf16 into 50257 rows: 38 us, where reading dy
+// and writing dW at the rate of a large copy take 20; 131072: 103 us and 54.  The
+// rows of dy, 1.5 KB each in no order of addresses, arrive at 3.4 TB/s, with 8 or
+// 16 of them in flight a thread.
 //
 // Up to 2048 positions, whose four launches would be latency, embed_small_kernel
 // does all but the zeros: a work-group reads all ids, sorts its group's positions
@@ -394,37 +398,45 @@ __global__ __launch_bounds__(kGroupThreads) void embed_small_kernel(EmbedGradArg
   });
 }
 
-// A wave sums 64 VEC columns of a piece of S positions, lane l the columns
-// VEC l .. of the wave's block, the loads of half a piece in flight at once.
-// The positions are the same for all lanes.
+// A thread sums VEC columns of a piece of S positions, the loads of kSumBatch
+// of them in flight at once.  Lanes go on into the next piece where a row is no
+// multiple of a wave's columns (the whole gradient of 65536 rows of 512 columns
+// 51.9 us, of 131072 rows of 768 103.3 us; with waves of their own for each piece,
+// a quarter of whose lanes 768 columns leave idle, 54.8 and 105.5 us).
 template <typename T, int VEC, int S>
 __global__ __launch_bounds__(kSumThreads) void embed_sum_kernel(EmbedGradArgs a) {
-  constexpr int kSumBatch = S / 2;
-  const int M = a.N, lane = threadIdx.x & 63;
-  const int blocks = (a.C + 64 * VEC - 1) / (64 * VEC);
-  const int item = __builtin_amdgcn_readfirstlane(
-      (int)(blockIdx.x * (kSumThreads / 64) + (threadIdx.x >> 6)));
-  const int piece = item / blocks;
-  const int c = (item % blocks) * 64 * VEC + lane * VEC;
-  const int64_t e0 = (int64_t)piece * S;
+  constexpr int kSumBatch = 8;  // (16 of pieces of 32: as fast)
+  const int M = a.N;
+  const uint32_t per = a.C / VEC;
+  const int64_t first = (int64_t)blockIdx.x * kSumThreads, piece0 = first / per;
+  const uint32_t column = (uint32_t)(first - piece0 * per) + threadIdx.x;
+  const int64_t piece = piece0 + column / per;
+  const int c = (int)(column % per) * VEC;
+  const int64_t e0 = piece * S;
   if (e0 >= M) return;
   const int n = (int)min((int64_t)S, M - e0);
   const int2* __restrict__ list = a.list + e0;
-  const bool in = c < a.C;
-  const T* __restrict__ dy = static_cast<const T*>(a.dy) + (in ? c : 0);
+  const T* __restrict__ dy = static_cast<const T*>(a.dy) + c;
   const int before = e0 ? list[-1].y : -2, after = e0 + n < M ? list[n].y : -2;
   float acc[VEC] = {};
   bool from_before = list[0].y == before;
 #pragma unroll 1  // (unrolled, most of a short list's time went into fetching code)
   for (int b = 0; b < n; b += kSumBatch) {
-    // (positions behind the piece's end: its last one again, unused)
-    int token[kSumBatch];
+    // (positions behind the end: the first one, unused; what lies behind the list
+    // in the workspace may be read)
+    int token[kSumBatch], pos[kSumBatch];
     Pack<T, VEC> d[kSumBatch];
 #pragma unroll
-    for (int e = 0; e < kSumBatch; ++e) {
-      const int2 at = list[min(b + e, n - 1)];
+    for (int e = 0; e < kSumBatch; e += 2) {
+      const int4 at = *reinterpret_cast<const int4*>(list + b + e);
+      pos[e] = b + e < n ? at.x : 0;
       token[e] = at.y;
-      d[e] = *reinterpret_cast<const Pack<T, VEC>*>(dy + (int64_t)at.x * a.dy_stride);
+      pos[e + 1] = b + e + 1 < n ? at.z : 0;
+      token[e + 1] = at.w;
+    }
+#pragma unroll
+    for (int e = 0; e < kSumBatch; ++e) {
+      d[e] = *reinterpret_cast<const Pack<T, VEC>*>(dy + (int64_t)pos[e] * a.dy_stride);
     }
     __builtin_amdgcn_sched_barrier(0);  // none of the loads moves to its use
     const int next = b + kSumBatch < n ? list[b + kSumBatch].y : after;
@@ -437,9 +449,9 @@ __global__ __launch_bounds__(kSumThreads) void embed_sum_kernel(EmbedGradArgs a)
       const int follows = ends ? after : e + 1 < kSumBatch ? token[(e + 1) % kSumBatch] : next;
       if (!ends && follows == token[e]) continue;
       const bool to_after = ends && follows == token[e];
-      if (in && token[e] >= 0) {
+      if (token[e] >= 0) {
         if (from_before || to_after) {
-          float* p = a.part + (2 * (int64_t)piece + !from_before) * a.C + c;
+          float* p = a.part + (2 * piece + !from_before) * a.C + c;
 #pragma unroll
           for (int k = 0; k < VEC; ++k) p[k] = acc[k];
         } else {
@@ -566,10 +578,9 @@ hipError_t launch_embed_t(const EmbedArgs& a, hipStream_t stream) {
 
 template <typename T, int VEC, int S>
 hipError_t launch_sum(const EmbedGradArgs& a, int64_t pieces, hipStream_t stream) {
-  const int64_t waves = pieces * ((a.C + 64 * VEC - 1) / (64 * VEC));
-  constexpr int per = kSumThreads / 64;
-  hipLaunchKernelGGL((embed_sum_kernel<T, VEC, S>), dim3((unsigned)((waves + per - 1) / per)),
-                     dim3(kSumThreads), 0, stream, a);
+  const int64_t threads = pieces * (a.C / VEC);
+  const dim3 grid((unsigned)((threads + kSumThreads - 1) / kSumThreads));
+  hipLaunchKernelGGL((embed_sum_kernel<T, VEC, S>), grid, dim3(kSumThreads), 0, stream, a);
   return hipGetLastError();
 }
 
@@ -619,8 +630,6 @@ hipError_t launch_grad_t(const EmbedGradArgs& a, bool vector, hipStream_t stream
   e = hipGetLastError();
   if (e != hipSuccess) return e;
   const int64_t pieces = ((int64_t)a.N + a.piece - 1) / a.piece;
-  // 16 bytes a lane, also where 768 columns leave half of every second wave idle
-  // (131072 positions: 59 us; lanes of 8 bytes, all of them busy, 75 us)
   e = vector ? launch_sum_piece<T, kVec>(a, pieces, stream)
              : launch_sum_piece<T, 1>(a, pieces, stream);
   if (e != hipSuccess) return e;
