@@ -4,6 +4,10 @@ Public surface (mirrors the reference's seams):
   mask creators   -- tagseq2tagseq_amd.mask_creators
   BlockMask       -- tagseq2tagseq_amd.block_mask.T2TBlockMask
   attention       -- tagseq2tagseq_amd.attention.flex_attention / FlexSelfAttention
+  prologue        -- tagseq2tagseq_amd.rope.qkv_rope / qk_norm_rope / qk_norm_rope_append
+  embedding       -- tagseq2tagseq_amd.embedding.embedding / ScaledEmbedding
+  losses          -- tagseq2tagseq_amd.head_loss / distill.distill_loss / head_distill
+  modules, models -- tagseq2tagseq_amd.modules / model.TS2TSModel
 """
 from .block_mask import T2TBlockMask, build_block_mask  # noqa: F401
 from .attention import FlexSelfAttention, T2TFlexAttentionFn, flex_attention  # noqa: F401

@@ -11,7 +11,9 @@
 // a zero gradient (their logits are not read); a target outside [0, V) or a
 // column i_k >= V gives the loss NaN and a zero gradient.
 //
-// HBM bound: the row is read once and its gradient written once.  The row
+// HBM bound: the row is read once and its gradient written once (8192 rows of 50257
+// bf16 columns, 64 slots, with counting and mean: 363 us, 4.5 TB/s of the 5.1 of a
+// large copy; 2048 rows without gradient: 59 us, 48 of them the kernel).  The row
 // stays in the registers of a work-group, packed as it was read.  An exponential
 // is exp2(z c - max c), one fused operation and the instruction; with an integer
 // T from 2 to 4, e^(z - max) is a power of e^((z - max) / T).  The rounding of
@@ -604,7 +606,7 @@ hipError_t launch_distill_t(const DistillArgs& a, hipStream_t stream) {
   // Rows in as few threads as still hold them: each thread has about 30 registers
   // beside its pieces, and what is left of them is further rows on the CU, whose
   // loads run while another row is computed (8192 rows of 50257: three rows of
-  // 512 threads 363 us, two of 1024 372 us).
+  // 512 threads 363 us, two of 1024 372 us; 2048 without gradient 59 and 64 us).
   if (pieces <= 13 * 512 && a.K <= 512) {
     if (a.unless_one) READ(512);
     if (pieces <= 4 * 512) ROW(512, 4);
