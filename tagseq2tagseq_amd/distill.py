@@ -188,7 +188,9 @@ def _head_pass(x, weight, teacher_idx, teacher_logits, targets, temperature, alp
                                   teacher_logits[r0:r0 + m],
                                   None if targets is None else targets[r0:r0 + m], temperature,
                                   alpha, ignore_index, inv, scale, row_loss[r0:r0 + m], grads)
-        if grads:  # (the padding columns are logits of zero weights: zeros)
+        if grads:
+            if ld != V:  # products of zero weights: not zeros in a row that is not finite
+                logits[:, V:].zero_()
             torch.mm(logits, w, out=dx[r0:r0 + m])
             part = _mm_f32(logits.t(), xs)
             dw = part if dw is None else dw.add_(part)

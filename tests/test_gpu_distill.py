@@ -601,6 +601,23 @@ def test_head_is_the_loss_of_its_logits(chunk, wdt):
     assert rows.shape == (40,)
 
 
+@pytest.mark.parametrize("V", [512, 515])
+def test_head_rows_that_do_not_count_may_hold_anything(V):
+    """Rows of ignored targets with infinities and NaN: no share of the loss, and a
+    gradient of zeros (that of the weight has 0 times them, as in torch)."""
+    x, w, idx, t, target = _head_case(40, 64, V, 6)
+    target[:] = torch.where(target == IGNORE, 1, target)
+    target[3:5] = IGNORE
+    kw = dict(temperature=2.0, alpha=0.5, ignore_index=IGNORE)
+    want = head_distill(x, w, idx, t, target, **kw)
+    x[3], x[4] = math.inf, math.nan
+    xl = x.clone().requires_grad_(True)
+    loss = head_distill(xl, w, idx, t, target, **kw)
+    assert torch.equal(loss.detach(), want)
+    (gx,) = torch.autograd.grad(loss, xl)
+    assert not gx[3:5].any() and gx.isfinite().all() and gx[5].any()
+
+
 def test_head_without_a_teacher_is_the_cross_entropy():
     """alpha 0: the loss of head_cross_entropy's logits, to the roundings of
     both row kernels (each under 1e-5 of a loss of about ln V)."""
