@@ -14,6 +14,7 @@ tensors (2-norms), 3 %.  The float32 model has 2^-16 of those errors; its
 bound, 1e-4, is the float32 attention's own.
 """
 import math
+import threading
 
 import pytest
 import torch
@@ -32,12 +33,12 @@ IGNORE = -100
 SPANS = [synth.DocSpan(doc_id=7, start=0, end=70), synth.DocSpan(doc_id=3, start=70, end=T)]
 
 
-def _student(dtype, seed=0):
+def _student(dtype, seed=0, **more):
     torch.manual_seed(seed)
     m = TS2TSTrainingModule.from_config(
         vocab_size=V, num_layers=LAYERS, model_dim=C, num_heads=H, max_seq_len=256, dropout=0.0,
         drop_path_rate=0.0, block_mask_creator=create_doc_causal_block_mask, qk_norm=True,
-        embedding_scale=SCALE, distill_alpha=ALPHA, distill_temperature=TAU)
+        embedding_scale=SCALE, distill_alpha=ALPHA, distill_temperature=TAU, **more)
     with torch.no_grad():
         m.embedding.weight.mul_(C ** -0.5)
         for layer in m.backbone.layers:
@@ -145,6 +146,57 @@ def test_steps_are_the_same_again():
         ends.append([loss.detach()] + [p.detach().clone() for p in m.parameters()])
     for a, b in zip(*ends):
         assert torch.equal(a, b)
+
+
+def _grads(m, batches, weight=1.0):
+    for batch in batches:
+        (m(batch) * weight).backward()
+    return [p.grad.clone() for p in m.parameters()]
+
+
+def test_checkpointed_layers_have_the_same_gradients():
+    """Layers that are computed again in the backward: the same bits."""
+    want = _grads(_student(torch.bfloat16), [_batch()])
+    got = _grads(_student(torch.bfloat16, activation_checkpointing=True), [_batch()])
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+
+
+def test_accumulated_and_scaled_losses():
+    """Two batches of a loss times 1/2: a factor that is a power of two moves no
+    rounding, and autograd adds the two gradients, each rounded, to one more."""
+    first, second = (_grads(_student(torch.bfloat16), [_batch(s)]) for s in (0, 1))
+    got = _grads(_student(torch.bfloat16), [_batch(0), _batch(1)], 0.5)
+    for a, x, y in zip(got, first, second):
+        assert torch.equal(a, x / 2 + y / 2)
+
+
+def test_two_threads_on_streams_of_their_own():
+    """Steps of two students at once: each has the bits that it has alone."""
+    want = [_grads(_student(torch.bfloat16, seed=s), [_batch(s)]) for s in (0, 1)]
+    models = [_student(torch.bfloat16, seed=s) for s in (0, 1)]
+    batches = [_batch(s) for s in (0, 1)]
+    torch.cuda.synchronize()
+    got = [[], []]
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(3):
+                models[i].zero_grad()
+                got[i].append(_grads(models[i], [batches[i]]))
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in (0, 1)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(60)
+        assert not t.is_alive()
+    for i in (0, 1):
+        assert len(got[i]) == 3
+        for run in got[i]:
+            for a, b in zip(run, want[i]):
+                assert torch.equal(a, b)
 
 
 def test_step_without_a_teacher_is_the_cross_entropy():
