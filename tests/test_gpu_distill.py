@@ -317,6 +317,26 @@ def test_more_rows_than_a_launch_takes():
         assert torch.equal(rows[part], want) and torch.equal(dz[part], d)
 
 
+def test_offsets_past_32_bits():
+    """Logit rows, ids and teacher rows more than 2^32 elements apart in all."""
+    z, idx, t, target = _case(5, 1000, 8, BF)
+
+    def far(x):
+        step = 1 << 30
+        rows = torch.empty(4 * step + x.shape[1], dtype=x.dtype, device=DEV).as_strided(
+            x.shape, (step, 1))
+        rows.copy_(x)
+        return rows
+
+    kw = dict(temperature=2.0, alpha=0.5, reduction="none")
+    a, b = far(z).requires_grad_(True), z.clone().requires_grad_(True)
+    got = distill_loss(a, far(idx.int()), far(t.to(BF)), target, **kw)
+    want = distill_loss(b, idx.int(), t.to(BF), target, **kw)
+    up = torch.arange(1.0, 6.0, device=DEV)
+    assert torch.equal(got, want)  # (rows of 2000 bytes: 16-byte boundaries in both)
+    assert torch.equal(torch.autograd.grad(got, a, up)[0], torch.autograd.grad(want, b, up)[0])
+
+
 def test_no_counted_rows_and_no_rows():
     z, idx, t, target = _case(5, 60, 3, F32)
     leaf = z.clone().requires_grad_(True)

@@ -224,6 +224,29 @@ def test_gradient_against_differences():
         assert abs(diff - float((dw.double() * u).sum())) <= 54 * U * size + 1e-12 * size
 
 
+def test_offsets_past_32_bits():
+    """A table and a gradient of more than 2^32 elements, rows of dy as far apart."""
+    V, C = 1 << 20, 4104
+    ids = torch.tensor([V - 1, 0, V - 2, V - 1, 1 << 19], device=DEV)
+    w = torch.empty(V, C, dtype=BF, device=DEV)
+    g = torch.Generator().manual_seed(3)
+    rows, dy = (torch.randn(5, C, generator=g).to(BF).to(DEV) for _ in range(2))
+    w[ids] = rows
+    out = embedding(ids, w, 2.0)
+    assert torch.equal(out, w[ids] * 2)
+    far = torch.empty(4 * (1 << 30) + C, dtype=BF, device=DEV).as_strided((5, C), (1 << 30, 1))
+    far.copy_(dy)
+    w.requires_grad_(True)
+    (dw,) = torch.autograd.grad(embedding(ids, w, 2.0), w, far)
+    d = dy.double()
+    want = {V - 1: d[0] + d[3], 0: d[1], V - 2: d[2], 1 << 19: d[4]}
+    for v, ref in want.items():
+        tol = (torch.finfo(BF).eps / 2 + 6 * U) * 2 * ref.abs() + 4 * U * 16
+        assert bool(((dw[v].double() - 2 * ref).abs() <= tol).all())
+    dw[ids] = 0
+    assert not any(bool(part.any()) for part in dw.split(1 << 17))
+
+
 def test_captured_lookup_and_gradient():
     tokens, w, dy = _case(1000, 500, 64, BF)
     w.requires_grad_(True)

@@ -361,6 +361,32 @@ def test_captured_forward_and_backward():
             assert torch.equal(a, b)
 
 
+def test_offsets_past_32_bits():
+    """Rows and cache heads more than 2^32 elements apart."""
+    H, Hkv, D, T, cap = 2, 2, 64, 3, 8
+    qkv, qw, kw, _, _ = _inputs(1, T, H, Hkv, D, BF, BF, 0)
+    cos, sin = rope_tables(D, cap, DEV)
+    far = (1 << 32) + 64
+    store = torch.empty(2 * far + 4096, dtype=BF, device=DEV)
+    rows = store.as_strided((1, T, 6 * D), (0, far, 1))
+    rows.copy_(qkv)
+    leaf = rows.requires_grad_(True)
+    out = qk_norm_rope(leaf, qw, kw, cos, sin, H)
+    near = qkv.clone().requires_grad_(True)
+    want = qk_norm_rope(near, qw, kw, cos, sin, H)
+    grads = _grads(want)
+    for a, b in zip(out, want):
+        assert torch.equal(a, b)
+    # (autograd.grad of a strided leaf gives its gradient contiguous)
+    assert torch.equal(torch.autograd.grad(out, leaf, grads)[0],
+                       torch.autograd.grad(want, near, grads)[0])
+    kc, vc = (store[1024 * (i + 1):].as_strided((1, Hkv, cap, D), (0, far, D, 1)) for i in (0, 1))
+    with torch.no_grad():
+        q = qk_norm_rope_append(qkv, qw, kw, cos, sin, H, 0, kc, vc)
+    for a, b in zip((q, kc[:, :, :T], vc[:, :, :T]), want):
+        assert torch.equal(a, b.detach())
+
+
 def test_captured_append():
     B, M, H, D, cap = 1, 1, 4, 64, 32
     qkv, qw, kw, _, _ = _inputs(B, M, H, H, D, BF, BF, 0)
