@@ -182,6 +182,16 @@ def test_every_width_of_the_held_float32_row(V):
     _check(*_case(2, V, 16, F32, seed=1), 1.0, 0.5)
 
 
+@pytest.mark.parametrize("dt", [BF, F32])
+def test_widest_row(dt):
+    V = 1 << 28
+    g = torch.Generator(device=DEV).manual_seed(1)
+    z = torch.randn(1, V, generator=g, device=DEV, dtype=dt)
+    idx = torch.tensor([[V - 1, 5, -1, V // 2]], device=DEV)
+    _check(z, idx, torch.tensor([[2.0, 1.0, 9.0, 0.5]], device=DEV),
+           torch.tensor([V - 1], device=DEV), 2.0, 0.5)
+
+
 def test_without_targets():
     z, idx, t, _ = _case(40, 777, 12, BF)
     _check(z, idx, t, None, 2.0, 1.0)

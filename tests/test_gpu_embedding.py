@@ -60,6 +60,8 @@ def _check_grad(dw, tokens, dy, V, scale, skip=()):
     (17, 600, 64, F32, 1.0), (300, 40, 520, BF, 22.6), (1537, 8192, 512, F32, 22.6),
     (4096, 50257, 768, BF, 27.7), (2049, 1000, 100, BF, 3.0), (333, 513, 30, F32, 0.1),
     (16384, 700, 96, BF, 9.8), (40000, 3000, 24, F32, 1.0), (33000, 200000, 264, BF, 1.0),
+    (3, 5, 1 << 20, BF, 1.0), (2500, 5, 30001, F32, 1.0), (3, 1 << 20, 8, BF, 2.0),
+    (2100, 1 << 20, 8, F32, 2.0),
 ])
 def test_rows_and_gradient(N, V, C, dt, scale):
     tokens, w, dy = _case(N, V, C, dt)

@@ -38,6 +38,8 @@ SHAPES = [
     (1, 301, 8, 8, 64, F32, F32, 0),
     (2, 19, 5, 1, 80, F32, BF, 2),
     (1, 2500, 12, 12, 64, BF, BF, 0),  # several rounds a work-group
+    (1, 3, 1001, 7, 16, BF, BF, 0),
+    (2, 2, 3, 700, 32, F32, F32, 0),
 ]
 IDS = ["B%d T%d H%d/%d D%d %s %s" % (*s[:5], str(s[5])[6:], str(s[6])[6:]) for s in SHAPES]
 
