@@ -17,10 +17,11 @@
 // stays in the registers of a work-group, packed as it was read.  An exponential
 // is exp2(z c - max c), one fused operation and the instruction; with an integer
 // T from 2 to 4, e^(z - max) is a power of e^((z - max) / T).  The rounding of
-// max c is a common factor of all exponentials, taken out of the sums' logarithms.
-// Rows whose maximum is near the type's largest magnitude (all columns
-// masked with the lowest value), where max c would overflow, are read again
-// and use (z - max) c.  Sums are fp32; KD is computed from
+// max c is a common factor of all exponentials, taken out of the sums' logarithms;
+// below |max c| = 2^24 it is at most 2^(1/2), 4 as a fourth power.  Rows whose
+// maximum is farther from 0 (all columns masked with a large negative value),
+// where that factor would grow past what fp32 holds, are read again and use
+// (z - max) c.  Sums are fp32; KD is computed from
 //   sum_k w_k ((t_k - max t) - (z(i_k) - max z)) / (T sum w) - ln sum w + ln sum_j
 // with w_k = e^((t_k - max t) / T), whose terms are small where the result is.
 // The gradient is first written without the teacher's and the target's terms;
@@ -169,7 +170,7 @@ __device__ __forceinline__ void combine(float (&x)[n], float (*red)[n]) {
 
 // The exponentials of a row.  P: 1, one softmax; 0, two of unrelated
 // temperatures; n >= 2, e^(z - max) is the n-th power of e^((z - max) / T).
-// Far: by differences, for maxima whose product with c could overflow.
+// Far: by differences, for maxima whose product with c rounds by more than 1/2.
 template <int P, bool Far>
 struct Exps {
   float m, c, nm, c1, nm1;
@@ -497,8 +498,9 @@ __device__ __forceinline__ void distill_row(const DistillArgs& a, int64_t row, c
   }
   const float ct = kLog2e * a.inv_temp;
   const float c = soft ? ct : kLog2e;  // of the only softmax, where there is one
-  // |max| c below the largest float, for c up to 144
-  if (fabsf(m[0]) < 1e36f) {
+  // Half a step of max c is the exponent of the factor that all exponentials share
+  // (of the other softmax's, for P = 0, with its own c).
+  if (fabsf(m[0]) * fmaxf(c, kLog2e) < 0x1p24f) {
     finish_row<T, NT, P, false>(a, row, at, held, sh, z_slot, z_target, m[0], m[1], taught, hard,
                                 c, ct, scale);
   } else {

@@ -260,6 +260,31 @@ def test_masked_logits(dt):
     _check(zz, idx, t, target, 2.0, 0.5)
 
 
+@pytest.mark.parametrize("tau", [1 / 64, 0.5, 1.0, 2.0, 4.0])
+@pytest.mark.parametrize("dt,V", [(BF, 203), (F32, 203), (BF, 131080), (F32, 65544)])
+def test_rows_far_from_zero(dt, V, tau):
+    """Rows wholly, or but for one column, at a value far from 0, and columns far
+    above the others.  A sum's exponentials are those of differences to the row's
+    maximum, whatever its size, so the tolerances at the head hold as they are
+    (temperatures are powers of two: T and 1 / T are exact)."""
+    far = (-1e4, -1e9, -1e10, -1e12, -1e30)
+    z, idx, t, target = _case(2 * len(far) + 3, V, 4, dt, empty=False)
+    for i, value in enumerate(far):
+        z[i] = value
+        z[len(far) + i] = value
+        z[len(far) + i, 17] = 0.5
+    z[-3, 17], z[-2, 17] = 1e10, 1e20
+    target[:] = torch.arange(len(target), device=DEV)
+    for alpha in (0.5, 1.0):
+        _check(z, idx, t, target, tau, alpha)
+        _, _, grad, size = _reference(z, idx, t, target, tau, alpha)
+        leaf, g = z.clone().requires_grad_(True), torch.tensor(-1 / 3, device=DEV)
+        loss = distill_loss(leaf, idx, t, target, temperature=tau, alpha=alpha, reduction="sum")
+        (dz,) = torch.autograd.grad(loss, leaf, g)
+        f = g.double()
+        _within(dz, grad * f, _grad_tol(dt, grad * f, size * f.abs()), "scaled gradient")
+
+
 def test_rows_that_are_not_numbers():
     z, idx, t, target = _case(8, 99, 4, F32, empty=False)
     target[:] = 7
