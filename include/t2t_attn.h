@@ -393,6 +393,8 @@ int64_t t2t_embedding_backward_workspace(int64_t N, int64_t V, int32_t C);
  * 16-byte aligned) is written; the row `padding` (-1: none) and those of ids
  * that do not occur are zero; ids outside [0, V) are left out.
  *   dy       [N][C] rows of the dtype with row stride dy_stride.
+ * N C at most 2^38, and below 2^37 where rows are read element by element (as
+ * for the lookup).
  */
 int t2t_embedding_backward(const int64_t *tokens, int64_t N, const void *dy, int64_t dy_stride,
                            int64_t V, int32_t C, int32_t dtype, float scale, int64_t padding,

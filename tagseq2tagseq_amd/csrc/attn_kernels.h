@@ -185,6 +185,7 @@ struct EmbedPlan {
   int64_t split_at, bounds_at, part_at, bytes;
 };
 EmbedPlan embed_plan(int64_t N, int64_t V, int C);
+bool embed_grad_fits(int64_t N, int64_t V, int C, bool f32, bool vector);
 hipError_t launch_embed_grad(EmbedGradArgs a, void* workspace, bool f32, bool vector,
                              hipStream_t stream);
 

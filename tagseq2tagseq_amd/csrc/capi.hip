@@ -780,6 +780,9 @@ int t2t_embedding_backward(const int64_t* tokens, int64_t N, const void* dy, int
     return fail(T2T_EINVAL, "dy or dweight NULL, misaligned, or a negative row stride");
   if (reinterpret_cast<uintptr_t>(dweight) % 16)
     return fail(T2T_EINVAL, "dweight must be 16-byte aligned");
+  if (!t2t::embed_grad_fits(N, V, C, dtype == T2T_DTYPE_F32, vec))
+    return fail(T2T_EUNSUPPORTED, "N=%lld C=%d: more than one launch of the gradient numbers",
+                (long long)N, C);
   const int64_t need = t2t_embedding_backward_workspace(N, V, C);
   if (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16)
     return fail(T2T_EINVAL, "workspace of %lld bytes (16-byte aligned), %lld needed",

@@ -660,6 +660,14 @@ EmbedPlan embed_plan(int64_t N, int64_t V, int C) {
   return p;
 }
 
+// The sum is one launch, which has fewer than 2^32 threads along an axis of its grid.
+bool embed_grad_fits(int64_t N, int64_t V, int C, bool f32, bool vector) {
+  if (N <= kEmbedSmall) return true;
+  const int64_t piece = embed_plan(N, V, C).piece, pieces = (N + piece - 1) / piece;
+  const int64_t threads = pieces * (C / (vector ? (f32 ? 4 : 8) : 1));
+  return threads <= (1ll << 32) - kSumThreads;
+}
+
 hipError_t launch_embed(const EmbedArgs& a, bool f32, bool vector, hipStream_t stream) {
   if (a.N == 0) return hipSuccess;
   if (f32) return vector ? launch_embed_t<float, 4>(a, stream) : launch_embed_t<float, 1>(a, stream);

@@ -55,6 +55,30 @@ def test_backward_entry_refuses(kw, rc, text):
     assert _backward(**kw) == rc and text in _err()
 
 
+
+@no_gpu
+@pytest.mark.parametrize("kw", [
+    dict(N=1 << 26, C=2049), dict(N=1 << 26, C=2049, dtype=1),
+    dict(N=1 << 26, C=2048, dy=ctypes.c_void_p(0x1002)),
+    dict(N=(1 << 30) + 64, C=255),
+])
+def test_backward_entry_refuses_what_a_launch_does_not_number(kw):
+    """A thread a column and piece of 32 positions: 2^32 of them and more, before
+    the first launch."""
+    assert _backward(ds=0, bytes=1 << 50, **kw) == -2 and "one launch" in _err()
+
+
+@no_gpu
+@pytest.mark.parametrize("kw", [
+    dict(N=1 << 26, C=2048), dict(N=(1 << 26) - 32, C=2048, dy=ctypes.c_void_p(0x1002)),
+    dict(N=1 << 30, C=127), dict(N=(1 << 31) - 4097, C=1),
+    dict(N=1 << 28, C=1 << 10, dtype=1),
+])
+def test_backward_entry_takes_what_a_launch_numbers(kw):
+    """(Refused for its workspace, which is checked behind the sizes.)"""
+    assert _backward(ds=0, bytes=0, **kw) == -1 and "workspace" in _err()
+
+
 def test_workspace_sizes():
     ws = _lib.lib().t2t_embedding_backward_workspace
     assert ws(-1, 5, 5) == ws(5, 0, 5) == ws(5, 5, 0) == ws(5, 1 << 21, 5) == 0
