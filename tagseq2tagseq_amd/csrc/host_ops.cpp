@@ -11,6 +11,7 @@
 // 64, a layer of 512 x 512 forward + backward 950 -> 750, twelve layers over
 // 2048 tokens 3710 -> 2460.  The functions keep nothing from one call to the
 // next.
+#include <ATen/SavedTensorHooks.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
@@ -879,8 +880,16 @@ Tensor embedding_ad(const Tensor& tokens, const Tensor& weight, double scale, in
   return EmbeddingAd::apply(tokens, weight, scale, padding);
 }
 
+// Whether hooks take what a graph saves: a recomputed region's, which drops it,
+// or a user's, which moves it elsewhere.
+bool saved_tensors_hooked() {
+  return !at::SavedTensorDefaultHooks::get_tls_state().stack.empty();
+}
+
 // A sum or mean is differentiated with an incoming gradient of 1 as a rule, so
-// the forward's pass over the logits writes its gradient.
+// the forward's pass over the logits writes its gradient.  Kept beside what the
+// graph saves, it would stay where hooks take the rest away, so it is then left
+// to the backward.
 struct DistillAd : torch::autograd::Function<DistillAd> {
   static Tensor forward(AutogradContext* ctx, const Tensor& logits, const Tensor& idx,
                         const Tensor& teacher, const c10::optional<Tensor>& target,
@@ -888,7 +897,7 @@ struct DistillAd : torch::autograd::Function<DistillAd> {
                         int64_t reduction) {
     auto [loss, grad, inv] =
         distill_loss(logits, idx, teacher, target, temperature, alpha, ignore_index, reduction,
-                     reduction != 0 && logits.requires_grad());
+                     reduction != 0 && logits.requires_grad() && !saved_tensors_hooked());
     ctx->save_for_backward({logits, idx, teacher, target.has_value() ? *target : Tensor(), inv});
     ctx->saved_data["x"] = std::vector<double>{temperature, alpha};
     ctx->saved_data["n"] = std::vector<int64_t>{ignore_index, reduction};
@@ -995,6 +1004,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("distill_loss", &distill_loss, no_gil);
   m.def("distill_loss_backward", &distill_loss_backward, no_gil);
   m.def("distill_rows_", &distill_rows_, no_gil);
+  m.def("saved_tensors_hooked", &saved_tensors_hooked);
   m.def("distill_count", &distill_count, no_gil);
   m.def("distill_mean", &distill_mean, no_gil);
   m.def("swiglu", &swiglu, no_gil);

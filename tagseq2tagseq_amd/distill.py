@@ -96,11 +96,13 @@ class DistillFn(torch.autograd.Function):
     with an incoming gradient of 1 as a rule, so its gradient is written by the
     forward's pass over the logits; the backward hands it over, having the rows
     computed again (on the device, without waiting) where the incoming gradient is
-    another."""
+    another.  Where hooks take what the graph saves (a recomputed region, offloading),
+    nothing is kept and the gradient is the backward's."""
 
     @staticmethod
     def forward(ctx, logits, teacher_idx, teacher_logits, targets, *args):
-        keep = args[-1] != 0 and ctx.needs_input_grad[0]
+        keep = (args[-1] != 0 and ctx.needs_input_grad[0]
+                and not _lib.host().saved_tensors_hooked())
         loss, grad, inv = _lib.host().distill_loss(logits, teacher_idx, teacher_logits, targets,
                                                    *args, keep)
         ctx.save_for_backward(logits, teacher_idx, teacher_logits, targets, inv)

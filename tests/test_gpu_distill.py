@@ -590,6 +590,32 @@ def test_what_else_may_watch_a_call():
     assert torch.equal(torch.autograd.grad(again, z)[0], want)
 
 
+@pytest.mark.parametrize("watched", [False, True])
+def test_offloaded_graphs_keep_no_gradient(watched):
+    """Where a user's hooks take what a graph saves, nothing of the logits' size
+    stays on the GPU beside the logits themselves, and the gradient is the same."""
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class Watch(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            return func(*args, **(kwargs or {}))
+
+    z, idx, t, target = _case(512, 8192, 4, F32)
+    leaf = z.clone().requires_grad_(True)
+    kw = dict(temperature=2.0, alpha=0.5, ignore_index=IGNORE)
+    (want,) = torch.autograd.grad(distill_loss(leaf, idx, t, target, **kw), leaf)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    with torch.autograd.graph.save_on_cpu():
+        if watched:
+            with Watch():
+                loss = distill_loss(leaf, idx, t, target, **kw)
+        else:
+            loss = distill_loss(leaf, idx, t, target, **kw)
+    assert torch.cuda.memory_allocated() - before < z.numel() * 4 // 2
+    assert torch.equal(torch.autograd.grad(loss, leaf)[0], want)
+
+
 def test_second_order_is_refused():
     z, idx, t, target = _case(4, 50, 3, F32)
     leaf = z.clone().requires_grad_(True)
@@ -709,3 +735,22 @@ def test_module():
     assert abs(float(loss) - float(rows.sum() / n)) <= 1e-4 * float(rows.sum() / n)
     _within(gx, grad @ w64 / n, 1e-4 * (grad.abs() @ w64.abs()) / n + 1e-9, "dx")
     _within(gw, grad.t() @ x64 / n, 1e-4 * (grad.abs().t() @ x64.abs()) / n + 1e-9, "dw")
+
+
+def test_recomputed_chunks_keep_no_logits():
+    """float32 rows of LinearDistillLoss: what lives between forward and backward
+    is less than one chunk's logits, and at no time more than a few chunks'."""
+    N, V, chunk = 2048, 8192, 256
+    _, idx, t, target = _case(N, V, 4, F32)
+    m = LinearDistillLoss(64, V, temperature=2.0, alpha=0.5, chunk=chunk).to(DEV)
+    x = torch.randn(N, 64, device=DEV, requires_grad=True)
+    torch.autograd.grad(m(x, target, idx, t), (x, m.weight))  # (what a first call loads stays)
+    one = chunk * V * 4
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    loss = m(x, target, idx, t)
+    assert torch.cuda.memory_allocated() - before < one
+    torch.autograd.grad(loss, (x, m.weight))
+    # a chunk's logits and their gradient, the weight's gradients (2 MB each)
+    assert torch.cuda.max_memory_allocated() - before < 3 * one
