@@ -38,7 +38,7 @@ import torch.utils.checkpoint
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .head_loss import AUTO_CHUNK_BYTES, _mm_f32, fused_head_applies, head_weight
+from .head_loss import AUTO_CHUNK_BYTES, _mm_f32, fused_head_applies, head_weight, scaled_rows
 from .modules import LinearCELoss
 
 _REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
@@ -217,7 +217,7 @@ class HeadDistillFn(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, g):
         dx, dw = ctx.saved_tensors
-        return (dx * g.to(dx.dtype), (dw[:ctx.V] * g).to(ctx.wdtype), *[None] * 7)
+        return (scaled_rows(dx, g), (dw[:ctx.V] * g).to(ctx.wdtype), *[None] * 7)
 
 
 def head_distill(x: torch.Tensor, weight: torch.Tensor, teacher_idx: torch.Tensor,

@@ -682,6 +682,24 @@ def test_head_is_the_loss_of_its_logits(chunk, wdt):
     assert rows.shape == (40,)
 
 
+def test_head_gradients_of_a_third():
+    """A loss divided by three: dx and dW are those of an incoming gradient of 1
+    times g in fp32, rounded once more (U, and half a step of bf16 for dx)."""
+    x, w, idx, t, target = _head_case(60, 64, 512, 6)
+    kw = dict(temperature=2.0, alpha=0.5)
+    w = w.float()
+    g = torch.tensor(1 / 3, device=DEV)
+
+    def grads(up):
+        xl, wl = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+        return torch.autograd.grad(head_distill(xl, wl, idx, t, target, **kw), (xl, wl), up)
+
+    for one, third in zip(grads(torch.ones_like(g)), grads(g)):
+        ref = one.double() * g.double()
+        tol = (torch.finfo(one.dtype).eps / 2 + U) * ref.abs()
+        _within(third, ref, tol + 1e-37, "a third")
+
+
 @pytest.mark.parametrize("V", [512, 515])
 def test_head_rows_that_do_not_count_may_hold_anything(V):
     """Rows of ignored targets with infinities and NaN: no share of the loss, and a
