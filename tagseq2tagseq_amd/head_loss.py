@@ -137,7 +137,7 @@ class HeadCEFn(torch.autograd.Function):
     @staticmethod
     def backward(ctx, g):
         dx, dw = ctx.saved_tensors
-        gx = dx * g.to(dx.dtype)
+        gx = scaled_rows(dx, g)
         gw = (dw[:ctx.V] * g).to(ctx.wdtype)
         return gx, gw, None, None, None
 

@@ -232,3 +232,36 @@ def test_head_loss_of_a_weight_on_another_device(V):
     w = torch.randn(V, 32, generator=g, device=DEV).to(torch.bfloat16)
     t = torch.randint(0, V, (40,), generator=g, device=DEV)
     assert torch.equal(head_loss_value(x, w.cpu(), t), head_loss_value(x, w, t))
+
+def test_gradients_of_a_third():
+    """A loss divided by three: dx and dW are those of an incoming gradient of 1
+    times g in fp32, rounded once more (2^-24, and half a step of bf16 for dx)."""
+    gen = torch.Generator().manual_seed(3)
+    x = torch.randn(60, 64, generator=gen).to(torch.bfloat16).to(DEV)
+    w = (torch.randn(512, 64, generator=gen) / 8).to(DEV)
+    t = torch.randint(0, 512, (60,), generator=gen).to(DEV)
+    g = torch.tensor(1 / 3, device=DEV)
+
+    def grads(up):
+        xl, wl = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+        return torch.autograd.grad(head_cross_entropy(xl, wl, t), (xl, wl), up)
+
+    for one, third in zip(grads(torch.ones_like(g)), grads(g)):
+        ref = one.double() * g.double()
+        tol = (torch.finfo(one.dtype).eps / 2 + 2.0 ** -24) * ref.abs() + 1e-37
+        assert bool(((third.double() - ref).abs() <= tol).all())
+
+
+def test_gradient_is_a_function_of_the_incoming_one():
+    """With create_graph, dx is recorded as g times the rows it scales."""
+    gen = torch.Generator().manual_seed(4)
+    x = torch.randn(9, 64, generator=gen).to(torch.bfloat16).to(DEV).requires_grad_(True)
+    w = (torch.randn(32, 64, generator=gen) / 8).to(torch.bfloat16).to(DEV)
+    t = torch.randint(0, 32, (9,), generator=gen).to(DEV)
+    (one,) = torch.autograd.grad(head_cross_entropy(x, w, t), x)
+    g = torch.tensor(0.3, device=DEV, requires_grad=True)
+    (dx,) = torch.autograd.grad(head_cross_entropy(x, w, t), x, g, create_graph=True)
+    (dg,) = torch.autograd.grad(dx.float().sum(), g)
+    # 576 terms, each rounded to bf16 at most once on the way, added in float32
+    size = one.double().abs().sum()
+    assert abs(float(dg) - float(one.double().sum())) <= float(size) * (2.0 ** -8 + 576 * 2.0 ** -24)
