@@ -393,6 +393,10 @@ Tensor qk_norm_rope_append(const Tensor& qkv_in, const Tensor& q_weight, const T
                                 pos.defined() ? pos.data_ptr<int64_t>() : nullptr, pos_sb,
                                 pos.defined() ? 0 : pos0, &qs, &ks, &vs, cap, stream_of(a.qkv)),
         "t2t_qk_norm_rope_append");
+  // written in place, which graphs that saved the caches have to see (inference
+  // tensors have no versions)
+  for (const Tensor* t : {&k_cache, &v_cache})
+    if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
   return q;
 }
 

@@ -389,6 +389,49 @@ def test_offsets_past_32_bits():
         assert torch.equal(a, b.detach())
 
 
+def _append_case():
+    qkv, qw, kw, cos, sin = _inputs(1, 2, 2, 2, 64, BF, BF, 6)
+    kc, vc = (torch.randn(1, 2, 8, 64, device=DEV).to(BF) for _ in range(2))
+    return (qkv, qw, kw, cos, sin), kc, vc
+
+
+@pytest.mark.parametrize("which", [0, 1])
+def test_append_is_seen_by_graphs_that_saved_the_cache(which):
+    """The append changes the caches in place: a graph that saved rows of one
+    refuses to be differentiated afterwards, as behind torch's own writes."""
+    args, *caches = _append_case()
+    w = torch.ones(64, device=DEV, dtype=BF, requires_grad=True)
+    y = (caches[which][:, :, 3:5] * w).sum()  # w's gradient needs the rows
+    at = torch.tensor([3, 4], device=DEV)
+    with torch.no_grad():
+        versions = [c._version for c in caches]
+        qk_norm_rope_append(*args, 2, at, *caches)
+        assert all(c._version > v for c, v in zip(caches, versions))
+    with pytest.raises(RuntimeError, match="modified"):
+        y.backward()
+    # a refused call changes nothing
+    versions = [c._version for c in caches]
+    with pytest.raises(ValueError, match="cache rows"):
+        qk_norm_rope_append(*args, 2, 7, *caches)
+    assert [c._version for c in caches] == versions
+
+
+def test_append_into_caches_made_for_inference():
+    """Inference tensors have no versions; a cache of them takes the append, in
+    and behind inference mode, and so does a plain cache in inference mode."""
+    args, kc, vc = _append_case()
+    want = [kc.clone(), vc.clone()]
+    qk_norm_rope_append(*args, 2, 1, *want)
+    with torch.inference_mode():
+        mine = [kc.clone(), vc.clone()]
+        qk_norm_rope_append(*args, 2, 1, *mine)
+        qk_norm_rope_append(*args, 2, 1, kc, vc)
+    with torch.no_grad():
+        qk_norm_rope_append(*args, 2, 1, *mine)
+    for a, b, c in zip(want, mine, (kc, vc)):
+        assert torch.equal(a, b) and torch.equal(a, c)
+
+
 def test_captured_append():
     B, M, H, D, cap = 1, 1, 4, 64, 32
     qkv, qw, kw, _, _ = _inputs(B, M, H, H, D, BF, BF, 0)
