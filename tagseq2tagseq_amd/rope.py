@@ -278,15 +278,17 @@ def qk_norm_rope_append(qkv: torch.Tensor, q_weight: torch.Tensor, k_weight: tor
     int64 tensor [M] or [B, M] of positions, read by the kernel (M at most 8).
     A device position outside the tables or the cache stores nothing and gives
     a query row of zeros; of rows at the same position the last is stored.
-    No gradient: for rows that autograd records, use ``qk_norm_rope``."""
+    No gradient: for rows that autograd records, use ``qk_norm_rope``; caches
+    that require one are refused too, except under torch.no_grad()."""
     rows = (qkv, q_weight, k_weight, cos, sin)
-    if (torch.is_grad_enabled() and any(t.requires_grad for t in rows)
+    tensors = (*rows, k_cache, v_cache)
+    if (torch.is_grad_enabled() and any(t.requires_grad for t in tensors)
             or forward_ad._current_level >= 0
-            and any(forward_ad.unpack_dual(t).tangent is not None for t in rows)):
+            and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors)):
         raise RuntimeError("qk_norm_rope_append has no gradient: call it under torch.no_grad()")
     at, pos0 = (pos, 0) if isinstance(pos, torch.Tensor) else (None, int(pos))
     args = (*rows, int(num_heads), at, pos0, k_cache, v_cache, float(eps))
-    watched = (*rows, k_cache, v_cache) if at is None else (*rows, k_cache, v_cache, at)
+    watched = tensors if at is None else (*tensors, at)
     if torch.compiler.is_compiling() or not _lib.only_recorded(*watched):
         return qk_norm_rope_append_op(*args)
     return _lib.host().qk_norm_rope_append(*args)

@@ -588,3 +588,16 @@ def test_refusals():
                             big.clone())
     with pytest.raises(RuntimeError, match="no gradient"):
         qk_norm_rope_append(qkv.requires_grad_(True), qw, kw, cos, sin, 2, 0, kc, vc)
+
+
+@pytest.mark.parametrize("which", [0, 1])
+def test_append_refuses_caches_with_a_gradient(which):
+    args, *caches = _append_case()
+    caches[which].requires_grad_(True)
+    before = [c.detach().clone() for c in caches]
+    with pytest.raises(RuntimeError, match="no gradient"):
+        qk_norm_rope_append(*args, 2, 1, *caches)
+    assert all(torch.equal(a, b) for a, b in zip(before, caches))
+    with torch.no_grad():  # as torch's own writes into a leaf
+        qk_norm_rope_append(*args, 2, 1, *caches)
+    assert not torch.equal(before[which], caches[which])
