@@ -118,6 +118,17 @@ class ScaledEmbedding(nn.Embedding):
                          dtype=dtype)
         self.scale = float(scale)
 
+    @classmethod
+    def from_pretrained(cls, embeddings: torch.Tensor, freeze: bool = True,
+                        padding_idx: Optional[int] = None,
+                        scale: float = 1.0) -> "ScaledEmbedding":
+        """A module of the table ``embeddings`` [V, C] itself."""
+        if embeddings.dim() != 2:
+            raise ValueError(f"embeddings must be [V, C], got shape {tuple(embeddings.shape)}")
+        m = cls(*embeddings.shape, scale, padding_idx, device="meta", dtype=embeddings.dtype)
+        m.weight = nn.Parameter(embeddings, requires_grad=not freeze)
+        return m
+
     def forward(self, tokens: torch.Tensor) -> torch.Tensor:
         if not self.weight.is_cuda:
             return super().forward(tokens) * self.scale

@@ -107,6 +107,21 @@ def test_shapes_of_the_traced_op():
         assert out.shape == (2, 3, 4)
 
 
+
+def test_module_from_a_table():
+    """nn.Embedding's constructor from a table, with the factor."""
+    w = torch.randn(7, 4)
+    m = ScaledEmbedding.from_pretrained(w, scale=3.0, padding_idx=-1)
+    t = torch.tensor([[1, 6], [0, 2]])
+    assert m.weight.data_ptr() == w.data_ptr() and not m.weight.requires_grad
+    assert (m.num_embeddings, m.embedding_dim, m.padding_idx, m.scale) == (7, 4, 6, 3.0)
+    assert torch.equal(m(t), w[t] * 3.0)
+    free = ScaledEmbedding.from_pretrained(w, freeze=False)
+    assert free.weight.requires_grad and free.scale == 1.0 and free.padding_idx is None
+    with pytest.raises(ValueError, match="V, C"):
+        ScaledEmbedding.from_pretrained(w[0])
+
+
 def test_module_on_the_cpu_and_in_the_training_module():
     m = ScaledEmbedding(7, 4, scale=3.0)
     t = torch.tensor([[1, 6], [0, 2]])
