@@ -166,9 +166,10 @@ void launch_tiles(const LinearArgs& p, hipStream_t stream) {
 }
 
 // The largest tile that still gives every CU work: 128 x 128 from two tiles
-// per CU (2048 x 4096 x 768: 21.1 us, 24.1 with 128 x 64; at 1.5 tiles per CU
-// 20.5 and 19.8), else 128 x 64 from one per CU (4096 x 768 x 768: 9.8 us,
-// 12.3 with 64 x 64; 2048 x 768 x 2048, 0.75 per CU: 16.0 and 12.7), else 64 x 64.  Two deep stages beat four shallow ones wherever a
+// per CU (2048 x 4096 x 768: 21.1 us, 24.1 with 128 x 64; 6.4e9 multiply-adds
+// in 1.5 tiles per CU: 20.5 and 19.8), else 128 x 64 from one per CU (4096 x
+// 768 x 768: 9.8 us, 12.3 with 64 x 64; 2048 x 768 x 2048, 0.75 per CU: 16.0
+// and 12.7), else 64 x 64.  Two deep stages beat four shallow ones wherever a
 // second work-group shares the CU (16384 x 2304 x 768: 70.9 against 89.1 us);
 // the gradient's 64 x 64 tiles, with their long contractions, want four
 // (512 x 768 x 4096: 19.5 against 24.6).
