@@ -342,8 +342,8 @@ __global__ __launch_bounds__(kGroupThreads) void embed_small_kernel(EmbedGradArg
       Pack<T, VEC> d[8];
 #pragma unroll
       for (int k = 0; k < 8; ++k)  // (behind the end: the last one again, unused)
-        d[k] = *reinterpret_cast<const Pack<T, VEC>*>(dy +
-                                                      (int64_t)list[min(s + k, e - 1)] * a.dy_stride);
+        d[k] = *reinterpret_cast<const Pack<T, VEC>*>(
+            dy + (int64_t)list[min(s + k, e - 1)] * a.dy_stride);
 #pragma unroll
       for (int k = 0; k < 8; ++k)
         if (s + k < e)
@@ -513,7 +513,8 @@ __global__ __launch_bounds__(64 * kJoinWaves) void embed_join_kernel(EmbedGradAr
     if (starts) {
       // Lane l: does piece + 1 + l start with the token?
       const int q = piece + 1 + lane;
-      const uint64_t more = __ballot(q < pieces && a.list[q < pieces ? (int64_t)q * S : e1].y == token);
+      const int64_t at = q < pieces ? (int64_t)q * S : e1;
+      const uint64_t more = __ballot(q < pieces && a.list[at].y == token);
       const int run = __ffsll((unsigned long long)~more) - 1;  // pieces behind; -1: 64 or more
       if (run < 0 || run >= kLongRun) {
         if (lane == 0) long_piece = piece;
@@ -670,7 +671,8 @@ bool embed_grad_fits(int64_t N, int64_t V, int C, bool f32, bool vector) {
 
 hipError_t launch_embed(const EmbedArgs& a, bool f32, bool vector, hipStream_t stream) {
   if (a.N == 0) return hipSuccess;
-  if (f32) return vector ? launch_embed_t<float, 4>(a, stream) : launch_embed_t<float, 1>(a, stream);
+  if (f32)
+    return vector ? launch_embed_t<float, 4>(a, stream) : launch_embed_t<float, 1>(a, stream);
   return vector ? launch_embed_t<__bf16, 8>(a, stream) : launch_embed_t<__bf16, 1>(a, stream);
 }
 

@@ -101,10 +101,12 @@ struct Place {
 };
 
 template <typename T>
-__global__ __launch_bounds__(kQkThreads, sizeof(T) == 4 ? 3 : 4) void qk_norm_rope_kernel(QkNormArgs a) {
+__global__ __launch_bounds__(kQkThreads, sizeof(T) == 4 ? 3 : 4)
+void qk_norm_rope_kernel(QkNormArgs a) {
   const Place at(a.lp_log2, a.tokens_log2, a.D);
   const int LP = 1 << a.lp_log2, half = at.half, j8 = at.j8;
-  const int64_t tokens = (int64_t)a.B * a.T, stride = (int64_t)gridDim.x * kQkWaves << a.tokens_log2;
+  const int64_t tokens = (int64_t)a.B * a.T;
+  const int64_t stride = (int64_t)gridDim.x * kQkWaves << a.tokens_log2;
   int64_t n0 = ((int64_t)blockIdx.x * kQkWaves + (threadIdx.x >> 6)) << a.tokens_log2;
   for (; n0 < tokens; n0 += stride) {
     const uint32_t n = (uint32_t)n0 + at.token;  // (at most 2^31 tokens)
@@ -300,7 +302,8 @@ __device__ __forceinline__ void bwd_rows(const QkNormBwdArgs& a, int which, uint
 }
 
 template <typename T>
-__global__ __launch_bounds__(kBwdThreads, sizeof(T) == 4 ? 3 : 4) void qk_norm_rope_bwd_kernel(QkNormBwdArgs a) {
+__global__ __launch_bounds__(kBwdThreads, sizeof(T) == 4 ? 3 : 4)
+void qk_norm_rope_bwd_kernel(QkNormBwdArgs a) {
   __shared__ float red[kBwdWaves][2 * 256];
   int which = 0;
   uint32_t group = blockIdx.x;

@@ -110,7 +110,9 @@ def embedding(tokens: torch.Tensor, weight: torch.Tensor, scale: float = 1.0,
 
 class ScaledEmbedding(nn.Embedding):
     """nn.Embedding (same parameters and state dict) with a factor on its rows,
-    on ``embedding``; a CPU table uses torch's lookup."""
+    on ``embedding``; a CPU table uses torch's lookup.  The table starts as
+    nn.Embedding's, N(0, 1): for rows of unit size behind the factor, and logits of
+    that size from a head that shares the table, multiply it by 1 / scale first."""
 
     def __init__(self, num_embeddings: int, embedding_dim: int, scale: float = 1.0,
                  padding_idx: Optional[int] = None, device=None, dtype=None):

@@ -216,7 +216,8 @@ class TS2TSTrainingModule(nn.Module):
                     distill_alpha: Optional[float] = None,
                     distill_temperature: float = 1.0) -> "TS2TSTrainingModule":
         """``qk_norm``: norms of the attention's query and key heads;
-        ``embedding_scale``: a factor on the embedding's rows (ScaledEmbedding);
+        ``embedding_scale``: a factor on the embedding's rows (ScaledEmbedding, whose
+        table starts at N(0, 1): multiply it by 1 / embedding_scale before training);
         ``distill_alpha``, ``distill_temperature``: the loss distils where a
         batch has a teacher's top logits (distill.LinearDistillLoss)."""
         backbone = TS2TSBackbone(num_layers=num_layers, model_dim=model_dim, num_heads=num_heads,
