@@ -700,6 +700,18 @@ def test_head_gradients_of_a_third():
         _within(third, ref, tol + 1e-37, "a third")
 
 
+def test_head_gradients_of_a_batch():
+    x, w, idx, t, target = _head_case(30, 64, 400, 5)
+    x.requires_grad_(True), w.requires_grad_(True)
+    loss = head_distill(x, w, idx, t, target, temperature=2.0, alpha=0.5)
+    many = torch.tensor([1.0, 1 / 3, -2.0], device=DEV)
+    dx, dw = torch.autograd.grad(loss, (x, w), many, is_grads_batched=True, retain_graph=True)
+    for i, g in enumerate(many):
+        a, b = torch.autograd.grad(loss, (x, w), g, retain_graph=True)
+        assert torch.equal(dx[i], a) and torch.equal(dw[i], b)
+
+
+
 @pytest.mark.parametrize("V", [512, 515])
 def test_head_rows_that_do_not_count_may_hold_anything(V):
     """Rows of ignored targets with infinities and NaN: no share of the loss, and a

@@ -264,4 +264,18 @@ def test_gradient_is_a_function_of_the_incoming_one():
     (dg,) = torch.autograd.grad(dx.float().sum(), g)
     # 576 terms, each rounded to bf16 at most once on the way, added in float32
     size = one.double().abs().sum()
-    assert abs(float(dg) - float(one.double().sum())) <= float(size) * (2.0 ** -8 + 576 * 2.0 ** -24)
+    tol = float(size) * (2.0 ** -8 + 576 * 2.0 ** -24)
+    assert abs(float(dg) - float(one.double().sum())) <= tol
+
+
+def test_batched_incoming_gradients():
+    gen = torch.Generator().manual_seed(5)
+    x = torch.randn(9, 64, generator=gen).to(torch.bfloat16).to(DEV).requires_grad_(True)
+    w = (torch.randn(32, 64, generator=gen) / 8).to(DEV).requires_grad_(True)
+    t = torch.randint(0, 32, (9,), generator=gen).to(DEV)
+    loss = head_cross_entropy(x, w, t)
+    many = torch.tensor([1.0, 1 / 3, -2.0], device=DEV)
+    dx, dw = torch.autograd.grad(loss, (x, w), many, is_grads_batched=True, retain_graph=True)
+    for i, g in enumerate(many):
+        a, b = torch.autograd.grad(loss, (x, w), g, retain_graph=True)
+        assert torch.equal(dx[i], a) and torch.equal(dw[i], b)

@@ -173,3 +173,18 @@ def test_gemm_tuning_file_has_validators_and_gfx950_shapes():
     assert any("50264" in s for s in shapes) and len(shapes) >= 10
     if not torch.cuda.is_available():
         assert gemm_tuning.use_tuned_gemms() is False
+
+
+def test_rows_scaled_by_the_incoming_gradient():
+    """In float32 with one rounding, recorded or not, and over a batch of gradients."""
+    from tagseq2tagseq_amd.head_loss import scaled_rows
+    torch.manual_seed(2)
+    dx, gs = torch.randn(5, 8).bfloat16(), torch.tensor([1.0, 1 / 3, -2.0])
+    want = torch.stack([(dx.float() * g).bfloat16() for g in gs])
+    with torch.no_grad():
+        assert torch.equal(torch.stack([scaled_rows(dx, g) for g in gs]), want)
+        assert torch.equal(torch.func.vmap(scaled_rows, (None, 0))(dx, gs), want)
+    g = gs[1].clone().requires_grad_(True)
+    got = scaled_rows(dx, g)
+    assert torch.equal(got.detach(), want[1])
+    assert torch.autograd.grad(got.sum(), g)[0].isfinite()
