@@ -372,6 +372,39 @@ int t2t_qk_norm_rope_backward(const t2t_tensor *dq, const t2t_tensor *dk, const 
                               void *workspace, int64_t workspace_bytes, void *stream);
 
 /*
+ * Attention prologue with any rotary form: the packed projection rows
+ * [Hq + 2 Hkv][D] (query heads, key heads, value heads) of B x T tokens to q,
+ * k, v, the first R dimensions of every query and key head rotated, the
+ * others and the values copied.  Pair i < R / 2 is (x[i], x[i + R/2]), or with
+ * interleaved != 0 (x[2i], x[2i + 1]); (a, b) becomes (a c + b s, b c - a s),
+ * c and s from table row p, in fp32 with one rounding.  p = pos0 + t, or int64
+ * pos[b pos_stride_b + t] on the device; such a position outside the table
+ * gives query and key rows of zeros.
+ *   qkv      dtype 0 = bf16, 1 = float32, strides in elements; 16-byte
+ *            aligned rows (views too).
+ *   cos, sin float32 [table_rows][R / 2], 16-byte aligned.
+ *   D        a multiple of 16, at most 512; R a multiple of 16, 16 <= R <= D.
+ *   q, k, v  [B, Hq | Hkv, T, D] views of the same dtype (out).
+ */
+int t2t_qkv_rotary(const void *qkv, int64_t stride_b, int64_t stride_t, int32_t B, int32_t T,
+                   int32_t Hq, int32_t Hkv, int32_t D, int32_t R, int32_t interleaved,
+                   int32_t dtype, const float *cos, const float *sin, int32_t table_rows,
+                   const int64_t *pos, int64_t pos_stride_b, int32_t pos0, const t2t_tensor *q,
+                   const t2t_tensor *k, const t2t_tensor *v, void *stream);
+
+/*
+ * Gradient of t2t_qkv_rotary: dqkv (its layout) from dq, dk, dv, every element
+ * written (not accumulated).  Tokens whose position has no table row get zeros
+ * in their query and key heads.
+ */
+int t2t_qkv_rotary_backward(const t2t_tensor *dq, const t2t_tensor *dk, const t2t_tensor *dv,
+                            void *dqkv, int64_t stride_b, int64_t stride_t, int32_t B, int32_t T,
+                            int32_t Hq, int32_t Hkv, int32_t D, int32_t R, int32_t interleaved,
+                            int32_t dtype, const float *cos, const float *sin, int32_t table_rows,
+                            const int64_t *pos, int64_t pos_stride_b, int32_t pos0,
+                            void *stream);
+
+/*
  * Scaled embedding lookup: out[i] = scale weight[tokens[i]] for N ids (int64),
  * computed in fp32 and rounded once; an id outside [0, V) gives a row of NaN.
  *   weight   [V][C], dtype 0 = bf16, 1 = float32, row stride weight_stride >= C

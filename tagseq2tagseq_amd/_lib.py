@@ -72,6 +72,10 @@ _SIGS = {
     "t2t_qk_norm_rope_backward_workspace": ([_I32] * 5, ctypes.c_int64),
     "t2t_qk_norm_rope_backward": ([_P] * 4 + [_I64, _I64] + [_I32] * 6 + [
         _P, _P, _I32, ctypes.c_float, _P, _P, _I32, _I32] + [_P] * 4 + [_I64, _P], ctypes.c_int),
+    "t2t_qkv_rotary": ([_P, _I64, _I64] + [_I32] * 8 + [_P, _P, _I32, _P, _I64, _I32] + [_P] * 4,
+                       ctypes.c_int),
+    "t2t_qkv_rotary_backward": ([_P] * 4 + [_I64, _I64] + [_I32] * 8 + [_P, _P, _I32, _P, _I64,
+                                _I32, _P], ctypes.c_int),
     "t2t_embedding": ([_P, _I64, _P, _I64, _I64, _I32, _I32, ctypes.c_float, _P, _P],
                       ctypes.c_int),
     "t2t_embedding_backward_workspace": ([_I64, _I64, _I32], ctypes.c_int64),

@@ -301,16 +301,24 @@ def flex_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
 class Rotary(nn.Module):
     """Rotary-embedding tables for [B, H, T, D] heads: half-split pairs, base
     10000, position = token index (float32 [max_seq_len, D/2] cos / sin, kept
-    in float32 whatever dtype the module is cast to)."""
+    in float32 whatever dtype the module is cast to); with ``form``
+    (rope.RotaryForm) that form's tables."""
 
-    def __init__(self, head_dim: int, max_seq_len: int, base: float = 10000.0):
+    def __init__(self, head_dim: int, max_seq_len: int, base: float = 10000.0, form=None):
         super().__init__()
         self.head_dim = head_dim
         self.max_seq_len = max_seq_len
-        self.base = base
+        self.base = base if form is None else form.base
+        self.form = form
+        # whether whole heads rotate half-split, as the prologues that fuse
+        # more than the rotation have it
+        self.whole_halves = form is None or (not form.interleaved
+                                             and form.dims(head_dim) == head_dim)
 
     def tables(self, device):
         from .rope import rope_tables
+        if self.form is not None:
+            return self.form.tables(self.head_dim, self.max_seq_len, device)
         return rope_tables(self.head_dim, self.max_seq_len, device, self.base)
 
 
@@ -329,13 +337,15 @@ class FlexSelfAttention(nn.Module):
 
     ``qk_norm=True`` RMS-normalises every query and key head before the
     rotation, in the same pass (rope.qk_norm_rope), with the weights
-    ``q_norm`` and ``k_norm`` [head_dim].
+    ``q_norm`` and ``k_norm`` [head_dim].  ``rotary`` (rope.RotaryForm): another
+    form of the rotary embedding (rope.qkv_rotary; with qk_norm, one that
+    rotates whole heads half-split).
     """
 
     NORM_EPS = 1e-6
 
     def __init__(self, dim: int, num_heads: int, max_seq_len: int, fp8_out_proj: bool = False,
-                 qk_norm: bool = False):
+                 qk_norm: bool = False, rotary=None):
         super().__init__()
         if dim % num_heads != 0:
             raise ValueError("dim must be divisible by num_heads")
@@ -344,7 +354,10 @@ class FlexSelfAttention(nn.Module):
         self.head_dim = dim // num_heads
         self.qkv = Linear(dim, 3 * dim, bias=False)
         self.proj = Linear(dim, dim, bias=False)
-        self.rotary = Rotary(self.head_dim, max_seq_len)
+        self.rotary = Rotary(self.head_dim, max_seq_len, form=rotary)
+        if qk_norm and not self.rotary.whole_halves:
+            raise ValueError("qk_norm=True rotates whole heads half-split: no interleaved or "
+                             "partial rotary form")
         self.qk_norm = qk_norm
         if qk_norm:
             self.q_norm = nn.Parameter(torch.ones(self.head_dim))
@@ -354,14 +367,21 @@ class FlexSelfAttention(nn.Module):
             warnings.warn("FlexSelfAttention(fp8_out_proj=True): the fp8 output projection is not "
                           "implemented; the projection runs in the module's dtype", stacklevel=2)
 
-    def forward(self, x: torch.Tensor, block_mask: T2TBlockMask) -> torch.Tensor:
-        from .rope import qk_norm_rope, qkv_rope
-        B, T, C = x.shape
-        cos, sin = self.rotary.tables(x.device)
+    def heads(self, qkv: torch.Tensor, pos0: int = 0):
+        """q, k, v [B, H, T, D] of projected rows [B, T, 3 C] at positions pos0 ..
+        pos0 + T - 1: split, normed (qk_norm) and rotated."""
+        from .rope import qk_norm_rope, qkv_rope, qkv_rotary
+        cos, sin = self.rotary.tables(qkv.device)
         if self.qk_norm:
-            q, k, v = qk_norm_rope(self.qkv(x), self.q_norm, self.k_norm, cos, sin,
-                                   self.num_heads, eps=self.NORM_EPS)
-        else:
-            q, k, v = qkv_rope(self.qkv(x), cos, sin, self.num_heads)
+            return qk_norm_rope(qkv, self.q_norm, self.k_norm, cos, sin, self.num_heads,
+                                pos0=pos0, eps=self.NORM_EPS)
+        if self.rotary.whole_halves:
+            return qkv_rope(qkv, cos, sin, self.num_heads, pos0)
+        return qkv_rotary(qkv, cos, sin, self.num_heads, pos=pos0,
+                          interleaved=self.rotary.form.interleaved)
+
+    def forward(self, x: torch.Tensor, block_mask: T2TBlockMask) -> torch.Tensor:
+        B, T, C = x.shape
+        q, k, v = self.heads(self.qkv(x))
         y = flex_attention(q, k, v, block_mask=block_mask)
         return self.proj(y.transpose(1, 2).reshape(B, T, C))

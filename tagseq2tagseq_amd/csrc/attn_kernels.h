@@ -147,6 +147,25 @@ hipError_t launch_qk_norm_rope(QkNormArgs a, bool f32, hipStream_t stream);
 hipError_t launch_qk_norm_rope_bwd(QkNormBwdArgs a, bool f32, void* dqw, void* dkw,
                                    hipStream_t stream);
 
+// Prologue with any rotary form: packed rows [B][T][(Hq + 2 Hkv) D] to q, k, v
+// views (or their gradients to packed rows), the first R dimensions of query
+// and key heads rotated.
+struct RotaryArgs {
+  void* packed;         // read by the forward, written by the backward
+  int64_t p_sb, p_st;
+  TensorView ops[3];    // q, k, v
+  const float* cos;     // [rows][R / 2]
+  const float* sin;
+  const int64_t* pos;   // [B or 1][T] positions (batch stride pos_sb), or NULL for pos0 + t
+  int64_t pos_sb;
+  int pos0, rows;       // positions outside [0, rows) have no table row
+  int B, T, Hq, Hkv, D, R;
+  bool interleaved;
+  int tokens, per_token;  // tokens a wave, lane groups a token; set by the launcher
+};
+
+hipError_t launch_rotary(RotaryArgs a, bool f32, bool backward, hipStream_t stream);
+
 // Scaled embedding lookup: out[i] = scale W[tokens[i]] (rows of C, contiguous
 // out); ids outside [0, V) give NaN rows.  vector: rows in 16-byte pieces.
 struct EmbedArgs {

@@ -721,6 +721,88 @@ int t2t_qk_norm_rope_backward(const t2t_tensor* dq, const t2t_tensor* dk, const 
 
 namespace {
 
+// Both directions of the rotary prologue; `packed` is read or written.
+int rotary(bool backward, void* packed, int64_t stride_b, int64_t stride_t, int32_t B, int32_t T,
+           int32_t Hq, int32_t Hkv, int32_t D, int32_t R, int32_t interleaved, int32_t dtype,
+           const float* cos, const float* sin, int32_t table_rows, const int64_t* pos,
+           int64_t pos_stride_b, int32_t pos0, const t2t_tensor* q, const t2t_tensor* k,
+           const t2t_tensor* v, void* stream) {
+  if (B < 0 || T < 0 || Hq < 1 || Hkv < 1)
+    return fail(T2T_EINVAL, "B=%d T=%d Hq=%d Hkv=%d", B, T, Hq, Hkv);
+  if (D < 16 || D > 512 || D % 16 != 0)
+    return fail(T2T_EUNSUPPORTED, "head dim D=%d (a multiple of 16, at most 512)", D);
+  if (R < 16 || R > D || R % 16 != 0)
+    return fail(T2T_EUNSUPPORTED, "%d rotated dimensions (a multiple of 16, at most D=%d)", R, D);
+  if (dtype != T2T_DTYPE_BF16 && dtype != T2T_DTYPE_F32)
+    return fail(T2T_EUNSUPPORTED, "dtype %d not supported here", dtype);
+  // (with the tokens past the end that a last wave's lanes number)
+  if ((int64_t)B * T > 0x7fffffffLL - 64 || (int64_t)Hq + 2 * (int64_t)Hkv > 1 << 20)
+    return fail(T2T_EUNSUPPORTED, "B=%d T=%d Hq=%d Hkv=%d: more tokens or heads than one launch "
+                "numbers", B, T, Hq, Hkv);
+  if (table_rows < 0) return fail(T2T_EINVAL, "negative table_rows");
+  if (pos) {
+    if (reinterpret_cast<uintptr_t>(pos) % 8 || pos_stride_b < 0)
+      return fail(T2T_EINVAL, "pos misaligned or with a negative stride");
+  } else if (pos0 < 0 || (int64_t)pos0 + T > table_rows) {
+    return fail(T2T_EINVAL, "positions %d..%lld exceed the %d table rows", pos0,
+                (long long)pos0 + T - 1, table_rows);
+  }
+  if (B == 0 || T == 0) return T2T_OK;
+  const int64_t align = dtype == T2T_DTYPE_F32 ? 4 : 8;
+  if (!packed || reinterpret_cast<uintptr_t>(packed) % 16 || stride_b < 0 || stride_t < 0 ||
+      stride_b % align || stride_t % align)
+    return fail(T2T_EINVAL, "qkv rows must start on 16-byte boundaries");
+  if (!cos || !sin || (reinterpret_cast<uintptr_t>(cos) | reinterpret_cast<uintptr_t>(sin)) % 16)
+    return fail(T2T_EINVAL, "cos / sin NULL or not 16-byte aligned");
+  if (int rc = check_head_views({q, k, v}, dtype)) return rc;
+  // rows that are written must not be one another's
+  const auto overlap = [](int64_t n, int64_t stride) { return n > 1 && stride == 0; };
+  if (backward) {
+    if (overlap(B, stride_b) || overlap(T, stride_t))
+      return fail(T2T_EINVAL, "dqkv rows overlap (stride 0)");
+  } else {
+    const int32_t heads[3] = {Hq, Hkv, Hkv};
+    const t2t_tensor* const views[3] = {q, k, v};
+    for (int i = 0; i < 3; ++i)
+      if (overlap(B, views[i]->stride_b) || overlap(heads[i], views[i]->stride_h) ||
+          overlap(T, views[i]->stride_t))
+        return fail(T2T_EINVAL, "q / k / v rows overlap (stride 0)");
+  }
+  t2t::RotaryArgs a{};
+  a.packed = packed; a.p_sb = stride_b; a.p_st = stride_t;
+  a.ops[0] = as_view(q); a.ops[1] = as_view(k); a.ops[2] = as_view(v);
+  a.cos = cos; a.sin = sin; a.pos = pos; a.pos_sb = pos_stride_b; a.pos0 = pos0;
+  a.rows = table_rows; a.interleaved = interleaved != 0;
+  a.B = B; a.T = T; a.Hq = Hq; a.Hkv = Hkv; a.D = D; a.R = R;
+  return hip_status(t2t::launch_rotary(a, dtype == T2T_DTYPE_F32, backward,
+                                       static_cast<hipStream_t>(stream)),
+                    backward ? "t2t_qkv_rotary_backward launch" : "t2t_qkv_rotary launch");
+}
+
+}  // namespace
+
+int t2t_qkv_rotary(const void* qkv, int64_t stride_b, int64_t stride_t, int32_t B, int32_t T,
+                   int32_t Hq, int32_t Hkv, int32_t D, int32_t R, int32_t interleaved,
+                   int32_t dtype, const float* cos, const float* sin, int32_t table_rows,
+                   const int64_t* pos, int64_t pos_stride_b, int32_t pos0, const t2t_tensor* q,
+                   const t2t_tensor* k, const t2t_tensor* v, void* stream) {
+  return rotary(false, const_cast<void*>(qkv), stride_b, stride_t, B, T, Hq, Hkv, D, R,
+                interleaved, dtype, cos, sin, table_rows, pos, pos_stride_b, pos0, q, k, v,
+                stream);
+}
+
+int t2t_qkv_rotary_backward(const t2t_tensor* dq, const t2t_tensor* dk, const t2t_tensor* dv,
+                            void* dqkv, int64_t stride_b, int64_t stride_t, int32_t B, int32_t T,
+                            int32_t Hq, int32_t Hkv, int32_t D, int32_t R, int32_t interleaved,
+                            int32_t dtype, const float* cos, const float* sin, int32_t table_rows,
+                            const int64_t* pos, int64_t pos_stride_b, int32_t pos0,
+                            void* stream) {
+  return rotary(true, dqkv, stride_b, stride_t, B, T, Hq, Hkv, D, R, interleaved, dtype, cos, sin,
+                table_rows, pos, pos_stride_b, pos0, dq, dk, dv, stream);
+}
+
+namespace {
+
 constexpr int64_t kEmbedMaxV = 1 << 20;
 
 int check_embed(const void* tokens, int64_t N, int64_t V, int32_t C, int32_t dtype) {

@@ -400,6 +400,115 @@ Tensor qk_norm_rope_append(const Tensor& qkv_in, const Tensor& q_weight, const T
   return q;
 }
 
+// ---- QKV split + any rotary form
+
+// What both directions take, checked: tables, head counts and positions (pos:
+// int64 [T] or [B, T] on the device, or undefined for pos0 + t).
+struct Rotary {
+  Tensor cos, sin, pos;
+  int64_t B = 0, T = 0, H = 0, Hkv = 0, D = 0, R = 0, pos_sb = 0;
+  int code = 0;
+  Rotary(const Tensor& rows, int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads,
+         int64_t head_dim, const Tensor& cos_in, const Tensor& sin_in,
+         const c10::optional<Tensor>& pos_in, int64_t pos0)
+      : B(batch), T(tokens), H(heads), Hkv(kv_heads), D(head_dim) {
+    TORCH_CHECK_NOT_IMPLEMENTED(
+        rows.scalar_type() == at::kBFloat16 || rows.scalar_type() == at::kFloat, "dtype ",
+        rows.scalar_type(), " is not supported (bfloat16 or float32)");
+    code = rows.scalar_type() == at::kFloat ? T2T_DTYPE_F32 : T2T_DTYPE_BF16;
+    TORCH_CHECK_VALUE(cos_in.dim() == 2 && sin_in.sizes() == cos_in.sizes() &&
+                          cos_in.size(1) >= 1 && cos_in.size(1) <= D / 2 &&
+                          cos_in.scalar_type() == at::kFloat &&
+                          sin_in.scalar_type() == at::kFloat,
+                      "cos ", cos_in.sizes(), " and sin ", sin_in.sizes(),
+                      " must be float32 [rows, R / 2] with R at most head_dim=", D);
+    need_gpu(rows, cos_in, sin_in);
+    TORCH_CHECK_VALUE(cos_in.device() == rows.device() && sin_in.device() == rows.device(),
+                      "operands on different devices");
+    const c10::DeviceGuard guard(rows.device());
+    cos = vector_rows(cos_in.contiguous());
+    sin = vector_rows(sin_in.contiguous());
+    R = 2 * cos.size(1);
+    TORCH_CHECK_VALUE(B <= INT32_MAX && T <= INT32_MAX && H <= INT32_MAX && D <= INT32_MAX,
+                      "rows ", rows.sizes(), " are too large");
+    if (pos_in.has_value()) {
+      TORCH_CHECK_VALUE(pos_in->is_cuda() && pos_in->device() == rows.device() &&
+                            pos_in->scalar_type() == at::kLong,
+                        "pos must be an int64 tensor on the rows' device");
+      const bool each = pos_in->dim() == 2;
+      TORCH_CHECK_VALUE((pos_in->dim() == 1 && pos_in->size(0) == T) ||
+                            (each && pos_in->size(0) == B && pos_in->size(1) == T),
+                        "pos ", pos_in->sizes(), " must be [", T, "] or [", B, ", ", T, "]");
+      pos = pos_in->contiguous();
+      pos_sb = each ? T : 0;
+    } else {
+      TORCH_CHECK_VALUE(pos0 >= 0 && pos0 <= rows_() && pos0 + T <= rows_(), "positions ", pos0,
+                        " .. ", pos0 + T - 1, " exceed the ", rows_(), " table rows");
+    }
+  }
+  int64_t rows_() const { return std::min<int64_t>(cos.size(0), INT32_MAX); }
+  const int64_t* positions() const {
+    return pos.defined() && pos.numel() ? pos.data_ptr<int64_t>() : nullptr;
+  }
+};
+
+std::tuple<Tensor, Tensor, Tensor> qkv_rotary(const Tensor& qkv_in, const Tensor& cos_in,
+                                              const Tensor& sin_in, int64_t heads,
+                                              int64_t kv_heads,
+                                              const c10::optional<Tensor>& pos_in, int64_t pos0,
+                                              bool interleaved) {
+  TORCH_CHECK_VALUE(qkv_in.dim() == 3, "qkv must be [B, T, (H + 2 Hkv) D], got shape ",
+                    qkv_in.sizes());
+  TORCH_CHECK_VALUE(heads > 0 && kv_heads > 0, "num_heads=", heads, " and num_kv_heads=", kv_heads,
+                    " must be positive");
+  // (as a quotient: twice a huge count would not fit)
+  TORCH_CHECK_VALUE(heads <= qkv_in.size(2) && kv_heads <= qkv_in.size(2) &&
+                        qkv_in.size(2) % (heads + 2 * kv_heads) == 0,
+                    "last dim ", qkv_in.size(2), " is not (num_heads + 2 num_kv_heads) * "
+                    "head_dim (num_heads=", heads, ", num_kv_heads=", kv_heads, ")");
+  const Rotary a(qkv_in, qkv_in.size(0), qkv_in.size(1), heads, kv_heads,
+                 qkv_in.size(2) / (heads + 2 * kv_heads), cos_in, sin_in, pos_in, pos0);
+  const c10::DeviceGuard guard(qkv_in.device());
+  const Tensor qkv = vector_rows(qkv_in);
+  Tensor q = at::empty({a.B, a.H, a.T, a.D}, qkv.options()),
+         k = at::empty({a.B, a.Hkv, a.T, a.D}, qkv.options()), v = at::empty_like(k);
+  if (q.numel() == 0) return {q, k, v};
+  const t2t_tensor qs = heads_of(q), ks = heads_of(k), vs = heads_of(v);
+  check(t2t_qkv_rotary(qkv.data_ptr(), a.B == 1 ? 0 : qkv.stride(0), a.T == 1 ? 0 : qkv.stride(1),
+                       a.B, a.T, a.H, a.Hkv, a.D, a.R, interleaved, a.code,
+                       a.cos.data_ptr<float>(), a.sin.data_ptr<float>(), a.rows_(), a.positions(),
+                       a.pos_sb, pos0, &qs, &ks, &vs, stream_of(qkv)),
+        "t2t_qkv_rotary");
+  return {q, k, v};
+}
+
+Tensor qkv_rotary_backward(const Tensor& dq_in, const Tensor& dk_in, const Tensor& dv_in,
+                           const Tensor& cos_in, const Tensor& sin_in,
+                           const c10::optional<Tensor>& pos_in, int64_t pos0, bool interleaved) {
+  TORCH_CHECK_VALUE(dq_in.dim() == 4 && dk_in.dim() == 4 && dk_in.sizes() == dv_in.sizes() &&
+                        dk_in.size(0) == dq_in.size(0) &&
+                        dk_in.sizes().slice(2) == dq_in.sizes().slice(2),
+                    "gradients ", dq_in.sizes(), ", ", dk_in.sizes(), ", ", dv_in.sizes(),
+                    " must be [B, H, T, D] and twice [B, Hkv, T, D]");
+  need_gpu(dq_in, dk_in, dv_in);
+  for (const Tensor* t : {&dk_in, &dv_in})
+    TORCH_CHECK_VALUE(t->scalar_type() == dq_in.scalar_type() && t->device() == dq_in.device(),
+                      "the gradients differ in dtype or device");
+  const Rotary a(dq_in, dq_in.size(0), dq_in.size(2), dq_in.size(1), dk_in.size(1), dq_in.size(3),
+                 cos_in, sin_in, pos_in, pos0);
+  const c10::DeviceGuard guard(dq_in.device());
+  const Tensor dq = vector_rows(dq_in), dk = vector_rows(dk_in), dv = vector_rows(dv_in);
+  Tensor dqkv = at::empty({a.B, a.T, (a.H + 2 * a.Hkv) * a.D}, dq.options());
+  if (dqkv.numel() == 0) return dqkv;
+  const t2t_tensor qs = heads_of(dq), ks = heads_of(dk), vs = heads_of(dv);
+  check(t2t_qkv_rotary_backward(&qs, &ks, &vs, dqkv.data_ptr(), dqkv.stride(0), dqkv.stride(1),
+                                a.B, a.T, a.H, a.Hkv, a.D, a.R, interleaved, a.code,
+                                a.cos.data_ptr<float>(), a.sin.data_ptr<float>(), a.rows_(),
+                                a.positions(), a.pos_sb, pos0, stream_of(dq)),
+        "t2t_qkv_rotary_backward");
+  return dqkv;
+}
+
 // ---- scaled embedding
 
 int embed_code(const Tensor& w) {
@@ -863,6 +972,70 @@ std::tuple<Tensor, Tensor, Tensor> qk_norm_rope_ad(const Tensor& qkv, const Tens
   return {o[0], o[1], o[2]};
 }
 
+// The rotation is linear, so each direction's gradient is the other one, and
+// both may be differentiated again.
+struct RotaryAd {
+  using Pos = c10::optional<Tensor>;
+  static void keep(AutogradContext* ctx, const Tensor& cos, const Tensor& sin, const Pos& pos,
+                   std::vector<int64_t> n) {
+    ctx->save_for_backward({cos, sin, pos.has_value() ? *pos : Tensor()});
+    ctx->saved_data["n"] = std::move(n);
+  }
+  struct Kept {
+    variable_list t;
+    std::vector<int64_t> n;  // heads, kv_heads, pos0, interleaved
+    Pos pos;
+    explicit Kept(AutogradContext* ctx)
+        : t(ctx->get_saved_variables()), n(ctx->saved_data["n"].toIntVector()) {
+      if (t[2].defined()) pos = t[2];
+    }
+  };
+  struct Forward : torch::autograd::Function<Forward> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& qkv, const Tensor& cos,
+                                 const Tensor& sin, int64_t heads, int64_t kv_heads,
+                                 const Pos& pos, int64_t pos0, bool interleaved) {
+      keep(ctx, cos, sin, pos, {heads, kv_heads, pos0, interleaved});
+      auto [q, k, v] = qkv_rotary(qkv, cos, sin, heads, kv_heads, pos, pos0, interleaved);
+      return {q, k, v};
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list g) {
+      const Kept a(ctx);
+      variable_list d(8);
+      d[0] = c10::GradMode::is_enabled()
+                 ? Backward::apply(g[0], g[1], g[2], a.t[0], a.t[1], a.pos, a.n[0], a.n[1], a.n[2],
+                                   a.n[3] != 0)
+                 : qkv_rotary_backward(g[0], g[1], g[2], a.t[0], a.t[1], a.pos, a.n[2],
+                                       a.n[3] != 0);
+      return d;
+    }
+  };
+  struct Backward : torch::autograd::Function<Backward> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& dq, const Tensor& dk,
+                          const Tensor& dv, const Tensor& cos, const Tensor& sin, const Pos& pos,
+                          int64_t heads, int64_t kv_heads, int64_t pos0, bool interleaved) {
+      keep(ctx, cos, sin, pos, {heads, kv_heads, pos0, interleaved});
+      return qkv_rotary_backward(dq, dk, dv, cos, sin, pos, pos0, interleaved);
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list g) {
+      const Kept a(ctx);
+      variable_list d =
+          Forward::apply(g[0], a.t[0], a.t[1], a.n[0], a.n[1], a.pos, a.n[2], a.n[3] != 0);
+      d.resize(10);
+      return d;
+    }
+  };
+};
+
+std::tuple<Tensor, Tensor, Tensor> qkv_rotary_ad(const Tensor& qkv, const Tensor& cos,
+                                                 const Tensor& sin, int64_t heads,
+                                                 int64_t kv_heads,
+                                                 const c10::optional<Tensor>& pos, int64_t pos0,
+                                                 bool interleaved) {
+  variable_list o =
+      RotaryAd::Forward::apply(qkv, cos, sin, heads, kv_heads, pos, pos0, interleaved);
+  return {o[0], o[1], o[2]};
+}
+
 struct EmbeddingAd : torch::autograd::Function<EmbeddingAd> {
   static Tensor forward(AutogradContext* ctx, const Tensor& tokens, const Tensor& weight,
                         double scale, int64_t padding) {
@@ -1001,6 +1174,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("qk_norm_rope_backward", &qk_norm_rope_backward, no_gil);
   m.def("qk_norm_rope_append", &qk_norm_rope_append, no_gil);
   m.def("qk_norm_rope_ad", &qk_norm_rope_ad, no_gil);
+  m.def("qkv_rotary", &qkv_rotary, no_gil);
+  m.def("qkv_rotary_backward", &qkv_rotary_backward, no_gil);
+  m.def("qkv_rotary_ad", &qkv_rotary_ad, no_gil);
   m.def("embedding_ad", &embedding_ad, no_gil);
   m.def("distill_loss_ad", &distill_loss_ad, no_gil);
   m.def("embedding", &embedding, no_gil);

@@ -135,10 +135,11 @@ class TS2TSModel:
                     block_mask_creator: Callable, fp8: bool = False, weight_tying: bool = True,
                     ignore_index: int = -100, tokenizer=None, link_detector=None,
                     layout_policy=None, qk_norm: bool = False,
-                    embedding_scale: Optional[float] = None) -> "TS2TSModel":
+                    embedding_scale: Optional[float] = None, rotary=None) -> "TS2TSModel":
         backbone = TS2TSBackbone(num_layers=num_layers, model_dim=model_dim, num_heads=num_heads,
                                  max_seq_len=max_seq_len, dropout=dropout,
-                                 drop_path_rate=drop_path_rate, fp8=fp8, qk_norm=qk_norm)
+                                 drop_path_rate=drop_path_rate, fp8=fp8, qk_norm=qk_norm,
+                                 rotary=rotary)
         table = nn.Embedding(vocab_size, model_dim)
         norm = RMSNorm(model_dim)
         if weight_tying:

@@ -91,15 +91,15 @@ class DropPath(nn.Module):
 
 class Layer(nn.Module):
     """model/modules/layer.py:11-35; ``qk_norm``: norms of the attention's query
-    and key heads (FlexSelfAttention)."""
+    and key heads, ``rotary``: form of the rotary embedding (FlexSelfAttention)."""
 
     def __init__(self, n_embd: int, n_head: int, dropout: float, max_seq_len: int, fp8: bool,
-                 drop_path_rate: float, qk_norm: bool = False):
+                 drop_path_rate: float, qk_norm: bool = False, rotary=None):
         super().__init__()
         self.drop_path = DropPath(drop_path_rate)
         self.ln_1 = RMSNorm(n_embd)
         self.attn = FlexSelfAttention(dim=n_embd, num_heads=n_head, max_seq_len=max_seq_len,
-                                      fp8_out_proj=fp8, qk_norm=qk_norm)
+                                      fp8_out_proj=fp8, qk_norm=qk_norm, rotary=rotary)
         self.ln_2 = RMSNorm(n_embd)
         self.mlp = GLU(in_dim=n_embd, out_dim=n_embd, hidden_dim=int(8 / 3 * n_embd),
                        activation="silu", dropout=dropout, fp8=fp8)
@@ -117,13 +117,14 @@ class TS2TSBackbone(nn.Module):
 
     def __init__(self, num_layers: int, model_dim: int, num_heads: int, max_seq_len: int,
                  dropout: float, drop_path_rate: float, fp8: bool = False,
-                 activation_checkpointing: bool = False, qk_norm: bool = False, **kwargs):
+                 activation_checkpointing: bool = False, qk_norm: bool = False, rotary=None,
+                 **kwargs):
         super().__init__()
         self.model_dim = model_dim
         self.max_seq_len = max_seq_len
         self.layers = nn.ModuleList([
             Layer(n_embd=model_dim, n_head=num_heads, max_seq_len=max_seq_len, dropout=dropout,
-                  drop_path_rate=drop_path_rate, fp8=fp8, qk_norm=qk_norm)
+                  drop_path_rate=drop_path_rate, fp8=fp8, qk_norm=qk_norm, rotary=rotary)
             for _ in range(num_layers)])
         self.skip_weights = nn.Parameter(torch.ones(num_layers // 2))
         self.activation_checkpointing = activation_checkpointing
@@ -214,8 +215,9 @@ class TS2TSTrainingModule(nn.Module):
                     activation_checkpointing: bool = False, qk_norm: bool = False,
                     embedding_scale: Optional[float] = None,
                     distill_alpha: Optional[float] = None,
-                    distill_temperature: float = 1.0) -> "TS2TSTrainingModule":
-        """``qk_norm``: norms of the attention's query and key heads;
+                    distill_temperature: float = 1.0, rotary=None) -> "TS2TSTrainingModule":
+        """``qk_norm``: norms of the attention's query and key heads; ``rotary``:
+        form of the rotary embedding (rope.RotaryForm);
         ``embedding_scale``: a factor on the embedding's rows (ScaledEmbedding, whose
         table starts at N(0, 1): multiply it by 1 / embedding_scale before training);
         ``distill_alpha``, ``distill_temperature``: the loss distils where a
@@ -224,7 +226,7 @@ class TS2TSTrainingModule(nn.Module):
                                  max_seq_len=max_seq_len, dropout=dropout,
                                  drop_path_rate=drop_path_rate, fp8=fp8,
                                  activation_checkpointing=activation_checkpointing,
-                                 qk_norm=qk_norm)
+                                 qk_norm=qk_norm, rotary=rotary)
         embedding = (nn.Embedding(vocab_size, model_dim) if embedding_scale is None else
                      ScaledEmbedding(vocab_size, model_dim, embedding_scale))
         norm = RMSNorm(model_dim)

@@ -23,9 +23,21 @@ logits bounded), and with fewer key / value heads than query heads:
 
 Kernels: ``t2t_qk_norm_rope``, ``t2t_qk_norm_rope_backward`` and
 ``t2t_qk_norm_rope_append`` (bf16 and float32).
+
+Other forms of the rotation -- interleaved pairs, the first dimensions of the
+head only, a position per token, tables scaled for contexts longer than the
+trained ones:
+
+    cos, sin = rotary_tables(rotary_dim, rows, device, scaling="by_parts", factor=4.0,
+                             original_len=8192)
+    q, k, v = qkv_rotary(qkv, cos, sin, num_heads, pos=positions, interleaved=True)
+
+Kernels: ``t2t_qkv_rotary`` and ``t2t_qkv_rotary_backward`` (bf16 and float32).
 """
 from __future__ import annotations
 
+import math
+from dataclasses import dataclass
 from typing import Dict, Optional, Tuple, Union
 
 import torch
@@ -34,7 +46,7 @@ from torch.autograd.function import once_differentiable
 
 from . import _lib
 
-_TABLES: Dict[Tuple[int, int, float, str], Tuple[torch.Tensor, torch.Tensor]] = {}
+_TABLES: Dict[Tuple, Tuple[torch.Tensor, torch.Tensor]] = {}
 
 
 def rope_tables(head_dim: int, rows: int, device, base: float = 10000.0):
@@ -47,6 +59,98 @@ def rope_tables(head_dim: int, rows: int, device, base: float = 10000.0):
         ang = torch.outer(torch.arange(rows, dtype=torch.float32), inv)
         _TABLES[key] = (ang.cos().to(device), ang.sin().to(device))
     return _TABLES[key]
+
+
+SCALINGS = ("linear", "base", "by_parts")
+
+
+def _rotary_angles(rotary_dim: int, rows: int, base: float, scaling: Optional[str], factor: float,
+                   original_len: int, fast: float, slow: float) -> torch.Tensor:
+    """Angles float64 [rows, rotary_dim / 2]; see rotary_tables."""
+    half = rotary_dim // 2
+    i = torch.arange(half, dtype=torch.float64)
+    if scaling == "base":
+        base = base * factor ** (rotary_dim / (rotary_dim - 2))
+    inv = base ** (-i / half)
+    if scaling == "linear":
+        inv = inv / factor
+    elif scaling == "by_parts":
+        turns = original_len * inv / (2 * math.pi)
+        keep = ((turns - slow) / (fast - slow)).clamp(0, 1)
+        inv = inv / factor * (1 - keep) + inv * keep
+    return torch.outer(torch.arange(rows, dtype=torch.float64), inv)
+
+
+def rotary_tables(rotary_dim: int, rows: int, device, base: float = 10000.0,
+                  scaling: Optional[str] = None, factor: float = 1.0, original_len: int = 0,
+                  fast: float = 32.0, slow: float = 1.0, magnitude: Optional[float] = None):
+    """(cos, sin) float32 [rows, rotary_dim / 2], the angles p * base^(-2 i /
+    rotary_dim) computed in float64 (a far position's angle keeps its fraction
+    of a turn).  Cached per arguments.
+
+    ``scaling`` fits a context ``factor`` times the trained one:
+      * "linear": every angle divided by factor (position interpolation);
+      * "base": base * factor^(rotary_dim / (rotary_dim - 2)), which divides the
+        slowest pair's angle by factor and leaves the fastest as it is;
+      * "by_parts": pairs that turn more than ``fast`` times over
+        ``original_len`` positions are left, those that turn less than ``slow``
+        times divided by factor, with a linear ramp over the turns between
+        (the interpolation by parts of the YaRN paper).
+    ``magnitude`` multiplies both tables; None is 1, or for "by_parts" the same
+    paper's 1 + 0.1 ln(factor), which sharpens the softmax as contexts grow."""
+    if rotary_dim < 2 or rotary_dim % 2 or rows < 0:
+        raise ValueError(f"rotary_dim={rotary_dim} must be even and positive, rows={rows} not "
+                         "negative")
+    if not (math.isfinite(base) and base > 0):
+        raise ValueError(f"base={base!r} must be positive and finite")
+    if scaling is None:
+        if factor != 1.0:
+            raise ValueError(f"factor={factor!r} needs a scaling ({', '.join(SCALINGS)})")
+    elif scaling not in SCALINGS:
+        raise ValueError(f"scaling={scaling!r} is none of {', '.join(SCALINGS)}")
+    if not (math.isfinite(factor) and factor >= 1.0):
+        raise ValueError(f"factor={factor!r} must be at least 1 and finite")
+    if scaling == "base" and rotary_dim < 4:
+        raise ValueError('scaling="base" needs rotary_dim of 4 or more')
+    if scaling == "by_parts" and not (original_len > 0 and 0 <= slow < fast
+                                      and math.isfinite(fast)):
+        raise ValueError(f'scaling="by_parts" needs original_len > 0 and 0 <= slow < fast, got '
+                         f"{original_len}, {slow!r}, {fast!r}")
+    if magnitude is None:
+        magnitude = 1.0 + 0.1 * math.log(factor) if scaling == "by_parts" else 1.0
+    if not math.isfinite(magnitude):
+        raise ValueError(f"magnitude={magnitude!r} must be finite")
+    key = ("rotary", rotary_dim, rows, float(base), scaling, float(factor), original_len,
+           float(fast), float(slow), float(magnitude), str(torch.device(device)))
+    if key not in _TABLES:
+        ang = _rotary_angles(rotary_dim, rows, base, scaling, factor, original_len, fast, slow)
+        _TABLES[key] = tuple((f * magnitude).float().to(device) for f in (ang.cos(), ang.sin()))
+    return _TABLES[key]
+
+
+@dataclass(frozen=True)
+class RotaryForm:
+    """A module's form of the rotary embedding: the ``fraction`` of the head that
+    rotates (its first dimensions), the pairs' layout and the tables' base and
+    scaling (rotary_tables)."""
+    fraction: float = 1.0
+    interleaved: bool = False
+    base: float = 10000.0
+    scaling: Optional[str] = None
+    factor: float = 1.0
+    original_len: int = 0
+
+    def dims(self, head_dim: int) -> int:
+        """Rotated dimensions of a head of head_dim."""
+        R = round(self.fraction * head_dim)
+        if not 16 <= R <= head_dim or R % 16:
+            raise ValueError(f"fraction={self.fraction!r} of head_dim={head_dim} is {R} rotated "
+                             "dimensions (a multiple of 16 up to head_dim)")
+        return R
+
+    def tables(self, head_dim: int, rows: int, device):
+        return rotary_tables(self.dims(head_dim), rows, device, self.base, self.scaling,
+                             self.factor, self.original_len)
 
 
 def _split_dims(qkv: torch.Tensor, num_heads: int):
@@ -292,3 +396,90 @@ def qk_norm_rope_append(qkv: torch.Tensor, q_weight: torch.Tensor, k_weight: tor
     if torch.compiler.is_compiling() or not _lib.only_recorded(*watched):
         return qk_norm_rope_append_op(*args)
     return _lib.host().qk_norm_rope_append(*args)
+
+
+# ---- any rotary form
+
+@torch.library.custom_op("t2t::qkv_rotary", mutates_args=())
+def qkv_rotary_op(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, num_heads: int,
+                  num_kv_heads: int, pos: Optional[torch.Tensor], pos0: int,
+                  interleaved: bool) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """q [B, H, T, D] and k, v [B, Hkv, T, D] from qkv [B, T, (H + 2 Hkv) D]."""
+    return _lib.host().qkv_rotary(qkv, cos, sin, num_heads, num_kv_heads, pos, pos0, interleaved)
+
+
+@qkv_rotary_op.register_fake
+def _qkv_rotary_fake(qkv, cos, sin, num_heads, num_kv_heads, pos, pos0, interleaved):
+    B, T, D = _qk_norm_dims(qkv, num_heads, num_kv_heads)
+    return tuple(qkv.new_empty((B, h, T, D)) for h in (num_heads, num_kv_heads, num_kv_heads))
+
+
+@torch.library.custom_op("t2t::qkv_rotary_backward", mutates_args=())
+def qkv_rotary_backward_op(dq: torch.Tensor, dk: torch.Tensor, dv: torch.Tensor,
+                           cos: torch.Tensor, sin: torch.Tensor, pos: Optional[torch.Tensor],
+                           pos0: int, interleaved: bool) -> torch.Tensor:
+    """dqkv [B, T, (H + 2 Hkv) D]."""
+    return _lib.host().qkv_rotary_backward(dq, dk, dv, cos, sin, pos, pos0, interleaved)
+
+
+@qkv_rotary_backward_op.register_fake
+def _qkv_rotary_backward_fake(dq, dk, dv, cos, sin, pos, pos0, interleaved):
+    B, H, T, D = dq.shape
+    return dq.new_empty((B, T, (H + 2 * dk.shape[1]) * D))
+
+
+# The rotation is linear, so each direction's gradient is the other one.
+def _qkv_rotary_setup(ctx, inputs, output):
+    _, cos, sin, ctx.heads, ctx.kv_heads, pos, ctx.pos0, ctx.interleaved = inputs
+    ctx.save_for_backward(cos, sin, pos)
+
+
+def _qkv_rotary_bwd(ctx, dq, dk, dv):
+    cos, sin, pos = ctx.saved_tensors
+    d = qkv_rotary_backward_op(dq, dk, dv, cos, sin, pos, ctx.pos0, ctx.interleaved)
+    return d, None, None, None, None, None, None, None
+
+
+def _qkv_rotary_backward_setup(ctx, inputs, output):
+    dq, dk, _, cos, sin, pos, ctx.pos0, ctx.interleaved = inputs
+    ctx.heads, ctx.kv_heads = dq.shape[1], dk.shape[1]
+    ctx.save_for_backward(cos, sin, pos)
+
+
+def _qkv_rotary_backward_bwd(ctx, d):
+    cos, sin, pos = ctx.saved_tensors
+    got = qkv_rotary_op(d, cos, sin, ctx.heads, ctx.kv_heads, pos, ctx.pos0, ctx.interleaved)
+    return *got, None, None, None, None, None
+
+
+qkv_rotary_op.register_autograd(_qkv_rotary_bwd, setup_context=_qkv_rotary_setup)
+qkv_rotary_backward_op.register_autograd(_qkv_rotary_backward_bwd,
+                                         setup_context=_qkv_rotary_backward_setup)
+
+
+def qkv_rotary(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, num_heads: int,
+               num_kv_heads: Optional[int] = None, pos: Union[int, torch.Tensor] = 0,
+               interleaved: bool = False):
+    """Split qkv [B, T, (H + 2 Hkv) D] (query heads, key heads, value heads;
+    Hkv = H unless ``num_kv_heads`` is given) into q [B, H, T, D] and k, v
+    [B, Hkv, T, D] (contiguous), the first R dimensions of every query and key
+    head rotated by tables cos, sin float32 [rows, R / 2] and the others copied.
+
+    ``interleaved``: pairs of neighbouring dimensions (x[2i], x[2i + 1]) instead
+    of (x[i], x[i + R/2]).  ``pos``: the first token's position, or a device
+    int64 tensor [T] or [B, T] of positions (read by the kernel, any order,
+    repeats too); one without a table row gives query and key rows of zeros and
+    no gradient.  bf16 or float32 rows, head_dim a multiple of 16 up to 512, R a
+    multiple of 16; fp32 arithmetic with one rounding.  Gradient for qkv."""
+    if (cos.requires_grad or sin.requires_grad) and torch.is_grad_enabled():
+        raise RuntimeError("the rotary tables get no gradient: detach cos and sin")
+    at, pos0 = (pos, 0) if isinstance(pos, torch.Tensor) else (None, int(pos))
+    args = (qkv, cos, sin, int(num_heads),
+            int(num_heads if num_kv_heads is None else num_kv_heads), at, pos0, bool(interleaved))
+    watched = (qkv, cos, sin) if at is None else (qkv, cos, sin, at)
+    if not torch.compiler.is_compiling():
+        if _lib.unwatched(*watched):
+            return _lib.host().qkv_rotary(*args)
+        if _lib.only_recorded(*watched):
+            return _lib.host().qkv_rotary_ad(*args)
+    return qkv_rotary_op(*args)  # a compiler, or something besides autograd watches
