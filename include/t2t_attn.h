@@ -150,6 +150,26 @@ int t2t_mask_meta(const int32_t *doc, const uint64_t *q_bits, const uint64_t *kv
                   const t2t_block_mask *out, void *stream);
 
 /*
+ * First token of each token's document: start[b][t] = the smallest t' such
+ * that tokens t' .. t of row b carry the same id (int32 [mask_batch][T], out).
+ */
+int t2t_doc_starts(const int32_t *doc, int32_t mask_batch, int32_t T, int32_t *start,
+                   void *stream);
+
+/*
+ * t2t_mask_meta of the mask with a sliding window: a token reads of its own
+ * document the `window` last tokens (itself among them) and the document's
+ * first `sinks` ones, and what a grant shows as before:
+ *   allowed = q >= k && (grant || (doc[q] == doc[k] &&
+ *             (q - k < window || 0 <= k - doc_start[q] < sinks))).
+ * window >= 1; doc_start (t2t_doc_starts of doc) may be NULL when sinks is 0.
+ */
+int t2t_mask_meta_window(const int32_t *doc, const uint64_t *q_bits, const uint64_t *kv_bits,
+                         const int32_t *doc_start, int32_t mask_batch, int32_t T, int32_t words,
+                         int32_t window, int32_t sinks, int8_t *tile_class,
+                         const t2t_block_mask *out, void *stream);
+
+/*
  * Masked attention forward.  Replaces the flex_attention forward
  * (torch/nn/attention/flex_attention.py:1396-1676; eager arithmetic
  * torch/_higher_order_ops/flex_attention.py:202-267) that FlexSelfAttention
@@ -291,6 +311,69 @@ int t2t_attn_decode(const t2t_tensor *q, const t2t_tensor *k, const t2t_tensor *
                     int32_t words, int32_t B, int32_t Hq, int32_t Hkv, int32_t Tq, int32_t Tkv,
                     int32_t D, int32_t dtype, float scale, void *workspace,
                     int64_t workspace_bytes, void *stream);
+
+/*
+ * t2t_attn_decode with the sliding window of t2t_mask_meta_window: a key of
+ * the row's own document is allowed iff q_pos[t] - j < window or
+ * 0 <= j - q_start[t] < sinks; q_start int32[Bm][Tq] is the first position of
+ * the row's document (NULL when sinks is 0).  Same workspace and limits.
+ */
+int t2t_attn_decode_window(const t2t_tensor *q, const t2t_tensor *k, const t2t_tensor *v,
+                           const t2t_tensor *o, float *lse2, const int32_t *key_doc,
+                           const uint64_t *key_bits, int64_t key_stride, const int32_t *q_pos,
+                           const int32_t *q_doc, const uint64_t *q_bits, int32_t mask_batch,
+                           int32_t words, int32_t B, int32_t Hq, int32_t Hkv, int32_t Tq,
+                           int32_t Tkv, int32_t D, int32_t dtype, float scale, int32_t window,
+                           int32_t sinks, const int32_t *q_start, void *workspace,
+                           int64_t workspace_bytes, void *stream);
+
+/* Positions of a t2t_kv8 cache block, which share a scale. */
+#define T2T_KV8_BLOCK 64
+/* Query rows per kv head, (Hq / Hkv) * Tq, of one t2t_kv8_attend. */
+#define T2T_KV8_MAX_ROWS 16
+
+/*
+ * Append to a key/value cache held in 8 bits: M new tokens of each of B
+ * sequences to positions p .. p + M - 1, p = pos0 or int64 pos[b pos_stride]
+ * on the device.  A cache holds, for every (b, kv head, block of 64
+ * positions), e4m3 codes and a float32 scale, a power of two:
+ *   k_codes [B][Hkv][blocks][64][D], v_codes [B][Hkv][blocks][D][64] (bytes),
+ *   k_scale, v_scale [B][Hkv][blocks]; a value is its code times its scale.
+ * Buffers start out as zeros.  What stands behind the new tokens is no longer
+ * part of the sequence; its codes are left as they were.  A block's scale
+ * becomes the larger of its own (if it holds positions before p) and the
+ * smallest power of two under which its new tokens are at most 448; the
+ * positions before p are written again under a scale that grew.  Rounding is
+ * to nearest, ties to even.  A token whose key or value is not finite is
+ * stored as NaN keys and zero values.  A device position p < 0 or
+ * p > capacity - M stores nothing.
+ *   k, v     [B, Hkv, M, D] views, dtype 0 = bf16, 1 = float32, 16-byte
+ *            aligned rows; D in {64, 128}.
+ *   capacity positions that may be written, at most 64 * blocks.
+ */
+int t2t_kv8_append(const t2t_tensor *k, const t2t_tensor *v, int32_t B, int32_t Hkv, int32_t M,
+                   int32_t D, int32_t dtype, const int64_t *pos, int64_t pos_stride, int64_t pos0,
+                   void *k_codes, void *v_codes, float *k_scale, float *v_scale, int64_t blocks,
+                   int32_t capacity, void *stream);
+
+/* Workspace (bytes) of t2t_kv8_attend. */
+int64_t t2t_kv8_attend_workspace(int32_t B, int32_t Hq, int32_t Hkv, int32_t Tq, int32_t Tkv,
+                                 int32_t D);
+
+/*
+ * t2t_attn_decode / t2t_attn_decode_window (window 0: none) over a cache of
+ * t2t_kv8_append: positions 0 .. Tkv - 1, Tkv <= 64 * blocks.  Supported: bf16
+ * q and o, D in {64, 128}, (Hq / Hkv) * Tq <= 16, words <= 8.
+ */
+int t2t_kv8_attend(const t2t_tensor *q, const void *k_codes, const void *v_codes,
+                   const float *k_scale, const float *v_scale, int64_t blocks,
+                   const t2t_tensor *o, float *lse2, const int32_t *key_doc,
+                   const uint64_t *key_bits, int64_t key_stride, const int32_t *q_pos,
+                   const int32_t *q_doc, const uint64_t *q_bits, int32_t mask_batch,
+                   int32_t words, int32_t B, int32_t Hq, int32_t Hkv, int32_t Tq, int32_t Tkv,
+                   int32_t D, int32_t dtype, float scale, int32_t window, int32_t sinks,
+                   const int32_t *q_start, void *workspace, int64_t workspace_bytes,
+                   void *stream);
 
 /*
  * RMS normalisation of token rows: y = x / sqrt(mean(x^2) + eps) * weight in

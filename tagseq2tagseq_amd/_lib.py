@@ -54,6 +54,15 @@ _SIGS = {
     "t2t_token_inputs": ([_P, _P, _I32, _P, _P, _I32, _P, _I32, _I32, _I32, _P, _P, _P, _P],
                          ctypes.c_int),
     "t2t_mask_meta": ([_P, _P, _P, _I32, _I32, _I32, _P, _P, _P], ctypes.c_int),
+    "t2t_doc_starts": ([_P, _I32, _I32, _P, _P], ctypes.c_int),
+    "t2t_mask_meta_window": ([_P] * 4 + [_I32] * 5 + [_P] * 3, ctypes.c_int),
+    "t2t_attn_decode_window": ([_P] * 7 + [_I64] + [_P] * 3 + [_I32] * 9 + [
+        ctypes.c_float, _I32, _I32, _P, _P, _I64, _P], ctypes.c_int),
+    "t2t_kv8_append": ([_P, _P] + [_I32] * 5 + [_P, _I64, _I64] + [_P] * 4 + [_I64, _I32, _P],
+                       ctypes.c_int),
+    "t2t_kv8_attend_workspace": ([_I32] * 6, ctypes.c_int64),
+    "t2t_kv8_attend": ([_P] * 5 + [_I64] + [_P] * 4 + [_I64] + [_P] * 3 + [_I32] * 9 + [
+        ctypes.c_float, _I32, _I32, _P, _P, _I64, _P], ctypes.c_int),
     "t2t_attn_fwd": ([_P] * 5 + [_I32] * 6 + [ctypes.c_float, _P, _P], ctypes.c_int),
     "t2t_attn_bwd": ([_P] * 10 + [_I32] * 6 + [ctypes.c_float, _P, _P], ctypes.c_int),
     "t2t_clock_probe": ([_P, _I32, _P, _P], ctypes.c_int),

@@ -367,18 +367,23 @@ class FlexSelfAttention(nn.Module):
             warnings.warn("FlexSelfAttention(fp8_out_proj=True): the fp8 output projection is not "
                           "implemented; the projection runs in the module's dtype", stacklevel=2)
 
-    def heads(self, qkv: torch.Tensor, pos0: int = 0):
-        """q, k, v [B, H, T, D] of projected rows [B, T, 3 C] at positions pos0 ..
-        pos0 + T - 1: split, normed (qk_norm) and rotated."""
+    def heads(self, qkv: torch.Tensor, pos=0):
+        """q, k, v [B, H, T, D] of projected rows [B, T, 3 C] at positions pos ..
+        pos + T - 1, or at those of a device int64 tensor [T]: split, normed
+        (qk_norm) and rotated."""
         from .rope import qk_norm_rope, qkv_rope, qkv_rotary
         cos, sin = self.rotary.tables(qkv.device)
+        on_device = isinstance(pos, torch.Tensor)
         if self.qk_norm:
+            if on_device:
+                cos, sin, pos = cos.index_select(0, pos), sin.index_select(0, pos), 0
             return qk_norm_rope(qkv, self.q_norm, self.k_norm, cos, sin, self.num_heads,
-                                pos0=pos0, eps=self.NORM_EPS)
-        if self.rotary.whole_halves:
-            return qkv_rope(qkv, cos, sin, self.num_heads, pos0)
-        return qkv_rotary(qkv, cos, sin, self.num_heads, pos=pos0,
-                          interleaved=self.rotary.form.interleaved)
+                                pos0=pos, eps=self.NORM_EPS)
+        if self.rotary.whole_halves and not on_device:
+            return qkv_rope(qkv, cos, sin, self.num_heads, pos)
+        form = self.rotary.form
+        return qkv_rotary(qkv, cos, sin, self.num_heads, pos=pos,
+                          interleaved=form is not None and form.interleaved)
 
     def forward(self, x: torch.Tensor, block_mask: T2TBlockMask) -> torch.Tensor:
         B, T, C = x.shape

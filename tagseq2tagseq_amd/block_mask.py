@@ -12,6 +12,11 @@ the GPU without materialising the [T, T] mask, plus launch orders and a
 128 x 128 allowed-pair bitmap per partial tile that the attention kernels use
 for element masking.
 
+With a sliding ``window`` a token reads of its own document the last ``window``
+tokens (itself among them) and the document's first ``sinks`` ones; what a
+grant word shows it reads as before.  A document is a run of tokens with one
+id: the same id again behind another document starts anew.
+
 ``to_block_mask()`` rebuilds a torch ``BlockMask`` from the same tables (via
 ``BlockMask.from_kv_blocks``) for interoperability with torch's own
 flex_attention, and ``from_torch_block_mask()`` goes the other way: a torch
@@ -56,6 +61,9 @@ class T2TBlockMask:
     # mask_mod of the torch BlockMask this mask was converted from (its
     # per-token inputs are then unknown: doc_ids are zeros and words 0)
     source_mask_mod: Optional[Callable] = field(default=None, repr=False)
+    window: Optional[int] = None   # of the document, in tokens; None: all of it
+    sinks: int = 0                 # first tokens of the document, always read
+    doc_start: Optional[torch.Tensor] = None  # int32 [Bm, T], with sinks
 
     @property
     def mask_batch(self) -> int:
@@ -91,16 +99,23 @@ class T2TBlockMask:
 
     def mask_mod(self):
         """The reference's mask_mod over this mask's per-token tensors
-        (cross_doc_mask.py:348-357; doc_causal when there are no words), or
-        the source BlockMask's own mask_mod for a converted mask."""
+        (cross_doc_mask.py:348-357; doc_causal when there are no words) with
+        the window's limits, or the source BlockMask's own mask_mod for a
+        converted mask."""
         if self.source_mask_mod is not None:
             return self.source_mask_mod
         doc, qb, kb = self.doc_ids, self.q_bits, self.kv_bits
-        W = self.words
+        W, window, sinks, start = self.words, self.window, self.sinks, self.doc_start
 
         def t2t_mask_mod(b, h, q_idx, kv_idx):
             bb = b if doc.shape[0] > 1 else 0
             same = doc[bb, q_idx] == doc[bb, kv_idx]
+            if window is not None:
+                near = q_idx - kv_idx < window
+                if sinks:
+                    at = kv_idx - start[bb, q_idx]
+                    near = near | ((at >= 0) & (at < sinks))
+                same = same & near
             for w in range(W):
                 same = same | ((qb[bb, w, q_idx] & kb[bb, w, kv_idx]) != 0)
             return (q_idx >= kv_idx) & same
@@ -146,6 +161,9 @@ class MaskInputs:
     doc_ids: torch.Tensor          # int32 [Bm, T]
     q_bits: torch.Tensor           # int64 [Bm, W, T]
     kv_bits: torch.Tensor          # int64 [Bm, W, T]
+    window: Optional[int] = None
+    sinks: int = 0
+    doc_start: Optional[torch.Tensor] = None  # int32 [Bm, T], with sinks
 
     @property
     def mask_batch(self) -> int:
@@ -156,9 +174,33 @@ class MaskInputs:
         return int(self.q_bits.shape[1])
 
 
+def check_window(window: Optional[int], sinks: int):
+    """(window, sinks) as ints, refused where they make no mask."""
+    if sinks < 0 or int(sinks) != sinks:
+        raise ValueError(f"sinks={sinks!r} must be a number of tokens")
+    if window is None:
+        if sinks:
+            raise ValueError(f"sinks={sinks!r} without a window: every token of a document is "
+                             "read already")
+        return None, 0
+    if window < 1 or int(window) != window:
+        raise ValueError(f"window={window!r} must be at least 1 token (None: no window)")
+    return int(window), int(sinks)
+
+
+def doc_starts(doc_ids: torch.Tensor) -> torch.Tensor:
+    """int32 [Bm, T]: the first token of each token's document (the run of
+    equal ids in doc_ids, int32 [T] or [Bm, T], that holds it)."""
+    if doc_ids.dim() == 1:
+        doc_ids = doc_ids.unsqueeze(0)
+    return _lib.host().doc_starts(doc_ids.to(torch.int32).contiguous())
+
+
 def mask_inputs(doc_ids: torch.Tensor, q_bits: Optional[torch.Tensor] = None,
-                kv_bits: Optional[torch.Tensor] = None) -> MaskInputs:
+                kv_bits: Optional[torch.Tensor] = None, window: Optional[int] = None,
+                sinks: int = 0) -> MaskInputs:
     """The inputs build_block_mask takes, normalised to [Bm, T] / [Bm, W, T]."""
+    window, sinks = check_window(window, sinks)
     if doc_ids.dim() == 1:
         doc_ids = doc_ids.unsqueeze(0)
     doc_ids = doc_ids.to(torch.int32).contiguous()
@@ -168,17 +210,21 @@ def mask_inputs(doc_ids: torch.Tensor, q_bits: Optional[torch.Tensor] = None,
     if qb.shape != kb.shape or qb.shape[0] != Bm or qb.shape[2] != T:
         raise ValueError(f"q_bits {tuple(qb.shape)} / kv_bits {tuple(kb.shape)} do not match "
                          f"doc_ids {tuple(doc_ids.shape)}")
-    return MaskInputs(T, doc_ids, qb, kb)
+    return MaskInputs(T, doc_ids, qb, kb, window, sinks, doc_starts(doc_ids) if sinks else None)
 
 
 def build_block_mask(doc_ids: torch.Tensor, q_bits: Optional[torch.Tensor] = None,
                      kv_bits: Optional[torch.Tensor] = None,
-                     stream: Optional[torch.cuda.Stream] = None) -> T2TBlockMask:
+                     stream: Optional[torch.cuda.Stream] = None, window: Optional[int] = None,
+                     sinks: int = 0) -> T2TBlockMask:
     """Run the metadata pass on the GPU.
 
     doc_ids: int32 [T] or [Bm, T] on a ROCm device.
     q_bits / kv_bits: int64 (or uint64) [W, T] or [Bm, W, T] grant words, or None.
+    window: last tokens of its own document that a token reads (None: all), and
+    sinks: first tokens of the document that it reads beside them.
     """
+    window, sinks = check_window(window, sinks)
     if not doc_ids.is_cuda:
         raise RuntimeError("build_block_mask needs doc_ids on a ROCm GPU device "
                            "(the masked-attention path has no CPU implementation)")
@@ -197,9 +243,10 @@ def build_block_mask(doc_ids: torch.Tensor, q_bits: Optional[torch.Tensor] = Non
         raise ValueError(f"{W} grant words exceed the supported {_lib.MAX_WORDS}")
     host = _lib.host()
     s = stream.cuda_stream if stream is not None else host.current_stream(device.index)
-    tile_class, *t = host.mask_meta(doc_ids, qb, kb, s)
+    tile_class, *t = host.mask_meta_window(doc_ids, qb, kb, window or 0, sinks, s)
     return T2TBlockMask(
         seq_len=T, doc_ids=doc_ids, q_bits=qb, kv_bits=kb, tile_class=tile_class,
+        window=window, sinks=sinks, doc_start=t[13] if sinks else None,
         **dict(zip(("kv_num_blocks", "kv_indices", "full_kv_num_blocks", "full_kv_indices",
                     "q_num_blocks", "q_indices", "full_q_num_blocks", "full_q_indices",
                     "row_order", "col_order", "kv_bits_off", "q_bits_slot", "tile_bits"), t)))

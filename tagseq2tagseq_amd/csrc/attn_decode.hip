@@ -28,6 +28,12 @@
 // Each (row, chunk) leaves (max, sum, unnormalised o[D]) in the
 // workspace; attn_decode_combine merges the chunks of a row into o (bf16)
 // and the log2-domain LSE.  Fully masked rows give o = 0 and LSE = -inf.
+//
+// With a sliding window of w positions and s sinks (Win) a key of the row's own
+// document is allowed only if pos(q) - j < w or 0 <= j - start(q) < s, start(q)
+// = the first position of the row's document; grants are as they were.  Without
+// grant words a chunk that lies outside every row's window and sinks ends
+// before it reads a key's document.
 #include "attn_kernels.h"
 
 namespace t2t {
@@ -48,6 +54,8 @@ struct DecodeArgs {
   int Bm, W, B, Hq, Hkv, Tq, Tkv, nch;
   float c;                   // scale * log2(e)
   float* part;               // [B][Hq][Tq][nch][D + 2]
+  int window, sinks;         // window 0: none
+  const int32_t* q_start;    // [Bm][Tq], or NULL without sinks
 };
 
 // Sum over the GL = D/8 lanes of a key group (8 or 16 adjacent, aligned
@@ -66,7 +74,7 @@ __device__ __forceinline__ float group_sum(float x) {
 
 // RMAX: compile-time bound on the R query rows (1, 2, 4 or 8), so the common
 // single-row step holds 8 + 8 accumulators per lane rather than 64 + 64.
-template <int D, int RMAX>
+template <int D, int RMAX, bool Win>
 __global__ __launch_bounds__(kDecThreads) void attn_decode_partial(DecodeArgs a) {
   constexpr int GL = D / 8;                    // lanes per key
   constexpr int NKG = kDecThreads / GL;        // key groups per work-group
@@ -74,7 +82,7 @@ __global__ __launch_bounds__(kDecThreads) void attn_decode_partial(DecodeArgs a)
   __shared__ float sc[RMAX][kDecChunk];        // scores (log2 units)
   __shared__ float red[kDecThreads / 64][RMAX][D];
   __shared__ float rmax[RMAX];
-  __shared__ int32_t qpos_s[RMAX], qdoc_s[RMAX];
+  __shared__ int32_t qpos_s[RMAX], qdoc_s[RMAX], qstart_s[RMAX];
   __shared__ uint64_t qbits_s[kMaxWords][RMAX];
 
   const int chunk = blockIdx.x, hk = blockIdx.y, b = blockIdx.z;
@@ -84,6 +92,29 @@ __global__ __launch_bounds__(kDecThreads) void attn_decode_partial(DecodeArgs a)
   const int R = G * a.Tq;
   const int mb = a.Bm > 1 ? b : 0;
   const int j0 = chunk * kDecChunk;
+
+  if constexpr (Win) {
+    if (a.W == 0) {
+      bool any = false;
+      for (int tq = 0; tq < a.Tq; ++tq) {
+        const int64_t p = a.q_pos[(size_t)mb * a.Tq + tq];
+        any = any || (j0 <= p && j0 + kDecChunk > p - a.window + 1);
+        if (a.q_start) {
+          const int64_t s = a.q_start[(size_t)mb * a.Tq + tq];
+          any = any || (j0 < s + a.sinks && j0 + kDecChunk > s);
+        }
+      }
+      if (!any) {  // an empty chunk
+        for (int x = tid; x < R * (D + 2); x += kDecThreads) {
+          const int r = x / (D + 2), col = x - r * (D + 2);
+          const int g = r / a.Tq, tq = r - g * a.Tq;
+          const size_t row = ((size_t)b * a.Hq + hk * G + g) * a.Tq + tq;
+          a.part[(row * a.nch + chunk) * (D + 2) + col] = col == 0 ? -INFINITY : 0.f;
+        }
+        return;
+      }
+    }
+  }
 
   const __bf16* kbase = static_cast<const __bf16*>(a.k.data) + b * a.k.sb + hk * a.k.sh + 8 * dg;
   const __bf16* vbase = static_cast<const __bf16*>(a.v.data) + b * a.v.sb + hk * a.v.sh + 8 * dg;
@@ -104,6 +135,7 @@ __global__ __launch_bounds__(kDecThreads) void attn_decode_partial(DecodeArgs a)
   if (tid < a.Tq) {
     qpos_s[tid] = a.q_pos[(size_t)mb * a.Tq + tid];
     qdoc_s[tid] = a.q_doc[(size_t)mb * a.Tq + tid];
+    if (Win) qstart_s[tid] = a.q_start ? a.q_start[(size_t)mb * a.Tq + tid] : 0;
     for (int w = 0; w < a.W; ++w)
       qbits_s[w][tid] = a.q_bits[((size_t)mb * a.W + w) * a.Tq + tid];
   }
@@ -136,7 +168,14 @@ __global__ __launch_bounds__(kDecThreads) void attn_decode_partial(DecodeArgs a)
     for (int tq = 0; tq < a.Tq; ++tq) {
       const int qd = qdoc_s[tq];
 #pragma unroll
-      for (int i = 0; i < KPG; ++i) allow[i] |= (dj[i] == qd ? 1u : 0u) << tq;
+      for (int i = 0; i < KPG; ++i) {
+        bool own = dj[i] == qd;
+        if constexpr (Win) {
+          const int64_t j = j0 + kg + NKG * i, at = j - qstart_s[tq];
+          own = own && (qpos_s[tq] - j < a.window || (at >= 0 && at < a.sinks));
+        }
+        allow[i] |= (own ? 1u : 0u) << tq;
+      }
     }
     for (int w = 0; w < a.W; ++w) {
       uint64_t kw[KPG];
@@ -317,16 +356,28 @@ __global__ __launch_bounds__(64) void attn_decode_combine(DecodeArgs a, TensorVi
   if (lane == 0) lse2[row] = L > 0.f ? M + log2f(L) : -INFINITY;
 }
 
-template <int D>
+template <int D, bool Win>
 void launch_partial(int R, dim3 grid, const DecodeArgs& a, hipStream_t stream) {
   if (R <= 1)
-    hipLaunchKernelGGL((attn_decode_partial<D, 1>), grid, dim3(kDecThreads), 0, stream, a);
+    hipLaunchKernelGGL((attn_decode_partial<D, 1, Win>), grid, dim3(kDecThreads), 0, stream, a);
   else if (R <= 2)
-    hipLaunchKernelGGL((attn_decode_partial<D, 2>), grid, dim3(kDecThreads), 0, stream, a);
+    hipLaunchKernelGGL((attn_decode_partial<D, 2, Win>), grid, dim3(kDecThreads), 0, stream, a);
   else if (R <= 4)
-    hipLaunchKernelGGL((attn_decode_partial<D, 4>), grid, dim3(kDecThreads), 0, stream, a);
+    hipLaunchKernelGGL((attn_decode_partial<D, 4, Win>), grid, dim3(kDecThreads), 0, stream, a);
   else
-    hipLaunchKernelGGL((attn_decode_partial<D, 8>), grid, dim3(kDecThreads), 0, stream, a);
+    hipLaunchKernelGGL((attn_decode_partial<D, 8, Win>), grid, dim3(kDecThreads), 0, stream, a);
+}
+
+template <int D>
+void launch_both(int R, const DecodeArgs& a, const TensorView& o, float* lse2,
+                 hipStream_t stream) {
+  const dim3 pgrid((unsigned)a.nch, (unsigned)a.Hkv, (unsigned)a.B);
+  const dim3 cgrid((unsigned)a.Tq, (unsigned)a.Hq, (unsigned)a.B);
+  if (a.window > 0)
+    launch_partial<D, true>(R, pgrid, a, stream);
+  else
+    launch_partial<D, false>(R, pgrid, a, stream);
+  hipLaunchKernelGGL(attn_decode_combine<D>, cgrid, dim3(64), 0, stream, a, o, lse2);
 }
 
 }  // namespace
@@ -341,21 +392,18 @@ hipError_t launch_attn_decode(const TensorView& q, const TensorView& k, const Te
                               const uint64_t* key_bits, int64_t key_stride, const int32_t* q_pos,
                               const int32_t* q_doc, const uint64_t* q_bits, int Bm, int W,
                               int B, int Hq, int Hkv, int Tq, int Tkv, int D, float scale,
+                              int window, int sinks, const int32_t* q_start,
                               float* workspace, hipStream_t stream) {
   DecodeArgs a{q,     k,      v,    key_doc, key_bits, key_stride, q_pos, q_doc,
                q_bits, Bm,    W,    B,       Hq,       Hkv,        Tq,    Tkv,
-               (Tkv + kDecChunk - 1) / kDecChunk, scale * kLog2e, workspace};
+               (Tkv + kDecChunk - 1) / kDecChunk, scale * kLog2e, workspace,
+               window, sinks, q_start};
   if (a.nch == 0) a.nch = 1;  // no keys: one chunk that finds nothing
-  const dim3 pgrid((unsigned)a.nch, (unsigned)Hkv, (unsigned)B);
-  const dim3 cgrid((unsigned)Tq, (unsigned)Hq, (unsigned)B);
   const int R = (Hq / Hkv) * Tq;
-  if (D == 64) {
-    launch_partial<64>(R, pgrid, a, stream);
-    hipLaunchKernelGGL(attn_decode_combine<64>, cgrid, dim3(64), 0, stream, a, o, lse2);
-  } else {
-    launch_partial<128>(R, pgrid, a, stream);
-    hipLaunchKernelGGL(attn_decode_combine<128>, cgrid, dim3(64), 0, stream, a, o, lse2);
-  }
+  if (D == 64)
+    launch_both<64>(R, a, o, lse2, stream);
+  else
+    launch_both<128>(R, a, o, lse2, stream);
   return hipGetLastError();
 }
 

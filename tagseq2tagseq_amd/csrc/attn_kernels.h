@@ -62,8 +62,13 @@ hipError_t launch_token_inputs(const int32_t* spans, const int32_t* n_spans, int
                                const uint64_t* links, int B, int T, int words, int32_t* doc,
                                uint64_t* q_bits, uint64_t* kv_bits, hipStream_t stream);
 
+hipError_t launch_doc_starts(const int32_t* doc, int Bm, int T, int32_t* start,
+                             hipStream_t stream);
+
+// window 0: none; start: doc_starts of doc, needed with sinks
 hipError_t launch_mask_meta(const int32_t* doc, const uint64_t* qbits, const uint64_t* kvbits,
-                            int T, int words, const MaskOut& out, hipStream_t stream);
+                            const int32_t* start, int window, int sinks, int T, int words,
+                            const MaskOut& out, hipStream_t stream);
 
 hipError_t launch_attn_fwd_bf16(const TensorView& q, const TensorView& k, const TensorView& v,
                                 const TensorView& o, float* lse2, const AttnDims& dims,
@@ -250,7 +255,52 @@ hipError_t launch_attn_decode(const TensorView& q, const TensorView& k, const Te
                               const uint64_t* key_bits, int64_t key_stride, const int32_t* q_pos,
                               const int32_t* q_doc, const uint64_t* q_bits, int Bm, int W,
                               int B, int Hq, int Hkv, int Tq, int Tkv, int D, float scale,
+                              int window, int sinks, const int32_t* q_start,
                               float* workspace, hipStream_t stream);
+
+// 8-bit key/value cache: codes [B][Hkv][blocks] of keys [64][D] and values
+// [D][64], scales [B][Hkv][blocks].
+constexpr int kKv8Block = 64;
+constexpr int kKv8MaxRows = 16;  // (Hq / Hkv) * Tq per launch
+
+struct Kv8AppendArgs {
+  TensorView k, v;           // [B][Hkv][M][D] new tokens
+  uint8_t* k_codes;
+  uint8_t* v_codes;
+  float* k_scale;
+  float* v_scale;
+  const int64_t* pos;        // first position of batch row b at pos[b pos_stride], or NULL
+  int64_t pos_stride;
+  int64_t pos0;
+  int B, Hkv, M, capacity;   // capacity: positions that may be written
+  int64_t blocks;
+};
+
+struct Kv8AttendArgs {
+  TensorView q, o;           // [B][Hq][Tq][D]
+  float* lse2;
+  const uint8_t* k_codes;
+  const uint8_t* v_codes;
+  const float* k_scale;
+  const float* v_scale;
+  int64_t blocks;
+  const int32_t* key_doc;    // as DecodeArgs of the bf16 cache
+  const uint64_t* key_bits;
+  int64_t key_stride;
+  const int32_t* q_pos;
+  const int32_t* q_doc;
+  const uint64_t* q_bits;
+  const int32_t* q_start;
+  int Bm, W, B, Hq, Hkv, Tq, Tkv;
+  float c;                   // scale * log2(e)
+  int window, sinks;         // window 0: none
+  float* part;               // [B][Hq][Tq][chunks][D + 2]
+  int chunks, chunk_blocks;  // set by the launcher
+};
+
+void kv8_split(int B, int Hkv, int Tkv, int* chunks, int* chunk_blocks);
+hipError_t launch_kv8_append(const Kv8AppendArgs& a, bool f32, int D, hipStream_t stream);
+hipError_t launch_kv8_attend(Kv8AttendArgs a, int D, hipStream_t stream);
 
 // Weight gradient C = A^T B over K rows (split-K, fp32 partials summed in order).
 int wgrad_splits(int M, int N, int K);

@@ -97,6 +97,17 @@ int check_dims(int B, int Hq, int Hkv, int T, int D, int dtype, bool f32_ok = fa
   return T2T_OK;
 }
 
+// Views of head rows [B, H, T, D] whose rows are read or written in 16-byte pieces.
+int check_head_views(const t2t_tensor* const (&views)[3], int32_t dtype) {
+  const int64_t align = dtype == T2T_DTYPE_F32 ? 4 : 8;
+  for (const t2t_tensor* t : views)
+    if (!t || !t->data || reinterpret_cast<uintptr_t>(t->data) % 16 || t->stride_b < 0 ||
+        t->stride_h < 0 || t->stride_t < 0 || t->stride_b % align || t->stride_h % align ||
+        t->stride_t % align)
+      return fail(T2T_EINVAL, "q / k / v view NULL, or its head rows off a 16-byte boundary");
+  return T2T_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -128,9 +139,33 @@ int t2t_token_inputs(const int32_t* spans, const int32_t* n_spans, int32_t max_s
                     "t2t_token_inputs launch");
 }
 
-int t2t_mask_meta(const int32_t* doc, const uint64_t* q_bits, const uint64_t* kv_bits,
-                  int32_t mask_batch, int32_t T, int32_t words, int8_t* tile_class,
-                  const t2t_block_mask* out, void* stream) {
+int t2t_doc_starts(const int32_t* doc, int32_t mask_batch, int32_t T, int32_t* start,
+                   void* stream) {
+  if (T < 0 || mask_batch < 0) return fail(T2T_EINVAL, "negative T or mask_batch");
+  if (mask_batch > 65535)
+    return fail(T2T_EUNSUPPORTED, "mask_batch=%d rows exceed one launch", mask_batch);
+  if (T > 0x7fffffff - 8192) return fail(T2T_EUNSUPPORTED, "T=%d tokens exceed one launch", T);
+  if (T == 0 || mask_batch == 0) return T2T_OK;
+  if (!doc || !start) return fail(T2T_EINVAL, "doc or start is NULL");
+  return hip_status(t2t::launch_doc_starts(doc, mask_batch, T, start,
+                                           static_cast<hipStream_t>(stream)),
+                    "t2t_doc_starts launch");
+}
+
+namespace {
+
+int check_window(int32_t window, int32_t sinks, const void* start, const char* what) {
+  if (window < 1) return fail(T2T_EINVAL, "window=%d must be at least 1", window);
+  if (sinks < 0) return fail(T2T_EINVAL, "sinks=%d is negative", sinks);
+  if (sinks > 0 && !start) return fail(T2T_EINVAL, "sinks need %s", what);
+  return T2T_OK;
+}
+
+// The metadata pass; window 0: none.
+int mask_meta(const int32_t* doc, const uint64_t* q_bits, const uint64_t* kv_bits,
+              const int32_t* doc_start, int32_t window, int32_t sinks, int32_t mask_batch,
+              int32_t T, int32_t words, int8_t* tile_class, const t2t_block_mask* out,
+              void* stream) {
   if (T < 0 || mask_batch < 0) return fail(T2T_EINVAL, "negative T or mask_batch");
   if (words < 0 || words > T2T_MAX_WORDS)
     return fail(T2T_EUNSUPPORTED, "words=%d outside [0, %d]", words, T2T_MAX_WORDS);
@@ -162,9 +197,30 @@ int t2t_mask_meta(const int32_t* doc, const uint64_t* q_bits, const uint64_t* kv
   o.row_order = out->row_order; o.col_order = out->col_order;
   o.kv_bits_off = out->kv_bits_off; o.q_bits_slot = out->q_bits_slot;
   o.tile_bits = out->tile_bits;
-  return hip_status(t2t::launch_mask_meta(doc, q_bits, kv_bits, T, words, o,
+  // (a window or sinks past the row are the whole row)
+  return hip_status(t2t::launch_mask_meta(doc, q_bits, kv_bits, sinks > 0 ? doc_start : nullptr,
+                                          std::min(window, T), std::min(sinks, T), T, words, o,
                                           static_cast<hipStream_t>(stream)),
                     "t2t_mask_meta launch");
+}
+
+}  // namespace
+
+int t2t_mask_meta(const int32_t* doc, const uint64_t* q_bits, const uint64_t* kv_bits,
+                  int32_t mask_batch, int32_t T, int32_t words, int8_t* tile_class,
+                  const t2t_block_mask* out, void* stream) {
+  return mask_meta(doc, q_bits, kv_bits, nullptr, 0, 0, mask_batch, T, words, tile_class, out,
+                   stream);
+}
+
+int t2t_mask_meta_window(const int32_t* doc, const uint64_t* q_bits, const uint64_t* kv_bits,
+                         const int32_t* doc_start, int32_t mask_batch, int32_t T, int32_t words,
+                         int32_t window, int32_t sinks, int8_t* tile_class,
+                         const t2t_block_mask* out, void* stream) {
+  if (T > 0 && mask_batch > 0)
+    if (int rc = check_window(window, sinks, doc_start, "doc_start")) return rc;
+  return mask_meta(doc, q_bits, kv_bits, doc_start, window, sinks, mask_batch, T, words,
+                   tile_class, out, stream);
 }
 
 int t2t_attn_fwd(const t2t_tensor* q, const t2t_tensor* k, const t2t_tensor* v,
@@ -428,13 +484,16 @@ int64_t t2t_attn_decode_workspace(int32_t B, int32_t Hq, int32_t Tq, int32_t Tkv
   return 4 * t2t::decode_workspace_floats(B, Hq, Tq, Tkv, D);
 }
 
-int t2t_attn_decode(const t2t_tensor* q, const t2t_tensor* k, const t2t_tensor* v,
-                    const t2t_tensor* o, float* lse2, const int32_t* key_doc,
-                    const uint64_t* key_bits, int64_t key_stride, const int32_t* q_pos,
-                    const int32_t* q_doc, const uint64_t* q_bits, int32_t mask_batch,
-                    int32_t words, int32_t B, int32_t Hq, int32_t Hkv, int32_t Tq, int32_t Tkv,
-                    int32_t D, int32_t dtype, float scale, void* workspace,
-                    int64_t workspace_bytes, void* stream) {
+namespace {
+
+// The decode step; window 0: none.
+int attn_decode(const t2t_tensor* q, const t2t_tensor* k, const t2t_tensor* v,
+                const t2t_tensor* o, float* lse2, const int32_t* key_doc,
+                const uint64_t* key_bits, int64_t key_stride, const int32_t* q_pos,
+                const int32_t* q_doc, const uint64_t* q_bits, int32_t mask_batch, int32_t words,
+                int32_t B, int32_t Hq, int32_t Hkv, int32_t Tq, int32_t Tkv, int32_t D,
+                int32_t dtype, float scale, int32_t window, int32_t sinks, const int32_t* q_start,
+                void* workspace, int64_t workspace_bytes, void* stream) {
   if (B < 0 || Hq < 0 || Hkv < 0 || Tq < 0 || Tkv < 0 || mask_batch < 0 || key_stride < 0)
     return fail(T2T_EINVAL, "negative size or stride");
   if (dtype != T2T_DTYPE_BF16) return fail(T2T_EUNSUPPORTED, "dtype %d is not bf16", dtype);
@@ -462,9 +521,159 @@ int t2t_attn_decode(const t2t_tensor* q, const t2t_tensor* k, const t2t_tensor* 
   return hip_status(t2t::launch_attn_decode(as_view(q), as_view(k), as_view(v), as_view(o), lse2,
                                             key_doc, key_bits, key_stride, q_pos, q_doc, q_bits,
                                             mask_batch, words, B, Hq, Hkv, Tq, Tkv, D, scale,
+                                            window, sinks, sinks > 0 ? q_start : nullptr,
                                             static_cast<float*>(workspace),
                                             static_cast<hipStream_t>(stream)),
                     "t2t_attn_decode launch");
+}
+
+}  // namespace
+
+int t2t_attn_decode(const t2t_tensor* q, const t2t_tensor* k, const t2t_tensor* v,
+                    const t2t_tensor* o, float* lse2, const int32_t* key_doc,
+                    const uint64_t* key_bits, int64_t key_stride, const int32_t* q_pos,
+                    const int32_t* q_doc, const uint64_t* q_bits, int32_t mask_batch,
+                    int32_t words, int32_t B, int32_t Hq, int32_t Hkv, int32_t Tq, int32_t Tkv,
+                    int32_t D, int32_t dtype, float scale, void* workspace,
+                    int64_t workspace_bytes, void* stream) {
+  return attn_decode(q, k, v, o, lse2, key_doc, key_bits, key_stride, q_pos, q_doc, q_bits,
+                     mask_batch, words, B, Hq, Hkv, Tq, Tkv, D, dtype, scale, 0, 0, nullptr,
+                     workspace, workspace_bytes, stream);
+}
+
+int t2t_attn_decode_window(const t2t_tensor* q, const t2t_tensor* k, const t2t_tensor* v,
+                           const t2t_tensor* o, float* lse2, const int32_t* key_doc,
+                           const uint64_t* key_bits, int64_t key_stride, const int32_t* q_pos,
+                           const int32_t* q_doc, const uint64_t* q_bits, int32_t mask_batch,
+                           int32_t words, int32_t B, int32_t Hq, int32_t Hkv, int32_t Tq,
+                           int32_t Tkv, int32_t D, int32_t dtype, float scale, int32_t window,
+                           int32_t sinks, const int32_t* q_start, void* workspace,
+                           int64_t workspace_bytes, void* stream) {
+  if (B > 0 && Hq > 0 && Tq > 0)
+    if (int rc = check_window(window, sinks, q_start, "q_start")) return rc;
+  return attn_decode(q, k, v, o, lse2, key_doc, key_bits, key_stride, q_pos, q_doc, q_bits,
+                     mask_batch, words, B, Hq, Hkv, Tq, Tkv, D, dtype, scale, window, sinks,
+                     q_start, workspace, workspace_bytes, stream);
+}
+
+namespace {
+
+int check_kv8(const void* k_codes, const void* v_codes, const float* k_scale,
+              const float* v_scale) {
+  for (const void* p : {k_codes, v_codes})
+    if (!p || reinterpret_cast<uintptr_t>(p) % 16)
+      return fail(T2T_EINVAL, "codes NULL or not 16-byte aligned");
+  if (!k_scale || !v_scale || k_codes == v_codes || k_scale == v_scale)
+    return fail(T2T_EINVAL, "scales NULL, or keys and values are one");
+  return T2T_OK;
+}
+
+}  // namespace
+
+static_assert(T2T_KV8_BLOCK == t2t::kKv8Block && T2T_KV8_MAX_ROWS == t2t::kKv8MaxRows,
+              "the header's cache layout");
+
+int t2t_kv8_append(const t2t_tensor* k, const t2t_tensor* v, int32_t B, int32_t Hkv, int32_t M,
+                   int32_t D, int32_t dtype, const int64_t* pos, int64_t pos_stride, int64_t pos0,
+                   void* k_codes, void* v_codes, float* k_scale, float* v_scale, int64_t blocks,
+                   int32_t capacity, void* stream) {
+  if (B < 0 || Hkv < 0 || M < 0 || blocks < 0 || capacity < 0)
+    return fail(T2T_EINVAL, "negative size");
+  if (D != 64 && D != 128) return fail(T2T_EUNSUPPORTED, "head dim %d (64 or 128)", D);
+  if (dtype != T2T_DTYPE_BF16 && dtype != T2T_DTYPE_F32)
+    return fail(T2T_EUNSUPPORTED, "dtype %d not supported here", dtype);
+  if (B > 65535 || Hkv > 65535)
+    return fail(T2T_EUNSUPPORTED, "B=%d or Hkv=%d exceeds one launch", B, Hkv);
+  if (capacity > 0x7fffffff - 2 * T2T_KV8_BLOCK || (int64_t)capacity > blocks * T2T_KV8_BLOCK)
+    return fail(T2T_EINVAL, "capacity=%d exceeds the %lld blocks", capacity, (long long)blocks);
+  if (pos) {
+    if (reinterpret_cast<uintptr_t>(pos) % 8 || pos_stride < 0)
+      return fail(T2T_EINVAL, "pos misaligned or with a negative stride");
+    if (M > capacity) return fail(T2T_EINVAL, "M=%d tokens exceed capacity=%d", M, capacity);
+  } else if (pos0 < 0 || pos0 > (int64_t)capacity - M) {
+    return fail(T2T_EINVAL, "positions %lld..%lld exceed capacity=%d", (long long)pos0,
+                (long long)pos0 + M - 1, capacity);
+  }
+  if (B == 0 || Hkv == 0 || M == 0) return T2T_OK;
+  if (int rc = check_head_views({k, k, v}, dtype)) return rc;
+  if (int rc = check_kv8(k_codes, v_codes, k_scale, v_scale)) return rc;
+  t2t::Kv8AppendArgs a{};
+  a.k = as_view(k); a.v = as_view(v);
+  a.k_codes = static_cast<uint8_t*>(k_codes); a.v_codes = static_cast<uint8_t*>(v_codes);
+  a.k_scale = k_scale; a.v_scale = v_scale;
+  a.pos = pos; a.pos_stride = pos_stride; a.pos0 = pos0;
+  a.B = B; a.Hkv = Hkv; a.M = M; a.capacity = capacity; a.blocks = blocks;
+  return hip_status(t2t::launch_kv8_append(a, dtype == T2T_DTYPE_F32, D,
+                                           static_cast<hipStream_t>(stream)),
+                    "t2t_kv8_append launch");
+}
+
+int64_t t2t_kv8_attend_workspace(int32_t B, int32_t Hq, int32_t Hkv, int32_t Tq, int32_t Tkv,
+                                 int32_t D) {
+  if (B <= 0 || Hq <= 0 || Hkv <= 0 || Tq <= 0 || Tkv < 0 || D < 0) return 0;
+  int chunks, each;
+  t2t::kv8_split(B, Hkv, Tkv, &chunks, &each);
+  return chunks == 1 ? 0 : 4 * (int64_t)B * Hq * Tq * chunks * (D + 2);
+}
+
+int t2t_kv8_attend(const t2t_tensor* q, const void* k_codes, const void* v_codes,
+                   const float* k_scale, const float* v_scale, int64_t blocks,
+                   const t2t_tensor* o, float* lse2, const int32_t* key_doc,
+                   const uint64_t* key_bits, int64_t key_stride, const int32_t* q_pos,
+                   const int32_t* q_doc, const uint64_t* q_bits, int32_t mask_batch,
+                   int32_t words, int32_t B, int32_t Hq, int32_t Hkv, int32_t Tq, int32_t Tkv,
+                   int32_t D, int32_t dtype, float scale, int32_t window, int32_t sinks,
+                   const int32_t* q_start, void* workspace, int64_t workspace_bytes,
+                   void* stream) {
+  if (B < 0 || Hq < 0 || Hkv < 0 || Tq < 0 || Tkv < 0 || mask_batch < 0 || key_stride < 0 ||
+      blocks < 0)
+    return fail(T2T_EINVAL, "negative size or stride");
+  if (dtype != T2T_DTYPE_BF16) return fail(T2T_EUNSUPPORTED, "dtype %d is not bf16", dtype);
+  if (D != 64 && D != 128) return fail(T2T_EUNSUPPORTED, "head dim %d (64 or 128)", D);
+  if (words < 0 || words > T2T_MAX_WORDS)
+    return fail(T2T_EUNSUPPORTED, "words=%d outside [0, %d]", words, T2T_MAX_WORDS);
+  if (int rc = check_scale(scale)) return rc;
+  if (window < 0) return fail(T2T_EINVAL, "window=%d is negative", window);
+  if (window > 0) {
+    if (int rc = check_window(window, sinks, q_start, "q_start")) return rc;
+  } else if (sinks != 0) {
+    return fail(T2T_EINVAL, "sinks=%d without a window", sinks);
+  }
+  if (B == 0 || Hq == 0 || Tq == 0) return T2T_OK;
+  if (Hkv == 0 || Hq % Hkv != 0)
+    return fail(T2T_EINVAL, "Hq=%d is not a multiple of Hkv=%d", Hq, Hkv);
+  if ((int64_t)(Hq / Hkv) * Tq > T2T_KV8_MAX_ROWS)
+    return fail(T2T_EUNSUPPORTED, "(Hq / Hkv) * Tq = %lld query rows per kv head exceeds %d",
+                (long long)(Hq / Hkv) * Tq, T2T_KV8_MAX_ROWS);
+  if (B > 65535 || Hq > 65535)
+    return fail(T2T_EUNSUPPORTED, "B=%d or Hq=%d exceeds one launch", B, Hq);
+  if (!(mask_batch == 1 || mask_batch == B))
+    return fail(T2T_EINVAL, "mask_batch %d does not broadcast to B=%d", mask_batch, B);
+  if (key_stride < Tkv)
+    return fail(T2T_EINVAL, "key_stride %lld < Tkv %d", (long long)key_stride, Tkv);
+  if (Tkv > 0x7fffffff - 1024 || (int64_t)Tkv > blocks * T2T_KV8_BLOCK)
+    return fail(T2T_EINVAL, "Tkv=%d exceeds the %lld blocks", Tkv, (long long)blocks);
+  if (int rc = check_head_views({q, q, o}, dtype)) return rc;
+  if (int rc = check_kv8(k_codes, v_codes, k_scale, v_scale)) return rc;
+  if (!lse2 || !key_doc || !q_pos || !q_doc || (words > 0 && (!key_bits || !q_bits)))
+    return fail(T2T_EINVAL, "NULL pointer argument");
+  const int64_t need = t2t_kv8_attend_workspace(B, Hq, Hkv, Tq, Tkv, D);
+  if (need > 0 && (!workspace || workspace_bytes < need))
+    return fail(T2T_EINVAL, "workspace of %lld bytes, %lld needed", (long long)workspace_bytes,
+                (long long)need);
+  t2t::Kv8AttendArgs a{};
+  a.q = as_view(q); a.o = as_view(o); a.lse2 = lse2;
+  a.k_codes = static_cast<const uint8_t*>(k_codes);
+  a.v_codes = static_cast<const uint8_t*>(v_codes);
+  a.k_scale = k_scale; a.v_scale = v_scale; a.blocks = blocks;
+  a.key_doc = key_doc; a.key_bits = key_bits; a.key_stride = key_stride;
+  a.q_pos = q_pos; a.q_doc = q_doc; a.q_bits = q_bits;
+  a.q_start = sinks > 0 ? q_start : nullptr;
+  a.Bm = mask_batch; a.W = words; a.B = B; a.Hq = Hq; a.Hkv = Hkv; a.Tq = Tq; a.Tkv = Tkv;
+  a.c = scale * t2t::kLog2e; a.window = window; a.sinks = sinks;
+  a.part = static_cast<float*>(workspace);
+  return hip_status(t2t::launch_kv8_attend(a, D, static_cast<hipStream_t>(stream)),
+                    "t2t_kv8_attend launch");
 }
 
 namespace {
@@ -594,16 +803,6 @@ int check_qk_norm(int32_t B, int32_t T, int32_t Hq, int32_t Hkv, int32_t D, int3
     return fail(T2T_EINVAL, "qkv rows must start on 16-byte boundaries");
   if (!cos || !sin || (reinterpret_cast<uintptr_t>(cos) | reinterpret_cast<uintptr_t>(sin)) % 16)
     return fail(T2T_EINVAL, "cos / sin NULL or not 16-byte aligned");
-  return T2T_OK;
-}
-
-int check_head_views(const t2t_tensor* const (&views)[3], int32_t dtype) {
-  const int64_t align = dtype == T2T_DTYPE_F32 ? 4 : 8;
-  for (const t2t_tensor* t : views)
-    if (!t || !t->data || reinterpret_cast<uintptr_t>(t->data) % 16 || t->stride_b < 0 ||
-        t->stride_h < 0 || t->stride_t < 0 || t->stride_b % align || t->stride_h % align ||
-        t->stride_t % align)
-      return fail(T2T_EINVAL, "q / k / v view NULL, or its head rows off a 16-byte boundary");
   return T2T_OK;
 }
 

@@ -509,6 +509,165 @@ Tensor qkv_rotary_backward(const Tensor& dq_in, const Tensor& dk_in, const Tenso
   return dqkv;
 }
 
+// ---- 8-bit key/value cache
+
+// Codes and scales of a cache, checked against the heads they are used with.
+// They are read and written in place, so never copied.
+struct Kv8 {
+  int64_t B, Hkv, blocks, D;
+  Kv8(const Tensor& k_codes, const Tensor& v_codes, const Tensor& k_scale, const Tensor& v_scale,
+      const Tensor& like) {
+    TORCH_CHECK_VALUE(k_codes.dim() == 5 && k_codes.size(3) == T2T_KV8_BLOCK &&
+                          v_codes.dim() == 5 && v_codes.size(4) == T2T_KV8_BLOCK &&
+                          v_codes.size(3) == k_codes.size(4) &&
+                          v_codes.sizes().slice(0, 3) == k_codes.sizes().slice(0, 3),
+                      "codes ", k_codes.sizes(), " and ", v_codes.sizes(), " must be [B, Hkv, "
+                      "blocks, ", T2T_KV8_BLOCK, ", D] and [B, Hkv, blocks, D, ", T2T_KV8_BLOCK,
+                      "]");
+    TORCH_CHECK_VALUE(k_scale.sizes() == k_codes.sizes().slice(0, 3) &&
+                          v_scale.sizes() == k_scale.sizes(),
+                      "scales ", k_scale.sizes(), " and ", v_scale.sizes(),
+                      " must be [B, Hkv, blocks]");
+    TORCH_CHECK_VALUE(k_codes.scalar_type() == at::kFloat8_e4m3fn &&
+                          v_codes.scalar_type() == at::kFloat8_e4m3fn &&
+                          k_scale.scalar_type() == at::kFloat &&
+                          v_scale.scalar_type() == at::kFloat,
+                      "codes must be float8_e4m3fn and scales float32");
+    need_gpu(like, k_codes, v_codes, k_scale, v_scale);
+    for (const Tensor* t : {&k_codes, &v_codes, &k_scale, &v_scale})
+      TORCH_CHECK_VALUE(t->is_contiguous() && t->device() == like.device(),
+                        "codes and scales must be contiguous and on the heads' device");
+    B = k_codes.size(0);
+    Hkv = k_codes.size(1);
+    blocks = k_codes.size(2);
+    D = k_codes.size(4);
+    TORCH_CHECK_NOT_IMPLEMENTED(D == 64 || D == 128, "head dim ", D, " is not supported (64 or "
+                                "128)");
+    TORCH_CHECK_VALUE(B <= INT32_MAX && Hkv <= INT32_MAX && blocks <= INT32_MAX / 64 - 16,
+                      "codes ", k_codes.sizes(), " are too large");
+  }
+};
+
+// pos: int64, one value or one a sequence, on the device, or undefined for pos0.
+void kv8_append(const Tensor& k_in, const Tensor& v_in, const c10::optional<Tensor>& pos_in,
+                int64_t pos0, const Tensor& k_codes, const Tensor& v_codes, const Tensor& k_scale,
+                const Tensor& v_scale, int64_t capacity) {
+  const Kv8 c(k_codes, v_codes, k_scale, v_scale, k_in);
+  TORCH_CHECK_VALUE(k_in.dim() == 4 && k_in.sizes() == v_in.sizes() && k_in.size(0) == c.B &&
+                        k_in.size(1) == c.Hkv && k_in.size(3) == c.D,
+                    "k ", k_in.sizes(), " and v ", v_in.sizes(), " must be [B, Hkv, M, D] of "
+                    "codes ", k_codes.sizes());
+  TORCH_CHECK_NOT_IMPLEMENTED(
+      k_in.scalar_type() == at::kBFloat16 || k_in.scalar_type() == at::kFloat, "dtype ",
+      k_in.scalar_type(), " is not supported (bfloat16 or float32)");
+  need_gpu(v_in);
+  TORCH_CHECK_VALUE(v_in.scalar_type() == k_in.scalar_type() && v_in.device() == k_in.device(),
+                    "k and v differ in dtype or device");
+  if (capacity < 0) capacity = c.blocks * T2T_KV8_BLOCK;
+  TORCH_CHECK_VALUE(capacity <= c.blocks * T2T_KV8_BLOCK, "capacity=", capacity, " exceeds the ",
+                    c.blocks, " blocks");
+  const c10::DeviceGuard guard(k_in.device());
+  const int64_t M = k_in.size(2);
+  Tensor pos;
+  if (pos_in.has_value()) {
+    TORCH_CHECK_VALUE(pos_in->is_cuda() && pos_in->device() == k_in.device() &&
+                          pos_in->scalar_type() == at::kLong,
+                      "pos must be an int64 tensor on the heads' device");
+    TORCH_CHECK_VALUE(pos_in->dim() <= 1 && (pos_in->numel() == 1 || pos_in->numel() == c.B),
+                      "pos ", pos_in->sizes(), " must be one position, or one for each of ", c.B,
+                      " sequences");
+    TORCH_CHECK_VALUE(M <= capacity, M, " tokens exceed capacity=", capacity);
+    pos = pos_in->contiguous();
+  } else {
+    TORCH_CHECK_VALUE(pos0 >= 0 && pos0 <= capacity - M, "positions ", pos0, " .. ",
+                      pos0 + M - 1, " exceed capacity=", capacity);
+  }
+  if (k_in.numel() == 0) return;
+  const Tensor k = vector_rows(k_in), v = vector_rows(v_in);
+  const t2t_tensor ks = heads_of(k), vs = heads_of(v);
+  check(t2t_kv8_append(&ks, &vs, c.B, c.Hkv, M, c.D,
+                       k.scalar_type() == at::kFloat ? T2T_DTYPE_F32 : T2T_DTYPE_BF16,
+                       pos.defined() ? pos.data_ptr<int64_t>() : nullptr,
+                       pos.defined() && pos.numel() > 1 ? 1 : 0, pos.defined() ? 0 : pos0,
+                       k_codes.data_ptr(), v_codes.data_ptr(), k_scale.data_ptr<float>(),
+                       v_scale.data_ptr<float>(), c.blocks, capacity, stream_of(k)),
+        "t2t_kv8_append");
+  // written in place, which graphs that saved the cache have to see (inference
+  // tensors have no versions)
+  for (const Tensor* t : {&k_codes, &v_codes, &k_scale, &v_scale})
+    if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+}
+
+std::tuple<Tensor, Tensor> kv8_attend(
+    const Tensor& q_in, const Tensor& k_codes, const Tensor& v_codes, const Tensor& k_scale,
+    const Tensor& v_scale, int64_t n_keys, const Tensor& key_doc,
+    const c10::optional<Tensor>& key_bits, const Tensor& q_pos, const Tensor& q_doc,
+    const c10::optional<Tensor>& q_bits, double scale, int64_t window, int64_t sinks,
+    const c10::optional<Tensor>& q_start) {
+  const Kv8 c(k_codes, v_codes, k_scale, v_scale, q_in);
+  TORCH_CHECK_NOT_IMPLEMENTED(q_in.scalar_type() == at::kBFloat16, "q dtype ", q_in.scalar_type(),
+                              " is not supported (bfloat16)");
+  TORCH_CHECK_VALUE(q_in.dim() == 4 && q_in.size(0) == c.B && q_in.size(3) == c.D && c.Hkv > 0 &&
+                        q_in.size(1) % c.Hkv == 0,
+                    "q ", q_in.sizes(), " must be [B, Hq, Tq, D] of codes ", k_codes.sizes(),
+                    ", Hq a multiple of Hkv");
+  const int64_t Hq = q_in.size(1), Tq = q_in.size(2);
+  TORCH_CHECK_NOT_IMPLEMENTED(Hq / c.Hkv * Tq <= T2T_KV8_MAX_ROWS, "(Hq / Hkv) * Tq = ",
+                              Hq / c.Hkv * Tq, " query rows per kv head exceeds ",
+                              T2T_KV8_MAX_ROWS);
+  TORCH_CHECK_VALUE(key_doc.dim() == 2 && (key_doc.size(0) == 1 || key_doc.size(0) == c.B),
+                    "key_doc ", key_doc.sizes(), " must be [1 or ", c.B, ", positions]");
+  const int64_t Bm = key_doc.size(0), cap = key_doc.size(1);
+  TORCH_CHECK_VALUE(n_keys >= 0 && n_keys <= cap && n_keys <= c.blocks * T2T_KV8_BLOCK,
+                    "n_keys=", n_keys, " exceeds the cache (", c.blocks * T2T_KV8_BLOCK,
+                    " positions, ", cap, " mask slots)");
+  TORCH_CHECK_VALUE(q_bits.has_value() == key_bits.has_value(),
+                    "q_bits and key_bits go together");
+  TORCH_CHECK_VALUE((sinks > 0) == q_start.has_value(), "q_start goes with sinks");
+  TORCH_CHECK_VALUE(scale > 0 && std::isfinite(scale), "scale=", scale, " must be positive and "
+                    "finite");
+  const int64_t W = key_bits.has_value() && key_bits->dim() == 3 ? key_bits->size(1) : 0;
+  TORCH_CHECK_NOT_IMPLEMENTED(W <= T2T_MAX_WORDS, W, " grant words exceed ", T2T_MAX_WORDS);
+  const auto takes = [&](const Tensor& t, at::ScalarType type, at::IntArrayRef shape,
+                         const char* name) {
+    TORCH_CHECK_VALUE(t.scalar_type() == type && t.is_contiguous() && t.sizes() == shape, name,
+                      " must be contiguous ", type, " ", shape, ", not ", t.scalar_type(), " ",
+                      t.sizes());
+    need_gpu(t);
+    TORCH_CHECK_VALUE(t.device() == q_in.device(), name, " is on another device");
+  };
+  const std::vector<int64_t> rows{Bm, Tq};
+  takes(key_doc, at::kInt, {Bm, cap}, "key_doc");
+  takes(q_pos, at::kInt, rows, "q_pos");
+  takes(q_doc, at::kInt, rows, "q_doc");
+  if (q_start.has_value()) takes(*q_start, at::kInt, rows, "q_start");
+  if (key_bits.has_value()) {
+    takes(*key_bits, at::kLong, {Bm, W, cap}, "key_bits");
+    takes(*q_bits, at::kLong, {Bm, W, Tq}, "q_bits");
+  }
+  const c10::DeviceGuard guard(q_in.device());
+  const Tensor q = vector_rows(q_in);
+  Tensor o = at::empty({c.B, Hq, Tq, c.D}, q.options());
+  Tensor lse2 = at::empty({c.B, Hq, Tq}, q.options().dtype(at::kFloat));
+  if (o.numel() == 0) return {o, lse2};
+  const int64_t bytes = t2t_kv8_attend_workspace(c.B, Hq, c.Hkv, Tq, n_keys, c.D);
+  Tensor ws = at::empty({bytes / 4}, lse2.options());
+  const t2t_tensor qs = heads_of(q), os = heads_of(o);
+  const auto bits = [](const c10::optional<Tensor>& t) {
+    return t.has_value() && t->numel() ? static_cast<const uint64_t*>(t->data_ptr()) : nullptr;
+  };
+  check(t2t_kv8_attend(&qs, k_codes.data_ptr(), v_codes.data_ptr(), k_scale.data_ptr<float>(),
+                       v_scale.data_ptr<float>(), c.blocks, &os, lse2.data_ptr<float>(),
+                       key_doc.data_ptr<int32_t>(), bits(key_bits), cap, q_pos.data_ptr<int32_t>(),
+                       q_doc.data_ptr<int32_t>(), bits(q_bits), Bm, W, c.B, Hq, c.Hkv, Tq, n_keys,
+                       c.D, T2T_DTYPE_BF16, static_cast<float>(scale),
+                       std::min<int64_t>(window, INT32_MAX), std::min<int64_t>(sinks, INT32_MAX),
+                       q_start.has_value() ? q_start->data_ptr<int32_t>() : nullptr,
+                       ws.data_ptr(), ws.numel() * 4, stream_of(q)),
+        "t2t_kv8_attend");
+  return {o, lse2};
+}
+
 // ---- scaled embedding
 
 int embed_code(const Tensor& w) {
@@ -848,9 +1007,12 @@ Tensor wgrad(const Tensor& dy, const Tensor& x, at::ScalarType out_dtype) {
 // (int64), in the order tile_class, the 13 tables of t2t_block_mask.  The
 // index tables are views of one allocation; the bitmaps, which dwarf them,
 // are their own.
-std::vector<Tensor> mask_meta(const Tensor& doc, const Tensor& q_bits, const Tensor& kv_bits,
-                              int64_t stream) {
+// window 0: none; sinks add t2t_doc_starts of doc behind the tables.
+std::vector<Tensor> mask_meta_window(const Tensor& doc, const Tensor& q_bits,
+                                     const Tensor& kv_bits, int64_t window, int64_t sinks,
+                                     int64_t stream_in) {
   need_gpu(doc, q_bits, kv_bits);
+  void* const stream = reinterpret_cast<void*>(static_cast<intptr_t>(stream_in));
   const c10::DeviceGuard guard(doc.device());
   const int64_t Bm = doc.size(0), T = doc.size(1), W = q_bits.size(1);
   const int64_t nt = (T + T2T_TILE - 1) / T2T_TILE;
@@ -886,13 +1048,42 @@ std::vector<Tensor> mask_meta(const Tensor& doc, const Tensor& q_bits, const Ten
   m.row_order = ptr(9); m.col_order = ptr(10); m.kv_bits_off = ptr(11); m.q_bits_slot = ptr(12);
   m.tile_bits = static_cast<uint32_t*>(t[13].data_ptr());
   m.tile_bits_slots = slots;
-  check(t2t_mask_meta(static_cast<const int32_t*>(doc.data_ptr()),
-                      W ? static_cast<const uint64_t*>(q_bits.data_ptr()) : nullptr,
-                      W ? static_cast<const uint64_t*>(kv_bits.data_ptr()) : nullptr, Bm, T, W,
-                      static_cast<int8_t*>(t[0].data_ptr()), &m,
-                      reinterpret_cast<void*>(static_cast<intptr_t>(stream))),
-        "t2t_mask_meta");
+  const int32_t* d = static_cast<const int32_t*>(doc.data_ptr());
+  const uint64_t* qb = W ? static_cast<const uint64_t*>(q_bits.data_ptr()) : nullptr;
+  const uint64_t* kb = W ? static_cast<const uint64_t*>(kv_bits.data_ptr()) : nullptr;
+  int8_t* cls = static_cast<int8_t*>(t[0].data_ptr());
+  if (window == 0) {
+    check(t2t_mask_meta(d, qb, kb, Bm, T, W, cls, &m, stream), "t2t_mask_meta");
+    return t;
+  }
+  const int32_t* start = nullptr;
+  if (sinks > 0) {
+    t.push_back(at::empty({Bm, T}, i32));
+    start = ptr(14);
+    check(t2t_doc_starts(d, Bm, T, ptr(14), stream), "t2t_doc_starts");
+  }
+  check(t2t_mask_meta_window(d, qb, kb, start, Bm, T, W, std::min<int64_t>(window, INT32_MAX),
+                             std::min<int64_t>(sinks, INT32_MAX), cls, &m, stream),
+        "t2t_mask_meta_window");
   return t;
+}
+
+std::vector<Tensor> mask_meta(const Tensor& doc, const Tensor& q_bits, const Tensor& kv_bits,
+                              int64_t stream) {
+  return mask_meta_window(doc, q_bits, kv_bits, 0, 0, stream);
+}
+
+// First token of each token's document, int32 of doc's shape [B, T].
+Tensor doc_starts(const Tensor& doc) {
+  need_gpu(doc);
+  TORCH_CHECK_VALUE(doc.dim() == 2 && doc.scalar_type() == at::kInt && doc.is_contiguous(),
+                    "doc must be contiguous int32 [B, T]");
+  const c10::DeviceGuard guard(doc.device());
+  Tensor start = at::empty_like(doc);
+  check(t2t_doc_starts(static_cast<const int32_t*>(doc.data_ptr()), doc.size(0), doc.size(1),
+                       static_cast<int32_t*>(start.data_ptr()), stream_of(doc)),
+        "t2t_doc_starts");
+  return start;
 }
 
 // doc [B, T] and, when words > 0, q / kv words [B, words, T] (else undefined)
@@ -1177,6 +1368,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("qkv_rotary", &qkv_rotary, no_gil);
   m.def("qkv_rotary_backward", &qkv_rotary_backward, no_gil);
   m.def("qkv_rotary_ad", &qkv_rotary_ad, no_gil);
+  m.def("kv8_append", &kv8_append, no_gil);
+  m.def("kv8_attend", &kv8_attend, no_gil);
   m.def("embedding_ad", &embedding_ad, no_gil);
   m.def("distill_loss_ad", &distill_loss_ad, no_gil);
   m.def("embedding", &embedding, no_gil);
@@ -1197,6 +1390,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     return wgrad(dy, x, f32 ? at::kFloat : at::kBFloat16);
   }, no_gil);
   m.def("mask_meta", &mask_meta, no_gil);
+  m.def("mask_meta_window", &mask_meta_window, no_gil);
+  m.def("doc_starts", &doc_starts, no_gil);
   m.def("token_inputs", &token_inputs, no_gil);
   m.def("current_stream", &current_stream);
   if (PyModule_AddFunctions(m.ptr(), kPredicates) != 0) throw py::error_already_set();

@@ -35,6 +35,19 @@
 // that of its first token, read from the lane holding it.  The grant-word
 // count is a template parameter, so a signature is exactly the registers it
 // needs and no loop over words is decided at run time.
+//
+// With a sliding window of w tokens and s sinks a document reads of itself only
+// the last w tokens and its first s:
+//   allowed = q >= k && (grant || (doc[q] == doc[k] &&
+//             (q - k < w || 0 <= k - start(q) < s)))
+// start(q) = the first token of the run of equal document ids that holds q
+// (doc_starts).  A key that a grant or a sink shows is seen by a whole query
+// run, any other key of the same document by the queries up to k + w - 1: still
+// one evaluation and one bit range per run and token.  A 16k row of six
+// documents, w 1024, s 4: doc_starts and the three launches below take 22 us
+// beside 17 us without a window, most of it the launches themselves.
+#include <utility>
+
 #include "attn_kernels.h"
 
 namespace t2t {
@@ -101,14 +114,19 @@ __device__ __forceinline__ bool sig_eq(const Sig<W>& a, const Sig<W>& b) {
   return eq;
 }
 
-// The non-causal part of the predicate for a query-side signature q and a
-// key-side signature k: same document, or a shared grant bit.
+// Whether a query-side signature q and a key-side signature k share a grant bit.
 template <int W>
-__device__ __forceinline__ bool sig_allowed(const Sig<W>& q, const Sig<W>& k) {
-  bool ok = q.doc == k.doc;
+__device__ __forceinline__ bool sig_granted(const Sig<W>& q, const Sig<W>& k) {
+  bool ok = false;
 #pragma unroll
   for (int w = 0; w < W; ++w) ok = ok || (q.w[w] & k.w[w]) != 0ull;
   return ok;
+}
+
+// The non-causal part of the predicate: same document, or a shared grant bit.
+template <int W>
+__device__ __forceinline__ bool sig_allowed(const Sig<W>& q, const Sig<W>& k) {
+  return q.doc == k.doc || sig_granted(q, k);
 }
 
 __device__ __forceinline__ int lane_id() { return threadIdx.x & 63; }
@@ -246,11 +264,14 @@ __device__ void wave_ordered(const int8_t* cls, int stride, int n, int8_t want,
 // evaluation sets a whole bit range; the causal and padding limits come last.
 constexpr int kTileWaves = kThreads / 64;
 
-template <int W>
+// Win: with the window's limits (start_all NULL without sinks).
+template <int W, bool Win>
 __global__ __launch_bounds__(kThreads) void mask_tiles(const int32_t* __restrict__ doc_all,
                                                        const uint64_t* __restrict__ qbits_all,
                                                        const uint64_t* __restrict__ kvbits_all,
-                                                       int T, MaskOut out) {
+                                                       const int32_t* __restrict__ start_all,
+                                                       int window, int sinks, int T,
+                                                       MaskOut out) {
   const int nt = out.nt;
   const int b = blockIdx.y;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -271,6 +292,21 @@ __global__ __launch_bounds__(kThreads) void mask_tiles(const int32_t* __restrict
                           load_sig<W>(doc, qbits, T, q0 + 64 + lane)};
   const Sig<W> ksig[2] = {load_sig<W>(doc, kbits, T, k0 + lane),
                           load_sig<W>(doc, kbits, T, k0 + 64 + lane)};
+  // first token of the document of queries q0 + lane and q0 + 64 + lane
+  int qstart[2] = {0, 0};
+  if constexpr (Win) {
+    if (start_all) {
+      const int32_t* start = start_all + (size_t)b * T;
+      qstart[0] = start[min(q0 + lane, T - 1)];
+      qstart[1] = start[min(q0 + 64 + lane, T - 1)];
+    }
+  }
+  // ... of the query run that begins at qa
+  auto run_start = [&](int qa) {
+    return qa < 64 ? __builtin_amdgcn_readlane(qstart[0], qa)
+                   : __builtin_amdgcn_readlane(qstart[1], qa - 64);
+  };
+  auto is_sink = [&](int start, int k) { return k >= start && k - start < sinks; };
   const TileSide<W> qs = mark_runs(qsig[0], qsig[1], qvalid);
   // Padding rows/columns are False pairs: such a tile can never be full.
   bool any_true = false;
@@ -281,12 +317,19 @@ __global__ __launch_bounds__(kThreads) void mask_tiles(const int32_t* __restrict
   // causal part
   for_each_run(qs, qvalid, open, [&](int qa, int qb, const Sig<W>& rsig) {
     bool t = false, f = false;
+    const int start = Win ? run_start(qa) : 0;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int kk = lane + 64 * i;
       const bool v = sig_allowed(rsig, ksig[i]);
-      const bool exists_ge = q0 + qb - 1 >= k0 + kk;  // some pair with q >= kv
-      const bool exists_lt = q0 + qa < k0 + kk;       // some pair with q < kv
+      bool exists_ge = q0 + qb - 1 >= k0 + kk;  // some pair with q >= kv
+      bool exists_lt = q0 + qa < k0 + kk;       // some pair with q < kv
+      if constexpr (Win) {
+        if (!sig_granted(rsig, ksig[i]) && !is_sink(start, k0 + kk)) {
+          exists_ge = exists_ge && q0 + qa - (k0 + kk) < window;
+          exists_lt = exists_lt || q0 + qb - 1 - (k0 + kk) >= window;
+        }
+      }
       t = t || (kk < kvalid && v && exists_ge);
       f = f || (kk < kvalid && (!v || exists_lt));
     }
@@ -302,13 +345,33 @@ __global__ __launch_bounds__(kThreads) void mask_tiles(const int32_t* __restrict
   uint32_t rows[2][4] = {}, cols[2][4] = {};
   for_each_run(ks, kvalid, always, [&](int a, int z, const Sig<W>& rsig) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-      if (sig_allowed(qsig[i], rsig)) set_bit_range(rows[i], a, z);
+    for (int i = 0; i < 2; ++i) {
+      if constexpr (Win) {
+        if (sig_granted(qsig[i], rsig)) {
+          set_bit_range(rows[i], a, z);
+        } else if (qsig[i].doc == rsig.doc) {
+          const int q = q0 + lane + 64 * i, s0 = qstart[i] - k0;
+          set_bit_range(rows[i], max(a, q - k0 - window + 1), z);
+          set_bit_range(rows[i], max(a, s0), min(z, s0 + sinks));
+        }
+      } else {
+        if (sig_allowed(qsig[i], rsig)) set_bit_range(rows[i], a, z);
+      }
+    }
   });
   for_each_run(qs, qvalid, always, [&](int a, int z, const Sig<W>& rsig) {
+    const int start = Win ? run_start(a) : 0;
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-      if (sig_allowed(rsig, ksig[i])) set_bit_range(cols[i], a, z);
+    for (int i = 0; i < 2; ++i) {
+      if constexpr (Win) {
+        const int k = k0 + lane + 64 * i;
+        const bool whole = sig_granted(rsig, ksig[i]) || is_sink(start, k);
+        if (sig_allowed(rsig, ksig[i]))
+          set_bit_range(cols[i], a, whole ? z : min(z, k + window - q0));
+      } else {
+        if (sig_allowed(rsig, ksig[i])) set_bit_range(cols[i], a, z);
+      }
+    }
   });
   uint32_t* dst = out.tile_bits + (size_t)(tri_slot(b, nt, qt) + kt) * kTileBitsWords;
 #pragma unroll
@@ -410,20 +473,87 @@ __global__ __launch_bounds__(kThreads) void mask_rank(MaskOut out) {
   rank_row_col(out, blockIdx.y, blockIdx.x, red);
 }
 
+// start[t] = the first token of the run of equal document ids that holds t.
+// grid (ceil(T / 256), Bm); block 256: the last run start at or before each
+// token of the block by ballots, and before the block by a search backwards,
+// 4096 tokens a step, whose loads do not wait for one another.
+constexpr int kStartSpan = 16;  // tokens a thread looks at in a step backwards
+
+__global__ __launch_bounds__(kThreads) void doc_starts(const int32_t* __restrict__ doc_all, int T,
+                                                       int32_t* __restrict__ start_all) {
+  __shared__ int last[kThreads / 64];
+  const int32_t* doc = doc_all + (size_t)blockIdx.y * T;
+  const int lane = lane_id(), wave = threadIdx.x >> 6;
+  const int t0 = blockIdx.x * kThreads, t = t0 + threadIdx.x;
+  const bool first = t < T && (t == 0 || doc[t] != doc[t - 1]);
+  const uint64_t m = __ballot(first);
+  if (lane == 0) last[wave] = m ? t0 + 64 * wave + 63 - __clzll((long long)m) : -1;
+  __syncthreads();
+  const uint64_t upto = m & (~0ull >> (63 - lane));
+  int s = upto ? t0 + 64 * wave + 63 - __clzll((long long)upto) : -1;
+  for (int w = 0; w < wave; ++w) s = upto ? s : max(s, last[w]);
+  __syncthreads();
+  // tokens of the run that enters the block: search [hi - 4096, hi)
+  if (t0 > 0 && __syncthreads_or(t < T && s < 0)) {
+    int found = -1;
+    for (int hi = t0; hi > 0 && found < 0; hi -= kThreads * kStartSpan) {
+      int best = -1;
+#pragma unroll
+      for (int i = 0; i < kStartSpan; ++i) {
+        const int u = hi - 1 - (int)threadIdx.x - kThreads * i;
+        const int d = doc[max(u, 0)], before = doc[max(u - 1, 0)];
+        if (u >= 0 && (u == 0 || d != before)) best = max(best, u);
+      }
+#pragma unroll
+      for (int off = 32; off > 0; off >>= 1) best = max(best, __shfl_xor(best, off, 64));
+      if (lane == 0) last[wave] = best;
+      __syncthreads();
+      for (int w = 0; w < kThreads / 64; ++w) found = max(found, last[w]);
+      __syncthreads();
+    }
+    if (s < 0) s = found;
+  }
+  if (t < T) start_all[(size_t)blockIdx.y * T + t] = s;
+}
+
+hipError_t launch_doc_starts(const int32_t* doc, int Bm, int T, int32_t* start,
+                             hipStream_t stream) {
+  if (Bm == 0 || T == 0) return hipSuccess;
+  hipLaunchKernelGGL(doc_starts, dim3((T + kThreads - 1) / kThreads, Bm), dim3(kThreads), 0,
+                     stream, doc, T, start);
+  return hipGetLastError();
+}
+
+namespace {
+
+template <bool Win, size_t... W>
+void start_tiles(std::index_sequence<W...>, int words, dim3 grid, hipStream_t stream,
+                 const int32_t* doc, const uint64_t* qbits, const uint64_t* kvbits,
+                 const int32_t* start, int window, int sinks, int T, const MaskOut& out) {
+  using TilesFn = void (*)(const int32_t*, const uint64_t*, const uint64_t*, const int32_t*, int,
+                           int, int, MaskOut);
+  static constexpr TilesFn kTilesByWords[] = {mask_tiles<W, Win>...};
+  hipLaunchKernelGGL(kTilesByWords[words], grid, dim3(kThreads), 0, stream, doc, qbits, kvbits,
+                     start, window, sinks, T, out);
+}
+
+}  // namespace
+
+// window 0: none
 hipError_t launch_mask_meta(const int32_t* doc, const uint64_t* qbits, const uint64_t* kvbits,
-                            int T, int words, const MaskOut& out, hipStream_t stream) {
+                            const int32_t* start, int window, int sinks, int T, int words,
+                            const MaskOut& out, hipStream_t stream) {
   const int nt = out.nt;
   if (nt == 0 || out.Bm == 0) return hipSuccess;
   if (words < 0 || words > kMaxWords) return hipErrorInvalidValue;
   const int64_t n_tri = (int64_t)nt * (nt + 1) / 2;
   const dim3 tiles((unsigned)((n_tri + kTileWaves - 1) / kTileWaves), out.Bm);
-  using TilesFn = void (*)(const int32_t*, const uint64_t*, const uint64_t*, int, MaskOut);
-  static constexpr TilesFn kTilesByWords[kMaxWords + 1] = {
-      mask_tiles<0>, mask_tiles<1>, mask_tiles<2>, mask_tiles<3>, mask_tiles<4>,
-      mask_tiles<5>, mask_tiles<6>, mask_tiles<7>, mask_tiles<8>};
-  static_assert(kMaxWords == 8, "one instantiation per grant-word count");
-  hipLaunchKernelGGL(kTilesByWords[words], tiles, dim3(kThreads), 0, stream, doc, qbits, kvbits,
-                     T, out);
+  constexpr auto kWords = std::make_index_sequence<kMaxWords + 1>{};
+  if (window > 0)
+    start_tiles<true>(kWords, words, tiles, stream, doc, qbits, kvbits, start, window, sinks, T,
+                      out);
+  else
+    start_tiles<false>(kWords, words, tiles, stream, doc, qbits, kvbits, nullptr, 0, 0, T, out);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   hipLaunchKernelGGL(mask_lists, dim3(nt, out.Bm), dim3(kThreads), 0, stream, out);

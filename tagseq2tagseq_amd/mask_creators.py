@@ -11,6 +11,9 @@ Mirrors model/graph_traversal/block_mask_creator.py and cross_doc_mask.py:
 * ``create_doc_link_block_mask(tokens, doc_spans, doc_links)`` -- the doc x doc
   link-bitmask form of the cross_doc_link mask (lower-triangular rows with the
   diagonal set), expressed in the same (q_bitmask, kv_bitmask) encoding
+* ``SlidingWindowMaskCreator(creator, window, sinks)`` -- any of them with a
+  sliding window (no counterpart in the reference); the creators' own keywords
+  ``window=`` and ``sinks=`` give the same mask
 * ``MASK_CREATORS`` / ``get_mask_creator`` / ``list_mask_creators`` /
   ``make_mask_creator_callable_from`` / ``make_mask_creator_callable`` -- :252-334
 
@@ -30,7 +33,7 @@ import numpy as np
 import torch
 
 from . import _lib
-from .block_mask import T2TBlockMask, build_block_mask, mask_inputs
+from .block_mask import T2TBlockMask, build_block_mask, check_window, mask_inputs
 
 logger = logging.getLogger(__name__)
 
@@ -149,10 +152,12 @@ def document_ids_host(seq_len: int, doc_spans: Sequence) -> np.ndarray:
 
 def _finish(doc, qb, kb, kwargs):
     """The creators' result: the BlockMask, or with ``inputs_only=True`` just
-    its per-token inputs (what the cached generation path reads)."""
+    its per-token inputs (what the cached generation path reads).  ``window``
+    and ``sinks``: of a sliding window (block_mask.build_block_mask)."""
+    limits = dict(window=kwargs.get("window"), sinks=kwargs.get("sinks", 0))
     if kwargs.get("inputs_only"):
-        return mask_inputs(doc, qb, kb)
-    return build_block_mask(doc, qb, kb)
+        return mask_inputs(doc, qb, kb, **limits)
+    return build_block_mask(doc, qb, kb, **limits)
 
 
 def create_doc_causal_block_mask(tokens: torch.Tensor, doc_spans: List[Any], **kwargs) -> T2TBlockMask:
@@ -288,6 +293,26 @@ class CrossDocLinkMaskCreator:
         return _finish(doc, qb, kb, kwargs)
 
 
+class SlidingWindowMaskCreator:
+    """The masks of ``creator`` (a ``(tokens, doc_spans, **kw)`` creator of this
+    module, or one that hands its keywords on to one) with a sliding window: a
+    token reads of its own document the last ``window`` tokens, itself among
+    them, and the first ``sinks`` ones; granted documents are read whole."""
+
+    def __init__(self, creator, window: int, sinks: int = 0):
+        if window is None:
+            raise ValueError("a sliding window needs a number of tokens")
+        self.creator = creator
+        self.window, self.sinks = check_window(window, sinks)
+
+    def __call__(self, tokens: torch.Tensor, doc_spans: List[Any], **kwargs):
+        bm = self.creator(tokens, doc_spans, **{**kwargs, "window": self.window,
+                                                "sinks": self.sinks})
+        if (getattr(bm, "window", None), getattr(bm, "sinks", 0)) != (self.window, self.sinks):
+            raise TypeError(f"{self.creator!r} does not take window= and sinks=")
+        return bm
+
+
 # Named creators; cross_doc_link is built from a link detector instead
 # (CrossDocLinkMaskCreator, wrapped with make_mask_creator_callable_from).
 MASK_CREATORS = dict(doc_causal=create_doc_causal_block_mask, causal=create_causal_block_mask)
@@ -329,5 +354,11 @@ def make_mask_creator_callable_from(creator):
     return _BatchMaskCreator(creator)
 
 
-def make_mask_creator_callable(mask_type: str):
-    return _BatchMaskCreator(get_mask_creator(mask_type))
+def make_mask_creator_callable(mask_type: str, window: Optional[int] = None, sinks: int = 0):
+    """The named creator as a (**batch) -> mask callable, with a sliding window
+    where one is given."""
+    creator = get_mask_creator(mask_type)
+    window, sinks = check_window(window, sinks)
+    if window is not None:
+        creator = SlidingWindowMaskCreator(creator, window, sinks)
+    return _BatchMaskCreator(creator)

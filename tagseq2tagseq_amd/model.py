@@ -24,6 +24,12 @@ such an edit.  New rows go through each layer with the decode-step kernel
 (``t2t_attn_decode``, up to 8 rows per kv head per launch); when more than
 ``prefill_rows`` rows are new, the whole sequence is recomputed through the
 block-mask kernels and the cache refilled.
+
+``kv_bits = 8`` holds the cache in 8 bits (kv8.py): half of its memory and of
+what a token's attention reads; rows that are recomputed as a whole sequence
+attend to the keys and values before their rounding.  A mask creator with a
+sliding window (mask_creators.SlidingWindowMaskCreator) limits the cached rows
+as it limits the whole sequence.
 """
 from __future__ import annotations
 
@@ -39,22 +45,32 @@ from .attention import flex_attention
 from .block_mask import T2TBlockMask, build_block_mask
 from .decode import MAX_ROWS, attn_decode
 from .embedding import embedding
+from .kv8 import KV8Cache
 from .modules import RMSNorm, TS2TSBackbone
-from .rope import qk_norm_rope_append, qkv_rope
+from .rope import qk_norm_rope_append
 from .rows import applies as rows_apply, rows_linear, rows_qkv_rope
 
 
 class KVCache:
     """Keys and values of every layer for the cached positions of one
     sequence (batch 1), with the token ids and mask inputs they were computed
-    under.  Storage: k, v bf16 [L][1][H][cap][D]; doc int32 [1][cap]; q / kv
-    words int64 [1][W][cap]."""
+    under.  Storage: k, v bf16 [L][1][H][cap][D], or with bits = 8 a KV8Cache a
+    layer; doc int32 [1][cap]; q / kv words int64 [1][W][cap]; with a sliding
+    window's sinks the documents' starts, int32 [1][cap]."""
 
     def __init__(self, num_layers: int, num_heads: int, head_dim: int, capacity: int,
-                 words: int, device, dtype=torch.bfloat16):
-        shape = (num_layers, 1, num_heads, capacity, head_dim)
-        self.k = torch.empty(shape, dtype=dtype, device=device)
-        self.v = torch.empty(shape, dtype=dtype, device=device)
+                 words: int, device, dtype=torch.bfloat16, bits: int = 16,
+                 window: Optional[int] = None, sinks: int = 0):
+        self.bits, self.window, self.sinks = bits, window, sinks
+        if bits == 8:
+            self.layers8 = [KV8Cache(1, num_heads, capacity, head_dim, device)
+                            for _ in range(num_layers)]
+        else:
+            shape = (num_layers, 1, num_heads, capacity, head_dim)
+            self.k = torch.empty(shape, dtype=dtype, device=device)
+            self.v = torch.empty(shape, dtype=dtype, device=device)
+        self.start = (torch.zeros((1, capacity), dtype=torch.int32, device=device) if sinks else
+                      None)
         self.tokens = torch.full((1, capacity), -1, dtype=torch.int64, device=device)
         self.doc = torch.empty((1, capacity), dtype=torch.int32, device=device)
         self.q_bits = torch.zeros((1, words, capacity), dtype=torch.int64, device=device)
@@ -62,6 +78,34 @@ class KVCache:
         self.capacity = capacity
         self.words = words
         self.length = 0
+
+    def fits(self, bm, bits: int) -> bool:
+        """Whether rows of the mask inputs ``bm`` belong into this cache."""
+        return ((self.words, self.window, self.sinks, self.bits)
+                == (bm.words, getattr(bm, "window", None), getattr(bm, "sinks", 0), bits))
+
+    def store(self, i: int, k: torch.Tensor, v: torch.Tensor, pos) -> None:
+        """Layer i's keys and values k, v [1, H, n, D] at positions pos .. pos +
+        n - 1 (pos an int, or for one row a device int64 tensor [1])."""
+        if self.bits == 8:
+            self.layers8[i].append(k, v, pos)
+        elif isinstance(pos, torch.Tensor):
+            self.k[i].index_copy_(2, pos, k)
+            self.v[i].index_copy_(2, pos, v)
+        else:
+            self.k[i, :, :, pos:pos + k.shape[2]] = k
+            self.v[i, :, :, pos:pos + k.shape[2]] = v
+
+    def attend(self, i: int, q: torch.Tensor, n_keys: int, q_pos, q_doc, q_bits, q_start,
+               out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Attention rows [1, H, n, D] of layer i's new rows q over the positions
+        before n_keys (in ``out`` where it is given)."""
+        mask = (n_keys, self.doc, self.kv_bits if self.words else None, q_pos, q_doc, q_bits)
+        limits = dict(window=self.window, sinks=self.sinks, q_start=q_start)
+        if self.bits == 8:
+            y = self.layers8[i].attend(q, *mask, **limits)[0]
+            return y if out is None else out.copy_(y)
+        return attn_decode(q, self.k[i], self.v[i], *mask, out=out, **limits)[0]
 
     def first_diff(self, tokens: torch.Tensor, bm, n: int) -> torch.Tensor:
         """Device int32 [1]: the first of positions 0 .. n - 1 whose token id
@@ -97,6 +141,8 @@ class KVCache:
     def store_inputs(self, tokens: torch.Tensor, bm, p0: int, p1: int) -> None:
         self.tokens[0, p0:p1] = tokens[0, p0:p1]
         self.doc[0, p0:p1] = bm.doc_ids[0, p0:p1]
+        if self.sinks:
+            self.start[0, p0:p1] = bm.doc_start[0, p0:p1]
         if self.words:
             self.q_bits[0, :, p0:p1] = bm.q_bits[0, :, p0:p1]
             self.kv_bits[0, :, p0:p1] = bm.kv_bits[0, :, p0:p1]
@@ -123,6 +169,7 @@ class TS2TSModel:
         self.embedding_scale = embedding_scale  # factor on the embedding's rows, or None
         self.kv_cache: Optional[KVCache] = None
         self.prefill_rows = 64
+        self.kv_bits = 16  # of the key/value cache: 16 (bf16) or 8
         self.use_graphs = True
         self.fuse_rows = True  # few-row steps on the fused row kernels (rows.py)
         self._graph: Optional[_DecodeGraph] = None
@@ -215,11 +262,12 @@ class TS2TSModel:
     def _layers(self):
         return self.backbone.layers
 
-    def _new_cache(self, words: int, device) -> KVCache:
+    def _new_cache(self, bm, device) -> KVCache:
         attn = self._layers()[0].attn
         return KVCache(len(self._layers()), attn.num_heads, attn.head_dim,
-                       self._layers()[0].attn.rotary.max_seq_len, words, device,
-                       self.embedding_weight.dtype)
+                       self._layers()[0].attn.rotary.max_seq_len, bm.words, device,
+                       self.embedding_weight.dtype, self.kv_bits, getattr(bm, "window", None),
+                       getattr(bm, "sinks", 0))
 
     @torch.no_grad()
     def forward_inference_last(self, tokens: torch.Tensor,
@@ -232,6 +280,8 @@ class TS2TSModel:
             # The key/value cache and the decode kernel are bf16; a float32
             # model recomputes the sequence on the float32 attention kernels.
             return self.forward_inference(tokens, doc_spans, **kwargs)[:, -1:]
+        if self.kv_bits not in (8, 16):
+            raise ValueError(f"kv_bits={self.kv_bits!r}: the cache holds 16 or 8 bits")
         # Per-token mask inputs only; the tile tables are built below if the
         # whole sequence has to be recomputed.
         bm = self.block_mask_creator(tokens=tokens, doc_spans=doc_spans or [], inputs_only=True,
@@ -242,8 +292,8 @@ class TS2TSModel:
             self.reset_cache()
             self._weights_seen = state
         cache = self.kv_cache
-        if cache is None or cache.words != bm.words or T > cache.capacity:
-            cache = self.kv_cache = self._new_cache(bm.words, tokens.device)
+        if cache is None or not cache.fits(bm, self.kv_bits) or T > cache.capacity:
+            cache = self.kv_cache = self._new_cache(bm, tokens.device)
             self._graph = None
         p = T - 1
         if self.use_graphs and p >= 1 and cache.length >= p:
@@ -264,7 +314,8 @@ class TS2TSModel:
         if full:
             p0 = 0
             if not isinstance(bm, T2TBlockMask):
-                bm = build_block_mask(bm.doc_ids, bm.q_bits, bm.kv_bits)
+                bm = build_block_mask(bm.doc_ids, bm.q_bits, bm.kv_bits, window=cache.window,
+                                      sinks=cache.sinks)
         cache.length = p0  # positions >= p0 are rewritten below
         cache.store_inputs(tokens, bm, p0, T)
         if self.use_graphs and not full and T - p0 == 1:
@@ -296,13 +347,10 @@ class TS2TSModel:
         tok = cache.tokens.index_select(1, buf.pos)
         qdoc = cache.doc.index_select(1, buf.pos)
         qbits = cache.q_bits.index_select(2, buf.pos) if cache.words else None
+        qstart = cache.start.index_select(1, buf.pos) if cache.sinks else None
         qpos = buf.pos.to(torch.int32).view(1, 1)
         x = self._embed(tok)
-        cos_t, sin_t = self._layers()[0].attn.rotary.tables(x.device)
         fused = self._rows_fusable(x)
-        if not fused:
-            cos = cos_t.index_select(0, buf.pos)
-            sin = sin_t.index_select(0, buf.pos)
         bb = self.backbone
         skips = []
         n_skip = len(bb.skip_weights)
@@ -310,21 +358,10 @@ class TS2TSModel:
         for i, layer in enumerate(bb.layers):
             if i >= n_skip and skips and not carried:
                 x = x + bb.skip_weights[i - n_skip] * skips.pop()
-            attn = layer.attn
             C = x.shape[-1]
             nxt = self._next_skip(i, skips) if fused else None
-            if attn.qk_norm:
-                q = self._normed_rows(layer, x, fused, buf.pos, cos_t, sin_t, cache.k[i],
-                                      cache.v[i])
-            elif fused:
-                q = rows_qkv_rope(x, attn.qkv.weight, attn.num_heads, cos_t, sin_t, buf.pos,
-                                  cache.k[i], cache.v[i], norm=layer.ln_1)
-            else:
-                q, k, v = qkv_rope(attn.qkv(layer.ln_1(x)), cos, sin, attn.num_heads, 0)
-                cache.k[i].index_copy_(2, buf.pos, k)
-                cache.v[i].index_copy_(2, buf.pos, v)
-            y, _ = attn_decode(q, cache.k[i], cache.v[i], cache.capacity, cache.doc,
-                               cache.kv_bits if cache.words else None, qpos, qdoc, qbits)
+            q, _, _ = self._new_rows(i, layer, x, fused, cache, buf.pos)
+            y = cache.attend(i, q, cache.capacity, qpos, qdoc, qbits, qstart)
             x = self._layer_tail(layer, y.transpose(1, 2).reshape(1, 1, C), x, fused, nxt)
             carried = nxt is not None
             if i < n_skip and not carried:
@@ -334,14 +371,24 @@ class TS2TSModel:
         return F.linear(self.norm(x), self.lm_head_weight)
 
     @staticmethod
-    def _normed_rows(layer, x, fused: bool, pos, cos, sin, k_cache, v_cache):
-        """Query rows of a layer with query / key norms; its keys and values go
-        to the cache rows at their positions (an int or a device tensor)."""
+    def _new_rows(i: int, layer, x, fused: bool, cache: KVCache, pos):
+        """Query rows of layer i for the rows x at positions pos .. (an int, or
+        for one row a device int64 tensor [1]), their keys and values put into the
+        cache; also these as the kernels left them, [1, H, n, D] (None, None
+        where they went to the cache alone)."""
         attn = layer.attn
+        cos, sin = attn.rotary.tables(x.device)
+        if cache.bits == 16 and fused and attn.rotary.whole_halves and not attn.qk_norm:
+            return rows_qkv_rope(x, attn.qkv.weight, attn.num_heads, cos, sin, pos, cache.k[i],
+                                 cache.v[i], norm=layer.ln_1), None, None
         h = (rows_linear(x, attn.qkv.weight, norm=layer.ln_1) if fused else
              attn.qkv(layer.ln_1(x)))
-        return qk_norm_rope_append(h, attn.q_norm, attn.k_norm, cos, sin, attn.num_heads, pos,
-                                   k_cache, v_cache, eps=attn.NORM_EPS)
+        if cache.bits == 16 and attn.qk_norm:
+            return qk_norm_rope_append(h, attn.q_norm, attn.k_norm, cos, sin, attn.num_heads, pos,
+                                       cache.k[i], cache.v[i], eps=attn.NORM_EPS), None, None
+        q, k, v = attn.heads(h, pos)
+        cache.store(i, k, v, pos)
+        return q, k, v
 
     def _rows_fusable(self, x) -> bool:
         """Whether the layers of a few-row step can run on the fused row
@@ -415,21 +462,12 @@ class TS2TSModel:
     def _layer_rows(self, i: int, layer, x, bm, cache: KVCache, p0: int, full: bool,
                     fused: bool, skip=None):
         """Layer.forward (model/modules/layer.py:32-35) over the new rows."""
-        attn = layer.attn
         B, n, C = x.shape
         T = p0 + n
-        cos, sin = attn.rotary.tables(x.device)
-        if attn.qk_norm:
-            q = self._normed_rows(layer, x, fused, p0, cos, sin, cache.k[i], cache.v[i])
-            k, v = cache.k[i, :, :, p0:T], cache.v[i, :, :, p0:T]
-        elif fused:
-            q = rows_qkv_rope(x, attn.qkv.weight, attn.num_heads, cos, sin, p0, cache.k[i],
-                              cache.v[i], norm=layer.ln_1)
-        else:
-            q, k, v = qkv_rope(attn.qkv(layer.ln_1(x)), cos, sin, attn.num_heads, p0)
-            cache.k[i, :, :, p0:T] = k
-            cache.v[i, :, :, p0:T] = v
+        q, k, v = self._new_rows(i, layer, x, fused, cache, p0)
         if full:
+            if k is None:
+                k, v = cache.k[i, :, :, p0:T], cache.v[i, :, :, p0:T]
             y = flex_attention(q, k, v, block_mask=bm)
         else:
             y = torch.empty_like(q)
@@ -437,11 +475,12 @@ class TS2TSModel:
             pos = torch.arange(p0, T, dtype=torch.int32, device=x.device)[None]
             for c0 in range(0, n, rows):
                 c1 = min(n, c0 + rows)
-                qb = bm.q_bits[:, :, p0 + c0:p0 + c1].contiguous() if bm.words else None
-                attn_decode(q[:, :, c0:c1], cache.k[i], cache.v[i], p0 + c1, cache.doc,
-                            cache.kv_bits if bm.words else None, pos[:, c0:c1].contiguous(),
-                            bm.doc_ids[:, p0 + c0:p0 + c1].contiguous(), qb,
-                            out=y[:, :, c0:c1])
+                at = slice(p0 + c0, p0 + c1)
+                cache.attend(i, q[:, :, c0:c1], p0 + c1, pos[:, c0:c1].contiguous(),
+                             bm.doc_ids[:, at].contiguous(),
+                             bm.q_bits[:, :, at].contiguous() if bm.words else None,
+                             bm.doc_start[:, at].contiguous() if cache.sinks else None,
+                             out=y[:, :, c0:c1])
         return self._layer_tail(layer, y.transpose(1, 2).reshape(B, n, C), x, fused, skip)
 
 
@@ -458,7 +497,7 @@ class _DecodeGraph:
 
     def __init__(self, model: TS2TSModel, cache: KVCache):
         self.cache = cache
-        self.pos = torch.zeros((1,), dtype=torch.int64, device=cache.k.device)
+        self.pos = torch.zeros((1,), dtype=torch.int64, device=cache.tokens.device)
         self.model = model
         self.fused = model.fuse_rows
         self.graph = None
