@@ -31,9 +31,11 @@
 //
 // With a sliding window of w positions and s sinks (Win) a key of the row's own
 // document is allowed only if pos(q) - j < w or 0 <= j - start(q) < s, start(q)
-// = the first position of the row's document; grants are as they were.  Without
-// grant words a chunk that lies outside every row's window and sinks ends
-// before it reads a key's document.
+// = the first position of the row's document; grants are as they were.  The
+// chunks are then those of the rows' PieceRange -- without grant words their
+// windows and sinks alone, wherever in the cache they are -- and a work-group
+// takes every gridDim.x-th of them: 12 heads of 64, a window of 4096 behind
+// 32768 positions 12 us with a work-group for every chunk of the cache.
 #include "attn_kernels.h"
 
 namespace t2t {
@@ -75,7 +77,7 @@ __device__ __forceinline__ float group_sum(float x) {
 // RMAX: compile-time bound on the R query rows (1, 2, 4 or 8), so the common
 // single-row step holds 8 + 8 accumulators per lane rather than 64 + 64.
 template <int D, int RMAX, bool Win>
-__global__ __launch_bounds__(kDecThreads) void attn_decode_partial(DecodeArgs a) {
+__device__ __forceinline__ void decode_chunk(const DecodeArgs& a, int chunk, int slot) {
   constexpr int GL = D / 8;                    // lanes per key
   constexpr int NKG = kDecThreads / GL;        // key groups per work-group
   constexpr int KPG = kDecChunk / NKG;         // keys per group
@@ -85,36 +87,13 @@ __global__ __launch_bounds__(kDecThreads) void attn_decode_partial(DecodeArgs a)
   __shared__ int32_t qpos_s[RMAX], qdoc_s[RMAX], qstart_s[RMAX];
   __shared__ uint64_t qbits_s[kMaxWords][RMAX];
 
-  const int chunk = blockIdx.x, hk = blockIdx.y, b = blockIdx.z;
+  const int hk = blockIdx.y, b = blockIdx.z;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int dg = tid % GL, kg = tid / GL;
   const int G = a.Hq / a.Hkv;
   const int R = G * a.Tq;
   const int mb = a.Bm > 1 ? b : 0;
   const int j0 = chunk * kDecChunk;
-
-  if constexpr (Win) {
-    if (a.W == 0) {
-      bool any = false;
-      for (int tq = 0; tq < a.Tq; ++tq) {
-        const int64_t p = a.q_pos[(size_t)mb * a.Tq + tq];
-        any = any || (j0 <= p && j0 + kDecChunk > p - a.window + 1);
-        if (a.q_start) {
-          const int64_t s = a.q_start[(size_t)mb * a.Tq + tq];
-          any = any || (j0 < s + a.sinks && j0 + kDecChunk > s);
-        }
-      }
-      if (!any) {  // an empty chunk
-        for (int x = tid; x < R * (D + 2); x += kDecThreads) {
-          const int r = x / (D + 2), col = x - r * (D + 2);
-          const int g = r / a.Tq, tq = r - g * a.Tq;
-          const size_t row = ((size_t)b * a.Hq + hk * G + g) * a.Tq + tq;
-          a.part[(row * a.nch + chunk) * (D + 2) + col] = col == 0 ? -INFINITY : 0.f;
-        }
-        return;
-      }
-    }
-  }
 
   const __bf16* kbase = static_cast<const __bf16*>(a.k.data) + b * a.k.sb + hk * a.k.sh + 8 * dg;
   const __bf16* vbase = static_cast<const __bf16*>(a.v.data) + b * a.v.sb + hk * a.v.sh + 8 * dg;
@@ -301,7 +280,27 @@ __global__ __launch_bounds__(kDecThreads) void attn_decode_partial(DecodeArgs a)
       for (int w = 0; w < kDecThreads / 64; ++w) val += red[w][r][col - 2];
     }
     const size_t row = ((size_t)b * a.Hq + hk * G + g) * a.Tq + tq;
-    a.part[(row * a.nch + chunk) * (D + 2) + col] = val;
+    a.part[(row * a.nch + slot) * (D + 2) + col] = val;
+  }
+}
+
+// Chunks of the rows of sequence b (with a window).
+__device__ __forceinline__ PieceRange<kDecChunk> window_chunks(const DecodeArgs& a, int b) {
+  const size_t row = (size_t)(a.Bm > 1 ? b : 0) * a.Tq;
+  return PieceRange<kDecChunk>(a.q_pos + row, a.q_start ? a.q_start + row : nullptr, a.Tq, a.Tkv,
+                               a.W == 0 ? a.window : 0, a.sinks);
+}
+
+template <int D, int RMAX, bool Win>
+__global__ __launch_bounds__(kDecThreads) void attn_decode_partial(DecodeArgs a) {
+  if constexpr (Win) {
+    const PieceRange<kDecChunk> range = window_chunks(a, blockIdx.z);
+    for (int i = blockIdx.x; i < range.count; i += gridDim.x) {
+      decode_chunk<D, RMAX, Win>(a, range.at(i), i);
+      __syncthreads();  // (its LDS is the next one's)
+    }
+  } else {
+    decode_chunk<D, RMAX, Win>(a, blockIdx.x, blockIdx.x);
   }
 }
 
@@ -309,7 +308,7 @@ __global__ __launch_bounds__(kDecThreads) void attn_decode_partial(DecodeArgs a)
 // chunk per lane; the weighted sum over chunks then issues its loads
 // independently (eight in flight per lane), so the merge costs a few memory
 // latencies whatever the chunk count.
-template <int D>
+template <int D, bool Win>
 __global__ __launch_bounds__(64) void attn_decode_combine(DecodeArgs a, TensorView o,
                                                           float* lse2) {
   constexpr int PER = D / 64;
@@ -318,25 +317,26 @@ __global__ __launch_bounds__(64) void attn_decode_combine(DecodeArgs a, TensorVi
   const int tq = blockIdx.x, h = blockIdx.y, b = blockIdx.z, lane = threadIdx.x;
   const size_t row = ((size_t)b * a.Hq + h) * a.Tq + tq;
   const float* pr = a.part + row * a.nch * S;
+  const int chunks = Win ? window_chunks(a, b).count : a.nch;
   float M = -INFINITY;
-  for (int c = lane; c < a.nch; c += 64) M = fmaxf(M, pr[(size_t)c * S]);
+  for (int c = lane; c < chunks; c += 64) M = fmaxf(M, pr[(size_t)c * S]);
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor(M, off, 64));
   float L = 0.f, acc[PER];
 #pragma unroll
   for (int e = 0; e < PER; ++e) acc[e] = 0.f;
   if (M != -INFINITY) {
-    for (int base = 0; base < a.nch; base += 64) {
+    for (int base = 0; base < chunks; base += 64) {
       const int c = base + lane;
       float w = 0.f;
-      if (c < a.nch) {
+      if (c < chunks) {
         const float m = pr[(size_t)c * S];
         w = m == -INFINITY ? 0.f : fast_exp2(m - M);
         L += w * pr[(size_t)c * S + 1];
       }
       wsh[lane] = w;
       __syncthreads();
-      const int n = min(64, a.nch - base);
+      const int n = min(64, chunks - base);
 #pragma unroll 8
       for (int k = 0; k < n; ++k) {
         const float wk = wsh[k];
@@ -373,11 +373,21 @@ void launch_both(int R, const DecodeArgs& a, const TensorView& o, float* lse2,
                  hipStream_t stream) {
   const dim3 pgrid((unsigned)a.nch, (unsigned)a.Hkv, (unsigned)a.B);
   const dim3 cgrid((unsigned)a.Tq, (unsigned)a.Hq, (unsigned)a.B);
-  if (a.window > 0)
-    launch_partial<D, true>(R, pgrid, a, stream);
-  else
+  if (a.window > 0) {
+    // a work-group for each chunk that rows next to one another read, which a
+    // window or sinks may begin and end inside
+    int64_t n = a.nch;
+    if (a.W == 0) {
+      n = ((int64_t)a.window + a.Tq + kDecChunk - 2) / kDecChunk + 1;
+      if (a.sinks > 0) n += ((int64_t)a.sinks + kDecChunk - 2) / kDecChunk + 1;
+    }
+    launch_partial<D, true>(R, dim3((unsigned)(n < a.nch ? n : a.nch), pgrid.y, pgrid.z), a,
+                            stream);
+    hipLaunchKernelGGL((attn_decode_combine<D, true>), cgrid, dim3(64), 0, stream, a, o, lse2);
+  } else {
     launch_partial<D, false>(R, pgrid, a, stream);
-  hipLaunchKernelGGL(attn_decode_combine<D>, cgrid, dim3(64), 0, stream, a, o, lse2);
+    hipLaunchKernelGGL((attn_decode_combine<D, false>), cgrid, dim3(64), 0, stream, a, o, lse2);
+  }
 }
 
 }  // namespace

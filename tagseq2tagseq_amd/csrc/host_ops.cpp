@@ -509,6 +509,106 @@ Tensor qkv_rotary_backward(const Tensor& dq_in, const Tensor& dk_in, const Tenso
   return dqkv;
 }
 
+// ---- decode step
+
+// Mask inputs of Tq new rows a sequence over a cache, checked.
+struct RowMask {
+  int64_t Bm, W, cap;
+  const Tensor &key_doc, &q_pos, &q_doc;
+  const c10::optional<Tensor>&key_bits, &q_bits, &q_start;
+  RowMask(const Tensor& q, int64_t B, int64_t Tq, const Tensor& key_doc_in,
+          const c10::optional<Tensor>& key_bits_in, const Tensor& q_pos_in,
+          const Tensor& q_doc_in, const c10::optional<Tensor>& q_bits_in, int64_t sinks,
+          const c10::optional<Tensor>& q_start_in)
+      : key_doc(key_doc_in), q_pos(q_pos_in), q_doc(q_doc_in), key_bits(key_bits_in),
+        q_bits(q_bits_in), q_start(q_start_in) {
+    W = key_bits.has_value() && key_bits->dim() == 3 ? key_bits->size(1) : 0;
+    TORCH_CHECK_VALUE(q_bits.has_value() == key_bits.has_value() &&
+                          (!q_bits.has_value() || (q_bits->dim() == 3 && q_bits->size(1) == W)),
+                      "q_bits and key_bits must both be given with the same word count (they go "
+                      "together)");
+    TORCH_CHECK_VALUE((sinks > 0) == q_start.has_value(), "q_start goes with sinks");
+    TORCH_CHECK_VALUE(key_doc.dim() == 2, "key_doc ", key_doc.sizes(), " must be [Bm, cap]");
+    Bm = key_doc.size(0);
+    cap = key_doc.size(1);
+    TORCH_CHECK_VALUE(Bm == 1 || Bm == B, "mask batch ", Bm, " does not broadcast to B=", B);
+    TORCH_CHECK_NOT_IMPLEMENTED(W <= T2T_MAX_WORDS, W, " grant words exceed ", T2T_MAX_WORDS);
+    const std::vector<int64_t> rows{Bm, Tq}, keys{Bm, cap}, kw{Bm, W, cap}, qw{Bm, W, Tq};
+    take(q, key_doc, at::kInt, keys, "key_doc");
+    take(q, q_pos, at::kInt, rows, "q_pos");
+    take(q, q_doc, at::kInt, rows, "q_doc");
+    if (q_start.has_value()) take(q, *q_start, at::kInt, rows, "q_start");
+    if (key_bits.has_value()) {
+      take(q, *key_bits, at::kLong, kw, "key_bits");
+      take(q, *q_bits, at::kLong, qw, "q_bits");
+    }
+  }
+  static void take(const Tensor& q, const Tensor& t, at::ScalarType type, at::IntArrayRef shape,
+                   const char* name) {
+    TORCH_CHECK_VALUE(t.scalar_type() == type && t.is_contiguous() && t.sizes() == shape, name,
+                      " must be contiguous ", type, " ", shape, ", not ", t.scalar_type(), " ",
+                      t.sizes());
+    TORCH_CHECK(t.device() == q.device(), name, " must be on q's device, the GPU ", q.device());
+  }
+  static const uint64_t* bits(const c10::optional<Tensor>& t) {
+    return t.has_value() && t->numel() ? static_cast<const uint64_t*>(t->data_ptr()) : nullptr;
+  }
+  const int32_t* start() const {
+    return q_start.has_value() ? q_start->data_ptr<int32_t>() : nullptr;
+  }
+};
+
+// window 0: none
+std::tuple<Tensor, Tensor> attn_decode(
+    const Tensor& q_in, const Tensor& k, const Tensor& v, int64_t n_keys, const Tensor& key_doc,
+    const c10::optional<Tensor>& key_bits, const Tensor& q_pos, const Tensor& q_doc,
+    const c10::optional<Tensor>& q_bits, double scale, const c10::optional<Tensor>& out,
+    int64_t window, int64_t sinks, const c10::optional<Tensor>& q_start) {
+  TORCH_CHECK_NOT_IMPLEMENTED(q_in.scalar_type() == at::kBFloat16 &&
+                                  k.scalar_type() == at::kBFloat16 &&
+                                  v.scalar_type() == at::kBFloat16,
+                              "bfloat16 only");
+  TORCH_CHECK(q_in.is_cuda() && k.is_cuda() && v.is_cuda(),
+              "the decode kernel needs ROCm GPU tensors");
+  TORCH_CHECK(k.device() == q_in.device() && v.device() == q_in.device(),
+              "the caches must be on q's device, ", q_in.device());
+  TORCH_CHECK_VALUE(q_in.dim() == 4 && k.dim() == 4, "q ", q_in.sizes(), " and the caches ",
+                    k.sizes(), " must be 4-D");
+  const int64_t B = q_in.size(0), Hq = q_in.size(1), Tq = q_in.size(2), D = q_in.size(3);
+  const RowMask m(q_in, B, Tq, key_doc, key_bits, q_pos, q_doc, q_bits, sinks, q_start);
+  TORCH_CHECK_VALUE(k.sizes() == v.sizes() && k.size(0) == B && k.size(3) == D, "caches ",
+                    k.sizes(), " / ", v.sizes(), " do not fit q ", q_in.sizes());
+  TORCH_CHECK_VALUE(n_keys >= 0 && n_keys <= std::min(m.cap, k.size(2)), "n_keys=", n_keys,
+                    " exceeds the cache (", k.size(2), " rows, ", m.cap, " mask slots)");
+  const c10::DeviceGuard guard(q_in.device());
+  const Tensor q = q_in.stride(3) == 1 ? q_in : q_in.contiguous();
+  Tensor o = out.has_value() ? *out : at::empty({B, Hq, Tq, D}, q.options());
+  if (out.has_value())
+    TORCH_CHECK_VALUE(o.sizes() == q.sizes() && o.scalar_type() == at::kBFloat16 &&
+                          o.device() == q.device(),
+                      "out ", o.sizes(), " must be bfloat16 of q's shape and on its device");
+  Tensor lse2 = at::empty({B, Hq, Tq}, q.options().dtype(at::kFloat));
+  Tensor ws = at::empty({t2t_attn_decode_workspace(B, Hq, Tq, n_keys, D) / 4}, lse2.options());
+  const t2t_tensor qs = view4(q), ks = view4(k), vs = view4(v), os = view4(o);
+  const int32_t *doc = key_doc.data_ptr<int32_t>(), *pos = q_pos.data_ptr<int32_t>(),
+                *qd = q_doc.data_ptr<int32_t>();
+  const float c = static_cast<float>(scale);
+  const int rc =
+      window == 0
+          ? t2t_attn_decode(&qs, &ks, &vs, &os, lse2.data_ptr<float>(), doc, m.bits(key_bits),
+                            m.cap, pos, qd, m.bits(q_bits), m.Bm, m.W, B, Hq, k.size(1), Tq,
+                            n_keys, D, T2T_DTYPE_BF16, c, ws.data_ptr(), ws.numel() * 4,
+                            stream_of(q))
+          : t2t_attn_decode_window(&qs, &ks, &vs, &os, lse2.data_ptr<float>(), doc,
+                                   m.bits(key_bits), m.cap, pos, qd, m.bits(q_bits), m.Bm, m.W, B,
+                                   Hq, k.size(1), Tq, n_keys, D, T2T_DTYPE_BF16, c,
+                                   std::min<int64_t>(window, INT32_MAX),
+                                   std::min<int64_t>(sinks, INT32_MAX), m.start(), ws.data_ptr(),
+                                   ws.numel() * 4, stream_of(q));
+  check(rc, "t2t_attn_decode");
+  return {o, lse2};
+}
+
 // ---- 8-bit key/value cache
 
 // Codes and scales of a cache, checked against the heads they are used with.
@@ -615,36 +715,12 @@ std::tuple<Tensor, Tensor> kv8_attend(
   TORCH_CHECK_NOT_IMPLEMENTED(Hq / c.Hkv * Tq <= T2T_KV8_MAX_ROWS, "(Hq / Hkv) * Tq = ",
                               Hq / c.Hkv * Tq, " query rows per kv head exceeds ",
                               T2T_KV8_MAX_ROWS);
-  TORCH_CHECK_VALUE(key_doc.dim() == 2 && (key_doc.size(0) == 1 || key_doc.size(0) == c.B),
-                    "key_doc ", key_doc.sizes(), " must be [1 or ", c.B, ", positions]");
-  const int64_t Bm = key_doc.size(0), cap = key_doc.size(1);
-  TORCH_CHECK_VALUE(n_keys >= 0 && n_keys <= cap && n_keys <= c.blocks * T2T_KV8_BLOCK,
+  const RowMask m(q_in, c.B, Tq, key_doc, key_bits, q_pos, q_doc, q_bits, sinks, q_start);
+  TORCH_CHECK_VALUE(n_keys >= 0 && n_keys <= m.cap && n_keys <= c.blocks * T2T_KV8_BLOCK,
                     "n_keys=", n_keys, " exceeds the cache (", c.blocks * T2T_KV8_BLOCK,
-                    " positions, ", cap, " mask slots)");
-  TORCH_CHECK_VALUE(q_bits.has_value() == key_bits.has_value(),
-                    "q_bits and key_bits go together");
-  TORCH_CHECK_VALUE((sinks > 0) == q_start.has_value(), "q_start goes with sinks");
+                    " positions, ", m.cap, " mask slots)");
   TORCH_CHECK_VALUE(scale > 0 && std::isfinite(scale), "scale=", scale, " must be positive and "
                     "finite");
-  const int64_t W = key_bits.has_value() && key_bits->dim() == 3 ? key_bits->size(1) : 0;
-  TORCH_CHECK_NOT_IMPLEMENTED(W <= T2T_MAX_WORDS, W, " grant words exceed ", T2T_MAX_WORDS);
-  const auto takes = [&](const Tensor& t, at::ScalarType type, at::IntArrayRef shape,
-                         const char* name) {
-    TORCH_CHECK_VALUE(t.scalar_type() == type && t.is_contiguous() && t.sizes() == shape, name,
-                      " must be contiguous ", type, " ", shape, ", not ", t.scalar_type(), " ",
-                      t.sizes());
-    need_gpu(t);
-    TORCH_CHECK_VALUE(t.device() == q_in.device(), name, " is on another device");
-  };
-  const std::vector<int64_t> rows{Bm, Tq};
-  takes(key_doc, at::kInt, {Bm, cap}, "key_doc");
-  takes(q_pos, at::kInt, rows, "q_pos");
-  takes(q_doc, at::kInt, rows, "q_doc");
-  if (q_start.has_value()) takes(*q_start, at::kInt, rows, "q_start");
-  if (key_bits.has_value()) {
-    takes(*key_bits, at::kLong, {Bm, W, cap}, "key_bits");
-    takes(*q_bits, at::kLong, {Bm, W, Tq}, "q_bits");
-  }
   const c10::DeviceGuard guard(q_in.device());
   const Tensor q = vector_rows(q_in);
   Tensor o = at::empty({c.B, Hq, Tq, c.D}, q.options());
@@ -653,17 +729,14 @@ std::tuple<Tensor, Tensor> kv8_attend(
   const int64_t bytes = t2t_kv8_attend_workspace(c.B, Hq, c.Hkv, Tq, n_keys, c.D);
   Tensor ws = at::empty({bytes / 4}, lse2.options());
   const t2t_tensor qs = heads_of(q), os = heads_of(o);
-  const auto bits = [](const c10::optional<Tensor>& t) {
-    return t.has_value() && t->numel() ? static_cast<const uint64_t*>(t->data_ptr()) : nullptr;
-  };
   check(t2t_kv8_attend(&qs, k_codes.data_ptr(), v_codes.data_ptr(), k_scale.data_ptr<float>(),
                        v_scale.data_ptr<float>(), c.blocks, &os, lse2.data_ptr<float>(),
-                       key_doc.data_ptr<int32_t>(), bits(key_bits), cap, q_pos.data_ptr<int32_t>(),
-                       q_doc.data_ptr<int32_t>(), bits(q_bits), Bm, W, c.B, Hq, c.Hkv, Tq, n_keys,
-                       c.D, T2T_DTYPE_BF16, static_cast<float>(scale),
-                       std::min<int64_t>(window, INT32_MAX), std::min<int64_t>(sinks, INT32_MAX),
-                       q_start.has_value() ? q_start->data_ptr<int32_t>() : nullptr,
-                       ws.data_ptr(), ws.numel() * 4, stream_of(q)),
+                       key_doc.data_ptr<int32_t>(), m.bits(key_bits), m.cap,
+                       q_pos.data_ptr<int32_t>(), q_doc.data_ptr<int32_t>(), m.bits(q_bits), m.Bm,
+                       m.W, c.B, Hq, c.Hkv, Tq, n_keys, c.D, T2T_DTYPE_BF16,
+                       static_cast<float>(scale), std::min<int64_t>(window, INT32_MAX),
+                       std::min<int64_t>(sinks, INT32_MAX), m.start(), ws.data_ptr(),
+                       ws.numel() * 4, stream_of(q)),
         "t2t_kv8_attend");
   return {o, lse2};
 }
@@ -1368,6 +1441,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("qkv_rotary", &qkv_rotary, no_gil);
   m.def("qkv_rotary_backward", &qkv_rotary_backward, no_gil);
   m.def("qkv_rotary_ad", &qkv_rotary_ad, no_gil);
+  m.def("attn_decode", &attn_decode, no_gil);
   m.def("kv8_append", &kv8_append, no_gil);
   m.def("kv8_attend", &kv8_attend, no_gil);
   m.def("embedding_ad", &embedding_ad, no_gil);

@@ -25,9 +25,8 @@
 // HBM bound: 2 D bytes a key and kv head.  At eight or more rows the products
 // alone would keep the vector units busy longer than the loads take, so they go
 // to the matrix unit whatever R: S^T = K Q^T and O^T = V^T P^T as 16x16x32 bf16
-// (e4m3 numbers are bf16 numbers, exactly; p is rounded to bf16 after the
-// running maximum and the value scale are in it, half a step of 2^-8 as in the
-// prefill kernels).  With A-operand row m of S tile t holding key
+// (e4m3 numbers are bf16 numbers, exactly, and p is taken as two of them, see
+// below).  With A-operand row m of S tile t holding key
 // 16 (m / 4) + 4 t + m % 4, lane (g, n) = (l / 16, l % 16) ends up with the
 // scores of keys 16 g + 0 .. 15 for row n, which in this order are the B operand
 // of the second product, whose A operand is then 16 neighbouring bytes of a row
@@ -260,7 +259,11 @@ __device__ __forceinline__ f32x4 mfma16(bf16x8 a, bf16x8 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
 
-template <int D>
+// Split: the rows' value sums are taken over p rounded to bf16 and over what
+// that rounding left, so that p counts with 16 bits.  Up to eight rows use half
+// of the products' 16 columns, and the other half takes the rests (Twice false:
+// column n + 8 is row n again); more rows take a second product.
+template <int D, bool Twice>
 __global__ __launch_bounds__(256) void kv8_attend_kernel(Kv8AttendArgs a) {
   constexpr int kPieces = D / 64;      // 16-byte pieces of a lane's part of a key
   constexpr int kTiles = D / 16;       // O^T tiles
@@ -271,7 +274,8 @@ __global__ __launch_bounds__(256) void kv8_attend_kernel(Kv8AttendArgs a) {
   const int chunk = blockIdx.x, hk = blockIdx.y, b = blockIdx.z;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int g = lane >> 4, n = lane & 15;
+  const int g = lane >> 4, column = lane & 15;
+  const int n = Twice ? column : column & 7;  // query row
   const int G = a.Hq / a.Hkv, R = G * a.Tq;
   const int mb = a.Bm > 1 ? b : 0;
   if (tid < a.Tq) {
@@ -290,10 +294,25 @@ __global__ __launch_bounds__(256) void kv8_attend_kernel(Kv8AttendArgs a) {
     for (int i = 0; i < 2 * kPieces; ++i) qraw[i] = reinterpret_cast<const uint4*>(q)[i];
   }
   __syncthreads();
+  // The blocks that these rows read, in equal shares of whole rounds of the
+  // waves.
+  const PieceRange<kBlk> range(spos, a.q_start ? sstart : nullptr, a.Tq, a.Tkv,
+                               a.W == 0 ? a.window : 0, a.sinks);
+  const int share = 4 * ((range.count + 4 * a.chunks - 1) / (4 * a.chunks));
+  const int end = min((chunk + 1) * share, range.count);
+  const size_t row0 = ((size_t)b * a.Hq + hk * G) * a.Tq;
+  float* pml = a.part + (size_t)a.B * a.Hq * a.Tq * a.chunks * D;
+  if (chunk * share >= range.count && a.chunks > 1) {  // no block: no sum either
+    if (tid < R) {
+      const size_t row = row0 + (size_t)(tid / a.Tq) * a.Tq + tid % a.Tq;
+      pml[(row * a.chunks + chunk) * 2] = -INFINITY;
+      pml[(row * a.chunks + chunk) * 2 + 1] = 0.f;
+    }
+    return;
+  }
   bf16x8 qf[2 * kPieces];
 #pragma unroll
   for (int i = 0; i < 2 * kPieces; ++i) qf[i] = *reinterpret_cast<const bf16x8*>(&qraw[i]);
-  const int64_t pos_n = spos[tq_n], start_n = sstart[tq_n];
 
   const int32_t* kdoc = a.key_doc + (size_t)mb * a.key_stride;
   const uint64_t* kbits = a.key_bits + (size_t)mb * a.W * a.key_stride;
@@ -307,19 +326,12 @@ __global__ __launch_bounds__(256) void kv8_attend_kernel(Kv8AttendArgs a) {
 #pragma unroll
   for (int i = 0; i < kTiles; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
   float m = -INFINITY, l = 0.f;
-  const int end = min((chunk + 1) * a.chunk_blocks, (a.Tkv + kBlk - 1) / kBlk);
-  for (int blk = chunk * a.chunk_blocks + wave; blk < end; blk += 4) {
-    const int j0 = blk * kBlk, j = j0 + lane;
-    // a block that no row's causal range, window or sinks reach (a grant
-    // reaches anything before the row)
-    bool near = n < R && j0 <= pos_n;
-    if (a.window > 0 && a.W == 0)
-      near = near && (j0 + kBlk > pos_n - a.window + 1 ||
-                      (a.q_start && j0 < start_n + a.sinks && j0 + kBlk > start_n));
-    if (!__any(near)) continue;
+  for (int v = chunk * share + wave; v < end; v += 4) {
+    const int blk = range.at(v);
+    const int j = blk * kBlk + lane;
     const bool in = j < a.Tkv;
     const int jd = in ? kdoc[j] : 0;
-    uint64_t mine = 0;  // bit i: key j0 + i is allowed for this lane's row
+    uint64_t mine = 0;  // bit i: key i of the block is allowed for this lane's row
     uint64_t any = 0;
     for (int tq = 0; tq < a.Tq; ++tq) {
       const int64_t p = spos[tq];
@@ -338,8 +350,9 @@ __global__ __launch_bounds__(256) void kv8_attend_kernel(Kv8AttendArgs a) {
     const uint32_t allowed = n < R ? (uint32_t)(mine >> (16 * g)) & 0xffffu : 0u;
 
     uint4 kraw[4][kPieces], vraw[kTiles];
-    const uint8_t* kp = kc + (int64_t)blk * kBlk * D + (16 * (n >> 2) + (n & 3)) * D + g * (D / 4);
-    const uint8_t* vp = vc + (int64_t)blk * kBlk * D + n * kBlk + 16 * g;
+    const uint8_t* kp = kc + (int64_t)blk * kBlk * D +
+                        (16 * (column >> 2) + (column & 3)) * D + g * (D / 4);
+    const uint8_t* vp = vc + (int64_t)blk * kBlk * D + column * kBlk + 16 * g;
 #pragma unroll
     for (int t = 0; t < 4; ++t)
 #pragma unroll
@@ -379,41 +392,50 @@ __global__ __launch_bounds__(256) void kv8_attend_kernel(Kv8AttendArgs a) {
         for (int e = 0; e < 4; ++e) o[i][e] *= keep;
       m = now;
     }
-    bf16x8 p[2];
+    bf16x8 p[2], rest[2];
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
       const float x = fast_exp2(s[e] - ref);
       l += x;
-      p[e >> 3][e & 7] = (__bf16)(x * vs);
+      const float y = x * vs;
+      const __bf16 hi = (__bf16)y;
+      const __bf16 lo = (__bf16)(y - (float)hi);
+      p[e >> 3][e & 7] = Twice || column < 8 ? hi : lo;
+      if (Twice) rest[e >> 3][e & 7] = lo;
     }
 #pragma unroll
     for (int i = 0; i < kTiles; ++i) {
-      o[i] = mfma16(decode8(vraw[i].x, vraw[i].y), p[0], o[i]);
-      o[i] = mfma16(decode8(vraw[i].z, vraw[i].w), p[1], o[i]);
+      const bf16x8 v0 = decode8(vraw[i].x, vraw[i].y), v1 = decode8(vraw[i].z, vraw[i].w);
+      o[i] = mfma16(v0, p[0], o[i]);
+      o[i] = mfma16(v1, p[1], o[i]);
+      if (Twice) {
+        o[i] = mfma16(v0, rest[0], o[i]);
+        o[i] = mfma16(v1, rest[1], o[i]);
+      }
     }
   }
 
-  // The four waves' sums of a row, joined.  Lane (g, n) holds o[16 i + 4 g + e]
-  // of row n.
+  // The four waves' sums of a row, joined.  Lane (g, column) holds
+  // o[16 i + 4 g + e] of its column.
   l = row_sum(l);
   if (g == 0) {
-    mls[wave][0][n] = m;
-    mls[wave][1][n] = l;
+    mls[wave][0][column] = m;
+    mls[wave][1][column] = l;
   }
 #pragma unroll
   for (int i = 0; i < kTiles; ++i)
-    *reinterpret_cast<f32x4*>(&osum[wave][n][16 * i + 4 * g]) = o[i];
+    *reinterpret_cast<f32x4*>(&osum[wave][column][16 * i + 4 * g]) = o[i];
   __syncthreads();
   for (int x = tid; x < R * D; x += 256) {
     const int r = x / D, d = x - r * D;
-    float M = fmaxf(fmaxf(mls[0][0][r], mls[1][0][r]), fmaxf(mls[2][0][r], mls[3][0][r]));
+    const float M = fmaxf(fmaxf(mls[0][0][r], mls[1][0][r]), fmaxf(mls[2][0][r], mls[3][0][r]));
     const float ref = M == -INFINITY ? 0.f : M;
-    float L = 0.f, v = 0.f;
+    float L = 0.f, sum = 0.f;
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
       const float f = fast_exp2(mls[w][0][r] - ref);
       L = fmaf(f, mls[w][1][r], L);
-      v = fmaf(f, osum[w][r][d], v);
+      sum = fmaf(f, Twice ? osum[w][r][d] : osum[w][r][d] + osum[w][r + 8][d], sum);
     }
     const int hq = hk * G + r / a.Tq, tq = r % a.Tq;
     const size_t row = ((size_t)b * a.Hq + hq) * a.Tq + tq;
@@ -421,71 +443,75 @@ __global__ __launch_bounds__(256) void kv8_attend_kernel(Kv8AttendArgs a) {
       // (a sum of NaN is a row's result, one of 0 a row without keys)
       const float inv = L == 0.f ? 0.f : 1.f / L;
       static_cast<__bf16*>(a.o.data)[b * a.o.sb + hq * a.o.sh + (int64_t)tq * a.o.st + d] =
-          (__bf16)(v * inv);
+          (__bf16)(sum * inv);
       if (d == 0) a.lse2[row] = L == 0.f ? -INFINITY : M + log2f(L);
     } else {
-      float* part = a.part + (row * a.chunks + chunk) * (D + 2);
-      part[2 + d] = v;
+      a.part[(row * a.chunks + chunk) * D + d] = sum;
       if (d == 0) {
-        part[0] = M;
-        part[1] = L;
+        pml[(row * a.chunks + chunk) * 2] = M;
+        pml[(row * a.chunks + chunk) * 2 + 1] = L;
       }
     }
   }
 }
 
-// One work-group per (new token, query head, batch row): the chunks' maxima
-// first, then their weights, then each wave adds every fourth chunk whose
-// weight is not 0.
+// One work-group per (new token, query head, batch row).  A lane holds one
+// chunk's (maximum, sum), so that every wave has all weights without LDS; the
+// sums are taken D / 4 lanes a chunk, and all of a lane's loads go out before
+// any is used: one memory latency whatever the number of chunks.
+constexpr int kMaxChunks = 64;
+
 template <int D>
 __global__ __launch_bounds__(256) void kv8_combine_kernel(Kv8AttendArgs a) {
-  constexpr int kPer = D / 64, kStep = D + 2;
-  __shared__ float wsh[256], red[4], lred[4], osh[4][D];
+  constexpr int kLanes = D / 4, kSlots = 256 / kLanes, kRounds = kMaxChunks / kSlots;
+  __shared__ __align__(16) float osh[4][D];
   const int tq = blockIdx.x, hq = blockIdx.y, b = blockIdx.z;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const size_t row = ((size_t)b * a.Hq + hq) * a.Tq + tq;
-  const float* part = a.part + row * a.chunks * kStep;
-  float M = -INFINITY;
-  for (int c = tid; c < a.chunks; c += 256) M = fmaxf(M, part[(size_t)c * kStep]);
+  const float* part = a.part + row * a.chunks * D;
+  const float* ml = a.part + (size_t)a.B * a.Hq * a.Tq * a.chunks * D + row * a.chunks * 2;
+  float2 own = make_float2(-INFINITY, 0.f);
+  if (lane < a.chunks) own = reinterpret_cast<const float2*>(ml)[lane];
+  float4 v[kRounds];
+#pragma unroll
+  for (int i = 0; i < kRounds; ++i) {
+    const int c = tid / kLanes + i * kSlots;
+    v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (c < a.chunks)
+      v[i] = *reinterpret_cast<const float4*>(part + (size_t)c * D + 4 * (tid % kLanes));
+  }
+  float M = own.x;
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor(M, off, 64));
-  if (lane == 0) red[wave] = M;
-  __syncthreads();
-  M = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-  const float ref = M == -INFINITY ? 0.f : M;
-  float L = 0.f, acc[kPer] = {};
-  for (int base = 0; base < a.chunks; base += 256) {
-    const int c = base + tid;
-    float w = 0.f;
-    if (c < a.chunks) {
-      w = fast_exp2(part[(size_t)c * kStep] - ref);
-      L = fmaf(w, part[(size_t)c * kStep + 1], L);
-    }
-    wsh[tid] = w;
-    __syncthreads();
-    const int count = min(256, a.chunks - base);
-#pragma unroll 4
-    for (int k = wave; k < count; k += 4) {
-      const float wk = wsh[k];
-      if (wk == 0.f) continue;
-#pragma unroll
-      for (int e = 0; e < kPer; ++e)
-        acc[e] = fmaf(wk, part[(size_t)(base + k) * kStep + 2 + lane + 64 * e], acc[e]);
-    }
-    __syncthreads();
-  }
+  const float w = fast_exp2(own.x - (M == -INFINITY ? 0.f : M));
+  float L = w * own.y;
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) L += __shfl_xor(L, off, 64);
-  if (lane == 0) lred[wave] = L;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-  for (int e = 0; e < kPer; ++e) osh[wave][lane + 64 * e] = acc[e];
+  for (int i = 0; i < kRounds; ++i) {
+    const float f = __shfl(w, (tid / kLanes + i * kSlots) & 63, 64);
+    if (f != 0.f) {  // (a chunk without a key has left no sums)
+      acc.x = fmaf(f, v[i].x, acc.x);
+      acc.y = fmaf(f, v[i].y, acc.y);
+      acc.z = fmaf(f, v[i].z, acc.z);
+      acc.w = fmaf(f, v[i].w, acc.w);
+    }
+  }
+#pragma unroll
+  for (int off = kLanes; off < 64; off <<= 1) {
+    acc.x += __shfl_xor(acc.x, off, 64);
+    acc.y += __shfl_xor(acc.y, off, 64);
+    acc.z += __shfl_xor(acc.z, off, 64);
+    acc.w += __shfl_xor(acc.w, off, 64);
+  }
+  if (lane < kLanes) *reinterpret_cast<float4*>(&osh[wave][4 * lane]) = acc;
   __syncthreads();
-  L = (lred[0] + lred[1]) + (lred[2] + lred[3]);
   if (tid < D) {
-    const float v = (osh[0][tid] + osh[1][tid]) + (osh[2][tid] + osh[3][tid]);
+    const float sum = (osh[0][tid] + osh[1][tid]) + (osh[2][tid] + osh[3][tid]);
     const float inv = L == 0.f ? 0.f : 1.f / L;
     static_cast<__bf16*>(a.o.data)[b * a.o.sb + hq * a.o.sh + (int64_t)tq * a.o.st + tid] =
-        (__bf16)(v * inv);
+        (__bf16)(sum * inv);
   }
   if (tid == 0) a.lse2[row] = L == 0.f ? -INFINITY : M + log2f(L);
 }
@@ -496,15 +522,14 @@ constexpr int kAimGroups = 1024;
 
 }  // namespace
 
-// Chunks are whole rounds of the four waves' blocks, as many as fill the aim.
-void kv8_split(int B, int Hkv, int Tkv, int* chunks, int* chunk_blocks) {
+// Chunks of a row's keys: as many as fill the aim, at most one for each round of
+// the four waves' blocks and as many as the second pass has lanes.
+int kv8_chunks(int B, int Hkv, int Tkv) {
   const int rounds = (Tkv + 4 * kBlk - 1) / (4 * kBlk);
   const int64_t pairs = (int64_t)B * Hkv;
-  const int want = (int)((kAimGroups + pairs - 1) / (pairs > 0 ? pairs : 1));
-  const int n = rounds < 1 ? 1 : (want < 1 ? 1 : (want < rounds ? want : rounds));
-  const int each = rounds < 1 ? 1 : (rounds + n - 1) / n;
-  *chunk_blocks = 4 * each;
-  *chunks = rounds < 1 ? 1 : (rounds + each - 1) / each;
+  const int64_t want = pairs > 0 ? (kAimGroups + pairs - 1) / pairs : 1;
+  const int n = (int)(want < kMaxChunks ? want : kMaxChunks);
+  return rounds < 1 ? 1 : n < rounds ? n : rounds;
 }
 
 hipError_t launch_kv8_append(const Kv8AppendArgs& a, bool f32, int D, hipStream_t stream) {
@@ -525,12 +550,17 @@ hipError_t launch_kv8_append(const Kv8AppendArgs& a, bool f32, int D, hipStream_
 }
 
 hipError_t launch_kv8_attend(Kv8AttendArgs a, int D, hipStream_t stream) {
-  kv8_split(a.B, a.Hkv, a.Tkv, &a.chunks, &a.chunk_blocks);
+  a.chunks = kv8_chunks(a.B, a.Hkv, a.Tkv);
   const dim3 grid(a.chunks, a.Hkv, a.B), rows(a.Tq, a.Hq, a.B);
-  if (D == 64)
-    hipLaunchKernelGGL(kv8_attend_kernel<64>, grid, dim3(256), 0, stream, a);
+  const bool twice = a.Hq / a.Hkv * a.Tq > 8;
+  if (D == 64 && twice)
+    hipLaunchKernelGGL((kv8_attend_kernel<64, true>), grid, dim3(256), 0, stream, a);
+  else if (D == 64)
+    hipLaunchKernelGGL((kv8_attend_kernel<64, false>), grid, dim3(256), 0, stream, a);
+  else if (twice)
+    hipLaunchKernelGGL((kv8_attend_kernel<128, true>), grid, dim3(256), 0, stream, a);
   else
-    hipLaunchKernelGGL(kv8_attend_kernel<128>, grid, dim3(256), 0, stream, a);
+    hipLaunchKernelGGL((kv8_attend_kernel<128, false>), grid, dim3(256), 0, stream, a);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || a.chunks == 1) return e;
   if (D == 64)

@@ -102,18 +102,7 @@ __global__ __launch_bounds__(kRotThreads) void rotary_kernel(RotaryArgs a) {
     const uint32_t n = (uint32_t)n0 + token;  // (at most 2^31 tokens)
     if (!in || n >= total) continue;
     const int b = n / (uint32_t)a.T, t = n - b * a.T;
-    const int64_t p = a.pos ? a.pos[b * a.pos_sb + t] : (int64_t)a.pos0 + t;
-    const bool known = p >= 0 && p < a.rows;
     T* row = static_cast<T*>(a.packed) + b * a.p_sb + (int64_t)t * a.p_st;
-    float c[8] = {}, s[8] = {};
-    if (turns && known) {
-      unpack(load_eight(a.cos + p * (a.R >> 1) + 8 * j), c);
-      unpack(load_eight(a.sin + p * (a.R >> 1) + 8 * j), s);
-      if constexpr (Back) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) s[e] = -s[e];
-      }
-    }
     // head h of the packed row in its view
     const auto view = [&](int h) {
       const int w = h < a.Hq ? 0 : h < rotated ? 1 : 2;
@@ -121,8 +110,8 @@ __global__ __launch_bounds__(kRotThreads) void rotary_kernel(RotaryArgs a) {
       return static_cast<T*>(o.data) + b * o.sb + (int64_t)t * o.st +
              (h - (w == 0 ? 0 : w == 1 ? a.Hq : rotated)) * o.sh;
     };
-    for (int h0 = head0; h0 < heads; h0 += kAhead * a.per_token) {
-      EightOf<T> r1[kAhead], r2[kAhead];
+    EightOf<T> r1[kAhead], r2[kAhead];
+    const auto load = [&](int h0) {
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) {
         const int h = h0 + i * a.per_token;
@@ -132,6 +121,21 @@ __global__ __launch_bounds__(kRotThreads) void rotary_kernel(RotaryArgs a) {
           r2[i] = load_eight(src + o2);
         }
       }
+    };
+    load(head0);  // (ahead of the position, which the angles wait for)
+    const int64_t p = a.pos ? a.pos[b * a.pos_sb + t] : (int64_t)a.pos0 + t;
+    const bool known = p >= 0 && p < a.rows;
+    float c[8] = {}, s[8] = {};
+    if (turns && known) {
+      unpack(load_eight(a.cos + p * (a.R >> 1) + 8 * j), c);
+      unpack(load_eight(a.sin + p * (a.R >> 1) + 8 * j), s);
+      if constexpr (Back) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s[e] = -s[e];
+      }
+    }
+    for (int h0 = head0; h0 < heads; h0 += kAhead * a.per_token) {
+      if (h0 != head0) load(h0);
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) {
         const int h = h0 + i * a.per_token;
