@@ -207,6 +207,23 @@ int t2t_attn_bwd(const t2t_tensor *q, const t2t_tensor *k, const t2t_tensor *v,
                  int32_t D, int32_t dtype, float scale, const t2t_block_mask *mask,
                  void *stream);
 
+/* Workspace (bytes) of t2t_attn_bwd_uneven; 0 where it runs as t2t_attn_bwd. */
+int64_t t2t_attn_bwd_uneven_workspace(int32_t B, int32_t Hkv, int32_t T, int32_t D,
+                                      int32_t dtype);
+
+/*
+ * t2t_attn_bwd for masks whose columns are uneven (a sliding window's, whose
+ * sinks are read by whole documents): where there are few columns, the queries
+ * of a long one are shared by several work-groups, whose fp32 sums of dK and
+ * dV are added in a fixed order (deterministic, no atomics).
+ */
+int t2t_attn_bwd_uneven(const t2t_tensor *q, const t2t_tensor *k, const t2t_tensor *v,
+                        const t2t_tensor *o, const t2t_tensor *dout, const float *lse2,
+                        float *delta, const t2t_tensor *dq, const t2t_tensor *dk,
+                        const t2t_tensor *dv, int32_t B, int32_t Hq, int32_t Hkv, int32_t T,
+                        int32_t D, int32_t dtype, float scale, const t2t_block_mask *mask,
+                        void *workspace, int64_t workspace_bytes, void *stream);
+
 /*
  * t2t_attn_bwd without the caller's Delta workspace, for callers that cannot
  * allocate device memory (code under HIP graph capture, tight serving loops,

@@ -7,13 +7,14 @@ Seams replaced (reference file:line):
     (model/modules/layer.py:16-21,33; monkey-patched at generate.py:167-178),
     i.e. torch/nn/attention/flex_attention.py:1396-1676.
   * FlexAttentionAutogradOp (torch/_higher_order_ops/flex_attention.py:628-767)
-    -- twice, over the same kernels: ``T2TFlexAttentionFn``, a plain
-    autograd.Function that eager calls use (saves q, k, v, out and the
-    log2-domain LSE; backward = atomic-free dK/dV + dQ kernels), and
+    -- over the same kernels: the host module's own record of a call that
+    nothing but autograd watches (saves q, k, v, out and the log2-domain LSE;
+    backward = atomic-free dK/dV + dQ kernels), ``T2TFlexAttentionFn``, a plain
+    autograd.Function with the same contents for other eager calls, and
     ``torch.ops.t2t.masked_attention`` / ``t2t::masked_attention_backward``,
     ``torch.library`` custom ops with fake implementations and registered
     autograd that compiled graphs trace.  ``flex_attention`` picks the custom
-    op while torch.compile traces and the Function otherwise: the custom op's
+    op while torch.compile traces and the others otherwise: the custom op's
     registered autograd costs several hundred microseconds of host time per
     call, the Function tens.
   * ``FlexSelfAttention(dim, num_heads, max_seq_len, fp8_out_proj)`` with
@@ -128,9 +129,11 @@ def attn_fwd(q, k, v, block_mask, scale: float):
 
 
 def attn_bwd(q, k, v, out, dout, lse2, block_mask, scale: float):
-    """Kernel call: returns (dq, dk, dv).  ``block_mask`` as in attn_fwd."""
+    """Kernel call: returns (dq, dk, dv).  ``block_mask`` as in attn_fwd; a
+    sliding window's mask gets the launch for uneven columns."""
     mask = _mask_struct(block_mask)
-    return _lib.host().attn_bwd(q, k, v, out, dout, lse2, ctypes.addressof(mask), scale)
+    return _lib.host().attn_bwd(q, k, v, out, dout, lse2, ctypes.addressof(mask), scale,
+                                getattr(block_mask, "window", None) is not None)
 
 
 class BwdPhases:
@@ -289,9 +292,12 @@ def flex_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
         out, lse2 = masked_attention(query, key, value, block_mask.tables(), float(scale))
     elif _lib.unwatched(query, key, value):
         out, lse2 = attn_fwd(query, key, value, block_mask, float(scale))
+    elif _lib.only_recorded(query, key, value):
+        # eager: the same kernels recorded by the host module, whose host cost
+        # per call is a fraction of the custom op's registered autograd
+        out, lse2 = _lib.host().attn_ad(query, key, value, block_mask.tables(), float(scale),
+                                        block_mask.window is not None)
     else:
-        # eager: the same kernels through a plain autograd.Function, whose host
-        # cost per call is a fraction of the custom op's registered autograd
         out, lse2 = T2TFlexAttentionFn.apply(query, key, value, block_mask, float(scale))
     if return_lse:
         return out, lse2 * LN2

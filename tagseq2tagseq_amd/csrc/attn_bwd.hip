@@ -41,7 +41,26 @@ struct BwdParams {
   float scale, scale_log2;
   int fuse_delta;  // dQ computes and writes Delta itself (kBwdDqDelta)
   MaskTables m;
+  float* part;     // split dK/dV: [B][Hkv][nt][splits][2][128][D] partial sums
+  int splits;
 };
+
+// Split dK/dV.  A window's columns are uneven: most are read by a window's
+// length of queries, those that hold sinks or granted documents by whole
+// documents, and where the columns are about as many as the CUs the longest one
+// is the launch's time.  The items (query head, query tile) of a column longer
+// than kSplitItems are then shared by up to `splits` work-groups, which leave
+// fp32 sums for bwd_dkdv_join to add in order.  2 rows of 4001 tokens, 16 / 4
+// heads of 128, nine linked documents, window 700 (256 columns of 4 to 128
+// items, 43 on average): 380 us in one work-group a column; 233 with the join's
+// 11 in up to four of 32 items, 240 in four of 16, 256 in eight of 16, which
+// write and read twice the sums.
+constexpr int kSplitItems = 32;
+constexpr int kMaxSplits = 4;
+
+__device__ __forceinline__ int column_pieces(int items, int splits) {
+  return max(1, min(splits, (items + kSplitItems - 1) / kSplitItems));
+}
 
 // Stores a transposed 32 x 32 f32 accumulator block (rows = d, cols = token)
 // scaled by `mul` as bf16 into out[token][d0 + d].
@@ -127,8 +146,13 @@ constexpr int kDkdvThreads = 64 * kDkdvWaves;
 // after the barrier that retired them (the next (head, tile) item's first
 // half is fetched during the current item's second half), so each copy has
 // one phase of compute to land in.
-template <int D>
+// Split: grid.z is (piece of the column, batch row), the last piece first, so
+// that work-groups without one (in a column of fewer pieces) lie together in the
+// order of dispatch: side by side with the others they would fall on the same
+// shader engines every time and leave those idle.
+template <int D, bool Split>
 __global__ __launch_bounds__(kDkdvThreads, 1) void bwd_dkdv_kernel(BwdParams p) {
+#ifdef __HIP_DEVICE_COMPILE__  // (the host's pass has no buffer resources)
   constexpr int KS = D / 16;
   constexpr int DT = D / 32;
   using U = UnitDma<D, kDkdvWaves>;
@@ -141,7 +165,8 @@ __global__ __launch_bounds__(kDkdvThreads, 1) void bwd_dkdv_kernel(BwdParams p) 
   // (16-byte aligned: rows are read four at a time)
   __shared__ __align__(16) float lse_lo[64], lse_hi[64], dl_lo[64], dl_hi[64];
 
-  const int hk = blockIdx.x, b = blockIdx.z;
+  const int hk = blockIdx.x, b = Split ? blockIdx.z % p.B : blockIdx.z;
+  const int piece = Split ? p.splits - 1 - blockIdx.z / p.B : 0;
   const int tid = threadIdx.x, wave = uniform(tid >> 6), lane = tid & 63;
   // Waves w and w + 4 share a SIMD; pairing key groups two apart there keeps
   // both busy on tiles whose upper key groups are masked for a whole half
@@ -160,7 +185,11 @@ __global__ __launch_bounds__(kDkdvThreads, 1) void bwd_dkdv_kernel(BwdParams p) 
   const int npart = uniform(p.m.q_num[col]);
   const int nfull = uniform(p.m.full_q_num[col]);
   const int nq = npart + nfull;
-  const int nu = G * nq;  // (query head, query tile) items
+  const int items = G * nq;  // (query head, query tile)
+  const int pieces = Split ? column_pieces(items, p.splits) : 1;
+  if (Split && piece >= pieces) return;
+  const int share = Split ? (items + pieces - 1) / pieces : items;
+  const int u0 = piece * share, nu = Split ? min(items, u0 + share) : items;
   const int32_t* pidx = p.m.q_idx + col * nt;
   const int32_t* fidx = p.m.full_q_idx + col * nt;
   const int32_t* pslot = p.m.q_bits_slot + col * nt;
@@ -341,13 +370,14 @@ __global__ __launch_bounds__(kDkdvThreads, 1) void bwd_dkdv_kernel(BwdParams p) 
 
   int2 e_next = make_int2(0, 0);
   uint4 wb = make_uint4(~0u, ~0u, ~0u, ~0u);
-  if (nu > 0) {
-    e_next = entry(0);
-    load_q_part(q_lo, lse_lo, hk * G, e_next.x * kTile);
-    load_do_part(do_lo, dl_lo, hk * G, e_next.x * kTile);
-    wb = tile_words(e_next, 0 < npart);
+  const int hh0 = Split && u0 < nu ? u0 / nq : 0, it0 = Split ? u0 - hh0 * nq : 0;
+  if (u0 < nu) {
+    e_next = entry(it0);
+    load_q_part(q_lo, lse_lo, hk * G + hh0, e_next.x * kTile);
+    load_do_part(do_lo, dl_lo, hk * G + hh0, e_next.x * kTile);
+    wb = tile_words(e_next, it0 < npart);
   }
-  for (int u = 0, hh = 0, it = 0; u < nu; ++u) {
+  for (int u = u0, hh = hh0, it = it0; u < nu; ++u) {
     const int h = hk * G + hh;
     const int q0 = e_next.x * kTile;
     const bool partial = it < npart;
@@ -420,6 +450,18 @@ __global__ __launch_bounds__(kDkdvThreads, 1) void bwd_dkdv_kernel(BwdParams p) 
           mine[dt][4 * a + 2] += x.z; mine[dt][4 * a + 3] += x.w;
         }
     }
+    if (Split && pieces > 1) {  // row kloc of this piece's sums
+      float* out = p.part + (((((size_t)b * p.Hkv + hk) * nt + kt) * p.splits + piece) * 2 + qh) *
+                                kTile * D + (size_t)kloc * D;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int a = 0; a < 4; ++a)
+          *reinterpret_cast<float4*>(out + 32 * dt + acc_row(4 * a, g)) =
+              make_float4(mine[dt][4 * a], mine[dt][4 * a + 1], mine[dt][4 * a + 2],
+                          mine[dt][4 * a + 3]);
+      return;
+    }
     __syncthreads();
     {
       __bf16* rows = qh == 0 ? k_s : v_s;  // bf16 row kloc of dK (qh 0) or dV (qh 1)
@@ -450,6 +492,41 @@ __global__ __launch_bounds__(kDkdvThreads, 1) void bwd_dkdv_kernel(BwdParams p) 
             *reinterpret_cast<const uint4*>(v_s + r * pitch<D>() + 8 * ch);
       }
     }
+  }
+#endif
+}
+
+// The pieces' sums of split columns, added in order, to dK and dV.  grid
+// (2 Hkv, nt, B); a thread takes 4 values a round.
+template <int D>
+__global__ __launch_bounds__(kThreads) void bwd_dkdv_join(BwdParams p) {
+  const int hk = blockIdx.x >> 1, which = blockIdx.x & 1, kt = blockIdx.y, b = blockIdx.z;
+  const size_t col = (size_t)(p.m.Bm > 1 ? b : 0) * p.m.nt + kt;
+  const int pieces = column_pieces(p.Hq / p.Hkv * (p.m.q_num[col] + p.m.full_q_num[col]), p.splits);
+  if (pieces == 1) return;
+  const float* in = p.part + ((((size_t)b * p.Hkv + hk) * p.m.nt + kt) * p.splits * 2 + which) *
+                                 kTile * D;
+  __bf16* out = which ? p.dv + b * p.dv_sb + hk * p.dv_sh : p.dk + b * p.dk_sb + hk * p.dk_sh;
+  const int64_t st = which ? p.dv_st : p.dk_st;
+  const float mul = which ? 1.f : p.scale;
+  const int rows = min(kTile, p.T - kt * kTile);
+  for (int x = threadIdx.x; x < rows * (D / 4); x += kThreads) {
+    const int r = x / (D / 4), c = 4 * (x % (D / 4));
+    float4 v[kMaxSplits];
+#pragma unroll
+    for (int i = 0; i < kMaxSplits; ++i)
+      v[i] = i < pieces ? *reinterpret_cast<const float4*>(in + (size_t)i * 2 * kTile * D +
+                                                           (size_t)r * D + c)
+                        : make_float4(0.f, 0.f, 0.f, 0.f);
+    float4 sum = v[0];
+#pragma unroll
+    for (int i = 1; i < kMaxSplits; ++i) {
+      sum.x += v[i].x; sum.y += v[i].y; sum.z += v[i].z; sum.w += v[i].w;
+    }
+    bf16x4 w;
+    w[0] = (__bf16)(sum.x * mul); w[1] = (__bf16)(sum.y * mul);
+    w[2] = (__bf16)(sum.z * mul); w[3] = (__bf16)(sum.w * mul);
+    *reinterpret_cast<bf16x4*>(out + (int64_t)(kt * kTile + r) * st + c) = w;
   }
 }
 
@@ -1140,6 +1217,8 @@ BwdParams make_bwd_params(const TensorView& q, const TensorView& k, const Tensor
   p.scale_log2 = dims.scale * kLog2e;
   p.fuse_delta = 0;
   p.m = mask;
+  p.part = nullptr;
+  p.splits = 1;
   return p;
 }
 
@@ -1164,11 +1243,11 @@ hipError_t launch_attn_bwd_phase(int phase, const TensorView& q, const TensorVie
   } else if (phase == kBwdDkDv) {
     const dim3 grid(dims.Hkv, nt, dims.B);
 #ifdef T2T_DKDV_CLASSIC
-    if (d64) hipLaunchKernelGGL(bwd_dkdv_kernel<64>, grid, dim3(kDkdvThreads), 0, stream, p);
-    else hipLaunchKernelGGL(bwd_dkdv_kernel<128>, grid, dim3(kDkdvThreads), 0, stream, p);
+    if (d64) hipLaunchKernelGGL((bwd_dkdv_kernel<64, false>), grid, dim3(kDkdvThreads), 0, stream, p);
+    else hipLaunchKernelGGL((bwd_dkdv_kernel<128, false>), grid, dim3(kDkdvThreads), 0, stream, p);
 #else
     if (d64) hipLaunchKernelGGL(bwd_dkdv_pair_kernel<64>, grid, dim3(kPairWaves * 64), 0, stream, p);
-    else hipLaunchKernelGGL(bwd_dkdv_kernel<128>, grid, dim3(kDkdvThreads), 0, stream, p);
+    else hipLaunchKernelGGL((bwd_dkdv_kernel<128, false>), grid, dim3(kDkdvThreads), 0, stream, p);
 #endif
   } else {  // kBwdDq, kBwdDqDelta
     BwdParams pq = p;
@@ -1177,6 +1256,37 @@ hipError_t launch_attn_bwd_phase(int phase, const TensorView& q, const TensorVie
     if (d64) hipLaunchKernelGGL(bwd_dq_kernel<64>, grid, dim3(kThreads), 0, stream, pq);
     else hipLaunchKernelGGL(bwd_dq_kernel<128>, grid, dim3(kThreads), 0, stream, pq);
   }
+  return hipGetLastError();
+}
+
+// Work-groups that share a column: only where at most two columns fall on a CU
+// (with more, the launch's order, longest column first, evens them out), as many
+// as keep the sums within 256 MiB.  D = 128 (the columns of D = 64 are two work-
+// groups a CU already, and a quarter as long for the same keys).
+int bwd_uneven_splits(int B, int Hkv, int T, int D) {
+  const int64_t columns = (int64_t)B * Hkv * ((T + kTile - 1) / kTile);
+  if (D != 128 || columns > 512 || columns == 0) return 1;
+  const int64_t fit = (256ll << 20) / (columns * 2 * kTile * D * 4);
+  return (int)(fit < kMaxSplits ? fit : kMaxSplits);
+}
+
+hipError_t launch_attn_bwd_dkdv_split(const TensorView& q, const TensorView& k,
+                                      const TensorView& v, const TensorView& dout,
+                                      const float* lse2, float* delta, const TensorView& dk,
+                                      const TensorView& dv, const AttnDims& dims,
+                                      const MaskTables& mask, int splits, float* workspace,
+                                      hipStream_t stream) {
+  const TensorView none{nullptr, 0, 0, 0};
+  BwdParams p = make_bwd_params(q, k, v, none, dout, lse2, delta, none, dk, dv, dims, mask);
+  p.part = workspace;
+  p.splits = splits;
+  const int nt = (dims.T + kTile - 1) / kTile;
+  hipLaunchKernelGGL((bwd_dkdv_kernel<128, true>), dim3(dims.Hkv, nt, dims.B * splits),
+                     dim3(kDkdvThreads), 0, stream, p);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL(bwd_dkdv_join<128>, dim3(2 * dims.Hkv, nt, dims.B), dim3(kThreads), 0, stream,
+                     p);
   return hipGetLastError();
 }
 

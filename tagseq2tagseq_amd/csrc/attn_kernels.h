@@ -92,6 +92,15 @@ enum BwdPhase { kBwdDelta = 0, kBwdDkDv = 1, kBwdDq = 2, kBwdDqDelta = 3 };
 // One backward phase.  Views a phase does not read may be empty (delta: o,
 // dout; dkdv: q, k, v, dout, lse2, delta, dk, dv; dq: q, k, v, dout, lse2,
 // delta, dq).
+// dK/dV with long columns shared by `splits` work-groups (bwd_uneven_splits; 1:
+// not worth it), their sums in workspace [B][Hkv][nt][splits][2][128][D].
+int bwd_uneven_splits(int B, int Hkv, int T, int D);
+hipError_t launch_attn_bwd_dkdv_split(const TensorView& q, const TensorView& k,
+                                      const TensorView& v, const TensorView& dout,
+                                      const float* lse2, float* delta, const TensorView& dk,
+                                      const TensorView& dv, const AttnDims& dims,
+                                      const MaskTables& mask, int splits, float* workspace,
+                                      hipStream_t stream);
 hipError_t launch_attn_bwd_phase(int phase, const TensorView& q, const TensorView& k,
                                  const TensorView& v, const TensorView& o,
                                  const TensorView& dout, const float* lse2, float* delta,

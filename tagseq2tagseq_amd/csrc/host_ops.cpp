@@ -107,7 +107,8 @@ std::tuple<Tensor, Tensor> attn_fwd(const Tensor& q, const Tensor& k, const Tens
 
 std::tuple<Tensor, Tensor, Tensor> attn_bwd(const Tensor& q, const Tensor& k, const Tensor& v,
                                             const Tensor& out, const Tensor& dout_in,
-                                            const Tensor& lse2, int64_t mask, double scale) {
+                                            const Tensor& lse2, int64_t mask, double scale,
+                                            bool uneven = false) {
   const int dtype = attention_code(q, k, v, out, dout_in);
   need_gpu(q, k, v, out, dout_in, lse2);
   const c10::DeviceGuard guard(q.device());
@@ -118,6 +119,16 @@ std::tuple<Tensor, Tensor, Tensor> attn_bwd(const Tensor& q, const Tensor& k, co
   Tensor delta = at::empty({B, Hq, T}, q.options().dtype(at::kFloat));
   const t2t_tensor qs = view4(q), ks = view4(k), vs = view4(v), os = view4(out),
                    ds = view4(dout), dqs = view4(dq), dks = view4(dk), dvs = view4(dv);
+  const int64_t bytes = uneven ? t2t_attn_bwd_uneven_workspace(B, Hkv, T, D, dtype) : 0;
+  if (bytes > 0) {
+    Tensor ws = at::empty({bytes / 4}, delta.options());
+    check(t2t_attn_bwd_uneven(&qs, &ks, &vs, &os, &ds, lse2.data_ptr<float>(),
+                              delta.data_ptr<float>(), &dqs, &dks, &dvs, B, Hq, Hkv, T, D, dtype,
+                              static_cast<float>(scale), mask_at(mask), ws.data_ptr(), bytes,
+                              stream_of(q)),
+          "t2t_attn_bwd_uneven");
+    return {dq, dk, dv};
+  }
   check(t2t_attn_bwd(&qs, &ks, &vs, &os, &ds, lse2.data_ptr<float>(), delta.data_ptr<float>(),
                      &dqs, &dks, &dvs, B, Hq, Hkv, T, D, dtype,
                      static_cast<float>(scale), mask_at(mask), stream_of(q)),
@@ -1095,7 +1106,7 @@ std::vector<Tensor> mask_meta_window(const Tensor& doc, const Tensor& q_bits,
   Tensor pool = at::empty({7 * padded(row) + 5 * padded(grid)}, i32);
   int64_t at_ = 0;
   const auto take = [&](at::IntArrayRef shape, int64_t n) {
-    Tensor t = pool.narrow(0, at_, n).view(shape);
+    Tensor t = at::as_strided(pool, shape, c10::contiguous_strides(shape), at_);
     at_ += padded(n);
     return t;
   };
@@ -1204,6 +1215,56 @@ variable_list once(variable_list grads, const char* what) {
   if (!c10::GradMode::is_enabled()) return grads;
   return torch::autograd::DelayedError(std::string(what) + " is differentiable once",
                                        static_cast<int64_t>(grads.size()))(std::move(grads));
+}
+
+// The mask's 13 tables (in t2t_block_mask's order) as the kernels take them.
+t2t_block_mask mask_of(const std::vector<Tensor>& t) {
+  TORCH_CHECK_VALUE(t.size() == 13, "a mask has 13 tables, not ", t.size());
+  need_gpu(t[0]);
+  const auto ptr = [&](int i) { return static_cast<int32_t*>(t[i].data_ptr()); };
+  t2t_block_mask m{};
+  m.mask_batch = t[0].size(0);
+  m.num_tiles = t[0].size(-1);
+  m.kv_num = ptr(0); m.kv_idx = ptr(1); m.full_kv_num = ptr(2); m.full_kv_idx = ptr(3);
+  m.q_num = ptr(4); m.q_idx = ptr(5); m.full_q_num = ptr(6); m.full_q_idx = ptr(7);
+  m.row_order = ptr(8); m.col_order = ptr(9); m.kv_bits_off = ptr(10); m.q_bits_slot = ptr(11);
+  m.tile_bits = static_cast<uint32_t*>(t[12].data_ptr());
+  m.tile_bits_slots = t[12].size(0);
+  return m;
+}
+
+// (the tables are the mask's own, which no one writes to: kept, not saved)
+struct AttentionAd : torch::autograd::Function<AttentionAd> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k,
+                               const Tensor& v, const std::vector<Tensor>& tables, double scale,
+                               bool uneven) {
+    const t2t_block_mask m = mask_of(tables);
+    auto [out, lse2] =
+        attn_fwd(q, k, v, static_cast<int64_t>(reinterpret_cast<intptr_t>(&m)), scale);
+    ctx->save_for_backward({q, k, v, out, lse2});
+    ctx->saved_data["tables"] = tables;
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["uneven"] = uneven;
+    ctx->mark_non_differentiable({lse2});
+    return {out, lse2};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    const variable_list t = ctx->get_saved_variables();
+    const t2t_block_mask m = mask_of(ctx->saved_data["tables"].toTensorVector());
+    auto [dq, dk, dv] = attn_bwd(t[0], t[1], t[2], t[3], g[0], t[4],
+                                 static_cast<int64_t>(reinterpret_cast<intptr_t>(&m)),
+                                 ctx->saved_data["scale"].toDouble(),
+                                 ctx->saved_data["uneven"].toBool());
+    variable_list d = once({dq, dk, dv}, "masked attention");
+    d.resize(6);
+    return d;
+  }
+};
+
+std::tuple<Tensor, Tensor> attn_ad(const Tensor& q, const Tensor& k, const Tensor& v,
+                                   const std::vector<Tensor>& tables, double scale, bool uneven) {
+  variable_list o = AttentionAd::apply(q, k, v, tables, scale, uneven);
+  return {o[0], o[1]};
 }
 
 struct QkNormAd : torch::autograd::Function<QkNormAd> {
@@ -1429,7 +1490,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   // Python threads run meanwhile
   const auto no_gil = py::call_guard<py::gil_scoped_release>();
   m.def("attn_fwd", &attn_fwd, no_gil);
-  m.def("attn_bwd", &attn_bwd, no_gil);
+  m.def("attn_bwd", &attn_bwd, py::arg("q"), py::arg("k"), py::arg("v"), py::arg("out"),
+        py::arg("dout"), py::arg("lse2"), py::arg("mask"), py::arg("scale"),
+        py::arg("uneven") = false, no_gil);
   m.def("rms_norm", &rms_norm, no_gil);
   m.def("rms_norm_backward", &rms_norm_backward, no_gil);
   m.def("qkv_rope", &qkv_rope, no_gil);
@@ -1441,6 +1504,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("qkv_rotary", &qkv_rotary, no_gil);
   m.def("qkv_rotary_backward", &qkv_rotary_backward, no_gil);
   m.def("qkv_rotary_ad", &qkv_rotary_ad, no_gil);
+  m.def("attn_ad", &attn_ad, no_gil);
   m.def("attn_decode", &attn_decode, no_gil);
   m.def("kv8_append", &kv8_append, no_gil);
   m.def("kv8_attend", &kv8_attend, no_gil);

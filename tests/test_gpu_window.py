@@ -478,3 +478,31 @@ def test_decode_captured_and_replayed():
         graph.replay()
         for a, b in zip(out, step()):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("B,T,H,Hkv,words", [(1, 4200, 8, 1, 0), (2, 2500, 8, 2, 2), (1, 100, 2, 1, 0),
+                                             (1, 2304, 4, 4, 1)])
+def test_columns_shared_by_work_groups(B, T, H, Hkv, words):
+    """Long columns of few heads of 128: dk and dv summed from several
+    work-groups' parts, within the same bounds and the same bits again."""
+    from tagseq2tagseq_amd import _lib
+    assert _lib.lib().t2t_attn_bwd_uneven_workspace(B, Hkv, T, 128, 0) > 0
+    rows = [_row(T, 5 * T + i, words, 3000) for i in range(B)]
+    window, sinks = 150, 5
+    bm = _build(rows, window, sinks)
+    items = (bm.q_num_blocks + bm.full_q_num_blocks) * (H // Hkv)
+    assert H == Hkv or T < 1000 or int(items.max()) > 32
+    dense = torch.stack([torch.from_numpy(_dense(*r, window, sinks)) for r in rows]).to(DEV)
+    g = torch.Generator().manual_seed(T)
+    q, k, v, do = (torch.randn(B, h, T, 128, generator=g).to(BF).to(DEV)
+                   for h in (H, Hkv, Hkv, H))
+    for t in (q, k, v):
+        t.requires_grad_(True)
+    out = flex_attention(q, k, v, block_mask=bm, enable_gqa=True)
+    got = (out, *torch.autograd.grad(out, (q, k, v), do, retain_graph=True))
+    again = torch.autograd.grad(out, (q, k, v), do)
+    assert all(torch.equal(a, b) for a, b in zip(got[1:], again))
+    for name, x, (ref, tol) in zip(("o", "dq", "dk", "dv"), got,
+                                   _attention_ref(q, k, v, do, dense, 2.0 ** -8)):
+        worst = float(((x.detach().double() - ref).abs() / tol).max())
+        assert worst <= 1, f"{name}: {worst:.3g} of the tolerance"
