@@ -348,7 +348,7 @@ struct Kv8AttendArgs {
   int chunks;                // set by the launcher
 };
 
-int kv8_chunks(int B, int Hkv, int Tkv);
+int kv8_chunks(int B, int Hkv, int Tkv, int D);
 hipError_t launch_kv8_append(const Kv8AppendArgs& a, bool f32, int D, hipStream_t stream);
 hipError_t launch_kv8_attend(Kv8AttendArgs a, int D, hipStream_t stream);
 

@@ -655,7 +655,7 @@ int t2t_kv8_append(const t2t_tensor* k, const t2t_tensor* v, int32_t B, int32_t 
 int64_t t2t_kv8_attend_workspace(int32_t B, int32_t Hq, int32_t Hkv, int32_t Tq, int32_t Tkv,
                                  int32_t D) {
   if (B <= 0 || Hq <= 0 || Hkv <= 0 || Tq <= 0 || Tkv < 0 || D < 0) return 0;
-  const int chunks = t2t::kv8_chunks(B, Hkv, Tkv);
+  const int chunks = t2t::kv8_chunks(B, Hkv, Tkv, D);
   return chunks == 1 ? 0 : 4 * (int64_t)B * Hq * Tq * chunks * (D + 2);
 }
 

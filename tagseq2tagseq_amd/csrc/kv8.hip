@@ -263,12 +263,12 @@ __device__ __forceinline__ f32x4 mfma16(bf16x8 a, bf16x8 b, f32x4 c) {
 // that rounding left, so that p counts with 16 bits.  Up to eight rows use half
 // of the products' 16 columns, and the other half takes the rests (Twice false:
 // column n + 8 is row n again); more rows take a second product.
-template <int D, bool Twice>
-__global__ __launch_bounds__(256) void kv8_attend_kernel(Kv8AttendArgs a) {
+template <int D, bool Twice, int Waves>
+__global__ __launch_bounds__(64 * Waves) void kv8_attend_kernel(Kv8AttendArgs a) {
   constexpr int kPieces = D / 64;      // 16-byte pieces of a lane's part of a key
   constexpr int kTiles = D / 16;       // O^T tiles
-  __shared__ __align__(16) float osum[4][16][D + 4];
-  __shared__ float mls[4][2][16];
+  __shared__ __align__(16) float osum[Waves][16][D + 4];
+  __shared__ float mls[Waves][2][16];
   __shared__ int32_t spos[16], sdoc[16], sstart[16];
   __shared__ uint64_t sbits[kMaxWords][16];
   const int chunk = blockIdx.x, hk = blockIdx.y, b = blockIdx.z;
@@ -298,7 +298,7 @@ __global__ __launch_bounds__(256) void kv8_attend_kernel(Kv8AttendArgs a) {
   // waves.
   const PieceRange<kBlk> range(spos, a.q_start ? sstart : nullptr, a.Tq, a.Tkv,
                                a.W == 0 ? a.window : 0, a.sinks);
-  const int share = 4 * ((range.count + 4 * a.chunks - 1) / (4 * a.chunks));
+  const int share = Waves * ((range.count + Waves * a.chunks - 1) / (Waves * a.chunks));
   const int end = min((chunk + 1) * share, range.count);
   const size_t row0 = ((size_t)b * a.Hq + hk * G) * a.Tq;
   float* pml = a.part + (size_t)a.B * a.Hq * a.Tq * a.chunks * D;
@@ -326,7 +326,7 @@ __global__ __launch_bounds__(256) void kv8_attend_kernel(Kv8AttendArgs a) {
 #pragma unroll
   for (int i = 0; i < kTiles; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
   float m = -INFINITY, l = 0.f;
-  for (int v = chunk * share + wave; v < end; v += 4) {
+  for (int v = chunk * share + wave; v < end; v += Waves) {
     const int blk = range.at(v);
     const int j = blk * kBlk + lane;
     const bool in = j < a.Tkv;
@@ -415,7 +415,7 @@ __global__ __launch_bounds__(256) void kv8_attend_kernel(Kv8AttendArgs a) {
     }
   }
 
-  // The four waves' sums of a row, joined.  Lane (g, column) holds
+  // The waves' sums of a row, joined.  Lane (g, column) holds
   // o[16 i + 4 g + e] of its column.
   l = row_sum(l);
   if (g == 0) {
@@ -426,13 +426,15 @@ __global__ __launch_bounds__(256) void kv8_attend_kernel(Kv8AttendArgs a) {
   for (int i = 0; i < kTiles; ++i)
     *reinterpret_cast<f32x4*>(&osum[wave][column][16 * i + 4 * g]) = o[i];
   __syncthreads();
-  for (int x = tid; x < R * D; x += 256) {
+  for (int x = tid; x < R * D; x += 64 * Waves) {
     const int r = x / D, d = x - r * D;
-    const float M = fmaxf(fmaxf(mls[0][0][r], mls[1][0][r]), fmaxf(mls[2][0][r], mls[3][0][r]));
+    float M = mls[0][0][r];
+#pragma unroll
+    for (int w = 1; w < Waves; ++w) M = fmaxf(M, mls[w][0][r]);
     const float ref = M == -INFINITY ? 0.f : M;
     float L = 0.f, sum = 0.f;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
+    for (int w = 0; w < Waves; ++w) {
       const float f = fast_exp2(mls[w][0][r] - ref);
       L = fmaf(f, mls[w][1][r], L);
       sum = fmaf(f, Twice ? osum[w][r][d] : osum[w][r][d] + osum[w][r + 8][d], sum);
@@ -520,16 +522,38 @@ __global__ __launch_bounds__(256) void kv8_combine_kernel(Kv8AttendArgs a) {
 // run under another's products.
 constexpr int kAimGroups = 1024;
 
+// Waves of a work-group that takes a whole row's keys in one pass where each
+// wave has one block at most: 12 heads of 64, 512 / 1024 / 2048 keys 5.3 / 6.6 /
+// 9.5 us against 6.8 / 6.9 / 6.9 in chunks and two passes (a wave's second block
+// costs what the second pass does); 16 x 8 heads of 128, 512 keys 7.2 against 8.9.
+template <int D>
+constexpr int kWideWaves = D == 64 ? 16 : 8;
+
+bool one_pass(int Tkv, int D) {
+  return Tkv <= kBlk * (D == 64 ? kWideWaves<64> : kWideWaves<128>);
+}
+
+template <int D, bool Twice>
+void start_attend(const Kv8AttendArgs& a, hipStream_t stream) {
+  const dim3 grid(a.chunks, a.Hkv, a.B);
+  if (one_pass(a.Tkv, D) && a.Tkv > 4 * kBlk)
+    hipLaunchKernelGGL((kv8_attend_kernel<D, Twice, kWideWaves<D>>), grid,
+                       dim3(64 * kWideWaves<D>), 0, stream, a);
+  else
+    hipLaunchKernelGGL((kv8_attend_kernel<D, Twice, 4>), grid, dim3(256), 0, stream, a);
+}
+
 }  // namespace
 
 // Chunks of a row's keys: as many as fill the aim, at most one for each round of
 // the four waves' blocks and as many as the second pass has lanes.
-int kv8_chunks(int B, int Hkv, int Tkv) {
+int kv8_chunks(int B, int Hkv, int Tkv, int D) {
+  if (one_pass(Tkv, D)) return 1;
   const int rounds = (Tkv + 4 * kBlk - 1) / (4 * kBlk);
   const int64_t pairs = (int64_t)B * Hkv;
   const int64_t want = pairs > 0 ? (kAimGroups + pairs - 1) / pairs : 1;
   const int n = (int)(want < kMaxChunks ? want : kMaxChunks);
-  return rounds < 1 ? 1 : n < rounds ? n : rounds;
+  return n < rounds ? n : rounds;
 }
 
 hipError_t launch_kv8_append(const Kv8AppendArgs& a, bool f32, int D, hipStream_t stream) {
@@ -550,19 +574,15 @@ hipError_t launch_kv8_append(const Kv8AppendArgs& a, bool f32, int D, hipStream_
 }
 
 hipError_t launch_kv8_attend(Kv8AttendArgs a, int D, hipStream_t stream) {
-  a.chunks = kv8_chunks(a.B, a.Hkv, a.Tkv);
-  const dim3 grid(a.chunks, a.Hkv, a.B), rows(a.Tq, a.Hq, a.B);
+  a.chunks = kv8_chunks(a.B, a.Hkv, a.Tkv, D);
   const bool twice = a.Hq / a.Hkv * a.Tq > 8;
-  if (D == 64 && twice)
-    hipLaunchKernelGGL((kv8_attend_kernel<64, true>), grid, dim3(256), 0, stream, a);
-  else if (D == 64)
-    hipLaunchKernelGGL((kv8_attend_kernel<64, false>), grid, dim3(256), 0, stream, a);
-  else if (twice)
-    hipLaunchKernelGGL((kv8_attend_kernel<128, true>), grid, dim3(256), 0, stream, a);
+  if (D == 64)
+    twice ? start_attend<64, true>(a, stream) : start_attend<64, false>(a, stream);
   else
-    hipLaunchKernelGGL((kv8_attend_kernel<128, false>), grid, dim3(256), 0, stream, a);
+    twice ? start_attend<128, true>(a, stream) : start_attend<128, false>(a, stream);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || a.chunks == 1) return e;
+  const dim3 rows(a.Tq, a.Hq, a.B);
   if (D == 64)
     hipLaunchKernelGGL(kv8_combine_kernel<64>, rows, dim3(256), 0, stream, a);
   else

@@ -68,18 +68,18 @@ def kv8_append(k: torch.Tensor, v: torch.Tensor, pos: Union[int, torch.Tensor],
     a block that pos begins starts from its new tokens.  A token whose key or
     value is not finite makes every row that reads it NaN.  A device position
     below 0 or above capacity - M stores nothing.  No gradient."""
-    tensors = (k, v, k_codes, v_codes, k_scale, v_scale)
-    _refuse_grad("kv8_append", *tensors)
     at, pos0 = (pos, 0) if isinstance(pos, torch.Tensor) else (None, int(pos))
     if capacity is not None and capacity < 0:
         raise ValueError(f"capacity={capacity} is negative")
     args = (k, v, at, pos0, k_codes, v_codes, k_scale, v_scale,
             -1 if capacity is None else int(capacity))
-    watched = tensors if at is None else (*tensors, at)
-    if torch.compiler.is_compiling() or not _lib.only_recorded(*watched):
-        kv8_append_op(*args)
-    else:
+    tensors = (k, v, k_codes, v_codes, k_scale, v_scale)
+    if (not torch.compiler.is_compiling()
+            and _lib.unwatched(*(tensors if at is None else (*tensors, at)))):
         _lib.host().kv8_append(*args)
+        return
+    _refuse_grad("kv8_append", *tensors)
+    kv8_append_op(*args)  # a compiler, or something besides autograd watches
 
 
 @torch.library.custom_op("t2t::kv8_attend", mutates_args=())
@@ -111,16 +111,16 @@ def attn_decode_kv8(q: torch.Tensor, k_codes: torch.Tensor, v_codes: torch.Tenso
     the window and what is returned are as there.  Rows without an allowed key
     give o = 0 and lse2 = -inf.  (Hq / Hkv) * Tq must be at most 16.  No
     gradient."""
-    _refuse_grad("attn_decode_kv8", q, k_codes, v_codes, k_scale, v_scale)
     window, sinks = check_window(window, sinks)
     if scale is None:
         scale = 1.0 / math.sqrt(q.shape[-1])
     args = (q, k_codes, v_codes, k_scale, v_scale, int(n_keys), key_doc, key_bits, q_pos, q_doc,
             q_bits, float(scale), window or 0, sinks, q_start)
-    if (torch.compiler.is_compiling()
-            or not _lib.only_recorded(*[t for t in args if isinstance(t, torch.Tensor)])):
-        return kv8_attend_op(*args)
-    return _lib.host().kv8_attend(*args)
+    if (not torch.compiler.is_compiling()
+            and _lib.unwatched(*[t for t in args if isinstance(t, torch.Tensor)])):
+        return _lib.host().kv8_attend(*args)
+    _refuse_grad("attn_decode_kv8", q, k_codes, v_codes, k_scale, v_scale)
+    return kv8_attend_op(*args)  # a compiler, or something besides autograd watches
 
 
 class KV8Cache:
