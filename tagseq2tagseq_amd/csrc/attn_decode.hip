@@ -35,7 +35,8 @@
 // chunks are then those of the rows' PieceRange -- without grant words their
 // windows and sinks alone, wherever in the cache they are -- and a work-group
 // takes every gridDim.x-th of them: 12 heads of 64, a window of 4096 behind
-// 32768 positions 12 us with a work-group for every chunk of the cache.
+// 32768 positions 8.7 + 4.1 us, where a work-group for every chunk of the cache
+// took 11.9 + 7.2.
 #include "attn_kernels.h"
 
 namespace t2t {

@@ -17,21 +17,27 @@
 // channel 2^-6 of the block's largest value keeps its three bits, where an
 // integer would have one left.  A token with a key or value that is not finite
 // is stored as NaN keys and zero values: every row that reads it is NaN, no
-// other row is touched.
+// other row is touched.  HBM bound for prompts: 16384 tokens of 12 heads of 64
+// 17.3 us, 4.4 TB/s of the tokens read and the codes written; one token is a
+// launch and its memory latencies in turn, 5.0 us.
 //
 // Attention (kv8_attend).  One work-group per (chunk of keys, kv head, batch
 // row), R = G Tq <= 16 query rows (G query heads a kv head, Tq new tokens), each
-// of its four waves on 64-key blocks of its own with a running maximum and sum.
-// HBM bound: 2 D bytes a key and kv head.  At eight or more rows the products
-// alone would keep the vector units busy longer than the loads take, so they go
-// to the matrix unit whatever R: S^T = K Q^T and O^T = V^T P^T as 16x16x32 bf16
+// of its 4 to 16 waves on 64-key blocks of its own with a running maximum and sum.
+// HBM bound: 2 D bytes a key and kv head.  From eight rows on the products alone
+// (R multiply-adds a byte of the 64 a CU makes in a cycle) would take the vector
+// units longer than memory takes for the byte, so they go to the matrix unit
+// whatever R: S^T = K Q^T and O^T = V^T P^T as 16x16x32 bf16
 // (e4m3 numbers are bf16 numbers, exactly, and p is taken as two of them, see
 // below).  With A-operand row m of S tile t holding key
 // 16 (m / 4) + 4 t + m % 4, lane (g, n) = (l / 16, l % 16) ends up with the
 // scores of keys 16 g + 0 .. 15 for row n, which in this order are the B operand
 // of the second product, whose A operand is then 16 neighbouring bytes of a row
 // of V^T: no shuffle and no LDS between global memory and the products.
-// Each (row, chunk) leaves (max, sum, unnormalised o[D]) for kv8_combine.
+// Each (row, chunk) leaves (max, sum, unnormalised o[D]) for kv8_combine.  12
+// heads of 64 over 32768 positions: 12.3 + 3.9 us, 4.1 TB/s; 16 sequences of 8192,
+// 32 / 8 heads of 128, two tokens: 45 + 4.7 us, 6.0 TB/s (part of it from the
+// last-level cache).
 #include "attn_kernels.h"
 
 namespace t2t {
@@ -39,7 +45,6 @@ namespace t2t {
 namespace {
 
 constexpr int kBlk = kKv8Block;
-constexpr float kLargest = 448.f;
 
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
@@ -85,10 +90,8 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(Kv8AppendArgs a) {
   constexpr int kPer = kBlk * kRowPieces / 256;        // pieces a thread
   constexpr int kPitch = kBlk + 16;                    // of a staged V^T row
   constexpr int kOut = kBlk * D / 16 / 256;            // 16-byte pieces a thread
-  __shared__ __align__(16) uint8_t ks[kBlk * D];
   __shared__ __align__(16) uint8_t vs[D * kPitch];
   __shared__ float top[2][4];
-  __shared__ int bad[kBlk];
   const int b = blockIdx.z, h = blockIdx.y, tid = threadIdx.x;
   const int64_t pos = a.pos ? a.pos[b * a.pos_stride] : a.pos0;
   if (pos < 0 || pos > (int64_t)a.capacity - a.M) return;
@@ -103,56 +106,53 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(Kv8AppendArgs a) {
   const T* k = static_cast<const T*>(a.k.data) + b * a.k.sb + h * a.k.sh;
   const T* v = static_cast<const T*>(a.v.data) + b * a.v.sb + h * a.v.sh;
 
-  // What the block holds already, in the pieces that this thread writes back.
+  // Values are written in 16-byte pieces: tokens t0 .. t0 + 15 of a row of V^T.
+  // What the block holds already in those with new and other tokens.
   const bool part = hi - lo < kBlk;
-  uint4 kold[kOut], vold[kOut];
+  const auto tokens = [&](int i) { return 16 * ((tid + 256 * i) % (kBlk / 16)); };
+  uint4 vold[kOut];
   float kwas = 0.f, vwas = 0.f;
-  if (part) {
 #pragma unroll
-    for (int i = 0; i < kOut; ++i) {
-      kold[i] = reinterpret_cast<const uint4*>(kc)[tid + 256 * i];
-      vold[i] = reinterpret_cast<const uint4*>(vc)[tid + 256 * i];
-    }
-    if (lo > 0) {
-      kwas = a.k_scale[at];
-      vwas = a.v_scale[at];
-    }
+  for (int i = 0; i < kOut; ++i) {
+    const int t0 = tokens(i);
+    vold[i] = make_uint4(0u, 0u, 0u, 0u);
+    if (part && t0 < hi && t0 + 16 > lo) vold[i] = reinterpret_cast<const uint4*>(vc)[tid + 256 * i];
   }
-  if (tid < kBlk) bad[tid] = 0;
-  __syncthreads();
+  if (lo > 0) {
+    kwas = a.k_scale[at];
+    vwas = a.v_scale[at];
+  }
   float x[kPer][8], y[kPer][8];
+  float km = 0.f, vm = 0.f;
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
     const int row = (tid + 256 * i) / kRowPieces, c = 8 * ((tid + 256 * i) % kRowPieces);
+    bool finite = true;
 #pragma unroll
     for (int e = 0; e < 8; ++e) x[i][e] = y[i][e] = 0.f;
     if (row >= lo && row < hi) {
       const int64_t t = first + row - pos;
       load_row8(k + t * a.k.st + c, x[i]);
       load_row8(v + t * a.v.st + c, y[i]);
-      bool finite = true;
 #pragma unroll
       for (int e = 0; e < 8; ++e)
         finite = finite && fabsf(x[i][e]) <= 3.4028234663852886e38f &&
                  fabsf(y[i][e]) <= 3.4028234663852886e38f;
-      if (!finite) bad[row] = 1;
     }
-  }
-  __syncthreads();
-  float km = 0.f, vm = 0.f;
-#pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    if (bad[(tid + 256 * i) / kRowPieces]) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        x[i][e] = __uint_as_float(0x7fc00000u);
-        y[i][e] = 0.f;
-      }
-    } else {
+    // (a token's lanes are neighbours in one wave)
+    constexpr uint64_t kAll = (1ull << kRowPieces) - 1;
+    const int shift = (tid & 63) / kRowPieces * kRowPieces;
+    if (((__ballot(finite) >> shift) & kAll) == kAll) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         km = fmaxf(km, fabsf(x[i][e]));
         vm = fmaxf(vm, fabsf(y[i][e]));
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        x[i][e] = __uint_as_float(0x7fc00000u);
+        y[i][e] = 0.f;
       }
     }
   }
@@ -187,29 +187,29 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(Kv8AppendArgs a) {
       kw[e] = encode4(x[i] + 4 * e);
       vw[e] = encode4(y[i] + 4 * e);
     }
-    *reinterpret_cast<uint2*>(ks + row * D + c) = make_uint2(kw[0], kw[1]);
+    *reinterpret_cast<uint2*>(kc + row * D + c) = make_uint2(kw[0], kw[1]);
 #pragma unroll
     for (int e = 0; e < 8; ++e)
       vs[(c + e) * kPitch + row] = (uint8_t)(vw[e >> 2] >> (8 * (e & 3)));
   }
-  __syncthreads();
   const float kg = kwas * kr, vg = vwas * vr;  // 1 where the scale stayed
-#pragma unroll
-  for (int i = 0; i < kOut; ++i) {
-    const int p = tid + 256 * i;
-    const int row = p / (D / 16);  // keys: the token of the piece
-    if (row >= lo && row < hi) {
-      reinterpret_cast<uint4*>(kc)[p] = reinterpret_cast<const uint4*>(ks)[p];
-    } else if (row < lo && kg != 1.f) {
-      const uint4 o = kold[i];
+  if (kg != 1.f) {  // (the lo rows before the new ones)
+    for (int p = tid; p < lo * (D / 16); p += 256) {
+      const uint4 o = reinterpret_cast<const uint4*>(kc)[p];
       reinterpret_cast<uint4*>(kc)[p] =
           make_uint4(rescale4(o.x, kg), rescale4(o.y, kg), rescale4(o.z, kg), rescale4(o.w, kg));
     }
-    const int d = p / (kBlk / 16), t0 = 16 * (p % (kBlk / 16));  // values: tokens t0 .. t0 + 15
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kOut; ++i) {
+    const int p = tid + 256 * i, d = p / (kBlk / 16), t0 = tokens(i);
+    const bool some = t0 < hi && t0 + 16 > lo;
+    if (!some && (t0 >= hi || vg == 1.f)) continue;
     uint4 n = *reinterpret_cast<const uint4*>(vs + d * kPitch + t0);
     if (part) {
-      if (t0 >= hi || (t0 + 16 <= lo && vg == 1.f)) continue;
-      const uint32_t o[4] = {vold[i].x, vold[i].y, vold[i].z, vold[i].w};
+      const uint4 was = some ? vold[i] : reinterpret_cast<const uint4*>(vc)[p];
+      const uint32_t o[4] = {was.x, was.y, was.z, was.w};
       uint32_t w[4] = {n.x, n.y, n.z, n.w};
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
@@ -362,6 +362,19 @@ __global__ __launch_bounds__(64 * Waves) void kv8_attend_kernel(Kv8AttendArgs a)
     for (int i = 0; i < kTiles; ++i)
       vraw[i] = *reinterpret_cast<const uint4*>(vp + i * 16 * kBlk);
     const float ks = kscale[blk] * a.c, vs = vscale[blk];
+    // Where no row may look there may be anything, NaN codes too, and 0 * NaN is
+    // NaN: zeros there.
+    if (any != ~0ull) {
+      const uint32_t some = (uint32_t)(any >> (16 * g));
+      uint32_t keep[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        keep[q] = (((some >> (4 * q)) & 0xfu) * 0x204081u & 0x1010101u) * 0xffu;
+#pragma unroll
+      for (int i = 0; i < kTiles; ++i)
+        vraw[i] = make_uint4(vraw[i].x & keep[0], vraw[i].y & keep[1], vraw[i].z & keep[2],
+                             vraw[i].w & keep[3]);
+    }
 
     float s[16];
     float top = -INFINITY;
@@ -546,7 +559,7 @@ void start_attend(const Kv8AttendArgs& a, hipStream_t stream) {
 }  // namespace
 
 // Chunks of a row's keys: as many as fill the aim, at most one for each round of
-// the four waves' blocks and as many as the second pass has lanes.
+// the waves' blocks and as many as the second pass has lanes.
 int kv8_chunks(int B, int Hkv, int Tkv, int D) {
   if (one_pass(Tkv, D)) return 1;
   const int rounds = (Tkv + 4 * kBlk - 1) / (4 * kBlk);

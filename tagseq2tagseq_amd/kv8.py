@@ -66,8 +66,9 @@ def kv8_append(k: torch.Tensor, v: torch.Tensor, pos: Union[int, torch.Tensor],
     it (its codes stay as they were).  A block's scale grows to what its new
     tokens need, and its positions before pos are written again where it did;
     a block that pos begins starts from its new tokens.  A token whose key or
-    value is not finite makes every row that reads it NaN.  A device position
-    below 0 or above capacity - M stores nothing.  No gradient."""
+    value is not finite makes every row that reads it NaN.  What the buffers
+    hold where nothing was stored is never looked at.  A device position below
+    0 or above capacity - M stores nothing.  No gradient."""
     at, pos0 = (pos, 0) if isinstance(pos, torch.Tensor) else (None, int(pos))
     if capacity is not None and capacity < 0:
         raise ValueError(f"capacity={capacity} is negative")
@@ -128,7 +129,7 @@ class KV8Cache:
     value heads of head_dim (64 or 128), all zeros."""
 
     def __init__(self, B: int, Hkv: int, capacity: int, head_dim: int, device):
-        if B < 0 or Hkv < 1 or capacity < 0 or head_dim not in (64, 128):
+        if B < 0 or Hkv < 1 or capacity < 1 or head_dim not in (64, 128):
             raise ValueError(f"B={B}, Hkv={Hkv}, capacity={capacity}, head_dim={head_dim}: no "
                              "cache (head_dim 64 or 128)")
         blocks = -(-capacity // BLOCK)

@@ -13,6 +13,7 @@ from tagseq2tagseq_amd import kv8
 from tagseq2tagseq_amd.kv8 import BLOCK, KV8Cache, attn_decode_kv8, kv8_append
 from tagseq2tagseq_amd.mask_creators import make_mask_creator_callable
 from tagseq2tagseq_amd.model import TS2TSModel
+from tagseq2tagseq_amd.rope import RotaryForm
 from tests.helpers import random_row, to_dev_words
 from tests.test_gpu_window import _dense, _spans, _starts, check_rows, logits_agree
 
@@ -295,6 +296,31 @@ def test_tokens_that_are_not_finite():
                 assert torch.equal(o[0, 0, t], want[0, 0, t])
 
 
+@pytest.mark.parametrize("n", [1, 17, 64, 100, 130])
+def test_what_was_never_stored_is_not_looked_at(n):
+    """NaN codes and scales around the tokens, as fresh memory may hold them,
+    and around the positions that a row's window leaves."""
+    g = torch.Generator().manual_seed(n)
+    clean, junk = KV8Cache(2, 2, 300, 64, DEV), KV8Cache(2, 2, 300, 64, DEV)
+    for t in junk.buffers():
+        t.view(torch.uint8).fill_(0xff)
+    k, v = _rows(2, 2, n, 64, BF, g)
+    for c in (clean, junk):
+        c.append(k, v, 0)
+    q = torch.randn(2, 2, 3, 64, generator=g).to(BF).to(DEV)
+    doc = torch.zeros(1, 300, dtype=torch.int32, device=DEV)
+    doc[:, n // 2:] = 1  # (two documents, the second to the end)
+    pos = torch.tensor([[n // 3, n - 1, n - 1]], dtype=torch.int32, device=DEV)
+    q_doc = doc[:, pos[0].long()]
+    for window in (None, 5):
+        want = clean.attend(q, n, doc, None, pos, q_doc, None, window=window)
+        assert want[0].isfinite().all()
+        for keys in (n, 300):
+            got = junk.attend(q, keys, doc, None, pos, q_doc, None, window=window)
+            ref = clean.attend(q, keys, doc, None, pos, q_doc, None, window=window)
+            assert all(torch.equal(a, b) for a, b in zip(got, ref))
+
+
 def test_strided_queries_and_masks_of_one_row():
     cache, q, mask, _, _ = _attend_case(2, 4, 2, 2, 64, 300, 0, None, 0)
     doc, _, pos, q_doc, _ = mask
@@ -480,19 +506,18 @@ def test_attention_refuses():
 
 # ---- the model's generation
 
-def _model(**kw):
+def _model(window=None, sinks=0, **kw):
     torch.manual_seed(0)
-    window = kw.pop("window", None)
+    creator = make_mask_creator_callable("doc_causal", window=window, sinks=sinks)
     m = TS2TSModel.from_config(
         vocab_size=211, num_layers=4, model_dim=128, num_heads=2, max_seq_len=450, dropout=0.0,
-        drop_path_rate=0.0, block_mask_creator=make_mask_creator_callable("doc_causal",
-                                                                          window=window), **kw)
+        drop_path_rate=0.0, block_mask_creator=creator, **kw)
     m.to(DEV, torch.bfloat16).eval()
     m.kv_bits = 8
     return m
 
 
-def _cached_rows_ref(m, tokens, spans, T, window):
+def _cached_rows_ref(m, tokens, spans, T):
     """Logits of the last row from the model's own cache, its attention in 64
     bits: every layer's projections as the model has them."""
     cache = m.kv_cache
@@ -515,17 +540,21 @@ def _cached_rows_ref(m, tokens, spans, T, window):
     return torch.nn.functional.linear(m.norm(x), m.lm_head_weight)
 
 
-@pytest.mark.parametrize("window", [None, 50])
 @pytest.mark.parametrize("fuse", [True, False])
-@pytest.mark.parametrize("qk_norm", [False, True])
+@pytest.mark.parametrize("window,sinks,kw", [
+    (None, 0, {}), (50, 0, {}), (None, 0, dict(qk_norm=True)), (50, 3, dict(qk_norm=True)),
+    # everything that long contexts add at once
+    (40, 4, dict(rotary=RotaryForm(fraction=0.5, interleaved=True, scaling="by_parts", factor=4.0,
+                                   original_len=128))),
+])
 @torch.no_grad()
-def test_generation(window, fuse, qk_norm):
-    m = _model(window=window, qk_norm=qk_norm)
+def test_generation(window, sinks, kw, fuse):
+    m = _model(window=window, sinks=sinks, **kw)
     m.fuse_rows = fuse
     tokens = torch.randint(0, 211, (1, 450), generator=torch.Generator().manual_seed(1)).to(DEV)
     for T in [390, 391, 392, 393, 400, 401, 449, 450]:  # whole, token by token, a few rows
         got = m.forward_inference_last(tokens[:, :T], _spans(T)).float()
-        logits_agree(got, _cached_rows_ref(m, tokens, _spans(T), T, window), f"T={T}")
+        logits_agree(got, _cached_rows_ref(m, tokens, _spans(T), T), f"T={T}")
     assert m.kv_cache.bits == 8 and m.kv_cache.length == 450
 
 
@@ -557,4 +586,4 @@ def test_an_edited_context_is_recomputed():
     tokens[0, 390] = 7
     for T in (397, 398):
         got = m.forward_inference_last(tokens[:, :T], _spans(T)).float()
-        logits_agree(got, _cached_rows_ref(m, tokens, _spans(T), T, None), f"T={T}")
+        logits_agree(got, _cached_rows_ref(m, tokens, _spans(T), T), f"T={T}")
