@@ -190,6 +190,15 @@ int t2t_attn_fwd(const t2t_tensor *q, const t2t_tensor *k, const t2t_tensor *v,
                  void *stream);
 
 /*
+ * t2t_attn_fwd (bf16) that also writes what rounding left of o, as bf16, into
+ * o_rest: for t2t_attn_bwd_uneven, whose rowsum(O * dO) then has 16 bits of O.
+ */
+int t2t_attn_fwd_rest(const t2t_tensor *q, const t2t_tensor *k, const t2t_tensor *v,
+                      const t2t_tensor *o, const t2t_tensor *o_rest, float *lse2, int32_t B,
+                      int32_t Hq, int32_t Hkv, int32_t T, int32_t D, int32_t dtype, float scale,
+                      const t2t_block_mask *mask, void *stream);
+
+/*
  * Masked attention backward.  Replaces flex_attention_backward as driven by
  * FlexAttentionAutogradOp.backward (torch/_higher_order_ops/flex_attention.py:689-767;
  * eager arithmetic sdpa_dense_backward :825-994).
@@ -215,14 +224,17 @@ int64_t t2t_attn_bwd_uneven_workspace(int32_t B, int32_t Hkv, int32_t T, int32_t
  * t2t_attn_bwd for masks whose columns are uneven (a sliding window's, whose
  * sinks are read by whole documents): where there are few columns, the queries
  * of a long one are shared by several work-groups, whose fp32 sums of dK and
- * dV are added in a fixed order (deterministic, no atomics).
+ * dV are added in a fixed order (deterministic, no atomics).  Rows of few keys,
+ * which such masks have, feel the roundings most: with o_rest (bf16, or NULL)
+ * Delta is taken from o + o_rest, and dS from P of at least 9 bits.
  */
 int t2t_attn_bwd_uneven(const t2t_tensor *q, const t2t_tensor *k, const t2t_tensor *v,
-                        const t2t_tensor *o, const t2t_tensor *dout, const float *lse2,
-                        float *delta, const t2t_tensor *dq, const t2t_tensor *dk,
-                        const t2t_tensor *dv, int32_t B, int32_t Hq, int32_t Hkv, int32_t T,
-                        int32_t D, int32_t dtype, float scale, const t2t_block_mask *mask,
-                        void *workspace, int64_t workspace_bytes, void *stream);
+                        const t2t_tensor *o, const t2t_tensor *o_rest, const t2t_tensor *dout,
+                        const float *lse2, float *delta, const t2t_tensor *dq,
+                        const t2t_tensor *dk, const t2t_tensor *dv, int32_t B, int32_t Hq,
+                        int32_t Hkv, int32_t T, int32_t D, int32_t dtype, float scale,
+                        const t2t_block_mask *mask, void *workspace, int64_t workspace_bytes,
+                        void *stream);
 
 /*
  * t2t_attn_bwd without the caller's Delta workspace, for callers that cannot

@@ -128,12 +128,17 @@ def attn_fwd(q, k, v, block_mask, scale: float):
     return _lib.host().attn_fwd(q, k, v, ctypes.addressof(mask), scale)
 
 
-def attn_bwd(q, k, v, out, dout, lse2, block_mask, scale: float):
+def _windowed(block_mask) -> bool:
+    return getattr(block_mask, "window", None) is not None
+
+
+def attn_bwd(q, k, v, out, dout, lse2, block_mask, scale: float, rest=None):
     """Kernel call: returns (dq, dk, dv).  ``block_mask`` as in attn_fwd; a
-    sliding window's mask gets the launch for uneven columns."""
+    sliding window's mask gets the launches for uneven columns and rows of few
+    keys, ``rest`` what the forward left of out's rounding for them."""
     mask = _mask_struct(block_mask)
     return _lib.host().attn_bwd(q, k, v, out, dout, lse2, ctypes.addressof(mask), scale,
-                                getattr(block_mask, "window", None) is not None)
+                                _windowed(block_mask), rest)
 
 
 class BwdPhases:
@@ -199,8 +204,10 @@ class T2TFlexAttentionFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, block_mask, scale):
-        out, lse2 = attn_fwd(q, k, v, block_mask, scale)
-        ctx.save_for_backward(q, k, v, out, lse2)
+        mask = _mask_struct(block_mask)
+        out, lse2, rest = _lib.host().attn_fwd_rest(q, k, v, ctypes.addressof(mask), scale,
+                                                    _windowed(block_mask))
+        ctx.save_for_backward(q, k, v, out, lse2, rest)
         ctx.block_mask = block_mask
         ctx.scale = scale
         ctx.mark_non_differentiable(lse2)
@@ -208,8 +215,8 @@ class T2TFlexAttentionFn(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dout, _dlse2):
-        q, k, v, out, lse2 = ctx.saved_tensors
-        dq, dk, dv = attn_bwd(q, k, v, out, dout, lse2, ctx.block_mask, ctx.scale)
+        q, k, v, out, lse2, rest = ctx.saved_tensors
+        dq, dk, dv = attn_bwd(q, k, v, out, dout, lse2, ctx.block_mask, ctx.scale, rest)
         return dq, dk, dv, None, None
 
 

@@ -31,6 +31,7 @@ struct BwdParams {
   const __bf16* k; int64_t k_sb, k_sh, k_st;
   const __bf16* v; int64_t v_sb, v_sh, v_st;
   const __bf16* o; int64_t o_sb, o_sh, o_st;
+  const __bf16* o_rest; int64_t r_sb, r_sh, r_st;  // with fuse_delta: or NULL
   const __bf16* dout; int64_t do_sb, do_sh, do_st;
   __bf16* dq; int64_t dq_sb, dq_sh, dq_st;
   __bf16* dk; int64_t dk_sb, dk_sh, dk_st;
@@ -543,6 +544,28 @@ __device__ __forceinline__ void masked_clear(f32x16& pacc, uint32_t wg) {
 
 constexpr int kPairWaves = 8;  // 4 key groups x (P / dV wave, dS / dK wave)
 
+// Entries 8 h .. 8 h + 7 of P in 16 bits each: 0 <= P < 2, so that a float's
+// sign and its exponent's highest bit are 0, and 7 exponent and 9 mantissa bits
+// are left (rounded to nearest; bf16 keeps 7).  dK over a row of 16384 tokens,
+// 12 heads, window 1024: 2.4e-3 off its 64-bit value instead of 2.9e-3 (the
+// roundings of dS and of dK itself are 1.7e-3 each), 122 us instead of 116.
+__device__ __forceinline__ bf16x8 pack_fine(const f32x16& acc, int h) {
+  uint32_t w[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const uint32_t lo = (__float_as_uint(acc[8 * h + 2 * j]) + 0x2000u) << 2;
+    const uint32_t hi = (__float_as_uint(acc[8 * h + 2 * j + 1]) + 0x2000u) << 2;
+    w[j] = __builtin_amdgcn_perm(hi, lo, 0x07060302u);
+  }
+  return __builtin_bit_cast(bf16x8, make_uint4(w[0], w[1], w[2], w[3]));
+}
+// Entry j of pack_fine.
+__device__ __forceinline__ float fine_entry(const bf16x8& x, int j) {
+  const uint4 v = __builtin_bit_cast(uint4, x);
+  const uint32_t w = j < 2 ? v.x : j < 4 ? v.y : j < 6 ? v.z : v.w;
+  return __uint_as_float(j & 1 ? (w >> 2) & 0x3fffc000u : (w & 0xffffu) << 14);
+}
+
 // dK, dV at D = 64 for one (b, kv head, 128-key tile), two work-groups per
 // CU, with the work of a key group split between two waves:
 //   P wave:  S = Q K^T, P = exp(S - LSE) (masked pairs cleared), dV^T += dO^T P
@@ -559,7 +582,8 @@ constexpr int kPairWaves = 8;  // 4 key groups x (P / dV wave, dS / dK wave)
 //   P waves:  S, P -> LDS  | dV, then the copies of the half two ahead
 //   dS waves: dP           | P <- LDS, dS, dK
 // with a barrier at the bar (P written to LDS as the bf16 MFMA operand it
-// already is) and one at the end.  The halves of a phase overlap across the
+// already is; Fine: in 9 mantissa bits, pack_fine, since a rounding of P to 7
+// in dS is as large as that of dS itself) and one at the end.  The halves of a phase overlap across the
 // two waves of a SIMD (the P wave's exponentials with the dS wave's dP
 // chain, the dS wave's dS with the P wave's dV).  Q, dO, LSE and Delta (in
 // accumulator-row order) and the column bitmap words travel by direct
@@ -567,7 +591,7 @@ constexpr int kPairWaves = 8;  // 4 key groups x (P / dV wave, dS / dK wave)
 // buffer freed at the start of the phase, so every copy has a whole phase
 // to land in; the end barrier waits only for the copies older than the
 // phase's own.
-template <int D>
+template <int D, bool Fine>
 __global__ __launch_bounds__(kPairWaves * 64) __attribute__((amdgpu_waves_per_eu(4, 4)))
 void bwd_dkdv_pair_kernel(BwdParams p) {
   static_assert(D == 64, "two work-groups per CU fit at D = 64 only");
@@ -828,8 +852,8 @@ void bwd_dkdv_pair_kernel(BwdParams p) {
           pa[blk] = pack_half(sacc, 0);
           pb[blk] = pack_half(sacc, 1);
           bf16x8* dst = p_s + ((kw * 2 + blk) * 2) * 64 + lane;
-          dst[0] = pa[blk];
-          dst[64] = pb[blk];
+          dst[0] = Fine ? pack_fine(sacc, 0) : pa[blk];
+          dst[64] = Fine ? pack_fine(sacc, 1) : pb[blk];
         }
         mid_barrier();
         // dV^T += dO^T P
@@ -890,8 +914,8 @@ void bwd_dkdv_pair_kernel(BwdParams p) {
           f32x16 ds;
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
-            ds[j] = (dp[blk][j] - dl[j]) * (float)xa[j];
-            ds[8 + j] = (dp[blk][8 + j] - dl[8 + j]) * (float)xb[j];
+            ds[j] = (dp[blk][j] - dl[j]) * (Fine ? fine_entry(xa, j) : (float)xa[j]);
+            ds[8 + j] = (dp[blk][8 + j] - dl[8 + j]) * (Fine ? fine_entry(xb, j) : (float)xb[j]);
           }
           const bf16x8 sa = pack_half(ds, 0), sb = pack_half(ds, 1);
           bf16x8 opd[2 * DT];
@@ -1028,7 +1052,7 @@ __global__ __launch_bounds__(kThreads, 2) void bwd_dq_kernel(BwdParams p) {
   // which is not stored, and its P is zero (neg_lse = -inf).
   const int qr = qvalid ? qrow : 0;
   const size_t rowstat = ((size_t)b * p.Hq + h) * T + qr;
-  bf16x8 qf[KS], dof[KS], of[KS];
+  bf16x8 qf[KS], dof[KS], of[KS], rest[KS];
   {
     const __bf16* qp = p.q + b * p.q_sb + h * p.q_sh + (int64_t)qr * p.q_st;
     const __bf16* dp = p.dout + b * p.do_sb + h * p.do_sh + (int64_t)qr * p.do_st;
@@ -1044,6 +1068,13 @@ __global__ __launch_bounds__(kThreads, 2) void bwd_dq_kernel(BwdParams p) {
     const __bf16* op = p.o + b * p.o_sb + h * p.o_sh + (int64_t)qr * p.o_st;
 #pragma unroll
     for (int s = 0; s < KS; ++s) of[s] = *reinterpret_cast<const bf16x8*>(op + 16 * s + 8 * g);
+    // (with o_rest 16 bits of O: Delta's error counts where a row has few keys
+    // -- dQ, window 4: 2.9e-3 off without, 2.4e-3 with -- and costs the reads,
+    // 81 to 84 us at 25 MB)
+    const __bf16* rp = p.o_rest + b * p.r_sb + h * p.r_sh + (int64_t)qr * p.r_st;
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+      rest[s] = p.o_rest ? *reinterpret_cast<const bf16x8*>(rp + 16 * s + 8 * g) : bf16x8{};
   }
   const float lrow = p.lse2[rowstat];
   float delta = p.fuse_delta ? 0.f : p.delta[rowstat];
@@ -1157,7 +1188,8 @@ __global__ __launch_bounds__(kThreads, 2) void bwd_dq_kernel(BwdParams p) {
 #pragma unroll
     for (int s = 0; s < KS; ++s)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) acc = fmaf((float)of[s][j], (float)dof[s][j], acc);
+      for (int j = 0; j < 8; ++j)
+        acc = fmaf((float)of[s][j] + (float)rest[s][j], (float)dof[s][j], acc);
     delta = halves_sum(acc);
     if (qvalid && g == 0) p.delta[rowstat] = delta;
   }
@@ -1215,6 +1247,8 @@ BwdParams make_bwd_params(const TensorView& q, const TensorView& k, const Tensor
   p.B = dims.B; p.Hq = dims.Hq; p.Hkv = dims.Hkv; p.T = dims.T;
   p.scale = dims.scale;
   p.scale_log2 = dims.scale * kLog2e;
+  p.o_rest = nullptr;
+  p.r_sb = p.r_sh = p.r_st = 0;
   p.fuse_delta = 0;
   p.m = mask;
   p.part = nullptr;
@@ -1226,11 +1260,14 @@ BwdParams make_bwd_params(const TensorView& q, const TensorView& k, const Tensor
 
 hipError_t launch_attn_bwd_phase(int phase, const TensorView& q, const TensorView& k,
                                  const TensorView& v, const TensorView& o,
-                                 const TensorView& dout, const float* lse2, float* delta,
+                                 const TensorView& o_rest, const TensorView& dout,
+                                 const float* lse2, float* delta,
                                  const TensorView& dq, const TensorView& dk, const TensorView& dv,
                                  const AttnDims& dims, const MaskTables& mask,
                                  hipStream_t stream) {
-  const BwdParams p = make_bwd_params(q, k, v, o, dout, lse2, delta, dq, dk, dv, dims, mask);
+  BwdParams p = make_bwd_params(q, k, v, o, dout, lse2, delta, dq, dk, dv, dims, mask);
+  p.o_rest = static_cast<const __bf16*>(o_rest.data);
+  p.r_sb = o_rest.sb; p.r_sh = o_rest.sh; p.r_st = o_rest.st;
   const int nt = (dims.T + kTile - 1) / kTile;
   if (nt == 0 || dims.B == 0 || dims.Hq == 0) return hipSuccess;
   const bool d64 = dims.D == 64;
@@ -1240,13 +1277,16 @@ hipError_t launch_attn_bwd_phase(int phase, const TensorView& q, const TensorVie
     const dim3 grid((unsigned)((rows + rows_per_block - 1) / rows_per_block));
     if (d64) hipLaunchKernelGGL(bwd_delta_kernel<64>, grid, dim3(kThreads), 0, stream, p);
     else hipLaunchKernelGGL(bwd_delta_kernel<128>, grid, dim3(kThreads), 0, stream, p);
-  } else if (phase == kBwdDkDv) {
+  } else if (phase == kBwdDkDv || phase == kBwdDkDvFine) {
     const dim3 grid(dims.Hkv, nt, dims.B);
 #ifdef T2T_DKDV_CLASSIC
     if (d64) hipLaunchKernelGGL((bwd_dkdv_kernel<64, false>), grid, dim3(kDkdvThreads), 0, stream, p);
     else hipLaunchKernelGGL((bwd_dkdv_kernel<128, false>), grid, dim3(kDkdvThreads), 0, stream, p);
 #else
-    if (d64) hipLaunchKernelGGL(bwd_dkdv_pair_kernel<64>, grid, dim3(kPairWaves * 64), 0, stream, p);
+    if (d64 && phase == kBwdDkDvFine)
+      hipLaunchKernelGGL((bwd_dkdv_pair_kernel<64, true>), grid, dim3(kPairWaves * 64), 0, stream, p);
+    else if (d64)
+      hipLaunchKernelGGL((bwd_dkdv_pair_kernel<64, false>), grid, dim3(kPairWaves * 64), 0, stream, p);
     else hipLaunchKernelGGL((bwd_dkdv_kernel<128, false>), grid, dim3(kDkdvThreads), 0, stream, p);
 #endif
   } else {  // kBwdDq, kBwdDqDelta

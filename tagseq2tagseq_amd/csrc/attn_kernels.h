@@ -70,9 +70,10 @@ hipError_t launch_mask_meta(const int32_t* doc, const uint64_t* qbits, const uin
                             const int32_t* start, int window, int sinks, int T, int words,
                             const MaskOut& out, hipStream_t stream);
 
+// o_rest (may be empty): what rounding to bf16 left of o, as bf16.
 hipError_t launch_attn_fwd_bf16(const TensorView& q, const TensorView& k, const TensorView& v,
-                                const TensorView& o, float* lse2, const AttnDims& dims,
-                                const MaskTables& mask, hipStream_t stream);
+                                const TensorView& o, const TensorView& o_rest, float* lse2,
+                                const AttnDims& dims, const MaskTables& mask, hipStream_t stream);
 
 // Float32 q / k / v / o (D in {64, 128}); same tables and LSE convention.
 hipError_t launch_attn_fwd_f32(const TensorView& q, const TensorView& k, const TensorView& v,
@@ -87,11 +88,10 @@ hipError_t launch_attn_bwd_f32(const TensorView& q, const TensorView& k, const T
                                hipStream_t stream);
 
 // kBwdDqDelta: dQ that also computes and writes Delta (run before dK/dV).
-enum BwdPhase { kBwdDelta = 0, kBwdDkDv = 1, kBwdDq = 2, kBwdDqDelta = 3 };
+// kBwdDkDvFine: dK/dV whose dS is taken from P of 9 bits instead of 7 (D = 64,
+// where P passes through LDS; D = 128 takes it unrounded in either).
+enum BwdPhase { kBwdDelta = 0, kBwdDkDv = 1, kBwdDq = 2, kBwdDqDelta = 3, kBwdDkDvFine = 4 };
 
-// One backward phase.  Views a phase does not read may be empty (delta: o,
-// dout; dkdv: q, k, v, dout, lse2, delta, dk, dv; dq: q, k, v, dout, lse2,
-// delta, dq).
 // dK/dV with long columns shared by `splits` work-groups (bwd_uneven_splits; 1:
 // not worth it), their sums in workspace [B][Hkv][nt][splits][2][128][D].
 int bwd_uneven_splits(int B, int Hkv, int T, int D);
@@ -101,9 +101,12 @@ hipError_t launch_attn_bwd_dkdv_split(const TensorView& q, const TensorView& k,
                                       const TensorView& dv, const AttnDims& dims,
                                       const MaskTables& mask, int splits, float* workspace,
                                       hipStream_t stream);
+// One backward phase.  Views a phase does not read may be empty (delta: o,
+// dout; dkdv: q, k, v, dout, lse2, delta, dk, dv; dq: q, k, v, dout, lse2,
+// delta, dq; with Delta o, and o_rest if not empty).
 hipError_t launch_attn_bwd_phase(int phase, const TensorView& q, const TensorView& k,
                                  const TensorView& v, const TensorView& o,
-                                 const TensorView& dout, const float* lse2, float* delta,
+                                 const TensorView& o_rest, const TensorView& dout, const float* lse2, float* delta,
                                  const TensorView& dq, const TensorView& dk, const TensorView& dv,
                                  const AttnDims& dims, const MaskTables& mask,
                                  hipStream_t stream);

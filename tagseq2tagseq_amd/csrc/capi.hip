@@ -223,10 +223,12 @@ int t2t_mask_meta_window(const int32_t* doc, const uint64_t* q_bits, const uint6
                    tile_class, out, stream);
 }
 
-int t2t_attn_fwd(const t2t_tensor* q, const t2t_tensor* k, const t2t_tensor* v,
-                 const t2t_tensor* o, float* lse2, int32_t B, int32_t Hq, int32_t Hkv,
-                 int32_t T, int32_t D, int32_t dtype, float scale, const t2t_block_mask* mask,
-                 void* stream) {
+namespace {
+
+// The forward; o_rest: NULL, or where what rounding left of o goes (bf16).
+int attn_fwd(const t2t_tensor* q, const t2t_tensor* k, const t2t_tensor* v, const t2t_tensor* o,
+             const t2t_tensor* o_rest, float* lse2, int32_t B, int32_t Hq, int32_t Hkv, int32_t T,
+             int32_t D, int32_t dtype, float scale, const t2t_block_mask* mask, void* stream) {
   int rc = check_dims(B, Hq, Hkv, T, D, dtype, true);
   if (rc) return rc;
   rc = check_scale(scale);
@@ -234,7 +236,7 @@ int t2t_attn_fwd(const t2t_tensor* q, const t2t_tensor* k, const t2t_tensor* v,
   if (B == 0 || Hq == 0 || T == 0) return T2T_OK;
   const int es = dtype == T2T_DTYPE_F32 ? 4 : 2;
   if (!view_ok(q, T, D, es) || !view_ok(k, T, D, es) || !view_ok(v, T, D, es) ||
-      !view_ok(o, T, D, es))
+      !view_ok(o, T, D, es) || (o_rest && !view_ok(o_rest, T, D, es)))
     return fail(T2T_EINVAL, "q/k/v/o view invalid (NULL, misaligned, bad stride or slice >= 2 GiB)");
   if (!lse2) return fail(T2T_EINVAL, "lse2 is NULL");
   rc = check_mask(mask, B, T, true, false);
@@ -246,8 +248,27 @@ int t2t_attn_fwd(const t2t_tensor* q, const t2t_tensor* k, const t2t_tensor* v,
                                                lse2, dims, as_tables(mask), st),
                       "t2t_attn_fwd launch");
   return hip_status(t2t::launch_attn_fwd_bf16(as_view(q), as_view(k), as_view(v), as_view(o),
-                                              lse2, dims, as_tables(mask), st),
+                                              o_rest ? as_view(o_rest) : t2t::TensorView{}, lse2,
+                                              dims, as_tables(mask), st),
                     "t2t_attn_fwd launch");
+}
+
+}  // namespace
+
+int t2t_attn_fwd(const t2t_tensor* q, const t2t_tensor* k, const t2t_tensor* v,
+                 const t2t_tensor* o, float* lse2, int32_t B, int32_t Hq, int32_t Hkv,
+                 int32_t T, int32_t D, int32_t dtype, float scale, const t2t_block_mask* mask,
+                 void* stream) {
+  return attn_fwd(q, k, v, o, nullptr, lse2, B, Hq, Hkv, T, D, dtype, scale, mask, stream);
+}
+
+int t2t_attn_fwd_rest(const t2t_tensor* q, const t2t_tensor* k, const t2t_tensor* v,
+                      const t2t_tensor* o, const t2t_tensor* o_rest, float* lse2, int32_t B,
+                      int32_t Hq, int32_t Hkv, int32_t T, int32_t D, int32_t dtype, float scale,
+                      const t2t_block_mask* mask, void* stream) {
+  if (dtype != T2T_DTYPE_BF16) return fail(T2T_EUNSUPPORTED, "dtype %d is not bf16", dtype);
+  if (!o_rest) return fail(T2T_EINVAL, "o_rest is NULL");
+  return attn_fwd(q, k, v, o, o_rest, lse2, B, Hq, Hkv, T, D, dtype, scale, mask, stream);
 }
 
 int t2t_attn_bwd_preprocess(const t2t_tensor* o, const t2t_tensor* dout, float* delta,
@@ -262,16 +283,18 @@ int t2t_attn_bwd_preprocess(const t2t_tensor* o, const t2t_tensor* dout, float* 
   t2t::AttnDims dims{B, Hq, Hq, T, D, 1.f};
   t2t::MaskTables m{};
   return hip_status(t2t::launch_attn_bwd_phase(t2t::kBwdDelta, none, none, none, as_view(o),
-                                               as_view(dout), nullptr, delta, none, none, none,
+                                               none, as_view(dout), nullptr, delta, none, none, none,
                                                dims, m, static_cast<hipStream_t>(stream)),
                     "t2t_attn_bwd_preprocess launch");
 }
 
-int t2t_attn_bwd_dkdv(const t2t_tensor* q, const t2t_tensor* k, const t2t_tensor* v,
-                      const t2t_tensor* dout, const float* lse2, const float* delta,
-                      const t2t_tensor* dk, const t2t_tensor* dv, int32_t B, int32_t Hq,
-                      int32_t Hkv, int32_t T, int32_t D, int32_t dtype, float scale,
-                      const t2t_block_mask* mask, void* stream) {
+namespace {
+
+int attn_bwd_dkdv(int phase, const t2t_tensor* q, const t2t_tensor* k, const t2t_tensor* v,
+                  const t2t_tensor* dout, const float* lse2, const float* delta,
+                  const t2t_tensor* dk, const t2t_tensor* dv, int32_t B, int32_t Hq, int32_t Hkv,
+                  int32_t T, int32_t D, int32_t dtype, float scale, const t2t_block_mask* mask,
+                  void* stream) {
   int rc = check_dims(B, Hq, Hkv, T, D, dtype);
   if (rc) return rc;
   rc = check_scale(scale);
@@ -285,12 +308,23 @@ int t2t_attn_bwd_dkdv(const t2t_tensor* q, const t2t_tensor* k, const t2t_tensor
   if (rc) return rc;
   const t2t::TensorView none{nullptr, 0, 0, 0};
   t2t::AttnDims dims{B, Hq, Hkv, T, D, scale};
-  return hip_status(t2t::launch_attn_bwd_phase(t2t::kBwdDkDv, as_view(q), as_view(k), as_view(v),
+  return hip_status(t2t::launch_attn_bwd_phase(phase, as_view(q), as_view(k), as_view(v), none,
                                                none, as_view(dout), lse2,
                                                const_cast<float*>(delta), none, as_view(dk),
                                                as_view(dv), dims, as_tables(mask),
                                                static_cast<hipStream_t>(stream)),
                     "t2t_attn_bwd_dkdv launch");
+}
+
+}  // namespace
+
+int t2t_attn_bwd_dkdv(const t2t_tensor* q, const t2t_tensor* k, const t2t_tensor* v,
+                      const t2t_tensor* dout, const float* lse2, const float* delta,
+                      const t2t_tensor* dk, const t2t_tensor* dv, int32_t B, int32_t Hq,
+                      int32_t Hkv, int32_t T, int32_t D, int32_t dtype, float scale,
+                      const t2t_block_mask* mask, void* stream) {
+  return attn_bwd_dkdv(t2t::kBwdDkDv, q, k, v, dout, lse2, delta, dk, dv, B, Hq, Hkv, T, D, dtype,
+                       scale, mask, stream);
 }
 
 int t2t_attn_bwd_dq(const t2t_tensor* q, const t2t_tensor* k, const t2t_tensor* v,
@@ -310,7 +344,7 @@ int t2t_attn_bwd_dq(const t2t_tensor* q, const t2t_tensor* k, const t2t_tensor* 
   const t2t::TensorView none{nullptr, 0, 0, 0};
   t2t::AttnDims dims{B, Hq, Hkv, T, D, scale};
   return hip_status(t2t::launch_attn_bwd_phase(t2t::kBwdDq, as_view(q), as_view(k), as_view(v),
-                                               none, as_view(dout), lse2,
+                                               none, none, as_view(dout), lse2,
                                                const_cast<float*>(delta), as_view(dq), none,
                                                none, dims, as_tables(mask),
                                                static_cast<hipStream_t>(stream)),
@@ -327,9 +361,10 @@ int64_t t2t_attn_bwd_uneven_workspace(int32_t B, int32_t Hkv, int32_t T, int32_t
 
 namespace {
 
-// The backward; uneven: with the workspace that long columns are shared over.
+// The backward; uneven: with the workspace that long columns are shared over,
+// finer in dS.  o_rest: NULL, or t2t_attn_fwd_rest's.
 int attn_bwd(const t2t_tensor* q, const t2t_tensor* k, const t2t_tensor* v, const t2t_tensor* o,
-             const t2t_tensor* dout, const float* lse2, float* delta, const t2t_tensor* dq,
+             const t2t_tensor* o_rest, const t2t_tensor* dout, const float* lse2, float* delta, const t2t_tensor* dq,
              const t2t_tensor* dk, const t2t_tensor* dv, int32_t B, int32_t Hq, int32_t Hkv,
              int32_t T, int32_t D, int32_t dtype, float scale, const t2t_block_mask* mask,
              bool uneven, void* workspace, int64_t workspace_bytes, void* stream) {
@@ -342,7 +377,8 @@ int attn_bwd(const t2t_tensor* q, const t2t_tensor* k, const t2t_tensor* v, cons
   const int es = dtype == T2T_DTYPE_F32 ? 4 : 2;
   if (!view_ok(q, T, D, es) || !view_ok(k, T, D, es) || !view_ok(v, T, D, es) ||
       !view_ok(o, T, D, es) || !view_ok(dout, T, D, es) || !view_ok(dq, T, D, es) ||
-      !view_ok(dk, T, D, es) || !view_ok(dv, T, D, es))
+      !view_ok(dk, T, D, es) || !view_ok(dv, T, D, es) ||
+      (o_rest && !view_ok(o_rest, T, D, es)))
     return fail(T2T_EINVAL, "tensor view invalid (NULL, misaligned, bad stride or slice >= 2 GiB)");
   if (!lse2 || !delta) return fail(T2T_EINVAL, "lse2/delta is NULL");
   rc = check_mask(mask, B, T, true, true);
@@ -362,8 +398,9 @@ int attn_bwd(const t2t_tensor* q, const t2t_tensor* k, const t2t_tensor* v, cons
   // dQ first: it computes each row's Delta = rowsum(O * dO) from the dO rows
   // it holds and writes it for dK/dV, so no separate Delta launch is needed.
   rc = hip_status(t2t::launch_attn_bwd_phase(t2t::kBwdDqDelta, as_view(q), as_view(k),
-                                             as_view(v), as_view(o), as_view(dout), lse2, delta,
-                                             as_view(dq), t2t::TensorView{nullptr, 0, 0, 0},
+                                             as_view(v), as_view(o),
+                                             o_rest ? as_view(o_rest) : t2t::TensorView{},
+                                             as_view(dout), lse2, delta, as_view(dq), t2t::TensorView{nullptr, 0, 0, 0},
                                              t2t::TensorView{nullptr, 0, 0, 0}, dims,
                                              as_tables(mask), static_cast<hipStream_t>(stream)),
                   "t2t_attn_bwd dQ launch");
@@ -375,8 +412,8 @@ int attn_bwd(const t2t_tensor* q, const t2t_tensor* k, const t2t_tensor* v, cons
                           t2t::bwd_uneven_splits(B, Hkv, T, D), static_cast<float*>(workspace),
                           static_cast<hipStream_t>(stream)),
                       "t2t_attn_bwd_uneven dK/dV launch");
-  return t2t_attn_bwd_dkdv(q, k, v, dout, lse2, delta, dk, dv, B, Hq, Hkv, T, D, dtype, scale,
-                           mask, stream);
+  return attn_bwd_dkdv(uneven ? t2t::kBwdDkDvFine : t2t::kBwdDkDv, q, k, v, dout, lse2, delta, dk,
+                       dv, B, Hq, Hkv, T, D, dtype, scale, mask, stream);
 }
 
 }  // namespace
@@ -387,18 +424,21 @@ int t2t_attn_bwd(const t2t_tensor* q, const t2t_tensor* k, const t2t_tensor* v,
                  const t2t_tensor* dv, int32_t B, int32_t Hq, int32_t Hkv, int32_t T,
                  int32_t D, int32_t dtype, float scale, const t2t_block_mask* mask,
                  void* stream) {
-  return attn_bwd(q, k, v, o, dout, lse2, delta, dq, dk, dv, B, Hq, Hkv, T, D, dtype, scale, mask,
-                  false, nullptr, 0, stream);
+  return attn_bwd(q, k, v, o, nullptr, dout, lse2, delta, dq, dk, dv, B, Hq, Hkv, T, D, dtype,
+                  scale, mask, false, nullptr, 0, stream);
 }
 
 int t2t_attn_bwd_uneven(const t2t_tensor* q, const t2t_tensor* k, const t2t_tensor* v,
-                        const t2t_tensor* o, const t2t_tensor* dout, const float* lse2,
-                        float* delta, const t2t_tensor* dq, const t2t_tensor* dk,
-                        const t2t_tensor* dv, int32_t B, int32_t Hq, int32_t Hkv, int32_t T,
-                        int32_t D, int32_t dtype, float scale, const t2t_block_mask* mask,
-                        void* workspace, int64_t workspace_bytes, void* stream) {
-  return attn_bwd(q, k, v, o, dout, lse2, delta, dq, dk, dv, B, Hq, Hkv, T, D, dtype, scale, mask,
-                  true, workspace, workspace_bytes, stream);
+                        const t2t_tensor* o, const t2t_tensor* o_rest, const t2t_tensor* dout,
+                        const float* lse2, float* delta, const t2t_tensor* dq,
+                        const t2t_tensor* dk, const t2t_tensor* dv, int32_t B, int32_t Hq,
+                        int32_t Hkv, int32_t T, int32_t D, int32_t dtype, float scale,
+                        const t2t_block_mask* mask, void* workspace, int64_t workspace_bytes,
+                        void* stream) {
+  if (o_rest && dtype != T2T_DTYPE_BF16)
+    return fail(T2T_EUNSUPPORTED, "o_rest goes with bf16, not dtype %d", dtype);
+  return attn_bwd(q, k, v, o, o_rest, dout, lse2, delta, dq, dk, dv, B, Hq, Hkv, T, D, dtype,
+                  scale, mask, true, workspace, workspace_bytes, stream);
 }
 
 // Delta workspace of t2t_attn_bwd_noalloc: a file-scope device array instead

@@ -88,8 +88,10 @@ const t2t_block_mask* mask_at(int64_t address) {
 
 // ---- attention (mask: address of the caller's t2t_block_mask, alive during the call)
 
-std::tuple<Tensor, Tensor> attn_fwd(const Tensor& q, const Tensor& k, const Tensor& v,
-                                    int64_t mask, double scale) {
+// rest: with what rounding left of a bf16 out (else undefined), for attn_bwd
+std::tuple<Tensor, Tensor, Tensor> attn_fwd_rest(const Tensor& q, const Tensor& k,
+                                                 const Tensor& v, int64_t mask, double scale,
+                                                 bool rest) {
   const int dtype = attention_code(q, k, v);
   need_gpu(q, k, v);
   const c10::DeviceGuard guard(q.device());
@@ -99,16 +101,31 @@ std::tuple<Tensor, Tensor> attn_fwd(const Tensor& q, const Tensor& k, const Tens
   Tensor out = at::empty({B, T, Hq, D}, q.options()).transpose(1, 2);
   Tensor lse2 = at::empty({B, Hq, T}, q.options().dtype(at::kFloat));
   const t2t_tensor qs = view4(q), ks = view4(k), vs = view4(v), os = view4(out);
+  if (rest && dtype == T2T_DTYPE_BF16) {
+    Tensor left = at::empty_like(out);
+    const t2t_tensor rs = view4(left);
+    check(t2t_attn_fwd_rest(&qs, &ks, &vs, &os, &rs, lse2.data_ptr<float>(), B, Hq, Hkv, T, D,
+                            dtype, static_cast<float>(scale), mask_at(mask), stream_of(q)),
+          "t2t_attn_fwd_rest");
+    return {out, lse2, left};
+  }
   check(t2t_attn_fwd(&qs, &ks, &vs, &os, lse2.data_ptr<float>(), B, Hq, Hkv, T, D,
                      dtype, static_cast<float>(scale), mask_at(mask), stream_of(q)),
         "t2t_attn_fwd");
+  return {out, lse2, Tensor()};
+}
+
+std::tuple<Tensor, Tensor> attn_fwd(const Tensor& q, const Tensor& k, const Tensor& v,
+                                    int64_t mask, double scale) {
+  auto [out, lse2, none] = attn_fwd_rest(q, k, v, mask, scale, false);
   return {out, lse2};
 }
 
+// uneven: t2t_attn_bwd_uneven, with rest where the forward has left one
 std::tuple<Tensor, Tensor, Tensor> attn_bwd(const Tensor& q, const Tensor& k, const Tensor& v,
                                             const Tensor& out, const Tensor& dout_in,
                                             const Tensor& lse2, int64_t mask, double scale,
-                                            bool uneven = false) {
+                                            bool uneven, const c10::optional<Tensor>& rest) {
   const int dtype = attention_code(q, k, v, out, dout_in);
   need_gpu(q, k, v, out, dout_in, lse2);
   const c10::DeviceGuard guard(q.device());
@@ -119,13 +136,21 @@ std::tuple<Tensor, Tensor, Tensor> attn_bwd(const Tensor& q, const Tensor& k, co
   Tensor delta = at::empty({B, Hq, T}, q.options().dtype(at::kFloat));
   const t2t_tensor qs = view4(q), ks = view4(k), vs = view4(v), os = view4(out),
                    ds = view4(dout), dqs = view4(dq), dks = view4(dk), dvs = view4(dv);
-  const int64_t bytes = uneven ? t2t_attn_bwd_uneven_workspace(B, Hkv, T, D, dtype) : 0;
-  if (bytes > 0) {
-    Tensor ws = at::empty({bytes / 4}, delta.options());
-    check(t2t_attn_bwd_uneven(&qs, &ks, &vs, &os, &ds, lse2.data_ptr<float>(),
-                              delta.data_ptr<float>(), &dqs, &dks, &dvs, B, Hq, Hkv, T, D, dtype,
-                              static_cast<float>(scale), mask_at(mask), ws.data_ptr(), bytes,
-                              stream_of(q)),
+  if (uneven) {
+    const int64_t bytes = t2t_attn_bwd_uneven_workspace(B, Hkv, T, D, dtype);
+    Tensor ws;
+    if (bytes > 0) ws = at::empty({bytes / 4}, delta.options());
+    t2t_tensor rs{};
+    if (rest.has_value()) {
+      need_gpu(*rest);
+      TORCH_CHECK_VALUE(rest->sizes() == out.sizes() && rest->scalar_type() == out.scalar_type(),
+                        "rest ", rest->sizes(), " ", rest->scalar_type(), " is not out's");
+      rs = view4(*rest);
+    }
+    check(t2t_attn_bwd_uneven(&qs, &ks, &vs, &os, rest.has_value() ? &rs : nullptr, &ds,
+                              lse2.data_ptr<float>(), delta.data_ptr<float>(), &dqs, &dks, &dvs,
+                              B, Hq, Hkv, T, D, dtype, static_cast<float>(scale), mask_at(mask),
+                              bytes > 0 ? ws.data_ptr() : nullptr, bytes, stream_of(q)),
           "t2t_attn_bwd_uneven");
     return {dq, dk, dv};
   }
@@ -1239,9 +1264,9 @@ struct AttentionAd : torch::autograd::Function<AttentionAd> {
                                const Tensor& v, const std::vector<Tensor>& tables, double scale,
                                bool uneven) {
     const t2t_block_mask m = mask_of(tables);
-    auto [out, lse2] =
-        attn_fwd(q, k, v, static_cast<int64_t>(reinterpret_cast<intptr_t>(&m)), scale);
-    ctx->save_for_backward({q, k, v, out, lse2});
+    auto [out, lse2, rest] =
+        attn_fwd_rest(q, k, v, static_cast<int64_t>(reinterpret_cast<intptr_t>(&m)), scale, uneven);
+    ctx->save_for_backward({q, k, v, out, lse2, rest});
     ctx->saved_data["tables"] = tables;
     ctx->saved_data["scale"] = scale;
     ctx->saved_data["uneven"] = uneven;
@@ -1254,7 +1279,8 @@ struct AttentionAd : torch::autograd::Function<AttentionAd> {
     auto [dq, dk, dv] = attn_bwd(t[0], t[1], t[2], t[3], g[0], t[4],
                                  static_cast<int64_t>(reinterpret_cast<intptr_t>(&m)),
                                  ctx->saved_data["scale"].toDouble(),
-                                 ctx->saved_data["uneven"].toBool());
+                                 ctx->saved_data["uneven"].toBool(),
+                                 t[5].defined() ? c10::make_optional(t[5]) : c10::nullopt);
     variable_list d = once({dq, dk, dv}, "masked attention");
     d.resize(6);
     return d;
@@ -1490,9 +1516,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   // Python threads run meanwhile
   const auto no_gil = py::call_guard<py::gil_scoped_release>();
   m.def("attn_fwd", &attn_fwd, no_gil);
+  m.def("attn_fwd_rest", &attn_fwd_rest, no_gil);
   m.def("attn_bwd", &attn_bwd, py::arg("q"), py::arg("k"), py::arg("v"), py::arg("out"),
         py::arg("dout"), py::arg("lse2"), py::arg("mask"), py::arg("scale"),
-        py::arg("uneven") = false, no_gil);
+        py::arg("uneven") = false, py::arg("rest") = py::none(), no_gil);
   m.def("rms_norm", &rms_norm, no_gil);
   m.def("rms_norm_backward", &rms_norm_backward, no_gil);
   m.def("qkv_rope", &qkv_rope, no_gil);

@@ -506,3 +506,40 @@ def test_columns_shared_by_work_groups(B, T, H, Hkv, words):
                                    _attention_ref(q, k, v, do, dense, 2.0 ** -8)):
         worst = float(((x.detach().double() - ref).abs() / tol).max())
         assert worst <= 1, f"{name}: {worst:.3g} of the tolerance"
+
+
+# A rounding to bf16 is off by 2^-7 / m / sqrt(12) (root of the mean square)
+# relative to a value of mantissa m, over mantissas spread as 1 / m
+# 2^-7 sqrt(3 / (8 ln 2) / 12) = 1.66e-3.  dS is rounded once, and what it is
+# summed to once; P of 9 bits adds a quarter of one: 2.38e-3 in all, and 5 % for
+# the sample.
+ONE_ROUNDING = 2.0 ** -7 * math.sqrt(3 / (8 * math.log(2)) / 12)
+TWO_ROUNDINGS = 1.05 * ONE_ROUNDING * math.sqrt(2 + 1 / 16)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("window,sinks", [(4, 0), (40, 0), (300, 4)])
+def test_gradients_round_twice(D, window, sinks):
+    T, H = 1500, 4
+    rows = [_row(T, 3, 0, 400)]
+    bm = _build(rows, window, sinks)
+    dense = torch.from_numpy(_dense(*rows[0], window, sinks))[None].to(DEV)
+    g = torch.Generator().manual_seed(D + window)
+    q, k, v, do = (torch.randn(1, H, T, D, generator=g).to(BF).to(DEV) for _ in range(4))
+    for t in (q, k, v):
+        t.requires_grad_(True)
+    out = flex_attention(q, k, v, block_mask=bm)
+    got = torch.autograd.grad(out, (q, k, v), do, retain_graph=True)
+    want = [r for r, _ in _attention_ref(q, k, v, do, dense, 2.0 ** -8)][1:]
+    for name, a, b in zip(("dq", "dk", "dv"), got, want):
+        off = float((a.double() - b).norm() / b.norm())
+        assert off <= TWO_ROUNDINGS, f"{name}: {off:.3g}"
+
+    class Seen(torch.overrides.TorchFunctionMode):
+        def __torch_function__(self, func, types, args=(), kwargs=None):
+            return func(*args, **(kwargs or {}))
+
+    with Seen():  # (a call that more than autograd watches)
+        out2 = flex_attention(q, k, v, block_mask=bm)
+    assert torch.equal(out, out2)
+    assert all(torch.equal(a, b) for a, b in zip(got, torch.autograd.grad(out2, (q, k, v), do)))

@@ -95,7 +95,7 @@ def test_nothing_to_do_is_no_error():
 
 def _backward(**kw):
     v = _view(stride_h=128, stride_t=128)
-    a = dict(q=v, k=v, v=v, o=v, do=v, lse2=P, delta=P, dq=v, dk=v, dv=v, B=1, Hq=2, Hkv=1, T=256,
+    a = dict(q=v, k=v, v=v, o=v, rest=v, do=v, lse2=P, delta=P, dq=v, dk=v, dv=v, B=1, Hq=2, Hkv=1, T=256,
              D=128, dtype=0, scale=0.1, mask=_tables(), ws=P, ws_bytes=1 << 40)
     a.update(kw)
     return L.t2t_attn_bwd_uneven(*a.values(), None)
@@ -106,10 +106,24 @@ def _backward(**kw):
     (dict(ws=None), -1, "workspace"), (dict(ws=ctypes.c_void_p(0x1008)), -1, "16-byte"),
     (dict(ws_bytes=1000), -1, "workspace"), (dict(D=96), -2, "head dim"), (dict(Hq=3, Hkv=2), -1, "GQA"),
     (dict(scale=-1.0), -1, "scale"), (dict(lse2=None), -1, "lse2"), (dict(mask=None), -1, "mask"),
-    (dict(dk=None), -1, "view"),
+    (dict(dk=None), -1, "view"), (dict(dtype=1), -2, "o_rest"),
+    (dict(rest=_view(data=None)), -1, "view"),
 ])
 def test_backward_entry_refuses(kw, rc, text):
     assert _backward(**kw) == rc and text in _err()
+
+
+@no_gpu
+@pytest.mark.parametrize("kw,rc,text", [
+    (dict(rest=None), -1, "o_rest"), (dict(dtype=1), -2, "not bf16"), (dict(lse2=None), -1, "lse2"),
+    (dict(rest=_view(data=None)), -1, "view"), (dict(D=96), -2, "head dim"), (dict(mask=None), -1, "mask"),
+])
+def test_forward_entry_refuses(kw, rc, text):
+    v = _view(stride_h=128, stride_t=128)
+    a = dict(q=v, k=v, v=v, o=v, rest=v, lse2=P, B=1, Hq=2, Hkv=1, T=256, D=128, dtype=0,
+             scale=0.1, mask=_tables())
+    a.update(kw)
+    assert L.t2t_attn_fwd_rest(*a.values(), None) == rc and text in _err()
 
 
 def test_backward_workspace():
