@@ -21,6 +21,7 @@ and ``t2t_kv8_attend``.
 from __future__ import annotations
 
 import math
+from operator import index
 from typing import Optional, Tuple, Union
 
 import torch
@@ -69,11 +70,11 @@ def kv8_append(k: torch.Tensor, v: torch.Tensor, pos: Union[int, torch.Tensor],
     value is not finite makes every row that reads it NaN.  What the buffers
     hold where nothing was stored is never looked at.  A device position below
     0 or above capacity - M stores nothing.  No gradient."""
-    at, pos0 = (pos, 0) if isinstance(pos, torch.Tensor) else (None, int(pos))
+    at, pos0 = (pos, 0) if isinstance(pos, torch.Tensor) else (None, index(pos))
     if capacity is not None and capacity < 0:
         raise ValueError(f"capacity={capacity} is negative")
     args = (k, v, at, pos0, k_codes, v_codes, k_scale, v_scale,
-            -1 if capacity is None else int(capacity))
+            -1 if capacity is None else index(capacity))
     tensors = (k, v, k_codes, v_codes, k_scale, v_scale)
     if (not torch.compiler.is_compiling()
             and _lib.unwatched(*(tensors if at is None else (*tensors, at)))):
@@ -115,7 +116,7 @@ def attn_decode_kv8(q: torch.Tensor, k_codes: torch.Tensor, v_codes: torch.Tenso
     window, sinks = check_window(window, sinks)
     if scale is None:
         scale = 1.0 / math.sqrt(q.shape[-1])
-    args = (q, k_codes, v_codes, k_scale, v_scale, int(n_keys), key_doc, key_bits, q_pos, q_doc,
+    args = (q, k_codes, v_codes, k_scale, v_scale, index(n_keys), key_doc, key_bits, q_pos, q_doc,
             q_bits, float(scale), window or 0, sinks, q_start)
     if (not torch.compiler.is_compiling()
             and _lib.unwatched(*[t for t in args if isinstance(t, torch.Tensor)])):

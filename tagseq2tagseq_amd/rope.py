@@ -38,6 +38,7 @@ from __future__ import annotations
 
 import math
 from dataclasses import dataclass
+from operator import index
 from typing import Dict, Optional, Tuple, Union
 
 import torch
@@ -473,9 +474,9 @@ def qkv_rotary(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, num_head
     multiple of 16; fp32 arithmetic with one rounding.  Gradient for qkv."""
     if (cos.requires_grad or sin.requires_grad) and torch.is_grad_enabled():
         raise RuntimeError("the rotary tables get no gradient: detach cos and sin")
-    at, pos0 = (pos, 0) if isinstance(pos, torch.Tensor) else (None, int(pos))
-    args = (qkv, cos, sin, int(num_heads),
-            int(num_heads if num_kv_heads is None else num_kv_heads), at, pos0, bool(interleaved))
+    at, pos0 = (pos, 0) if isinstance(pos, torch.Tensor) else (None, index(pos))
+    args = (qkv, cos, sin, index(num_heads),
+            index(num_heads if num_kv_heads is None else num_kv_heads), at, pos0, bool(interleaved))
     watched = (qkv, cos, sin) if at is None else (qkv, cos, sin, at)
     if not torch.compiler.is_compiling():
         if _lib.unwatched(*watched):

@@ -543,3 +543,91 @@ def test_gradients_round_twice(D, window, sinks):
         out2 = flex_attention(q, k, v, block_mask=bm)
     assert torch.equal(out, out2)
     assert all(torch.equal(a, b) for a, b in zip(got, torch.autograd.grad(out2, (q, k, v), do)))
+
+
+def _recorded(dtype, D=64, T=700, window=90, sinks=3, seed=0):
+    rows = [_row(T, seed, 1, 300)]
+    bm = _build(rows, window, sinks)
+    g = torch.Generator().manual_seed(seed)
+    q, k, v, do = (torch.randn(1, 2, T, D, generator=g).to(dtype).to(DEV) for _ in range(4))
+    return bm, [t.requires_grad_(True) for t in (q, k, v)], do
+
+
+@pytest.mark.parametrize("dtype", [BF, torch.float32])
+def test_recomputed_and_offloaded_regions(dtype):
+    """Where a checkpoint or hooks take what the call's graph saves."""
+    from torch.utils.checkpoint import checkpoint
+    bm, x, do = _recorded(dtype)
+
+    def call(q, k, v):
+        return flex_attention(q, k, v, block_mask=bm)
+    out = call(*x)
+    want = torch.autograd.grad(out, x, do)
+    got = [checkpoint(call, *x, use_reentrant=False), checkpoint(call, *x, use_reentrant=True)]
+    with torch.autograd.graph.save_on_cpu():
+        got.append(call(*x))
+    for o in got:
+        assert torch.equal(o, out)
+        o.backward(do)
+        for t, w in zip(x, want):
+            assert torch.equal(t.grad, w)
+            t.grad = None
+
+
+@pytest.mark.parametrize("dtype,D", [(BF, 64), (BF, 128), (torch.float32, 64)])
+def test_training_captured_and_replayed(dtype, D):
+    """The mask, forward and backward in one graph, replayed with other inputs
+    beside eager calls."""
+    T, H, window, sinks = 900, 2, 120, 4
+    doc = torch.from_numpy(_row(T, 1, 0, 300)[0]).to(DEV).int()[None]
+    g = torch.Generator().manual_seed(1)
+    x = [torch.randn(1, H, T, D, generator=g).to(dtype).to(DEV).requires_grad_(True)
+         for _ in range(3)]
+    do = torch.randn(1, H, T, D, generator=g).to(dtype).to(DEV)
+
+    def step(leaves):
+        bm = build_block_mask(doc, window=window, sinks=sinks)
+        out = flex_attention(*leaves, block_mask=bm)
+        return [out.detach(), *torch.autograd.grad(out, leaves, do)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step(x)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step(x)
+    for i in range(4):
+        with torch.no_grad():
+            for t in (*x, do):
+                t.copy_(torch.randn(t.shape, generator=g).to(dtype).to(DEV))
+            doc.copy_(torch.from_numpy(_row(T, 2 + i, 0, 300)[0]).to(DEV).int()[None])
+        graph.replay()
+        torch.cuda.synchronize()
+        own = [t.detach().clone().requires_grad_(True) for t in x]
+        for a, b in zip(outs, step(own)):
+            assert torch.equal(a, b)
+
+
+def test_training_on_other_streams_and_threads():
+    import threading
+    bm, x, do = _recorded(BF, D=128, T=2500, window=400)
+    want = torch.autograd.grad(flex_attention(*x, block_mask=bm), x, do)
+    torch.cuda.synchronize()
+    bad = []
+
+    def work():
+        own = [t.detach().clone().requires_grad_(True) for t in x]
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            for _ in range(10):
+                got = torch.autograd.grad(flex_attention(*own, block_mask=bm), own, do)
+            s.synchronize()
+            if not all(torch.equal(a, b) for a, b in zip(got, want)):
+                bad.append(1)
+    threads = [threading.Thread(target=work) for _ in range(2)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert not bad

@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from tagseq2tagseq_amd import _lib
-from tagseq2tagseq_amd.kv8 import KV8Cache
+from tagseq2tagseq_amd.kv8 import KV8Cache, attn_decode_kv8, kv8_append
 
 no_gpu = pytest.mark.skipif(torch.cuda.is_available(),
                             reason="placeholder-pointer checks run on CPU-only hosts")
@@ -112,3 +112,13 @@ def test_python_layer_refuses_host_memory():
 def test_no_cache_of_such_sizes(args):
     with pytest.raises(ValueError, match="no cache"):
         KV8Cache(*args, "cpu")
+
+
+def test_positions_that_are_no_whole_numbers_are_refused():
+    none = torch.zeros(1)
+    with pytest.raises(TypeError):
+        kv8_append(none, none, 3.0, none, none, none, none)
+    with pytest.raises(TypeError):
+        kv8_append(none, none, 3, none, none, none, none, capacity=64.5)
+    with pytest.raises(TypeError):
+        attn_decode_kv8(none, none, none, none, none, 2.5, none, None, none, none, None)

@@ -178,3 +178,10 @@ def test_module_forms():
     assert not part.rotary.whole_halves and part.rotary.tables("cpu")[0].shape == (32, 16)
     plain = FlexSelfAttention(128, 2, 32)
     assert plain.rotary.whole_halves and plain.rotary.form is None
+
+
+@pytest.mark.parametrize("change", [dict(pos=1.0), dict(num_heads=2.0), dict(num_kv_heads=1.5)])
+def test_numbers_that_are_not_whole_are_refused(change):
+    cs = torch.zeros(8, 16)
+    with pytest.raises(TypeError):
+        qkv_rotary(torch.zeros(1, 4, 192), cs, cs, **{"num_heads": 1, **change})
