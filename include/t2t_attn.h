@@ -385,7 +385,7 @@ int t2t_kv8_append(const t2t_tensor *k, const t2t_tensor *v, int32_t B, int32_t 
                    void *k_codes, void *v_codes, float *k_scale, float *v_scale, int64_t blocks,
                    int32_t capacity, void *stream);
 
-/* Workspace (bytes) of t2t_kv8_attend. */
+/* Workspace (bytes, 16-byte aligned) of t2t_kv8_attend. */
 int64_t t2t_kv8_attend_workspace(int32_t B, int32_t Hq, int32_t Hkv, int32_t Tq, int32_t Tkv,
                                  int32_t D);
 

@@ -36,7 +36,7 @@
 // windows and sinks alone, wherever in the cache they are -- and a work-group
 // takes every gridDim.x-th of them: 12 heads of 64, a window of 4096 behind
 // 32768 positions 8.7 + 4.1 us, where a work-group for every chunk of the cache
-// took 11.9 + 7.2.
+// took 11.9 + 7.2; a window of 512 7.0 + 2.5.
 #include "attn_kernels.h"
 
 namespace t2t {
@@ -45,6 +45,7 @@ namespace {
 
 constexpr int kDecThreads = 256;
 constexpr int kDecChunk = 256;  // keys per work-group
+constexpr int kDecHalf = 128;   // ... of a window, where its chunks are few (launch_both)
 
 struct DecodeArgs {
   TensorView q, k, v;  // q [B][Hq][Tq][D]; k, v [B][Hkv][cap][D]
@@ -59,6 +60,7 @@ struct DecodeArgs {
   float* part;               // [B][Hq][Tq][nch][D + 2]
   int window, sinks;         // window 0: none
   const int32_t* q_start;    // [Bm][Tq], or NULL without sinks
+  bool half;                 // with a window: chunks of kDecHalf keys, if they fit
 };
 
 // Sum over the GL = D/8 lanes of a key group (8 or 16 adjacent, aligned
@@ -77,12 +79,12 @@ __device__ __forceinline__ float group_sum(float x) {
 
 // RMAX: compile-time bound on the R query rows (1, 2, 4 or 8), so the common
 // single-row step holds 8 + 8 accumulators per lane rather than 64 + 64.
-template <int D, int RMAX, bool Win>
+template <int D, int RMAX, bool Win, int Chunk = kDecChunk>
 __device__ __forceinline__ void decode_chunk(const DecodeArgs& a, int chunk, int slot) {
   constexpr int GL = D / 8;                    // lanes per key
   constexpr int NKG = kDecThreads / GL;        // key groups per work-group
-  constexpr int KPG = kDecChunk / NKG;         // keys per group
-  __shared__ float sc[RMAX][kDecChunk];        // scores (log2 units)
+  constexpr int KPG = Chunk / NKG;             // keys per group
+  __shared__ float sc[RMAX][Chunk];            // scores (log2 units)
   __shared__ float red[kDecThreads / 64][RMAX][D];
   __shared__ float rmax[RMAX];
   __shared__ int32_t qpos_s[RMAX], qdoc_s[RMAX], qstart_s[RMAX];
@@ -94,7 +96,7 @@ __device__ __forceinline__ void decode_chunk(const DecodeArgs& a, int chunk, int
   const int G = a.Hq / a.Hkv;
   const int R = G * a.Tq;
   const int mb = a.Bm > 1 ? b : 0;
-  const int j0 = chunk * kDecChunk;
+  const int j0 = chunk * Chunk;
 
   const __bf16* kbase = static_cast<const __bf16*>(a.k.data) + b * a.k.sb + hk * a.k.sh + 8 * dg;
   const __bf16* vbase = static_cast<const __bf16*>(a.v.data) + b * a.v.sb + hk * a.v.sh + 8 * dg;
@@ -214,7 +216,7 @@ __device__ __forceinline__ void decode_chunk(const DecodeArgs& a, int chunk, int
   // Chunk row max: wave w reduces rows w, w + 4.
   for (int r = wave; r < R; r += kDecThreads / 64) {
     float m = -INFINITY;
-    for (int x = lane; x < kDecChunk; x += 64) m = fmaxf(m, sc[r][x]);
+    for (int x = lane; x < Chunk; x += 64) m = fmaxf(m, sc[r][x]);
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
     if (lane == 0) rmax[r] = m;
@@ -286,19 +288,40 @@ __device__ __forceinline__ void decode_chunk(const DecodeArgs& a, int chunk, int
 }
 
 // Chunks of the rows of sequence b (with a window).
-__device__ __forceinline__ PieceRange<kDecChunk> window_chunks(const DecodeArgs& a, int b) {
+template <int Chunk>
+__device__ __forceinline__ PieceRange<Chunk> window_chunks(const DecodeArgs& a, int b) {
   const size_t row = (size_t)(a.Bm > 1 ? b : 0) * a.Tq;
-  return PieceRange<kDecChunk>(a.q_pos + row, a.q_start ? a.q_start + row : nullptr, a.Tq, a.Tkv,
-                               a.W == 0 ? a.window : 0, a.sinks);
+  return PieceRange<Chunk>(a.q_pos + row, a.q_start ? a.q_start + row : nullptr, a.Tq, a.Tkv,
+                           a.W == 0 ? a.window : 0, a.sinks);
 }
 
-template <int D, int RMAX, bool Win>
+// How many of kDecHalf keys; -1: chunks of kDecChunk (the workspace has a slot for
+// each of the cache's, which rows far apart can pass in halves).
+__device__ __forceinline__ int half_chunks(const DecodeArgs& a, int b) {
+  if (!a.half) return -1;
+  const int n = window_chunks<kDecHalf>(a, b).count;
+  return n <= a.nch ? n : -1;
+}
+
+// Half: a.half, whose chunks the kernel has too.
+template <int D, int RMAX, bool Win, bool Half>
 __global__ __launch_bounds__(kDecThreads) void attn_decode_partial(DecodeArgs a) {
   if constexpr (Win) {
-    const PieceRange<kDecChunk> range = window_chunks(a, blockIdx.z);
+    if constexpr (Half) {
+      const int n = half_chunks(a, blockIdx.z);
+      if (n >= 0) {
+        const auto half = window_chunks<kDecHalf>(a, blockIdx.z);
+        for (int i = blockIdx.x; i < n; i += gridDim.x) {
+          decode_chunk<D, RMAX, Win, kDecHalf>(a, half.at(i), i);
+          __syncthreads();  // (its LDS is the next one's)
+        }
+        return;
+      }
+    }
+    const auto range = window_chunks<kDecChunk>(a, blockIdx.z);
     for (int i = blockIdx.x; i < range.count; i += gridDim.x) {
       decode_chunk<D, RMAX, Win>(a, range.at(i), i);
-      __syncthreads();  // (its LDS is the next one's)
+      __syncthreads();
     }
   } else {
     decode_chunk<D, RMAX, Win>(a, blockIdx.x, blockIdx.x);
@@ -308,7 +331,9 @@ __global__ __launch_bounds__(kDecThreads) void attn_decode_partial(DecodeArgs a)
 // One wave per (new token, query head, batch row).  The chunk maxima load one
 // chunk per lane; the weighted sum over chunks then issues its loads
 // independently (eight in flight per lane), so the merge costs a few memory
-// latencies whatever the chunk count.
+// latencies whatever the chunk count.  With a window, whose chunks are few, the
+// first kAhead values go out with the maxima, which they do not wait for (0.3 to
+// 1 us of a call; none, or a loss of as much, at the 64 chunks of a 16k cache).
 template <int D, bool Win>
 __global__ __launch_bounds__(64) void attn_decode_combine(DecodeArgs a, TensorView o,
                                                           float* lse2) {
@@ -318,7 +343,18 @@ __global__ __launch_bounds__(64) void attn_decode_combine(DecodeArgs a, TensorVi
   const int tq = blockIdx.x, h = blockIdx.y, b = blockIdx.z, lane = threadIdx.x;
   const size_t row = ((size_t)b * a.Hq + h) * a.Tq + tq;
   const float* pr = a.part + row * a.nch * S;
-  const int chunks = Win ? window_chunks(a, b).count : a.nch;
+  int chunks = a.nch;
+  if constexpr (Win) {
+    chunks = half_chunks(a, b);
+    if (chunks < 0) chunks = window_chunks<kDecChunk>(a, b).count;
+  }
+  constexpr int kAhead = Win ? 32 / PER : 0;
+  float ahead[kAhead + 1][PER];
+#pragma unroll
+  for (int k = 0; k < kAhead; ++k)
+#pragma unroll
+    for (int e = 0; e < PER; ++e)
+      ahead[k][e] = k < chunks ? pr[(size_t)k * S + 2 + lane + 64 * e] : 0.f;
   float M = -INFINITY;
   for (int c = lane; c < chunks; c += 64) M = fmaxf(M, pr[(size_t)c * S]);
 #pragma unroll
@@ -338,8 +374,18 @@ __global__ __launch_bounds__(64) void attn_decode_combine(DecodeArgs a, TensorVi
       wsh[lane] = w;
       __syncthreads();
       const int n = min(64, chunks - base);
+      int k = 0;
+      if (base == 0) {
+#pragma unroll
+        for (; k < kAhead; ++k)
+          if (k < n) {
+            const float wk = wsh[k];
+#pragma unroll
+            for (int e = 0; e < PER; ++e) acc[e] = fmaf(wk, ahead[k][e], acc[e]);
+          }
+      }
 #pragma unroll 8
-      for (int k = 0; k < n; ++k) {
+      for (; k < n; ++k) {
         const float wk = wsh[k];
 #pragma unroll
         for (int e = 0; e < PER; ++e)
@@ -357,36 +403,46 @@ __global__ __launch_bounds__(64) void attn_decode_combine(DecodeArgs a, TensorVi
   if (lane == 0) lse2[row] = L > 0.f ? M + log2f(L) : -INFINITY;
 }
 
-template <int D, bool Win>
+template <int D, bool Win, bool Half>
 void launch_partial(int R, dim3 grid, const DecodeArgs& a, hipStream_t stream) {
   if (R <= 1)
-    hipLaunchKernelGGL((attn_decode_partial<D, 1, Win>), grid, dim3(kDecThreads), 0, stream, a);
+    hipLaunchKernelGGL((attn_decode_partial<D, 1, Win, Half>), grid, dim3(kDecThreads), 0, stream, a);
   else if (R <= 2)
-    hipLaunchKernelGGL((attn_decode_partial<D, 2, Win>), grid, dim3(kDecThreads), 0, stream, a);
+    hipLaunchKernelGGL((attn_decode_partial<D, 2, Win, Half>), grid, dim3(kDecThreads), 0, stream, a);
   else if (R <= 4)
-    hipLaunchKernelGGL((attn_decode_partial<D, 4, Win>), grid, dim3(kDecThreads), 0, stream, a);
+    hipLaunchKernelGGL((attn_decode_partial<D, 4, Win, Half>), grid, dim3(kDecThreads), 0, stream, a);
   else
-    hipLaunchKernelGGL((attn_decode_partial<D, 8, Win>), grid, dim3(kDecThreads), 0, stream, a);
+    hipLaunchKernelGGL((attn_decode_partial<D, 8, Win, Half>), grid, dim3(kDecThreads), 0, stream, a);
 }
 
 template <int D>
-void launch_both(int R, const DecodeArgs& a, const TensorView& o, float* lse2,
+void launch_both(int R, DecodeArgs& a, const TensorView& o, float* lse2,
                  hipStream_t stream) {
   const dim3 pgrid((unsigned)a.nch, (unsigned)a.Hkv, (unsigned)a.B);
   const dim3 cgrid((unsigned)a.Tq, (unsigned)a.Hq, (unsigned)a.B);
   if (a.window > 0) {
     // a work-group for each chunk that rows next to one another read, which a
     // window or sinks may begin and end inside
-    int64_t n = a.nch;
-    if (a.W == 0) {
-      n = ((int64_t)a.window + a.Tq + kDecChunk - 2) / kDecChunk + 1;
-      if (a.sinks > 0) n += ((int64_t)a.sinks + kDecChunk - 2) / kDecChunk + 1;
-    }
-    launch_partial<D, true>(R, dim3((unsigned)(n < a.nch ? n : a.nch), pgrid.y, pgrid.z), a,
-                            stream);
+    const auto touched = [&](int chunk) -> int64_t {
+      if (a.W > 0) return a.nch;
+      int64_t n = ((int64_t)a.window + a.Tq + chunk - 2) / chunk + 1;
+      if (a.sinks > 0) n += ((int64_t)a.sinks + chunk - 2) / chunk + 1;
+      return n;
+    };
+    // Halves of chunks where whole ones leave a quarter of the CUs without a
+    // work-group: the time is then one's chain of loads and products; with more,
+    // the halves' sums cost what they save.  us, chunks of 256 / 128 keys: 12
+    // heads of 64, windows of 512 (36 work-groups) 10.9 / 9.6, 4096 (216) 12.2 /
+    // 12.5, 16000 (768) 21.6 / 25.4; 32 / 8 heads of 128 (24, 144, 512) 24.2 /
+    // 18.0, 25.5 / 21.2, 50.9 / 51.4.
+    a.half = a.W == 0 && touched(kDecChunk) * a.Hkv * a.B <= 192;
+    const int64_t n = touched(a.half ? kDecHalf : kDecChunk);
+    const dim3 grid((unsigned)(n < a.nch ? n : a.nch), pgrid.y, pgrid.z);
+    a.half ? launch_partial<D, true, true>(R, grid, a, stream)
+           : launch_partial<D, true, false>(R, grid, a, stream);
     hipLaunchKernelGGL((attn_decode_combine<D, true>), cgrid, dim3(64), 0, stream, a, o, lse2);
   } else {
-    launch_partial<D, false>(R, pgrid, a, stream);
+    launch_partial<D, false, false>(R, pgrid, a, stream);
     hipLaunchKernelGGL((attn_decode_combine<D, false>), cgrid, dim3(64), 0, stream, a, o, lse2);
   }
 }
@@ -408,7 +464,7 @@ hipError_t launch_attn_decode(const TensorView& q, const TensorView& k, const Te
   DecodeArgs a{q,     k,      v,    key_doc, key_bits, key_stride, q_pos, q_doc,
                q_bits, Bm,    W,    B,       Hq,       Hkv,        Tq,    Tkv,
                (Tkv + kDecChunk - 1) / kDecChunk, scale * kLog2e, workspace,
-               window, sinks, q_start};
+               window, sinks, q_start, false};
   if (a.nch == 0) a.nch = 1;  // no keys: one chunk that finds nothing
   const int R = (Hq / Hkv) * Tq;
   if (D == 64)

@@ -741,9 +741,10 @@ int t2t_kv8_attend(const t2t_tensor* q, const void* k_codes, const void* v_codes
   if (!lse2 || !key_doc || !q_pos || !q_doc || (words > 0 && (!key_bits || !q_bits)))
     return fail(T2T_EINVAL, "NULL pointer argument");
   const int64_t need = t2t_kv8_attend_workspace(B, Hq, Hkv, Tq, Tkv, D);
-  if (need > 0 && (!workspace || workspace_bytes < need))
-    return fail(T2T_EINVAL, "workspace of %lld bytes, %lld needed", (long long)workspace_bytes,
-                (long long)need);
+  if (need > 0 && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16 ||
+                   workspace_bytes < need))
+    return fail(T2T_EINVAL, "workspace of %lld bytes (16-byte aligned), %lld needed",
+                (long long)workspace_bytes, (long long)need);
   t2t::Kv8AttendArgs a{};
   a.q = as_view(q); a.o = as_view(o); a.lse2 = lse2;
   a.k_codes = static_cast<const uint8_t*>(k_codes);

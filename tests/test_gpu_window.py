@@ -631,3 +631,25 @@ def test_training_on_other_streams_and_threads():
     [t.start() for t in threads]
     [t.join() for t in threads]
     assert not bad
+
+
+@pytest.mark.parametrize("window,sinks", [(40, 0), (300, 130)])
+@pytest.mark.parametrize("D", [64, 128])
+def test_decode_rows_far_apart(D, window, sinks):
+    """Rows whose windows lie apart read a hull of more pieces than rows next to
+    one another: up to the whole cache, in whole and in half chunks."""
+    cap, M = 5000, 4
+    g = torch.Generator().manual_seed(window)
+    k, v = (torch.randn(2, 2, cap, D, generator=g).to(BF).to(DEV) for _ in range(2))
+    q = torch.randn(2, 2, M, D, generator=g).to(BF).to(DEV)
+    doc = torch.zeros(2, cap, dtype=torch.int32, device=DEV)
+    at = torch.arange(cap, device=DEV)
+    for row in ([0, 1, 2, 3], [0, 1700, 3333, 4999], [4999, 20, 4000, 4100], [2550, 2600, 4999, 5200]):
+        pos = torch.tensor([row, row[::-1]], dtype=torch.int32, device=DEV)
+        start = torch.clamp(pos - 900, min=0)
+        far = pos[..., None].long() - at
+        since = at - start[..., None].long()
+        ok = (far >= 0) & ((far < window) | ((since >= 0) & (since < sinks)))
+        o, lse2 = attn_decode(q, k, v, cap, doc, None, pos, torch.zeros_like(pos), None,
+                              window=window, sinks=sinks, q_start=start if sinks else None)
+        check_rows(o, lse2, q, k, v, ok, 0.0)

@@ -73,6 +73,7 @@ def _attend(**kw):
     (dict(kc=ODD), -1, "codes"), (dict(vc=P), -1, "are one"), (dict(lse2=None), -1, "NULL"),
     (dict(key_doc=None), -1, "NULL"), (dict(words=1), -1, "NULL"),
     (dict(ws=None), -1, "workspace"), (dict(ws_bytes=8), -1, "workspace"),
+    (dict(ws=ODD), -1, "16-byte"),
     (dict(B=70000, Bm=1), -2, "one launch"),
 ])
 def test_attend_entry_refuses(kw, rc, text):
