@@ -583,14 +583,14 @@ __device__ __forceinline__ float fine_entry(const bf16x8& x, int j) {
 //   dS waves: dP           | P <- LDS, dS, dK
 // with a barrier at the bar (P written to LDS as the bf16 MFMA operand it
 // already is; Fine: in 9 mantissa bits, pack_fine, since a rounding of P to 7
-// in dS is as large as that of dS itself) and one at the end.  The halves of a phase overlap across the
-// two waves of a SIMD (the P wave's exponentials with the dS wave's dP
-// chain, the dS wave's dS with the P wave's dV).  Q, dO, LSE and Delta (in
-// accumulator-row order) and the column bitmap words travel by direct
-// global->LDS copies into three buffers, issued two phases ahead into the
-// buffer freed at the start of the phase, so every copy has a whole phase
-// to land in; the end barrier waits only for the copies older than the
-// phase's own.
+// in dS is as large as that of dS itself) and one at the end.  The halves of a
+// phase overlap across the two waves of a SIMD (the P wave's exponentials with
+// the dS wave's dP chain, the dS wave's dS with the P wave's dV).  Q, dO, LSE
+// and Delta (in accumulator-row order) and the column bitmap words travel by
+// direct global->LDS copies into three buffers, issued two phases ahead into
+// the buffer freed at the start of the phase, so every copy has a whole phase
+// to land in; the end barrier waits only for the copies older than the phase's
+// own.
 template <int D, bool Fine>
 __global__ __launch_bounds__(kPairWaves * 64) __attribute__((amdgpu_waves_per_eu(4, 4)))
 void bwd_dkdv_pair_kernel(BwdParams p) {
@@ -1284,9 +1284,11 @@ hipError_t launch_attn_bwd_phase(int phase, const TensorView& q, const TensorVie
     else hipLaunchKernelGGL((bwd_dkdv_kernel<128, false>), grid, dim3(kDkdvThreads), 0, stream, p);
 #else
     if (d64 && phase == kBwdDkDvFine)
-      hipLaunchKernelGGL((bwd_dkdv_pair_kernel<64, true>), grid, dim3(kPairWaves * 64), 0, stream, p);
+      hipLaunchKernelGGL((bwd_dkdv_pair_kernel<64, true>), grid, dim3(kPairWaves * 64), 0, stream,
+                         p);
     else if (d64)
-      hipLaunchKernelGGL((bwd_dkdv_pair_kernel<64, false>), grid, dim3(kPairWaves * 64), 0, stream, p);
+      hipLaunchKernelGGL((bwd_dkdv_pair_kernel<64, false>), grid, dim3(kPairWaves * 64), 0, stream,
+                         p);
     else hipLaunchKernelGGL((bwd_dkdv_kernel<128, false>), grid, dim3(kDkdvThreads), 0, stream, p);
 #endif
   } else {  // kBwdDq, kBwdDqDelta

@@ -35,8 +35,8 @@
 // chunks are then those of the rows' PieceRange -- without grant words their
 // windows and sinks alone, wherever in the cache they are -- and a work-group
 // takes every gridDim.x-th of them: 12 heads of 64, a window of 4096 behind
-// 32768 positions 8.7 + 4.1 us, where a work-group for every chunk of the cache
-// took 11.9 + 7.2; a window of 512 7.0 + 2.5.
+// 32768 positions 8.8 + 3.6 us, where a work-group for every chunk of the cache
+// took 11.9 + 7.2.
 #include "attn_kernels.h"
 
 namespace t2t {
@@ -406,13 +406,17 @@ __global__ __launch_bounds__(64) void attn_decode_combine(DecodeArgs a, TensorVi
 template <int D, bool Win, bool Half>
 void launch_partial(int R, dim3 grid, const DecodeArgs& a, hipStream_t stream) {
   if (R <= 1)
-    hipLaunchKernelGGL((attn_decode_partial<D, 1, Win, Half>), grid, dim3(kDecThreads), 0, stream, a);
+    hipLaunchKernelGGL((attn_decode_partial<D, 1, Win, Half>), grid, dim3(kDecThreads), 0,
+                       stream, a);
   else if (R <= 2)
-    hipLaunchKernelGGL((attn_decode_partial<D, 2, Win, Half>), grid, dim3(kDecThreads), 0, stream, a);
+    hipLaunchKernelGGL((attn_decode_partial<D, 2, Win, Half>), grid, dim3(kDecThreads), 0,
+                       stream, a);
   else if (R <= 4)
-    hipLaunchKernelGGL((attn_decode_partial<D, 4, Win, Half>), grid, dim3(kDecThreads), 0, stream, a);
+    hipLaunchKernelGGL((attn_decode_partial<D, 4, Win, Half>), grid, dim3(kDecThreads), 0,
+                       stream, a);
   else
-    hipLaunchKernelGGL((attn_decode_partial<D, 8, Win, Half>), grid, dim3(kDecThreads), 0, stream, a);
+    hipLaunchKernelGGL((attn_decode_partial<D, 8, Win, Half>), grid, dim3(kDecThreads), 0,
+                       stream, a);
 }
 
 template <int D>

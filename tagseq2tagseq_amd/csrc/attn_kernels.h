@@ -106,10 +106,10 @@ hipError_t launch_attn_bwd_dkdv_split(const TensorView& q, const TensorView& k,
 // delta, dq; with Delta o, and o_rest if not empty).
 hipError_t launch_attn_bwd_phase(int phase, const TensorView& q, const TensorView& k,
                                  const TensorView& v, const TensorView& o,
-                                 const TensorView& o_rest, const TensorView& dout, const float* lse2, float* delta,
-                                 const TensorView& dq, const TensorView& dk, const TensorView& dv,
-                                 const AttnDims& dims, const MaskTables& mask,
-                                 hipStream_t stream);
+                                 const TensorView& o_rest, const TensorView& dout,
+                                 const float* lse2, float* delta, const TensorView& dq,
+                                 const TensorView& dk, const TensorView& dv, const AttnDims& dims,
+                                 const MaskTables& mask, hipStream_t stream);
 
 // Attention-module prologue: qkv [B][T][3][H][D] rows (strides sb, st) to
 // rotated q, k and plain v views, and the transposed map for the gradients.

@@ -364,10 +364,11 @@ namespace {
 // The backward; uneven: with the workspace that long columns are shared over,
 // finer in dS.  o_rest: NULL, or t2t_attn_fwd_rest's.
 int attn_bwd(const t2t_tensor* q, const t2t_tensor* k, const t2t_tensor* v, const t2t_tensor* o,
-             const t2t_tensor* o_rest, const t2t_tensor* dout, const float* lse2, float* delta, const t2t_tensor* dq,
-             const t2t_tensor* dk, const t2t_tensor* dv, int32_t B, int32_t Hq, int32_t Hkv,
-             int32_t T, int32_t D, int32_t dtype, float scale, const t2t_block_mask* mask,
-             bool uneven, void* workspace, int64_t workspace_bytes, void* stream) {
+             const t2t_tensor* o_rest, const t2t_tensor* dout, const float* lse2, float* delta,
+             const t2t_tensor* dq, const t2t_tensor* dk, const t2t_tensor* dv, int32_t B,
+             int32_t Hq, int32_t Hkv, int32_t T, int32_t D, int32_t dtype, float scale,
+             const t2t_block_mask* mask, bool uneven, void* workspace, int64_t workspace_bytes,
+             void* stream) {
   // Validate every argument before launching anything.
   int rc = check_dims(B, Hq, Hkv, T, D, dtype, true);
   if (rc) return rc;
@@ -400,8 +401,8 @@ int attn_bwd(const t2t_tensor* q, const t2t_tensor* k, const t2t_tensor* v, cons
   rc = hip_status(t2t::launch_attn_bwd_phase(t2t::kBwdDqDelta, as_view(q), as_view(k),
                                              as_view(v), as_view(o),
                                              o_rest ? as_view(o_rest) : t2t::TensorView{},
-                                             as_view(dout), lse2, delta, as_view(dq), t2t::TensorView{nullptr, 0, 0, 0},
-                                             t2t::TensorView{nullptr, 0, 0, 0}, dims,
+                                             as_view(dout), lse2, delta, as_view(dq),
+                                             t2t::TensorView{}, t2t::TensorView{}, dims,
                                              as_tables(mask), static_cast<hipStream_t>(stream)),
                   "t2t_attn_bwd dQ launch");
   if (rc) return rc;
