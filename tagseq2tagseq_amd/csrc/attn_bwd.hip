@@ -1162,7 +1162,11 @@ __global__ __launch_bounds__(kThreads, 2) void bwd_dq_kernel(BwdParams p) {
       const float pv = fast_exp2(fmaf(sacc[i], c, neg_lse));
       dpacc[i] = pv * dpacc[i];  // dS^T
     }
-    // dQ^T += K^T dS^T (contraction over the 32 keys of the block).
+    // dQ^T += K^T dS^T (contraction over the 32 keys of the block).  dS is
+    // rounded to bf16 once, as everywhere here: as two bf16 numbers the gradients
+    // are 1.7e-3 off their 64-bit values instead of 2.4e-3 (their own rounding
+    // alone is 1.7e-3), for 84 to 105 us here and 123 to 163 in dK/dV (16384
+    // tokens, 12 heads of 64, window 1024).
     __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int h2 = 0; h2 < 2; ++h2) {
