@@ -1,6 +1,7 @@
 // Argument blocks and launchers for the masked-attention kernels.
 #pragma once
 
+#include "piece_range.h"
 #include "t2t_common.h"
 
 namespace t2t {
@@ -269,46 +270,6 @@ hipError_t launch_attn_decode(const TensorView& q, const TensorView& k, const Te
                               int B, int Hq, int Hkv, int Tq, int Tkv, int D, float scale,
                               int window, int sinks, const int32_t* q_start,
                               float* workspace, hipStream_t stream);
-
-// Which pieces of a cache (kPiece positions each) the new rows of one sequence
-// read: their causal range, or with a window and no grant words the hull of
-// their windows and, before it, the hull of their sinks.  Piece i < count is
-// piece at(i) of the cache.
-template <int kPiece>
-struct PieceRange {
-  int sink0 = 0, sinks = 0, near0 = 0, count = 0;
-
-  // rows tokens at q_pos, documents from q_start (NULL: no sinks); window 0:
-  // none, or whole it has no effect
-  __device__ PieceRange(const int32_t* q_pos, const int32_t* q_start, int rows, int keys,
-                        int window, int n_sinks) {
-    int near_lo = 0x7fffffff, near_hi = -1, sink_lo = 0x7fffffff, sink_hi = -1;
-    for (int t = 0; t < rows; ++t) {
-      const int p = q_pos[t], last = min(p, keys - 1);
-      if (last < 0) continue;
-      const int64_t lo = window > 0 ? max((int64_t)p - window + 1, (int64_t)0) : 0;
-      if (lo <= last) {
-        near_lo = min(near_lo, (int)lo / kPiece);
-        near_hi = max(near_hi, last / kPiece);
-      }
-      if (q_start) {
-        const int64_t s = q_start[t], e = min(s + n_sinks - 1, (int64_t)last);
-        if (e >= 0 && s <= e) {
-          sink_lo = min(sink_lo, (int)max(s, (int64_t)0) / kPiece);
-          sink_hi = max(sink_hi, (int)e / kPiece);
-        }
-      }
-    }
-    // (sinks that the windows' hull holds are read there; none lie behind it)
-    sink_hi = min(sink_hi, near_hi < 0 ? sink_hi : near_lo - 1);
-    sink0 = sink_lo;
-    sinks = max(0, sink_hi - sink_lo + 1);
-    if (sink_hi < 0) sinks = 0;
-    near0 = near_lo;
-    count = sinks + (near_hi < 0 ? 0 : near_hi - near_lo + 1);
-  }
-  __device__ int at(int i) const { return i < sinks ? sink0 + i : near0 + i - sinks; }
-};
 
 // 8-bit key/value cache: codes [B][Hkv][blocks] of keys [64][D] and values
 // [D][64], scales [B][Hkv][blocks].

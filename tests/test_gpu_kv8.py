@@ -15,7 +15,8 @@ from tagseq2tagseq_amd.mask_creators import make_mask_creator_callable
 from tagseq2tagseq_amd.model import TS2TSModel
 from tagseq2tagseq_amd.rope import RotaryForm
 from tests.helpers import random_row, to_dev_words
-from tests.test_gpu_window import _dense, _spans, _starts, check_rows, logits_agree
+from tests.test_gpu_window import (PAST_THE_CACHE, _dense, _spans, _starts, check_rows,
+                                   logits_agree)
 
 pytestmark = pytest.mark.gpu
 
@@ -587,3 +588,23 @@ def test_an_edited_context_is_recomputed():
     for T in (397, 398):
         got = m.forward_inference_last(tokens[:, :T], _spans(T)).float()
         logits_agree(got, _cached_rows_ref(m, tokens, _spans(T), T), f"T={T}")
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("window,sinks", [(40, 4), (4, 4), (300, 130)])
+def test_rows_past_the_cache_keep_their_sinks(D, window, sinks):
+    cap = 5000
+    g = torch.Generator().manual_seed(window)
+    cache = KV8Cache(1, 2, cap, D, DEV)
+    cache.append(*_rows(1, 2, cap, D, BF, g, 0.25), 0)
+    k, v = cache.values(F32)
+    q = (0.5 * torch.randn(1, 2, 2, D, generator=g)).to(BF).to(DEV)
+    doc = torch.zeros(1, cap, dtype=torch.int32, device=DEV)
+    at = torch.arange(cap, device=DEV)
+    for rows in PAST_THE_CACHE:
+        pos, start = (torch.tensor([x], dtype=torch.int32, device=DEV) for x in zip(*rows))
+        far, since = (x[..., None].long() - at for x in (pos, start))
+        ok = (far >= 0) & ((far < window) | ((since <= 0) & (-since < sinks)))
+        o, lse2 = cache.attend(q, cap, doc, None, pos, torch.zeros_like(pos), None,
+                               window=window, sinks=sinks, q_start=start)
+        check_rows(o, lse2, q, k, v, ok, 2.0 ** -16)  # (p in two bf16 numbers)

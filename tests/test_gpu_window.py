@@ -653,3 +653,27 @@ def test_decode_rows_far_apart(D, window, sinks):
         o, lse2 = attn_decode(q, k, v, cap, doc, None, pos, torch.zeros_like(pos), None,
                               window=window, sinks=sinks, q_start=start if sinks else None)
         check_rows(o, lse2, q, k, v, ok, 0.0)
+
+
+# (position, document's start) of rows whose windows hold no key of the cache, and
+# whose sinks lie behind the other rows' windows
+PAST_THE_CACHE = [[(100, 0), (5200, 4300)], [(10, 0), (10000, 4000)], [(9000, 2000), (2, 0)]]
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("window,sinks", [(40, 4), (4, 4), (300, 130)])
+def test_decode_rows_past_the_cache_keep_their_sinks(D, window, sinks):
+    cap = 5000
+    g = torch.Generator().manual_seed(window)
+    k, v = (torch.randn(1, 2, cap, D, generator=g).to(BF).to(DEV) for _ in range(2))
+    q = torch.randn(1, 2, 2, D, generator=g).to(BF).to(DEV)
+    doc = torch.zeros(1, cap, dtype=torch.int32, device=DEV)
+    at = torch.arange(cap, device=DEV)
+    for rows in PAST_THE_CACHE:
+        pos, start = (torch.tensor([x], dtype=torch.int32, device=DEV) for x in zip(*rows))
+        far, since = (x[..., None].long() - at for x in (pos, start))
+        ok = (far >= 0) & ((far < window) | ((since <= 0) & (-since < sinks)))
+        assert bool(ok.any(-1).all())
+        o, lse2 = attn_decode(q, k, v, cap, doc, None, pos, torch.zeros_like(pos), None,
+                              window=window, sinks=sinks, q_start=start)
+        check_rows(o, lse2, q, k, v, ok, 0.0)
