@@ -39,7 +39,7 @@ from __future__ import annotations
 import math
 from dataclasses import dataclass
 from operator import index
-from typing import Dict, Optional, Tuple, Union
+from typing import Callable, Dict, Optional, Tuple, Union
 
 import torch
 from torch.autograd import forward_ad
@@ -50,16 +50,32 @@ from . import _lib
 _TABLES: Dict[Tuple, Tuple[torch.Tensor, torch.Tensor]] = {}
 
 
+def _tables(key: Tuple, make: Callable[[], Tuple[torch.Tensor, torch.Tensor]]):
+    """The tables of ``key``, made once.  What is kept serves every later call, so
+    nothing of the mode that the first one runs under may stay in it: made
+    outside of inference mode (a backward cannot save inference tensors), and
+    kept only if they hold memory of their own (not fake tensors, nor those of a
+    function transform)."""
+    if key in _TABLES:
+        return _TABLES[key]
+    with torch.inference_mode(False):
+        pair = make()
+    if all(type(t) is torch.Tensor
+           and (torch.compiler.is_dynamo_compiling()
+                or not torch._C._functorch.is_functorch_wrapped_tensor(t)) for t in pair):
+        _TABLES[key] = pair
+    return pair
+
+
 def rope_tables(head_dim: int, rows: int, device, base: float = 10000.0):
     """(cos, sin) float32 [rows, head_dim / 2]: angle[p][i] = p * base^(-i / (D/2)).
     Cached per (head_dim, rows, base, device)."""
-    key = (head_dim, rows, float(base), str(torch.device(device)))
-    if key not in _TABLES:
+    def make():
         half = head_dim // 2
         inv = base ** (-torch.arange(0, half, dtype=torch.float32) / half)
         ang = torch.outer(torch.arange(rows, dtype=torch.float32), inv)
-        _TABLES[key] = (ang.cos().to(device), ang.sin().to(device))
-    return _TABLES[key]
+        return ang.cos().to(device), ang.sin().to(device)
+    return _tables((head_dim, rows, float(base), str(torch.device(device))), make)
 
 
 SCALINGS = ("linear", "base", "by_parts")
@@ -123,10 +139,11 @@ def rotary_tables(rotary_dim: int, rows: int, device, base: float = 10000.0,
         raise ValueError(f"magnitude={magnitude!r} must be finite")
     key = ("rotary", rotary_dim, rows, float(base), scaling, float(factor), original_len,
            float(fast), float(slow), float(magnitude), str(torch.device(device)))
-    if key not in _TABLES:
+
+    def make():
         ang = _rotary_angles(rotary_dim, rows, base, scaling, factor, original_len, fast, slow)
-        _TABLES[key] = tuple((f * magnitude).float().to(device) for f in (ang.cos(), ang.sin()))
-    return _TABLES[key]
+        return tuple((f * magnitude).float().to(device) for f in (ang.cos(), ang.sin()))
+    return _tables(key, make)
 
 
 @dataclass(frozen=True)

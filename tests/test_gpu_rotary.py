@@ -10,7 +10,8 @@ import torch
 from torch.fx.experimental.proxy_tensor import make_fx
 
 from tagseq2tagseq_amd import rope
-from tagseq2tagseq_amd.rope import qkv_rope, qkv_rotary, rope_tables, rotary_tables
+from tagseq2tagseq_amd.attention import FlexSelfAttention
+from tagseq2tagseq_amd.rope import RotaryForm, qkv_rope, qkv_rotary, rope_tables, rotary_tables
 
 pytestmark = pytest.mark.gpu
 
@@ -282,3 +283,24 @@ def test_positions_changed_before_the_backward_are_noticed():
     pos.add_(1)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         torch.autograd.grad(out, qkv, grads)
+
+
+@pytest.mark.parametrize("form", [
+    None, RotaryForm(base=10001.0), RotaryForm(fraction=0.5, interleaved=True, base=10001.0)])
+def test_training_behind_an_evaluation_in_inference_mode(form):
+    """Tables made under inference mode serve the backward that saves them."""
+    T = 333  # (no other test's: the first call here makes them)
+    torch.manual_seed(0)
+    mod = FlexSelfAttention(128, 2, T, rotary=form).to(DEV, BF)
+    x = torch.randn(1, T, 384, device=DEV).to(BF)
+    with torch.inference_mode():
+        want = mod.heads(x)
+    x.requires_grad_(True)
+    out = mod.heads(x)
+    grads = [torch.randn_like(t) for t in out]
+    got, = torch.autograd.grad(out, x, grads)
+    assert all(torch.equal(a, b) for a, b in zip(out, want))
+    if form is not None:
+        cos, sin = mod.rotary.tables(DEV)
+        again = qkv_rotary(x, cos, sin, 2, interleaved=form.interleaved)
+        assert torch.equal(torch.autograd.grad(again, x, grads)[0], got)

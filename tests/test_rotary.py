@@ -185,3 +185,52 @@ def test_numbers_that_are_not_whole_are_refused(change):
     cs = torch.zeros(8, 16)
     with pytest.raises(TypeError):
         qkv_rotary(torch.zeros(1, 4, 192), cs, cs, **{"num_heads": 1, **change})
+
+
+# every test its own row count: the tables are kept by their arguments
+def _made_under(mode, rows):
+    with mode:
+        first = [*rope_tables(32, rows, "cpu"), *rotary_tables(32, rows, "cpu")]
+    return first, [*rope_tables(32, rows, "cpu"), *rotary_tables(32, rows, "cpu")]
+
+
+def test_tables_made_in_inference_mode_serve_training():
+    for t in _made_under(torch.inference_mode(), 101)[1]:
+        assert not t.is_inference()
+        x = torch.ones(101, 16, requires_grad=True)
+        (x * t).sum().backward()  # (saves the table)
+        assert torch.equal(x.grad, t)
+
+
+def test_tables_of_fake_tensors_are_not_kept():
+    from torch._subclasses.fake_tensor import FakeTensor, FakeTensorMode
+    first, later = _made_under(FakeTensorMode(), 102)
+    assert all(isinstance(t, FakeTensor) for t in first)
+    assert all(type(t) is torch.Tensor for t in later)
+
+
+def test_tables_of_a_function_transform_are_not_kept():
+    def f(x):
+        cos, sin = rotary_tables(32, 103, "cpu")
+        c2, s2 = rope_tables(32, 103, "cpu")
+        return (x * (cos + sin + c2 + s2)).sum()
+    torch.func.grad(f)(torch.ones(103, 16))
+    for t in (*rope_tables(32, 103, "cpu"), *rotary_tables(32, 103, "cpu")):
+        assert t.data_ptr() != 0 and float(t[0].abs().max()) in (0.0, 1.0)
+
+
+@pytest.mark.parametrize("tables", [rope_tables, rotary_tables])
+@pytest.mark.parametrize("inference", [False, True])
+def test_tables_made_while_compiling(tables, inference):
+    rows = 104 + inference
+
+    @torch.compile(backend="eager", fullgraph=True)
+    def f(x):
+        cos, sin = tables(32, rows, x.device)
+        return x * cos + sin
+    x = torch.ones(rows, 16)
+    with torch.inference_mode(inference):
+        got = f(x)
+    cos, sin = tables(32, rows, "cpu")
+    assert torch.equal(got, cos + sin) and not cos.is_inference()
+    assert tables(32, rows, "cpu")[0] is cos
