@@ -67,15 +67,25 @@ def _tables(key: Tuple, make: Callable[[], Tuple[torch.Tensor, torch.Tensor]]):
     return pair
 
 
+def _where(device) -> torch.device:
+    """The device of a call: "cuda" is the current one, which may change."""
+    device = torch.device(device)
+    if device.type == "cuda" and device.index is None:
+        return torch.device("cuda", torch.cuda.current_device())
+    return device
+
+
 def rope_tables(head_dim: int, rows: int, device, base: float = 10000.0):
     """(cos, sin) float32 [rows, head_dim / 2]: angle[p][i] = p * base^(-i / (D/2)).
     Cached per (head_dim, rows, base, device)."""
+    device = _where(device)
+
     def make():
         half = head_dim // 2
         inv = base ** (-torch.arange(0, half, dtype=torch.float32) / half)
         ang = torch.outer(torch.arange(rows, dtype=torch.float32), inv)
         return ang.cos().to(device), ang.sin().to(device)
-    return _tables((head_dim, rows, float(base), str(torch.device(device))), make)
+    return _tables((head_dim, rows, float(base), str(device)), make)
 
 
 SCALINGS = ("linear", "base", "by_parts")
@@ -137,8 +147,9 @@ def rotary_tables(rotary_dim: int, rows: int, device, base: float = 10000.0,
         magnitude = 1.0 + 0.1 * math.log(factor) if scaling == "by_parts" else 1.0
     if not math.isfinite(magnitude):
         raise ValueError(f"magnitude={magnitude!r} must be finite")
+    device = _where(device)
     key = ("rotary", rotary_dim, rows, float(base), scaling, float(factor), original_len,
-           float(fast), float(slow), float(magnitude), str(torch.device(device)))
+           float(fast), float(slow), float(magnitude), str(device))
 
     def make():
         ang = _rotary_angles(rotary_dim, rows, base, scaling, factor, original_len, fast, slow)

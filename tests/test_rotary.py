@@ -234,3 +234,19 @@ def test_tables_made_while_compiling(tables, inference):
     cos, sin = tables(32, rows, "cpu")
     assert torch.equal(got, cos + sin) and not cos.is_inference()
     assert tables(32, rows, "cpu")[0] is cos
+
+
+@pytest.mark.parametrize("tables", [rope_tables, rotary_tables])
+def test_a_device_without_an_index_is_the_current_one(tables, monkeypatch):
+    """Kept by the device that the call means, not by its name."""
+    from tagseq2tagseq_amd import rope
+    now = [0]
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: now[0])
+    keys = []
+    monkeypatch.setattr(rope, "_tables", lambda key, make: keys.append(key))
+    tables(32, 106, "cuda")
+    now[0] = 1
+    tables(32, 106, "cuda")
+    tables(32, 106, torch.device("cuda", 1))
+    tables(32, 106, "cuda:0")
+    assert keys[0] != keys[1] == keys[2] and keys[0] == keys[3]
