@@ -5,8 +5,8 @@ autograd (the gradient is one pass too).
 Replaces the head split and rotary embedding inside the reference's attention
 module (tunalab ``FlexSelfAttention``, constructed and called at
 model/modules/layer.py:16-21,33; the package is not part of the reference, so
-the rotary variant -- half-split pairs, base 10000, position = token index --
-is the textbook form and its parity with tunalab is unpinned).
+the rotary variant -- half-split pairs turned by the negative angle, base 10000,
+position = token index -- and its parity with tunalab are unpinned).
 
     q, k, v = qkv_rope(qkv, cos, sin, num_heads)       # qkv: [B, T, 3 C]
     cos, sin = rope_tables(head_dim, rows, device)      # float32 [rows, D/2]
@@ -110,7 +110,8 @@ def _rotary_angles(rotary_dim: int, rows: int, base: float, scaling: Optional[st
 
 def rotary_tables(rotary_dim: int, rows: int, device, base: float = 10000.0,
                   scaling: Optional[str] = None, factor: float = 1.0, original_len: int = 0,
-                  fast: float = 32.0, slow: float = 1.0, magnitude: Optional[float] = None):
+                  fast: float = 32.0, slow: float = 1.0, magnitude: Optional[float] = None,
+                  positive: bool = False):
     """(cos, sin) float32 [rows, rotary_dim / 2], the angles p * base^(-2 i /
     rotary_dim) computed in float64 (a far position's angle keeps its fraction
     of a turn).  Cached per arguments.
@@ -124,7 +125,13 @@ def rotary_tables(rotary_dim: int, rows: int, device, base: float = 10000.0,
         times divided by factor, with a linear ramp over the turns between
         (the interpolation by parts of the YaRN paper).
     ``magnitude`` multiplies both tables; None is 1, or for "by_parts" the same
-    paper's 1 + 0.1 ln(factor), which sharpens the softmax as contexts grow."""
+    paper's 1 + 0.1 ln(factor), which sharpens the softmax as contexts grow.
+
+    ``positive``: for a rotation by the positive angle, (a cos - b sin, b cos +
+    a sin) of a pair (a, b), as the RoFormer paper and most published weights
+    have it; the kernels' own is the negative one, (a cos + b sin, b cos - a sin),
+    so that the sines come negated.  Weights serve the direction that they were
+    trained in only."""
     if rotary_dim < 2 or rotary_dim % 2 or rows < 0:
         raise ValueError(f"rotary_dim={rotary_dim} must be even and positive, rows={rows} not "
                          "negative")
@@ -149,25 +156,28 @@ def rotary_tables(rotary_dim: int, rows: int, device, base: float = 10000.0,
         raise ValueError(f"magnitude={magnitude!r} must be finite")
     device = _where(device)
     key = ("rotary", rotary_dim, rows, float(base), scaling, float(factor), original_len,
-           float(fast), float(slow), float(magnitude), str(device))
+           float(fast), float(slow), float(magnitude), bool(positive), str(device))
 
     def make():
         ang = _rotary_angles(rotary_dim, rows, base, scaling, factor, original_len, fast, slow)
-        return tuple((f * magnitude).float().to(device) for f in (ang.cos(), ang.sin()))
+        turn = -magnitude if positive else magnitude
+        return (ang.cos() * magnitude).float().to(device), (ang.sin() * turn).float().to(device)
     return _tables(key, make)
 
 
 @dataclass(frozen=True)
 class RotaryForm:
     """A module's form of the rotary embedding: the ``fraction`` of the head that
-    rotates (its first dimensions), the pairs' layout and the tables' base and
-    scaling (rotary_tables)."""
+    rotates (its first dimensions), the pairs' layout, and the tables' base,
+    scaling and direction (rotary_tables; ``positive`` for weights trained with
+    the published rotation)."""
     fraction: float = 1.0
     interleaved: bool = False
     base: float = 10000.0
     scaling: Optional[str] = None
     factor: float = 1.0
     original_len: int = 0
+    positive: bool = False
 
     def dims(self, head_dim: int) -> int:
         """Rotated dimensions of a head of head_dim."""
@@ -179,7 +189,7 @@ class RotaryForm:
 
     def tables(self, head_dim: int, rows: int, device):
         return rotary_tables(self.dims(head_dim), rows, device, self.base, self.scaling,
-                             self.factor, self.original_len)
+                             self.factor, self.original_len, positive=self.positive)
 
 
 def _split_dims(qkv: torch.Tensor, num_heads: int):
@@ -277,7 +287,8 @@ def qkv_rope_torch(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, num_
 def qkv_rope(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, num_heads: int,
              pos0: int = 0):
     """Split qkv [B, T, 3 C] into rotated q, k and v, each [B, H, T, D]
-    (contiguous), with positions pos0 .. pos0 + T - 1 (table rows).  bf16 runs
+    (contiguous), with positions pos0 .. pos0 + T - 1 (table rows); the pair
+    (a, b) = (x[i], x[i + D/2]) becomes (a cos + b sin, b cos - a sin).  bf16 runs
     the kernel; float32 (module not cast to bf16) the torch composition."""
     if qkv.dtype == torch.float32:
         return qkv_rope_torch(qkv, cos, sin, num_heads, pos0)
@@ -493,6 +504,8 @@ def qkv_rotary(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, num_head
     Hkv = H unless ``num_kv_heads`` is given) into q [B, H, T, D] and k, v
     [B, Hkv, T, D] (contiguous), the first R dimensions of every query and key
     head rotated by tables cos, sin float32 [rows, R / 2] and the others copied.
+    A pair (a, b) becomes (a cos + b sin, b cos - a sin), as in qkv_rope: it turns
+    by the tables' negative angle (rotary_tables' ``positive`` for the other way).
 
     ``interleaved``: pairs of neighbouring dimensions (x[2i], x[2i + 1]) instead
     of (x[i], x[i + R/2]).  ``pos``: the first token's position, or a device

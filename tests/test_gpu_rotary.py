@@ -304,3 +304,38 @@ def test_training_behind_an_evaluation_in_inference_mode(form):
         cos, sin = mod.rotary.tables(DEV)
         again = qkv_rotary(x, cos, sin, 2, interleaved=form.interleaved)
         assert torch.equal(torch.autograd.grad(again, x, grads)[0], got)
+
+
+@pytest.mark.parametrize("positive", [False, True])
+@pytest.mark.parametrize("interleaved,fraction", [(False, 1.0), (False, 0.5), (True, 1.0),
+                                                  (True, 0.25)])
+def test_modules_turn_either_way(positive, interleaved, fraction):
+    """The rotation by -angle, or by the published one's +angle: (a + i b) e^(i p w)
+    with angles of 64 bits, at a range of positions and at those of a tensor."""
+    T, D, H = 150, 64, 2
+    R = int(fraction * D)
+    form = RotaryForm(fraction=fraction, interleaved=interleaved, base=700.0, positive=positive)
+    mod = FlexSelfAttention(H * D, H, T, rotary=form).to(DEV, BF)
+    g = torch.Generator().manual_seed(R)
+    qkv = torch.randn(1, T, 3 * H * D, generator=g).to(BF).to(DEV)
+    rows = qkv.double().view(1, T, 3, H, D).permute(2, 0, 3, 1, 4)
+    w = 700.0 ** (-torch.arange(R // 2, dtype=torch.float64, device=DEV) * 2 / R)
+
+    def published(x, at):
+        r = x[..., :R]
+        a, b = (r[..., 0::2], r[..., 1::2]) if interleaved else r.chunk(2, -1)
+        ang = torch.outer(at.double(), w) * (1 if positive else -1)
+        z = torch.complex(a, b) * torch.polar(torch.ones_like(ang), ang)
+        turned = (torch.stack([z.real, z.imag], -1).flatten(-2) if interleaved else
+                  torch.cat([z.real, z.imag], -1))
+        return torch.cat([turned, x[..., R:]], -1)
+    order = torch.randperm(T, generator=g).to(DEV)
+    for pos, at in ((0, torch.arange(T, device=DEV)), (order, order)):
+        q, k, v = mod.heads(qkv, pos)
+        assert torch.equal(v.double(), rows[2])
+        for x, y in ((q, rows[0]), (k, rows[1])):
+            want = published(y, at)
+            # |a c| + |b s| <= sqrt(2) |(a, b)|; tables and arithmetic 3 roundings of
+            # U of that (whole halves at base 700: rope.rotary_tables' too)
+            size = y.abs().amax(-1, keepdim=True) * 2
+            assert bool(((x.double() - want).abs() <= 2.0 ** -8 * want.abs() + 4 * U * size).all())

@@ -250,3 +250,20 @@ def test_a_device_without_an_index_is_the_current_one(tables, monkeypatch):
     tables(32, 106, torch.device("cuda", 1))
     tables(32, 106, "cuda:0")
     assert keys[0] != keys[1] == keys[2] and keys[0] == keys[3]
+
+
+def test_the_tables_turn_either_way():
+    """A pair (a, b) becomes (a cos + b sin, b cos - a sin) of the tables: by the
+    negative angle, or with positive=True by the published rotation's."""
+    for kw in (dict(), dict(scaling="by_parts", factor=4.0, original_len=16)):
+        cos, sin = rotary_tables(32, 40, "cpu", **kw)
+        c2, s2 = rotary_tables(32, 40, "cpu", positive=True, **kw)
+        assert torch.equal(c2, cos) and torch.equal(s2, -sin)
+    form = RotaryForm(fraction=0.5, interleaved=True, base=500.0, positive=True)
+    cos, sin = form.tables(64, 9, "cpu")
+    want = rotary_tables(32, 9, "cpu", base=500.0, positive=True)
+    assert torch.equal(cos, want[0]) and torch.equal(sin, want[1])
+    i = torch.arange(16, dtype=torch.float64)
+    ang = torch.outer(torch.arange(9, dtype=torch.float64), 500.0 ** (-i / 16))
+    # published: (a cos - b sin, a sin + b cos), here with s = -sin
+    assert torch.allclose(sin.double(), -ang.sin(), atol=2 ** -24)
