@@ -169,8 +169,8 @@ def rotary_tables(rotary_dim: int, rows: int, device, base: float = 10000.0,
 class RotaryForm:
     """A module's form of the rotary embedding: the ``fraction`` of the head that
     rotates (its first dimensions), the pairs' layout, and the tables' base,
-    scaling and direction (rotary_tables; ``positive`` for weights trained with
-    the published rotation)."""
+    scaling, magnitude and direction (rotary_tables; ``positive`` for weights
+    trained with the published rotation)."""
     fraction: float = 1.0
     interleaved: bool = False
     base: float = 10000.0
@@ -178,6 +178,9 @@ class RotaryForm:
     factor: float = 1.0
     original_len: int = 0
     positive: bool = False
+    fast: float = 32.0
+    slow: float = 1.0
+    magnitude: Optional[float] = None
 
     def dims(self, head_dim: int) -> int:
         """Rotated dimensions of a head of head_dim."""
@@ -189,7 +192,8 @@ class RotaryForm:
 
     def tables(self, head_dim: int, rows: int, device):
         return rotary_tables(self.dims(head_dim), rows, device, self.base, self.scaling,
-                             self.factor, self.original_len, positive=self.positive)
+                             self.factor, self.original_len, self.fast, self.slow,
+                             self.magnitude, self.positive)
 
 
 def _split_dims(qkv: torch.Tensor, num_heads: int):

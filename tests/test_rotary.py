@@ -1,6 +1,7 @@
 """The prologue with any rotary form where no GPU is needed: refusals of the C
 entries and of the Python layer, the tables' scalings, and the modules' forms."""
 import ctypes
+import inspect
 import math
 
 import pytest
@@ -267,3 +268,13 @@ def test_the_tables_turn_either_way():
     ang = torch.outer(torch.arange(9, dtype=torch.float64), 500.0 ** (-i / 16))
     # published: (a cos - b sin, a sin + b cos), here with s = -sin
     assert torch.allclose(sin.double(), -ang.sin(), atol=2 ** -24)
+
+
+def test_a_form_hands_on_every_argument_of_the_tables():
+    kw = dict(scaling="by_parts", factor=4.0, original_len=64, fast=8.0, slow=2.0, magnitude=1.5,
+              base=300.0, positive=True)
+    for a, b in zip(RotaryForm(**kw).tables(64, 50, "cpu"), rotary_tables(64, 50, "cpu", **kw)):
+        assert torch.equal(a, b)
+    names = set(RotaryForm.__dataclass_fields__) - {"fraction", "interleaved"}
+    assert names == set(kw) == set(inspect.signature(rotary_tables).parameters) - {
+        "rotary_dim", "rows", "device"}
