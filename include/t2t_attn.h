@@ -191,7 +191,8 @@ int t2t_attn_fwd(const t2t_tensor *q, const t2t_tensor *k, const t2t_tensor *v,
 
 /*
  * t2t_attn_fwd (bf16) that also writes what rounding left of o, as bf16, into
- * o_rest: for t2t_attn_bwd_uneven, whose rowsum(O * dO) then has 16 bits of O.
+ * o_rest: for t2t_attn_bwd_rest and t2t_attn_bwd_uneven, whose rowsum(O * dO)
+ * then has 16 bits of O.
  */
 int t2t_attn_fwd_rest(const t2t_tensor *q, const t2t_tensor *k, const t2t_tensor *v,
                       const t2t_tensor *o, const t2t_tensor *o_rest, float *lse2, int32_t B,
@@ -216,17 +217,37 @@ int t2t_attn_bwd(const t2t_tensor *q, const t2t_tensor *k, const t2t_tensor *v,
                  int32_t D, int32_t dtype, float scale, const t2t_block_mask *mask,
                  void *stream);
 
-/* Workspace (bytes) of t2t_attn_bwd_uneven; 0 where it runs as t2t_attn_bwd. */
+/*
+ * t2t_attn_bwd for masks whose rows have few keys (a sliding window's), which
+ * feel the roundings most: with o_rest (bf16, or NULL) Delta is taken from o +
+ * o_rest, and dS from P of at least 9 bits.
+ */
+int t2t_attn_bwd_rest(const t2t_tensor *q, const t2t_tensor *k, const t2t_tensor *v,
+                      const t2t_tensor *o, const t2t_tensor *o_rest, const t2t_tensor *dout,
+                      const float *lse2, float *delta, const t2t_tensor *dq,
+                      const t2t_tensor *dk, const t2t_tensor *dv, int32_t B, int32_t Hq,
+                      int32_t Hkv, int32_t T, int32_t D, int32_t dtype, float scale,
+                      const t2t_block_mask *mask, void *stream);
+
+/*
+ * How many work-groups t2t_attn_bwd_uneven shares the longest column of such a
+ * call by; 1: t2t_attn_bwd_rest runs the same launches without a workspace.
+ */
+int32_t t2t_attn_bwd_uneven_pieces(int32_t B, int32_t Hq, int32_t Hkv, int32_t T, int32_t D,
+                                   int32_t dtype);
+
+/*
+ * Workspace (bytes) of t2t_attn_bwd_uneven, whatever the number of query heads;
+ * 0 where no column is shared.
+ */
 int64_t t2t_attn_bwd_uneven_workspace(int32_t B, int32_t Hkv, int32_t T, int32_t D,
                                       int32_t dtype);
 
 /*
- * t2t_attn_bwd for masks whose columns are uneven (a sliding window's, whose
- * sinks are read by whole documents): where there are few columns, the queries
- * of a long one are shared by several work-groups, whose fp32 sums of dK and
- * dV are added in a fixed order (deterministic, no atomics).  Rows of few keys,
- * which such masks have, feel the roundings most: with o_rest (bf16, or NULL)
- * Delta is taken from o + o_rest, and dS from P of at least 9 bits.
+ * t2t_attn_bwd_rest for masks whose columns are uneven too (a sliding window's,
+ * whose sinks are read by whole documents): where there are few columns, the
+ * queries of a long one are shared by several work-groups, whose fp32 sums of
+ * dK and dV are added in a fixed order (deterministic, no atomics).
  */
 int t2t_attn_bwd_uneven(const t2t_tensor *q, const t2t_tensor *k, const t2t_tensor *v,
                         const t2t_tensor *o, const t2t_tensor *o_rest, const t2t_tensor *dout,

@@ -67,6 +67,8 @@ _SIGS = {
     "t2t_attn_bwd": ([_P] * 10 + [_I32] * 6 + [ctypes.c_float, _P, _P], ctypes.c_int),
     "t2t_attn_bwd_uneven_workspace": ([_I32] * 5, ctypes.c_int64),
     "t2t_attn_fwd_rest": ([_P] * 6 + [_I32] * 6 + [ctypes.c_float, _P, _P], ctypes.c_int),
+    "t2t_attn_bwd_rest": ([_P] * 11 + [_I32] * 6 + [ctypes.c_float, _P, _P], ctypes.c_int),
+    "t2t_attn_bwd_uneven_pieces": ([_I32] * 6, ctypes.c_int32),
     "t2t_attn_bwd_uneven": ([_P] * 11 + [_I32] * 6 + [ctypes.c_float, _P, _P, _I64, _P],
                             ctypes.c_int),
     "t2t_clock_probe": ([_P, _I32, _P, _P], ctypes.c_int),

@@ -1306,14 +1306,16 @@ hipError_t launch_attn_bwd_phase(int phase, const TensorView& q, const TensorVie
 }
 
 // Work-groups that share a column: only where at most two columns fall on a CU
-// (with more, the launch's order, longest column first, evens them out), as many
-// as keep the sums within 256 MiB.  D = 128 (the columns of D = 64 are two work-
-// groups a CU already, and a quarter as long for the same keys).
-int bwd_uneven_splits(int B, int Hkv, int T, int D) {
-  const int64_t columns = (int64_t)B * Hkv * ((T + kTile - 1) / kTile);
+// (with more, the launch's order, longest column first, evens them out), whose
+// sums are 256 MiB at most; as many as the longest column that the call can have
+// is shared by, 1 where that is none.  D = 128 (the kernel of D = 64 has two
+// work-groups a CU, and no form that shares a column).
+int bwd_uneven_splits(int B, int Hq, int Hkv, int T, int D) {
+  const int64_t nt = ((int64_t)T + kTile - 1) / kTile;
+  const int64_t columns = (int64_t)B * Hkv * nt;
   if (D != 128 || columns > 512 || columns == 0) return 1;
-  const int64_t fit = (256ll << 20) / (columns * 2 * kTile * D * 4);
-  return (int)(fit < kMaxSplits ? fit : kMaxSplits);
+  const int64_t pieces = (Hq / Hkv * nt + kSplitItems - 1) / kSplitItems;
+  return (int)(pieces < 1 ? 1 : pieces < kMaxSplits ? pieces : kMaxSplits);
 }
 
 hipError_t launch_attn_bwd_dkdv_split(const TensorView& q, const TensorView& k,

@@ -94,8 +94,8 @@ hipError_t launch_attn_bwd_f32(const TensorView& q, const TensorView& k, const T
 enum BwdPhase { kBwdDelta = 0, kBwdDkDv = 1, kBwdDq = 2, kBwdDqDelta = 3, kBwdDkDvFine = 4 };
 
 // dK/dV with long columns shared by `splits` work-groups (bwd_uneven_splits; 1:
-// not worth it), their sums in workspace [B][Hkv][nt][splits][2][128][D].
-int bwd_uneven_splits(int B, int Hkv, int T, int D);
+// none), their sums in workspace [B][Hkv][nt][splits][2][128][D].
+int bwd_uneven_splits(int B, int Hq, int Hkv, int T, int D);
 hipError_t launch_attn_bwd_dkdv_split(const TensorView& q, const TensorView& k,
                                       const TensorView& v, const TensorView& dout,
                                       const float* lse2, float* delta, const TensorView& dk,

@@ -354,21 +354,29 @@ int t2t_attn_bwd_dq(const t2t_tensor* q, const t2t_tensor* k, const t2t_tensor* 
 int64_t t2t_attn_bwd_uneven_workspace(int32_t B, int32_t Hkv, int32_t T, int32_t D,
                                       int32_t dtype) {
   if (B <= 0 || Hkv <= 0 || T <= 0 || dtype != T2T_DTYPE_BF16) return 0;
-  const int splits = t2t::bwd_uneven_splits(B, Hkv, T, D);
+  // (query heads past any count: columns as long as they get)
+  const int splits = t2t::bwd_uneven_splits(B, 0x7fffffff, Hkv, T, D);
   if (splits == 1) return 0;
   return (int64_t)B * Hkv * ((T + t2t::kTile - 1) / t2t::kTile) * splits * 2 * t2t::kTile * D * 4;
 }
 
+int32_t t2t_attn_bwd_uneven_pieces(int32_t B, int32_t Hq, int32_t Hkv, int32_t T, int32_t D,
+                                   int32_t dtype) {
+  if (B <= 0 || Hq <= 0 || Hkv <= 0 || T <= 0 || dtype != T2T_DTYPE_BF16) return 1;
+  return t2t::bwd_uneven_splits(B, Hq, Hkv, T, D);
+}
+
 namespace {
 
-// The backward; uneven: with the workspace that long columns are shared over,
-// finer in dS.  o_rest: NULL, or t2t_attn_fwd_rest's.
+// The backward; fine: with dS from P of at least 9 bits; shared: with the
+// workspace that long columns are shared over.  o_rest: NULL, or
+// t2t_attn_fwd_rest's.
 int attn_bwd(const t2t_tensor* q, const t2t_tensor* k, const t2t_tensor* v, const t2t_tensor* o,
              const t2t_tensor* o_rest, const t2t_tensor* dout, const float* lse2, float* delta,
              const t2t_tensor* dq, const t2t_tensor* dk, const t2t_tensor* dv, int32_t B,
              int32_t Hq, int32_t Hkv, int32_t T, int32_t D, int32_t dtype, float scale,
-             const t2t_block_mask* mask, bool uneven, void* workspace, int64_t workspace_bytes,
-             void* stream) {
+             const t2t_block_mask* mask, bool fine, bool shared, void* workspace,
+             int64_t workspace_bytes, void* stream) {
   // Validate every argument before launching anything.
   int rc = check_dims(B, Hq, Hkv, T, D, dtype, true);
   if (rc) return rc;
@@ -384,7 +392,7 @@ int attn_bwd(const t2t_tensor* q, const t2t_tensor* k, const t2t_tensor* v, cons
   if (!lse2 || !delta) return fail(T2T_EINVAL, "lse2/delta is NULL");
   rc = check_mask(mask, B, T, true, true);
   if (rc) return rc;
-  const int64_t need = uneven ? t2t_attn_bwd_uneven_workspace(B, Hkv, T, D, dtype) : 0;
+  const int64_t need = shared ? t2t_attn_bwd_uneven_workspace(B, Hkv, T, D, dtype) : 0;
   if (need > 0 && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16 ||
                    workspace_bytes < need))
     return fail(T2T_EINVAL, "workspace of %lld bytes (16-byte aligned), %lld needed",
@@ -406,14 +414,14 @@ int attn_bwd(const t2t_tensor* q, const t2t_tensor* k, const t2t_tensor* v, cons
                                              as_tables(mask), static_cast<hipStream_t>(stream)),
                   "t2t_attn_bwd dQ launch");
   if (rc) return rc;
-  if (need > 0)
+  const int splits = need > 0 ? t2t::bwd_uneven_splits(B, Hq, Hkv, T, D) : 1;
+  if (splits > 1)
     return hip_status(t2t::launch_attn_bwd_dkdv_split(
                           as_view(q), as_view(k), as_view(v), as_view(dout), lse2, delta,
-                          as_view(dk), as_view(dv), dims, as_tables(mask),
-                          t2t::bwd_uneven_splits(B, Hkv, T, D), static_cast<float*>(workspace),
-                          static_cast<hipStream_t>(stream)),
+                          as_view(dk), as_view(dv), dims, as_tables(mask), splits,
+                          static_cast<float*>(workspace), static_cast<hipStream_t>(stream)),
                       "t2t_attn_bwd_uneven dK/dV launch");
-  return attn_bwd_dkdv(uneven ? t2t::kBwdDkDvFine : t2t::kBwdDkDv, q, k, v, dout, lse2, delta, dk,
+  return attn_bwd_dkdv(fine ? t2t::kBwdDkDvFine : t2t::kBwdDkDv, q, k, v, dout, lse2, delta, dk,
                        dv, B, Hq, Hkv, T, D, dtype, scale, mask, stream);
 }
 
@@ -426,7 +434,19 @@ int t2t_attn_bwd(const t2t_tensor* q, const t2t_tensor* k, const t2t_tensor* v,
                  int32_t D, int32_t dtype, float scale, const t2t_block_mask* mask,
                  void* stream) {
   return attn_bwd(q, k, v, o, nullptr, dout, lse2, delta, dq, dk, dv, B, Hq, Hkv, T, D, dtype,
-                  scale, mask, false, nullptr, 0, stream);
+                  scale, mask, false, false, nullptr, 0, stream);
+}
+
+int t2t_attn_bwd_rest(const t2t_tensor* q, const t2t_tensor* k, const t2t_tensor* v,
+                      const t2t_tensor* o, const t2t_tensor* o_rest, const t2t_tensor* dout,
+                      const float* lse2, float* delta, const t2t_tensor* dq, const t2t_tensor* dk,
+                      const t2t_tensor* dv, int32_t B, int32_t Hq, int32_t Hkv, int32_t T,
+                      int32_t D, int32_t dtype, float scale, const t2t_block_mask* mask,
+                      void* stream) {
+  if (o_rest && dtype != T2T_DTYPE_BF16)
+    return fail(T2T_EUNSUPPORTED, "o_rest goes with bf16, not dtype %d", dtype);
+  return attn_bwd(q, k, v, o, o_rest, dout, lse2, delta, dq, dk, dv, B, Hq, Hkv, T, D, dtype,
+                  scale, mask, true, false, nullptr, 0, stream);
 }
 
 int t2t_attn_bwd_uneven(const t2t_tensor* q, const t2t_tensor* k, const t2t_tensor* v,
@@ -439,7 +459,7 @@ int t2t_attn_bwd_uneven(const t2t_tensor* q, const t2t_tensor* k, const t2t_tens
   if (o_rest && dtype != T2T_DTYPE_BF16)
     return fail(T2T_EUNSUPPORTED, "o_rest goes with bf16, not dtype %d", dtype);
   return attn_bwd(q, k, v, o, o_rest, dout, lse2, delta, dq, dk, dv, B, Hq, Hkv, T, D, dtype,
-                  scale, mask, true, workspace, workspace_bytes, stream);
+                  scale, mask, true, true, workspace, workspace_bytes, stream);
 }
 
 // Delta workspace of t2t_attn_bwd_noalloc: a file-scope device array instead

@@ -121,7 +121,8 @@ std::tuple<Tensor, Tensor> attn_fwd(const Tensor& q, const Tensor& k, const Tens
   return {out, lse2};
 }
 
-// uneven: t2t_attn_bwd_uneven, with rest where the forward has left one
+// uneven: t2t_attn_bwd_uneven, or t2t_attn_bwd_rest where no column can be long;
+// with rest where the forward has left one
 std::tuple<Tensor, Tensor, Tensor> attn_bwd(const Tensor& q, const Tensor& k, const Tensor& v,
                                             const Tensor& out, const Tensor& dout_in,
                                             const Tensor& lse2, int64_t mask, double scale,
@@ -137,9 +138,6 @@ std::tuple<Tensor, Tensor, Tensor> attn_bwd(const Tensor& q, const Tensor& k, co
   const t2t_tensor qs = view4(q), ks = view4(k), vs = view4(v), os = view4(out),
                    ds = view4(dout), dqs = view4(dq), dks = view4(dk), dvs = view4(dv);
   if (uneven) {
-    const int64_t bytes = t2t_attn_bwd_uneven_workspace(B, Hkv, T, D, dtype);
-    Tensor ws;
-    if (bytes > 0) ws = at::empty({bytes / 4}, delta.options());
     t2t_tensor rs{};
     if (rest.has_value()) {
       need_gpu(*rest);
@@ -147,10 +145,20 @@ std::tuple<Tensor, Tensor, Tensor> attn_bwd(const Tensor& q, const Tensor& k, co
                         "rest ", rest->sizes(), " ", rest->scalar_type(), " is not out's");
       rs = view4(*rest);
     }
-    check(t2t_attn_bwd_uneven(&qs, &ks, &vs, &os, rest.has_value() ? &rs : nullptr, &ds,
-                              lse2.data_ptr<float>(), delta.data_ptr<float>(), &dqs, &dks, &dvs,
-                              B, Hq, Hkv, T, D, dtype, static_cast<float>(scale), mask_at(mask),
-                              bytes > 0 ? ws.data_ptr() : nullptr, bytes, stream_of(q)),
+    const t2t_tensor* left = rest.has_value() ? &rs : nullptr;
+    if (t2t_attn_bwd_uneven_pieces(B, Hq, Hkv, T, D, dtype) == 1) {
+      check(t2t_attn_bwd_rest(&qs, &ks, &vs, &os, left, &ds, lse2.data_ptr<float>(),
+                              delta.data_ptr<float>(), &dqs, &dks, &dvs, B, Hq, Hkv, T, D, dtype,
+                              static_cast<float>(scale), mask_at(mask), stream_of(q)),
+            "t2t_attn_bwd_rest");
+      return {dq, dk, dv};
+    }
+    const int64_t bytes = t2t_attn_bwd_uneven_workspace(B, Hkv, T, D, dtype);
+    Tensor ws = at::empty({bytes / 4}, delta.options());
+    check(t2t_attn_bwd_uneven(&qs, &ks, &vs, &os, left, &ds, lse2.data_ptr<float>(),
+                              delta.data_ptr<float>(), &dqs, &dks, &dvs, B, Hq, Hkv, T, D, dtype,
+                              static_cast<float>(scale), mask_at(mask), ws.data_ptr(), bytes,
+                              stream_of(q)),
           "t2t_attn_bwd_uneven");
     return {dq, dk, dv};
   }

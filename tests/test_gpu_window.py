@@ -677,3 +677,48 @@ def test_decode_rows_past_the_cache_keep_their_sinks(D, window, sinks):
         o, lse2 = attn_decode(q, k, v, cap, doc, None, pos, torch.zeros_like(pos), None,
                               window=window, sinks=sinks, q_start=start)
         check_rows(o, lse2, q, k, v, ok, 0.0)
+
+
+@pytest.mark.parametrize("B,T,H,Hkv,words,pieces", [(1, 4230, 8, 8, 0, 2), (1, 2304, 8, 4, 1, 2),
+                                                    (1, 2304, 8, 2, 0, 3), (2, 2200, 8, 1, 1, 4)])
+def test_every_number_of_shares(B, T, H, Hkv, words, pieces):
+    """Columns of more than 32 items, shared by two to four work-groups."""
+    from tagseq2tagseq_amd import _lib
+    assert _lib.lib().t2t_attn_bwd_uneven_pieces(B, H, Hkv, T, 128, 0) == pieces
+    # one document: its sinks' column is read by the whole row
+    rows = [_row(T, 5 * T + i, words, 3000) for i in range(B)]
+    rows = [(np.zeros(T, dtype=np.int32), *r[1:]) for r in rows]
+    window, sinks = 150, 5
+    bm = _build(rows, window, sinks)
+    items = (bm.q_num_blocks + bm.full_q_num_blocks) * (H // Hkv)
+    assert int(items.max()) > 32 * (pieces - 1)
+    dense = torch.stack([torch.from_numpy(_dense(*r, window, sinks)) for r in rows]).to(DEV)
+    g = torch.Generator().manual_seed(T)
+    q, k, v, do = (torch.randn(B, h, T, 128, generator=g).to(BF).to(DEV)
+                   for h in (H, Hkv, Hkv, H))
+    for t in (q, k, v):
+        t.requires_grad_(True)
+    out = flex_attention(q, k, v, block_mask=bm, enable_gqa=True)
+    got = (out, *torch.autograd.grad(out, (q, k, v), do, retain_graph=True))
+    again = torch.autograd.grad(out, (q, k, v), do)
+    assert all(torch.equal(a, b) for a, b in zip(got[1:], again))
+    for name, x, (ref, tol) in zip(("o", "dq", "dk", "dv"), got,
+                                   _attention_ref(q, k, v, do, dense, 2.0 ** -8)):
+        worst = float(((x.detach().double() - ref).abs() / tol).max())
+        assert worst <= 1, f"{name}: {worst:.3g} of the tolerance"
+
+
+def test_columns_that_cannot_be_long_take_no_workspace():
+    """4 x 4 heads of 128 over 4096 tokens: 32 items a column at most."""
+    B, H, T = 4, 4, 4096
+    bm = build_block_mask(torch.zeros(B, T, dtype=torch.int32, device=DEV), window=500, sinks=4)
+    q, k, v, do = (torch.randn(B, H, T, 128, device=DEV).to(BF) for _ in range(4))
+    for t in (q, k, v):
+        t.requires_grad_(True)
+    out = flex_attention(q, k, v, block_mask=bm)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    grads = torch.autograd.grad(out, (q, k, v), do)
+    results = sum(t.numel() * t.element_size() for t in grads) + B * H * T * 4
+    assert torch.cuda.max_memory_allocated() - before < results + (8 << 20)

@@ -168,3 +168,30 @@ def test_window_creators_need_a_window_and_a_gpu():
     one = torch.zeros(1, 1, dtype=torch.int32)
     with pytest.raises(RuntimeError, match="GPU tensors"):
         attn_decode(k[:, :, :1], k, k, 4, one.repeat(1, 4), None, one, one, None, window=2)
+
+
+def test_columns_are_shared_only_where_one_can_be_long():
+    """A column has at most (Hq / Hkv) ceil(T / 128) items, a work-group takes 32."""
+    w = L.t2t_attn_bwd_uneven_pieces
+    assert w(4, 4, 4, 4096, 128, 0) == 1 and w(1, 8, 8, 100, 128, 0) == 1   # 32 items; 1
+    assert w(4, 4, 4, 4097, 128, 0) == 1                                     # 528 columns
+    assert w(1, 4, 4, 4097, 128, 0) == 2 and w(1, 8, 4, 2304, 128, 0) == 2   # 33; 36
+    assert w(1, 8, 2, 2304, 128, 0) == 3 and w(2, 16, 4, 4001, 128, 0) == 4  # 72; 128
+    assert w(1, 64, 1, 32768, 128, 0) == 4
+    assert w(1, 64, 1, 32768, 64, 0) == 1 and w(1, 64, 1, 32768, 128, 1) == 1
+    assert w(0, 1, 1, 9, 128, 0) == 1 and w(1, 0, 1, 9, 128, 0) == 1 and w(1, 1, 0, 9, 128, 0) == 1
+    assert w(1, 1, 1, 2 ** 31 - 1, 128, 0) == 1 and w(1, 1, 1, -5, 128, 0) == 1
+
+
+@no_gpu
+@pytest.mark.parametrize("kw,rc,text", [
+    (dict(D=96), -2, "head dim"), (dict(Hq=3, Hkv=2), -1, "GQA"), (dict(scale=-1.0), -1, "scale"),
+    (dict(lse2=None), -1, "lse2"), (dict(mask=None), -1, "mask"), (dict(dk=None), -1, "view"),
+    (dict(dtype=1), -2, "o_rest"), (dict(rest=_view(data=None)), -1, "view"),
+])
+def test_backward_entry_without_a_workspace_refuses(kw, rc, text):
+    v = _view(stride_h=128, stride_t=128)
+    a = dict(q=v, k=v, v=v, o=v, rest=v, do=v, lse2=P, delta=P, dq=v, dk=v, dv=v, B=1, Hq=2, Hkv=1,
+             T=256, D=128, dtype=0, scale=0.1, mask=_tables())
+    a.update(kw)
+    assert L.t2t_attn_bwd_rest(*a.values(), None) == rc and text in _err()
