@@ -544,17 +544,19 @@ __device__ __forceinline__ void masked_clear(f32x16& pacc, uint32_t wg) {
 
 constexpr int kPairWaves = 8;  // 4 key groups x (P / dV wave, dS / dK wave)
 
-// Entries 8 h .. 8 h + 7 of P in 16 bits each: 0 <= P < 2, so that a float's
+// Entries 8 h .. 8 h + 7 of P in 16 bits each: 0 <= P <= 1, so that a float's
 // sign and its exponent's highest bit are 0, and 7 exponent and 9 mantissa bits
-// are left (rounded to nearest; bf16 keeps 7).  dK over a row of 16384 tokens,
+// are left (rounded to nearest; bf16 keeps 7).  P is taken as 1 where it is more:
+// LSE is a float, off by 1 where it passes 2^24, and P then by factors of 2.  dK over a row of 16384 tokens,
 // 12 heads, window 1024: 2.4e-3 off its 64-bit value instead of 2.9e-3 (the
 // roundings of dS and of dK itself are 1.7e-3 each), 122 us instead of 116.
 __device__ __forceinline__ bf16x8 pack_fine(const f32x16& acc, int h) {
   uint32_t w[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const uint32_t lo = (__float_as_uint(acc[8 * h + 2 * j]) + 0x2000u) << 2;
-    const uint32_t hi = (__float_as_uint(acc[8 * h + 2 * j + 1]) + 0x2000u) << 2;
+    const uint32_t lo = (min(__float_as_uint(acc[8 * h + 2 * j]), 0x3f800000u) + 0x2000u) << 2;
+    const uint32_t hi =
+        (min(__float_as_uint(acc[8 * h + 2 * j + 1]), 0x3f800000u) + 0x2000u) << 2;
     w[j] = __builtin_amdgcn_perm(hi, lo, 0x07060302u);
   }
   return __builtin_bit_cast(bf16x8, make_uint4(w[0], w[1], w[2], w[3]));

@@ -722,3 +722,39 @@ def test_columns_that_cannot_be_long_take_no_workspace():
     grads = torch.autograd.grad(out, (q, k, v), do)
     results = sum(t.numel() * t.element_size() for t in grads) + B * H * T * 4
     assert torch.cuda.max_memory_allocated() - before < results + (8 << 20)
+
+
+def test_scores_past_the_steps_of_their_sums():
+    """Scores of 2^25 to 2^26 in log2 units, where the log-sum-exp of a row, a
+    float, has steps of 4.
+
+    Documents of two tokens with one key twice: the second token's P is 1/2 for
+    both, and its log-sum-exp is one more than the score.  Off by at most half a
+    step each in the score's rounding and in the sum's, 4 in all, P is 2^-5 .. 2^3
+    to the kernel, and at most 1 where it knows that: dK of the first token,
+    c P (dP - Delta) q, is 2^-4 to 2 of its value, but for the roundings of q k
+    (none: all its terms are one power of two's multiple), P, dS and dK (2^-8
+    each at most) and of Delta (16 bits of O)."""
+    n, D = 256, 64
+    T = 2 * n
+    doc = (torch.arange(T, device=DEV) // 2).int()
+    bm = build_block_mask(doc, window=2)
+    g = torch.Generator().manual_seed(0)
+    q, k = torch.zeros(1, 1, T, D), torch.zeros(1, 1, T, D)
+    a = 2.0 ** torch.linspace(10.6, 11.3, n)  # (8 a 2^11 log2(e) of scores)
+    q[0, 0, 1::2] = a[:, None]
+    k[0, 0] = 2048.0
+    v, do = torch.randn(1, 1, T, D, generator=g), torch.randn(1, 1, T, D, generator=g)
+    q, k, v, do = (t.to(BF).to(DEV) for t in (q, k, v, do))
+    score = (q.double() * k.double()).sum(-1)[0, 0, 1::2] / 8 / math.log(2.0)
+    assert 2 ** 25 < float(score.min()) and float(score.max()) < 2 ** 26
+    for t in (q, k, v):
+        t.requires_grad_(True)
+    _, dk, _ = torch.autograd.grad(flex_attention(q, k, v, block_mask=bm), (q, k, v), do)
+    v64, do64 = v.detach().double()[0, 0].view(n, 2, D), do.double()[0, 0].view(n, 2, D)[:, 1]
+    diff = ((v64[:, 0] - v64[:, 1]) / 2 * do64).sum(-1)  # dP - Delta of the first token
+    clear = diff.abs() > 2.0 ** -6 * (v64.abs().amax(1) * do64.abs()).sum(-1)
+    want = (diff / 2 / 8)[:, None] * q.detach().double()[0, 0, 1::2]
+    ratio = (dk.double()[0, 0, 0::2] / want)[clear]
+    assert int(clear.sum()) > n / 2
+    assert 2.0 ** -4 * 0.95 < float(ratio.min()) and float(ratio.max()) < 2 * 1.05
