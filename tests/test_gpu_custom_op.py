@@ -81,3 +81,16 @@ def test_compiled_layer_matches_eager():
                         layer.attn.qkv.weight.grad])
     for a, b in zip(*results):
         assert torch.allclose(a.float(), b.float(), atol=2e-2, rtol=2e-2)
+
+
+def test_one_compiled_function_takes_both_head_dims():
+    """The second head dim makes it a symbol of the graph, and so the scale."""
+    def fn(q, k, v, bm):
+        return flex_attention(q, k, v, block_mask=bm, enable_gqa=True)
+    compiled = torch.compile(fn, backend="aot_eager", fullgraph=True)
+    for D in (64, 128, 64):
+        q, k, v, bm = _inputs(D=D)
+        assert torch.equal(compiled(q, k, v, bm), fn(q, k, v, bm))
+    for scale in (0.0, -1.0, math.inf, math.nan):
+        with pytest.raises(ValueError, match="positive finite"):
+            flex_attention(q, k, v, block_mask=bm, enable_gqa=True, scale=scale)
