@@ -13,7 +13,8 @@ Seams replaced (reference file:line):
     autograd.Function with the same contents for other eager calls, and
     ``torch.ops.t2t.masked_attention`` / ``t2t::masked_attention_backward``,
     ``torch.library`` custom ops with fake implementations and registered
-    autograd that compiled graphs trace.  ``flex_attention`` picks the custom
+    autograd that compiled graphs trace (``windowed_attention`` and its backward
+    for a sliding window's mask).  ``flex_attention`` picks the custom
     op while torch.compile traces and the others otherwise: the custom op's
     registered autograd costs several hundred microseconds of host time per
     call, the Function tens.
@@ -132,13 +133,15 @@ def _windowed(block_mask) -> bool:
     return getattr(block_mask, "window", None) is not None
 
 
-def attn_bwd(q, k, v, out, dout, lse2, block_mask, scale: float, rest=None):
+def attn_bwd(q, k, v, out, dout, lse2, block_mask, scale: float, rest=None,
+             windowed: bool = False):
     """Kernel call: returns (dq, dk, dv).  ``block_mask`` as in attn_fwd; a
-    sliding window's mask gets the launches for uneven columns and rows of few
-    keys, ``rest`` what the forward left of out's rounding for them."""
+    sliding window's mask (or tables that are one's, ``windowed``) gets the
+    launches for uneven columns and rows of few keys, ``rest`` what the forward
+    left of out's rounding for them."""
     mask = _mask_struct(block_mask)
     return _lib.host().attn_bwd(q, k, v, out, dout, lse2, ctypes.addressof(mask), scale,
-                                _windowed(block_mask), rest)
+                                windowed or _windowed(block_mask), rest)
 
 
 class BwdPhases:
@@ -267,6 +270,55 @@ def _masked_attention_bwd(ctx, dout, _dlse2):
 masked_attention.register_autograd(_masked_attention_bwd, setup_context=_masked_attention_setup)
 
 
+@torch.library.custom_op("t2t::windowed_attention", mutates_args=())
+def windowed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                       tables: List[torch.Tensor],
+                       scale: float) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """masked_attention of a sliding window's tables that is to be recorded:
+    (out, lse2, rest), rest what rounding left of a bf16 out (float32: empty)."""
+    mask = _mask_struct(tables)
+    out, lse2, rest = _lib.host().attn_fwd_rest(q, k, v, ctypes.addressof(mask), scale, True)
+    return out, lse2, q.new_empty(0) if rest is None else rest
+
+
+@windowed_attention.register_fake
+def _windowed_attention_fake(q, k, v, tables, scale):
+    out, lse2 = _masked_attention_fake(q, k, v, tables, scale)
+    return out, lse2, torch.empty_like(out) if q.dtype == torch.bfloat16 else q.new_empty(0)
+
+
+@torch.library.custom_op("t2t::windowed_attention_backward", mutates_args=())
+def windowed_attention_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                                out: torch.Tensor, rest: torch.Tensor, dout: torch.Tensor,
+                                lse2: torch.Tensor, tables: List[torch.Tensor],
+                                scale: float) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(dq, dk, dv) of windowed_attention."""
+    return attn_bwd(q, k, v, out, dout, lse2, tables, scale,
+                    rest if q.dtype == torch.bfloat16 else None, True)
+
+
+@windowed_attention_backward.register_fake
+def _windowed_attention_backward_fake(q, k, v, out, rest, dout, lse2, tables, scale):
+    return _masked_attention_backward_fake(q, k, v, out, dout, lse2, tables, scale)
+
+
+def _windowed_attention_setup(ctx, inputs, output):
+    q, k, v, tables, scale = inputs
+    ctx.save_for_backward(q, k, v, *output, *tables)
+    ctx.scale = scale
+
+
+def _windowed_attention_bwd(ctx, dout, _dlse2, _drest):
+    q, k, v, out, lse2, rest, *tables = ctx.saved_tensors
+    grads = windowed_attention_backward(q, k, v, out, rest, dout.contiguous(), lse2, tables,
+                                        ctx.scale)
+    return *grads, [None] * len(tables), None
+
+
+windowed_attention.register_autograd(_windowed_attention_bwd,
+                                     setup_context=_windowed_attention_setup)
+
+
 def flex_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
                    score_mod=None, block_mask: Optional[T2TBlockMask] = None,
                    scale: Optional[float] = None, enable_gqa: bool = False,
@@ -296,7 +348,11 @@ def flex_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
         raise ValueError(f"scale={scale!r}: the gfx950 kernels need a positive finite scale")
     if torch.compiler.is_compiling():
         # compiled graphs trace the custom op (schema + fake implementation)
-        out, lse2 = masked_attention(query, key, value, block_mask.tables(), float(scale))
+        recorded = torch.is_grad_enabled() and (query.requires_grad or key.requires_grad
+                                                or value.requires_grad)
+        args = (query, key, value, block_mask.tables(), float(scale))
+        out, lse2 = (windowed_attention(*args)[:2] if recorded and _windowed(block_mask) else
+                     masked_attention(*args))
     elif _lib.unwatched(query, key, value):
         out, lse2 = attn_fwd(query, key, value, block_mask, float(scale))
     elif _lib.only_recorded(query, key, value):

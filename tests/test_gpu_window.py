@@ -758,3 +758,28 @@ def test_scores_past_the_steps_of_their_sums():
     ratio = (dk.double()[0, 0, 0::2] / want)[clear]
     assert int(clear.sum()) > n / 2
     assert 2.0 ** -4 * 0.95 < float(ratio.min()) and float(ratio.max()) < 2 * 1.05
+
+
+@pytest.mark.parametrize("dtype,D,H,Hkv,T", [(BF, 64, 4, 2, 700), (BF, 128, 8, 1, 1300),
+                                             (F32, 64, 2, 2, 300)])
+def test_compiled_windowed_attention_is_the_eager_one(dtype, D, H, Hkv, T):
+    """Outputs and gradients bit for bit, and without a graph to record."""
+    from tagseq2tagseq_amd.attention import windowed_attention
+    bm = _build([_row(T, T, 1, 300)], 90, 3)
+    g = torch.Generator().manual_seed(T)
+    q, k, v, do = (torch.randn(1, h, T, D, generator=g).to(dtype).to(DEV)
+                   for h in (H, Hkv, Hkv, H))
+
+    def fn(q, k, v):
+        return flex_attention(q, k, v, block_mask=bm, enable_gqa=True)
+    results = []
+    for f in (fn, torch.compile(fn, backend="aot_eager", fullgraph=True)):
+        x = [t.clone().requires_grad_(True) for t in (q, k, v)]
+        out = f(*x)
+        results.append([out.detach(), *torch.autograd.grad(out, x, do)])
+        with torch.no_grad():
+            results[-1].append(f(q, k, v))
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
+    x = [t.clone().requires_grad_(True) for t in (q, k, v)]
+    torch.library.opcheck(windowed_attention, (*x, bm.tables(), D ** -0.5))
