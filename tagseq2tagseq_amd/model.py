@@ -21,7 +21,8 @@ mode -- and is dropped when any of them changes (an optimizer step,
 load_state_dict, an in-place edit, train() / eval()).  Writes through a
 parameter's ``.data`` bypass its version counter; call ``reset_cache()`` after
 such an edit.  New rows go through each layer with the decode-step kernel
-(``t2t_attn_decode``, up to 8 rows per kv head per launch); when more than
+(``t2t_attn_decode``, up to 8 rows per kv head per launch, over the 8-bit
+cache ``t2t_kv8_attend``, up to 16); when more than
 ``prefill_rows`` rows are new, the whole sequence is recomputed through the
 block-mask kernels and the cache refilled.
 
@@ -45,6 +46,7 @@ from .attention import flex_attention
 from .block_mask import T2TBlockMask, build_block_mask
 from .decode import MAX_ROWS, attn_decode
 from .embedding import embedding
+from .kv8 import MAX_ROWS as MAX_ROWS_8
 from .kv8 import KV8Cache
 from .modules import RMSNorm, TS2TSBackbone
 from .rope import qk_norm_rope_append
@@ -62,6 +64,8 @@ class KVCache:
                  words: int, device, dtype=torch.bfloat16, bits: int = 16,
                  window: Optional[int] = None, sinks: int = 0):
         self.bits, self.window, self.sinks = bits, window, sinks
+        # new rows a launch of attend (one query head per kv head in this model)
+        self.max_rows = MAX_ROWS_8 if bits == 8 else MAX_ROWS
         if bits == 8:
             self.layers8 = [KV8Cache(1, num_heads, capacity, head_dim, device)
                             for _ in range(num_layers)]
@@ -471,7 +475,7 @@ class TS2TSModel:
             y = flex_attention(q, k, v, block_mask=bm)
         else:
             y = torch.empty_like(q)
-            rows = MAX_ROWS  # one query head per kv head in this model
+            rows = cache.max_rows
             pos = torch.arange(p0, T, dtype=torch.int32, device=x.device)[None]
             for c0 in range(0, n, rows):
                 c1 = min(n, c0 + rows)

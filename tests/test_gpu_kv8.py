@@ -608,3 +608,24 @@ def test_rows_past_the_cache_keep_their_sinks(D, window, sinks):
         o, lse2 = cache.attend(q, cap, doc, None, pos, torch.zeros_like(pos), None,
                                window=window, sinks=sinks, q_start=start)
         check_rows(o, lse2, q, k, v, ok, 2.0 ** -16)  # (p in two bf16 numbers)
+
+
+@pytest.mark.parametrize("bits,launches", [(8, [1, 1, 2, 3]), (16, [1, 2, 3, 5])])
+@torch.no_grad()
+def test_new_rows_go_through_as_many_at_once_as_the_cache_takes(bits, launches, monkeypatch):
+    from tagseq2tagseq_amd.model import KVCache
+    m = _model(window=50, sinks=2)
+    m.kv_bits = bits
+    seen = []
+    attend = KVCache.attend
+    monkeypatch.setattr(KVCache, "attend",
+                        lambda self, i, q, *a, **kw: (seen.append(q.shape[2]),
+                                                      attend(self, i, q, *a, **kw))[1])
+    tokens = torch.randint(0, 211, (1, 450), generator=torch.Generator().manual_seed(4)).to(DEV)
+    m.forward_inference_last(tokens[:, :300], _spans(300))
+    T = 300
+    for n, count in zip((2, 16, 17, 40), launches):
+        seen.clear()
+        T += n
+        m.forward_inference_last(tokens[:, :T], _spans(T))
+        assert len(seen) == 4 * count and sum(seen) == 4 * n
