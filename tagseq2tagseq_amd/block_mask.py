@@ -14,8 +14,10 @@ for element masking.
 
 With a sliding ``window`` a token reads of its own document the last ``window``
 tokens (itself among them) and the document's first ``sinks`` ones; what a
-grant word shows it reads as before.  A document is a run of tokens with one
-id: the same id again behind another document starts anew.
+grant word shows it reads as before.  Documents are told apart by their ids
+alone: where one id comes back behind another document, the window reaches the
+earlier tokens of that id too, as a mask without one does.  Only sinks are
+counted from the start of the token's own run of equal ids.
 
 ``to_block_mask()`` rebuilds a torch ``BlockMask`` from the same tables (via
 ``BlockMask.from_kv_blocks``) for interoperability with torch's own
@@ -221,8 +223,9 @@ def build_block_mask(doc_ids: torch.Tensor, q_bits: Optional[torch.Tensor] = Non
 
     doc_ids: int32 [T] or [Bm, T] on a ROCm device.
     q_bits / kv_bits: int64 (or uint64) [W, T] or [Bm, W, T] grant words, or None.
-    window: last tokens of its own document that a token reads (None: all), and
-    sinks: first tokens of the document that it reads beside them.
+    window: a token reads the tokens of its own document id among the last
+    ``window`` (None: all), and
+    sinks: the first ones of its own run of that id beside them.
     """
     window, sinks = check_window(window, sinks)
     if not doc_ids.is_cuda:
