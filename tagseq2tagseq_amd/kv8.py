@@ -67,9 +67,12 @@ def kv8_append(k: torch.Tensor, v: torch.Tensor, pos: Union[int, torch.Tensor],
     it (its codes stay as they were).  A block's scale grows to what its new
     tokens need, and its positions before pos are written again where it did;
     a block that pos begins starts from its new tokens.  A token whose key or
-    value is not finite makes every row that reads it NaN.  What the buffers
-    hold where nothing was stored is never looked at.  A device position below
-    0 or above capacity - M stores nothing.  No gradient."""
+    value is not finite makes every row that reads it NaN.  What the codes hold
+    where nothing was stored is never looked at, nor are the scales of blocks
+    that no token is in; a block that pos begins inside keeps the scale it has,
+    so scales start out as zeros (KV8Cache's do) where positions may be left out.
+    A device position below 0 or above capacity - M stores nothing.  No
+    gradient."""
     at, pos0 = (pos, 0) if isinstance(pos, torch.Tensor) else (None, index(pos))
     if capacity is not None and capacity < 0:
         raise ValueError(f"capacity={capacity} is negative")

@@ -629,3 +629,27 @@ def test_new_rows_go_through_as_many_at_once_as_the_cache_takes(bits, launches, 
         T += n
         m.forward_inference_last(tokens[:, :T], _spans(T))
         assert len(seen) == 4 * count and sum(seen) == 4 * n
+
+
+@pytest.mark.parametrize("pos", [5, 70, 127])
+def test_a_sequence_that_begins_inside_a_block(pos):
+    """Positions before the first token were never stored: their codes may be
+    anything, their scales are zeros."""
+    g = torch.Generator().manual_seed(pos)
+    clean, junk = KV8Cache(1, 2, 300, 64, DEV), KV8Cache(1, 2, 300, 64, DEV)
+    for t in junk.buffers()[:2]:
+        t.view(torch.uint8).fill_(0xff)
+    doc = torch.full((1, 300), 7, dtype=torch.int32, device=DEV)
+    doc[:, pos:] = 0
+    at = torch.tensor([[pos + 39]], dtype=torch.int32, device=DEV)
+    q = torch.randn(1, 2, 1, 64, generator=g).to(BF).to(DEV)
+    steps = [_rows(1, 2, n, 64, BF, g, 2.0 ** i) for i, n in enumerate((1, 30, 9))]
+    outs = []
+    for c in (clean, junk):
+        p = pos
+        for k, v in steps:  # (each under a larger scale)
+            c.append(k, v, p)
+            p += k.shape[2]
+        outs.append(c.attend(q, p, doc, None, at, torch.zeros_like(at), None))
+    assert outs[0][0].isfinite().all()
+    assert all(torch.equal(a, b) for a, b in zip(*outs))
