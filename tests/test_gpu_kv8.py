@@ -15,7 +15,7 @@ from tagseq2tagseq_amd.mask_creators import make_mask_creator_callable
 from tagseq2tagseq_amd.model import TS2TSModel
 from tagseq2tagseq_amd.rope import RotaryForm
 from tests.helpers import random_row, to_dev_words
-from tests.test_gpu_window import (PAST_THE_CACHE, _dense, _spans, _starts, check_rows,
+from tests.test_gpu_window import (ONE_ROUNDING, PAST_THE_CACHE, _dense, _spans, _starts, check_rows,
                                    logits_agree)
 
 pytestmark = pytest.mark.gpu
@@ -653,3 +653,29 @@ def test_a_sequence_that_begins_inside_a_block(pos):
         outs.append(c.attend(q, p, doc, None, at, torch.zeros_like(at), None))
     assert outs[0][0].isfinite().all()
     assert all(torch.equal(a, b) for a, b in zip(*outs))
+
+
+# A rounding to bf16 is off by 1.66e-3 in the mean square (test_gpu_window); o is
+# rounded once, and by how much is known: the distance to the nearest bf16 number
+# changes by no more than its argument, so that with x the sum before the rounding
+# |o - want| <= |x - want| + |bf16(x) - x| <= 2 |x - want| + |bf16(want) - want|.
+# (The mean of 1.66e-3 would not do: the channels' sizes differ by 2^8, and the
+# few hundred values of the largest ones, which are the norm, are off by 1.5e-3 to
+# 2e-3.)  p in two bf16 numbers adds 2^-8 of a rounding more, fp32 sums less than
+# 1e-5; p in one would add as much again as a rounding of o (an o of independent
+# values is as long as its terms' squares' sum).
+@pytest.mark.parametrize("window,sinks", [(3, 0), (40, 2), (None, 0)])
+@pytest.mark.parametrize("B,H,Hkv,M,D,T", [
+    (2, 4, 4, 1, 64, 700), (1, 4, 1, 2, 128, 500), (1, 8, 1, 2, 64, 900), (2, 6, 2, 5, 128, 300),
+    (8, 8, 4, 1, 64, 5000), (8, 6, 2, 3, 128, 5000),
+])
+def test_rows_round_once(B, H, Hkv, M, D, T, window, sinks):
+    """Up to eight rows a kv head and more, in one pass and in chunks."""
+    cache, q, mask, limits, ok = _attend_case(B, H, Hkv, M, D, T, 0, window, sinks)
+    o, _ = cache.attend(q, T, *mask, **limits)
+    k, v = (t[:, :, :T].repeat_interleave(H // Hkv, 1).double() for t in cache.values(F32))
+    s = (q.double() @ k.transpose(2, 3).contiguous()) * D ** -0.5
+    want = torch.softmax(s.masked_fill(~ok[:, None], -math.inf), -1) @ v
+    off = float((o.double() - want).norm() / want.norm())
+    once = float((want.to(BF).double() - want).norm() / want.norm())
+    assert off <= once + 0.05 * ONE_ROUNDING, f"{off:.3g}, one rounding {once:.3g}"

@@ -783,3 +783,73 @@ def test_compiled_windowed_attention_is_the_eager_one(dtype, D, H, Hkv, T):
         assert torch.equal(a, b)
     x = [t.clone().requires_grad_(True) for t in (q, k, v)]
     torch.library.opcheck(windowed_attention, (*x, bm.tables(), D ** -0.5))
+
+
+def _windowed_loss(p, tokens, spans, layers, H, form, window, sinks):
+    """Mean cross-entropy of the whole model in 64 bits, from parameters p."""
+    ids, target = tokens[0, :-1], tokens[0, 1:]
+    n, C = ids.shape[0], p["embedding.weight"].shape[1]
+    D = C // H
+    R = int(form.fraction * D)
+    doc = torch.full((n,), -1, dtype=torch.int64)
+    for s in spans:
+        doc[s.start:min(s.end, n)] = s.doc_id
+    mask = torch.from_numpy(_dense(doc.numpy(), None, None, window, sinks)).to(DEV)
+    w = (form.base ** (-torch.arange(R // 2, dtype=torch.float64, device=DEV) * 2 / R)
+         / form.factor)  # (positions divided)
+    ang = torch.arange(n, dtype=torch.float64, device=DEV)[:, None] * w
+    cos, sin = ang.cos(), ang.sin()
+
+    def turn(x):  # interleaved pairs by the negative angle
+        a, b = x[..., :R:2], x[..., 1:R:2]
+        y = torch.stack((a * cos + b * sin, b * cos - a * sin), -1).flatten(-2)
+        return torch.cat((y, x[..., R:]), -1)
+
+    def rms(x, w):
+        return x / torch.sqrt((x * x).mean(-1, keepdim=True) + 1e-6) * w
+
+    x = p["embedding.weight"][ids]
+    skips, n_skip = [], layers // 2
+    for i in range(layers):
+        at = f"backbone.layers.{i}."
+        if i >= n_skip and skips:
+            x = x + p["backbone.skip_weights"][i - n_skip] * skips.pop()
+        h = rms(x, p[at + "ln_1.weight"]) @ p[at + "attn.qkv.weight"].t()
+        a, b, v = h.view(n, 3, H, D).permute(1, 2, 0, 3)
+        s = (turn(a) @ turn(b).transpose(-1, -2) / math.sqrt(D)).masked_fill(~mask, -math.inf)
+        y = (torch.softmax(s, -1) @ v).transpose(0, 1).reshape(n, C)
+        x = x + y @ p[at + "attn.proj.weight"].t()
+        g, u = (rms(x, p[at + "ln_2.weight"]) @ p[at + "mlp.gate_up.weight"].t()).chunk(2, -1)
+        x = x + (torch.nn.functional.silu(g) * u) @ p[at + "mlp.down.weight"].t()
+        if i < n_skip:
+            skips.append(x)
+    z = rms(x, p["norm.weight"]) @ p["embedding.weight"].t()
+    return torch.nn.functional.cross_entropy(z, target)
+
+
+@pytest.mark.parametrize("dtype,bound", [(BF, 3e-2), (F32, 1e-4)])
+@pytest.mark.parametrize("window,sinks", [(8, 0), (20, 3)])
+def test_gradients_of_a_windowed_model(dtype, bound, window, sinks):
+    """A training step with a rotary form and a window with sinks against the
+    model in 64 bits.  Some 12 stored activations a layer and 2 layers, each
+    rounded by 2^-9.8 of itself in the mean square and independent: sqrt(24)
+    2^-9.8 = 0.6 % at the logits, 0.8 % behind a backward with as many; the bound
+    is over three times that.  float32 has 2^-16 of it; 1e-4 is its attention's."""
+    torch.manual_seed(0)
+    form = RotaryForm(fraction=0.5, interleaved=True, base=500.0, scaling="linear", factor=2.0)
+    m = TS2TSTrainingModule.from_config(
+        vocab_size=211, num_layers=2, model_dim=256, num_heads=4, max_seq_len=512, dropout=0.0,
+        drop_path_rate=0.0, rotary=form,
+        block_mask_creator=make_mask_creator_callable("doc_causal", window=window, sinks=sinks))
+    m = m.to(DEV, dtype)
+    tokens = torch.randint(0, 211, (1, 251), generator=torch.Generator().manual_seed(1)).to(DEV)
+    spans = _spans(250)
+    loss = m(dict(tokens=tokens, doc_spans=spans))
+    loss.backward()
+    named = m.state_dict()
+    p = {n: named[n].double().requires_grad_(True) for n, _ in m.named_parameters()}
+    ref = _windowed_loss(p, tokens, spans, 2, 4, form, window, sinks)
+    assert abs(float(loss.detach()) - float(ref.detach())) <= bound * float(ref.detach())
+    for (name, prm), want in zip(m.named_parameters(), torch.autograd.grad(ref, [*p.values()])):
+        off = float((prm.grad.double() - want).norm() / want.norm())
+        assert off <= bound, f"{name}: {off:.3g}"
