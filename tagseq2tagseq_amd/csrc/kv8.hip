@@ -18,8 +18,9 @@
 // integer would have one left.  A token with a key or value that is not finite
 // is stored as NaN keys and zero values: every row that reads it is NaN, no
 // other row is touched.  HBM bound for prompts: 16384 tokens of 12 heads of 64
-// 17.3 us, 4.4 TB/s of the tokens read and the codes written; one token is a
-// launch and its memory latencies in turn, 5.0 us.
+// 16.6 us, 4.5 TB/s of the tokens read and the codes written; one token is a
+// launch and its memory latencies in turn, 5.1 us, also where its block's scale
+// grows and the codes before it are written again.
 //
 // Attention (kv8_attend).  One work-group per (chunk of keys, kv head, batch
 // row), R = G Tq <= 16 query rows (G query heads a kv head, Tq new tokens), each
@@ -36,8 +37,10 @@
 // of V^T: no shuffle and no LDS between global memory and the products.
 // Each (row, chunk) leaves (max, sum, unnormalised o[D]) for kv8_combine.  12
 // heads of 64 over 32768 positions: 12.3 + 3.9 us, 4.1 TB/s; 16 sequences of 8192,
-// 32 / 8 heads of 128, two tokens: 45 + 4.7 us, 6.0 TB/s (part of it from the
-// last-level cache).
+// 32 / 8 heads of 128, two tokens: 44 + 4.7 us, 6.1 TB/s (part of it from the
+// last-level cache).  Through a window of 512 or 4096 behind the 32768 positions
+// 5.9 + 3.5 and 6.6 + 3.3: the chunks are as many as the cache's length asks for,
+// most of them without a block.
 #include "attn_kernels.h"
 
 namespace t2t {

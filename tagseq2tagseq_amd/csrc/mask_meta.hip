@@ -44,9 +44,9 @@
 // (doc_starts).  A key that a grant or a sink shows is seen by a whole query
 // run, any other key of the same document by the queries up to k + w - 1: still
 // one evaluation and one bit range per run and token.  A 16k row of six
-// documents: mask_tiles 7.0 us (w 1024, s 4) and 5.9 without a window, doc_starts
-// 5.5, lists and ranks 6.2 either way; memory latency and the launches bound
-// each of them.
+// documents, ahead of its attention (w 1024, s 4): doc_starts 6.2 us, mask_tiles
+// 6.7, lists 4.8, ranks 4.6; memory latency and the launches bound each of them.
+// Masks alone, one behind the other: 5.4, 6.7 (5.7 without a window), 3.2, 3.2.
 #include <utility>
 
 #include "attn_kernels.h"
@@ -477,7 +477,9 @@ __global__ __launch_bounds__(kThreads) void mask_rank(MaskOut out) {
 // start[t] = the first token of the run of equal document ids that holds t.
 // grid (ceil(T / 256), Bm); block 256: the last run start at or before each
 // token of the block by ballots, and before the block by a search backwards,
-// 4096 tokens a step, whose loads do not wait for one another.
+// 4096 tokens a step, whose loads do not wait for one another.  A block searches
+// as far as its document's start: 16384 tokens of six documents 5.4 us, of one
+// 12.6; 131072 of 48 documents 5.1, of one 79.
 constexpr int kStartSpan = 16;  // tokens a thread looks at in a step backwards
 
 __global__ __launch_bounds__(kThreads) void doc_starts(const int32_t* __restrict__ doc_all, int T,
