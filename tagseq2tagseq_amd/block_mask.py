@@ -246,7 +246,8 @@ def build_block_mask(doc_ids: torch.Tensor, q_bits: Optional[torch.Tensor] = Non
         raise ValueError(f"{W} grant words exceed the supported {_lib.MAX_WORDS}")
     host = _lib.host()
     s = stream.cuda_stream if stream is not None else host.current_stream(device.index)
-    tile_class, *t = host.mask_meta_window(doc_ids, qb, kb, window or 0, sinks, s)
+    tile_class, *t = (host.mask_meta(doc_ids, qb, kb, s) if window is None else
+                      host.mask_meta_window(doc_ids, qb, kb, window, sinks, s))
     return T2TBlockMask(
         seq_len=T, doc_ids=doc_ids, q_bits=qb, kv_bits=kb, tile_class=tile_class,
         window=window, sinks=sinks, doc_start=t[13] if sinks else None,
