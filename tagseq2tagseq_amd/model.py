@@ -58,8 +58,10 @@ class KVCache:
     sequence (batch 1), with the token ids and mask inputs they were computed
     under.  Storage: k, v bf16 [L][1][H][cap][D], or with bits = 8 a KV8Cache a
     layer; doc int32 [1][cap]; q / kv words int64 [1][W][cap]; with a sliding
-    window's sinks the documents' starts, int32 [1][cap]."""
+    window's sinks the documents' starts, int32 [1][cap].  Made outside of inference
+    mode, so that calls in and out of it may fill one cache in turn."""
 
+    @torch.inference_mode(False)
     def __init__(self, num_layers: int, num_heads: int, head_dim: int, capacity: int,
                  words: int, device, dtype=torch.bfloat16, bits: int = 16,
                  window: Optional[int] = None, sinks: int = 0):
@@ -499,6 +501,7 @@ class _DecodeGraph:
     kernels, or hipBLASLt GEMMs, torch elementwise / reduction kernels and
     the prologue kernel) write no memset nodes of their own."""
 
+    @torch.inference_mode(False)  # (as the cache)
     def __init__(self, model: TS2TSModel, cache: KVCache):
         self.cache = cache
         self.pos = torch.zeros((1,), dtype=torch.int64, device=cache.tokens.device)
@@ -507,6 +510,8 @@ class _DecodeGraph:
         self.graph = None
         self.logits = None
 
+    @torch.inference_mode(False)  # (torch keeps tensors of its own from a first capture too)
+    @torch.no_grad()
     def _capture(self):
         """Warm up on a side stream (default priority), then capture.  The
         buffers already hold the first step's values, so the warm-up run writes

@@ -22,7 +22,8 @@ from oracle import mask_oracle as mo
 from tagseq2tagseq_amd import synth
 from tagseq2tagseq_amd.decode import attn_decode
 from tagseq2tagseq_amd.mask_creators import (create_doc_causal_block_mask,
-                                             create_doc_link_block_mask)
+                                             create_doc_link_block_mask,
+                                             make_mask_creator_callable)
 from tagseq2tagseq_amd.model import TS2TSModel
 from tests.helpers import assert_close, random_row, to_dev_words
 
@@ -373,3 +374,23 @@ def test_first_input_diff_kernel(words):
             want = p if p is not None and p < n else n
             got = int(cache.first_diff(toks, bm, n).item())
             assert got == want, f"{which} at {p}, n={n}: got {got}, want {want}"
+
+
+@pytest.mark.parametrize("kv_bits", [16, 8])
+@pytest.mark.parametrize("graphs", [True, False])
+def test_a_cache_made_in_inference_mode_serves_other_calls(kv_bits, graphs):
+    torch.manual_seed(0)
+    m = TS2TSModel.from_config(
+        vocab_size=97, num_layers=2, model_dim=128, num_heads=2, max_seq_len=256, dropout=0.0,
+        drop_path_rate=0.0, block_mask_creator=make_mask_creator_callable("causal"))
+    m.to(DEV, torch.bfloat16).eval()
+    m.kv_bits, m.use_graphs = kv_bits, graphs
+    tokens = torch.randint(0, 97, (1, 200), generator=torch.Generator().manual_seed(1)).to(DEV)
+    runs = []
+    for modes in ((True, False, True, False), (False, True, False, True)):
+        m.reset_cache()
+        runs.append([])
+        for T, inference in zip((120, 121, 122, 130), modes):
+            with torch.inference_mode(inference):
+                runs[-1].append(m.forward_inference_last(tokens[:, :T], []))
+    assert all(torch.equal(a, b) for a, b in zip(*runs))
