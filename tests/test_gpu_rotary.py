@@ -5,12 +5,16 @@ Tolerance: a rotated value is a c + b s in fp32 (a product, a fused
 multiply-add: 2 roundings of U = 2^-24 of |a c| + |b s|), then half a step of
 its type; a copied value is exact.
 """
+import dataclasses
+
 import pytest
 import torch
 from torch.fx.experimental.proxy_tensor import make_fx
 
 from tagseq2tagseq_amd import rope
 from tagseq2tagseq_amd.attention import FlexSelfAttention
+from tagseq2tagseq_amd.mask_creators import make_mask_creator_callable
+from tagseq2tagseq_amd.model import TS2TSModel
 from tagseq2tagseq_amd.rope import RotaryForm, qkv_rope, qkv_rotary, rope_tables, rotary_tables
 
 pytestmark = pytest.mark.gpu
@@ -339,3 +343,38 @@ def test_modules_turn_either_way(positive, interleaved, fraction):
             # U of that (whole halves at base 700: rope.rotary_tables' too)
             size = y.abs().amax(-1, keepdim=True) * 2
             assert bool(((x.double() - want).abs() <= 2.0 ** -8 * want.abs() + 4 * U * size).all())
+
+
+@pytest.mark.parametrize("kv_bits", [16, 8])
+@pytest.mark.parametrize("kw", [dict(rotary=RotaryForm(positive=True)),
+                                dict(rotary=RotaryForm(positive=True), qk_norm=True),
+                                dict(rotary=RotaryForm(positive=True, interleaved=True,
+                                                       fraction=0.5))])
+@torch.no_grad()
+def test_generation_turns_as_the_whole_sequence_does(kw, kv_bits):
+    """Cached rows of the published direction: new tokens and a few rows at once
+    (8 bits: near the whole sequence's, whose keys are not rounded)."""
+    torch.manual_seed(0)
+    m = TS2TSModel.from_config(
+        vocab_size=97, num_layers=2, model_dim=128, num_heads=2, max_seq_len=256, dropout=0.0,
+        drop_path_rate=0.0, block_mask_creator=make_mask_creator_callable("causal"), **kw)
+    m.to(DEV, BF).eval()
+    m.kv_bits = kv_bits
+    tokens = torch.randint(0, 97, (1, 200), generator=torch.Generator().manual_seed(1)).to(DEV)
+    # bf16: as logits_agree's, two layers; e4m3 keys and values: 2^-4 / sqrt(12) of
+    # a value at most in the mean square, averaged over heads and keys: under 2 %
+    # of a layer's attention rows, which are part of the row they are added to
+    bound = 2e-2 if kv_bits == 16 else 6e-2
+    for T in (150, 151, 152, 160, 161):
+        got = m.forward_inference_last(tokens[:, :T], []).float()
+        want = m.forward_inference(tokens[:, :T], [])[:, -1:].float()
+        assert float((got - want).norm() / want.norm()) < bound
+    other = TS2TSModel.from_config(
+        vocab_size=97, num_layers=2, model_dim=128, num_heads=2, max_seq_len=256, dropout=0.0,
+        drop_path_rate=0.0, block_mask_creator=make_mask_creator_callable("causal"),
+        **{**kw, "rotary": dataclasses.replace(kw["rotary"], positive=False)}).to(DEV, BF).eval()
+    for a, b in zip(other.backbone.parameters(), m.backbone.parameters()):
+        a.copy_(b)
+    x = m._embed(tokens[:, :160])
+    bm = make_mask_creator_callable("causal")(tokens=tokens[:, :160])
+    assert not torch.allclose(other.backbone(x, bm), m.backbone(x, bm), atol=1e-3)
