@@ -547,10 +547,10 @@ constexpr int kPairWaves = 8;  // 4 key groups x (P / dV wave, dS / dK wave)
 // Entries 8 h .. 8 h + 7 of P in 16 bits each: 0 <= P <= 1, so that a float's
 // sign and its exponent's highest bit are 0, and 7 exponent and 9 mantissa bits
 // are left (rounded to nearest; bf16 keeps 7).  P is taken as 1 where it is more:
-// LSE is a float, off by 1 where it passes 2^24, and P then by factors of 2.  dK over a row of 16384 tokens,
-// 12 heads, window 1024: 2.4e-3 off its 64-bit value instead of 2.9e-3 (the
-// roundings of dS and of dK itself are 1.7e-3 each), 126 us instead of 114, 4 of
-// them for the minimum.
+// LSE is a float, off by 1 where it passes 2^24, and P then by factors of 2.  dK
+// over a row of 16384 tokens, 12 heads, window 1024: 2.4e-3 off its 64-bit value
+// instead of 2.9e-3 (the roundings of dS and of dK itself are 1.7e-3 each), 126 us
+// instead of 114, 4 of them for the minimum.
 __device__ __forceinline__ bf16x8 pack_fine(const f32x16& acc, int h) {
   uint32_t w[4];
 #pragma unroll

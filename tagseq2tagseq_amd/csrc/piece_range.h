@@ -1,5 +1,4 @@
-// Which pieces of a key/value cache the new rows of a sequence read.  Plain C++,
-// so that the host can check it too.
+// Plain C++, so that the host can check it too.
 #pragma once
 
 #include <cstdint>
@@ -14,8 +13,8 @@ namespace t2t {
 
 // Which pieces of a cache (kPiece positions each) the new rows of one sequence
 // read: their causal range, or with a window and no grant words the hull of
-// their windows (and of sinks behind it) and, before it, the hull of their sinks.  Piece i < count is
-// piece at(i) of the cache.
+// their windows (and of sinks behind it) and, before it, the hull of their
+// sinks.  Piece i < count is piece at(i) of the cache.
 template <int kPiece>
 struct PieceRange {
   int sink0 = 0, sinks = 0, near0 = 0, count = 0;
